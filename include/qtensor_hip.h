@@ -470,6 +470,48 @@ void qtensor_hip_adamw_tail_rows(const qtensor_tail_tensor *table, const int *ch
 void qtensor_hip_sgd_tail(const qtensor_tail_tensor *table, const int *chunk_tensor, int n_chunks, float *partial, int graft,
                           double lr, double momentum, double weight_decay, int nesterov, qtensor_stream_t stream);
 
+/* ---- an attention cache held in 4 bits (no counterpart in the reference, which has no models) --------
+ * Keys and values of the tokens of a batch of sequences.  A vector of a head (head_dim elements) is cut into segments of
+ * blocksize (64, 128 or 256; the last one shorter); a segment is an fp32 scale, fl(largest magnitude / 6), and 4-bit floating
+ * numbers (sign, two bits of exponent, one of mantissa: 0, 1/2, 1, 3/2, 2, 3, 4, 6), the one nearest to fl(element / scale),
+ * ties to the even code; it stands for number * scale.  A segment of zeroes has scale 0; one that holds a NaN or an
+ * infinity reads as NaN.
+ * codes: [pages][kv_heads][page_size][16 * ceil(head_dim / 32)] bytes, first element in the low nibble, what is behind
+ * head_dim zero; scales: [pages][kv_heads][ceil(head_dim / blocksize)][page_size]; both aligned to 16 bytes, for keys and for
+ * values.  page_size: a power of two from 16 to 4096. */
+typedef struct {
+    unsigned char *codes[2];    /* keys, values                                                */
+    float *scales[2];
+    int pages, page_size, kv_heads, head_dim, blocksize;
+} qtensor_cache;
+/* Which tokens a call is about.  Sequence b has lengths[b] tokens, token t in page table[b * table_stride + t / page_size];
+ * the call's tokens are the last starts[b + 1] - starts[b] of each sequence, packed end to end (starts[0] = 0, ascending,
+ * starts[batch] = tokens), or with starts == NULL the last one of each (tokens = batch).  All arrays on the device.  A token
+ * of a negative position (a sequence shorter than its part of the call) or without a page (beyond table_pages, or a page
+ * number outside the cache) is not written, reads as zeros and is not seen. */
+typedef struct {
+    const int *table, *lengths, *starts;
+    long long table_stride;
+    int table_pages, batch, tokens;
+} qtensor_cache_places;
+/* Vectors of the call's tokens: element d of head h of token t at base + t * token_stride + h * head_stride + d (in elements
+ * of fp32 or bf16). */
+typedef struct {
+    void *base;
+    int is_bf16;
+    long long token_stride, head_stride;
+} qtensor_cache_vectors;
+/* Encodes the call's keys and values into the cache; decodes them from it. */
+void qtensor_hip_cache_write(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *keys,
+                             const qtensor_cache_vectors *values, qtensor_stream_t stream);
+void qtensor_hip_cache_read(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *keys,
+                            const qtensor_cache_vectors *values, qtensor_stream_t stream);
+/* out = softmax(scale q k) v for the call's tokens, whose keys and values the cache already has: a token sees those of its
+ * sequence up to itself; with window > 0 only the last `window` of them (itself included) and the first `sinks` of the sequence.
+ * heads is a multiple of kv_heads, query head h reads head h / (heads / kv_heads).  A token that sees nothing gets zeros. */
+void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *q,
+                              const qtensor_cache_vectors *out, int heads, float scale, int window, int sinks, qtensor_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
