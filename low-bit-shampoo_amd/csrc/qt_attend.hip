@@ -1,138 +1,509 @@
 // Attention over a cache held in 4 bits (layout: qt_cache.h): out_i = sum_j p_ij v_j, p_ij = softmax_j(scale q_i . k_j) over the
 // tokens j that query i sees: j <= i and, with a window, i - j < window or j < sinks.
-#include "qt_cache.h"
+//
+// The cache is never expanded: its 4-bit numbers are operands of the scaled matrix instructions as they lie in memory.  Queries and
+// weights are split into pieces of 6 bits (qt_attend.h) and multiplied piece by piece; the fp32 scales of keys multiply scores, those of
+// values the weights before they are split.
+#include "qt_attend.h"
 
 namespace qt {
 namespace {
 
-struct AttendArgs {
-    CacheShape shape;
-    CachePlaces at;
-    const uint8_t *codes[2];
-    const float *scales[2];
-    const void *q;
-    void *out;
-    long long q_token, q_head, out_token, out_head;
-    int heads, group;
-    float factor;           // scale * log2 e
-    int window, sinks;      // window 0: no window
+constexpr int kTile = 128;              // tokens a wave takes at a time: one step of k of a matrix instruction with the weights
+constexpr int kRows = 16;               // queries (of all heads that share a head of the cache) in a tile of rows
+constexpr int kLeastTiles = 8;          // tiles below which a row of tiles is not cut: two for each wave
+
+struct Work {
+    int b, head, row_tile, piece, pieces, slot;      // slot: first partial result of this row of tiles
+    int per_piece;                                   // tiles of one piece
 };
 
-__device__ __forceinline__ float wave_max(float x) {
+__device__ __forceinline__ unsigned long long wave_scan(unsigned long long x) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x = fmaxf(x, __shfl_xor(x, off, 64));
-    return x;
-}
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+    for (int off = 1; off < 64; off <<= 1) {
+        const unsigned long long y = __shfl_up(x, off, 64);
+        if (lane >= off) x += y;
+    }
     return x;
 }
 
-// One wave per query and head: a token per lane for the scores of 64 tokens, then two elements per lane and byte for their values.
-template <bool BF16>
-__global__ __launch_bounds__(256) void attend_kernel(const AttendArgs a) {
-    __shared__ float s_q[4][256];
-    __shared__ float s_p[4][64][4];         // weight times the value's scale, per segment
-    __shared__ long long s_row[4][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int token = blockIdx.x, head = blockIdx.y * 4 + wave;
-    int b = token;
-    if (a.at.starts) b = sequence_of_block(a.at, token);
-    if (head >= a.heads || b >= a.at.batch) return;
-    if (a.at.starts && token < a.at.starts[b]) return;
-    const int dim = a.shape.head_dim, kv = head / a.group;
-    const int position = a.at.starts ? a.at.lengths[b] - (a.at.starts[b + 1] - token) : a.at.lengths[b] - 1;
-    for (int d = lane; d < 256; d += 64) {
-        const long long at = token * a.q_token + head * a.q_head + d;
-        s_q[wave][d] = d >= dim ? 0.0f : BF16 ? bf16_bits_to_float(((const uint16_t *)a.q)[at]) : ((const float *)a.q)[at];
+// Sum over the workgroup (total) and inclusive sum up to this thread, of 256 threads.
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long x, unsigned long long &total, unsigned long long *s) {
+    x = wave_scan(x);
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) s[wave] = x;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) x += s[w];
+        total += s[w];
     }
-    wave_lds_sync();
-    float best = -__builtin_inff(), sum = 0.0f;
-    float acc[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-    int first = 0;
-    const long long covered = (long long)a.at.table_pages << a.shape.page_shift;      // (lengths beyond the table: nothing is there)
-    const int end = (int)min((long long)position + 1, covered);
-    while (first < end) {
-        const int j = first + lane;
-        const bool seen = j < end && (!a.window || position - j < a.window || j < a.sinks);
-        const long long row = seen ? cache_row(a.shape, a.at, b, j, kv) : -1;
-        float score = -__builtin_inff();
-        if (row >= 0) {
-            const uint8_t *codes = a.codes[0] + row * a.shape.row_bytes;
-            const float *scale = a.scales[0] + cache_scale_at(a.shape, row);
-            score = 0.0f;
-            for (int c = 0; c < a.shape.row_bytes; c += 16) {
-                const uint4 w = *(const uint4 *)(codes + c);
-                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-                float part = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float *q = &s_q[wave][2 * c + 8 * i];
-                    const cache_f32x2 e0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i], 1.0f, 0), e1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i], 1.0f, 1),
-                                      e2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i], 1.0f, 2), e3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(v[i], 1.0f, 3);
-                    part += e0.x * q[0] + e0.y * q[1] + e1.x * q[2] + e1.y * q[3] + e2.x * q[4] + e2.y * q[5] + e3.x * q[6] + e3.y * q[7];
-                }
-                score += part * scale[(long long)((2 * c) >> a.shape.segment_shift) << a.shape.page_shift];
-            }
-            score *= a.factor;
+    return x;
+}
+
+__device__ __forceinline__ int row_tiles(const AttendArgs &a, const SequenceView &v) { return (v.count * a.group + kRows - 1) / kRows; }
+
+// How a call is cut: a row of tiles (a sequence, a head of the cache, sixteen queries) into pieces of about as many tiles as all the work
+// has per slot.  Finds the `index`th piece (BY_PIECE) or the first piece of the `index`th row of tiles; false beyond the last.
+template <bool BY_PIECE>
+__device__ __forceinline__ bool find_work(const AttendArgs &a, unsigned index, Work &w) {
+    __shared__ unsigned long long s_sums[4];
+    __shared__ Work s_work;
+    __shared__ int s_found;
+    unsigned long long all = 0;
+    for (int first = 0; first < a.at.batch; first += 256) {
+        const int b = first + (int)threadIdx.x;
+        unsigned long long mine = 0, total;
+        if (b < a.at.batch) {
+            const SequenceView v = view_sequence(a, b);
+            mine = (unsigned long long)row_tiles(a, v) * a.shape.kv_heads * v.tiles;
         }
-        const float top = fmaxf(best, wave_max(score));
-        const float base = top == -__builtin_inff() ? 0.0f : top;
-        const float fade = __builtin_amdgcn_exp2f(best - base);
-        const float p = row >= 0 ? __builtin_amdgcn_exp2f(score - base) : 0.0f;
-        sum = sum * fade + wave_sum(p);
-        best = top;
-        s_row[wave][lane] = row;
-        if (row >= 0)
-            for (int i = 0; i < a.shape.segments; ++i)
-                s_p[wave][lane][i] = p * a.scales[1][cache_scale_at(a.shape, row) + ((long long)i << a.shape.page_shift)];
-        wave_lds_sync();
+        block_scan(mine, total, s_sums);
+        all += total;
+    }
+    const int most = (int)max((unsigned long long)kLeastTiles, (all + a.slots - 1) / a.slots);
+    if (threadIdx.x == 0) s_found = 0;
+    unsigned long long before = 0;          // pieces or rows of tiles (high half) and partial results (low half) of the sequences before
+    for (int first = 0; first < a.at.batch; first += 256) {
+        const int b = first + (int)threadIdx.x;
+        unsigned long long mine = 0, total;
+        int items = 0, pieces = 1, tiles = 0;
+        if (b < a.at.batch) {
+            const SequenceView v = view_sequence(a, b);
+            items = row_tiles(a, v) * a.shape.kv_heads;
+            tiles = v.tiles;
+            pieces = max(1, (tiles + most - 1) / most);
+            mine = ((unsigned long long)(unsigned)(BY_PIECE ? items * pieces : items) << 32) + (unsigned)(pieces > 1 ? items * pieces : 0);
+        }
+        const unsigned long long upto = before + block_scan(mine, total, s_sums), from = upto - mine;
+        if (index >= (unsigned)(from >> 32) && index < (unsigned)(upto >> 32)) {
+            const int local = (int)(index - (unsigned)(from >> 32)), item = BY_PIECE ? local / pieces : local;
+            Work found;
+            found.b = b;
+            found.head = item % a.shape.kv_heads;
+            found.row_tile = item / a.shape.kv_heads;
+            found.piece = BY_PIECE ? local - item * pieces : 0;
+            found.pieces = pieces;
+            found.slot = (int)(unsigned)from + item * pieces;
+            found.per_piece = (tiles + pieces - 1) / pieces;
+            s_work = found;
+            s_found = 1;
+        }
+        before += total;
+        if (index < (unsigned)(before >> 32)) break;
+    }
+    __syncthreads();
+    w = s_work;
+    return s_found != 0;
+}
+
+// 32 consecutive elements of a query from element d on, zeros behind its end.
+template <bool BF16>
+__device__ __forceinline__ void load_query(const AttendArgs &a, long long at, int d, bool there, f32x16 &even, f32x16 &odd) {
+    const int valid = there ? a.shape.head_dim - d : 0;
+    if (BF16) {
+        const uint16_t *p = (const uint16_t *)a.q + at + d;
+        if (valid >= 32 && is_aligned16(p)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) acc[i][0] *= fade, acc[i][1] *= fade;
-        const int count = min(64, end - first);
-        for (int t = 0; t < count; ++t) {
-            const long long here = s_row[wave][t];
-            if (here < 0) continue;
+            for (int i = 0; i < 4; ++i) {
+                const uint4 w = ((const uint4 *)p)[i];
+                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) even[4 * i + e] = __uint_as_float(v[e] << 16), odd[4 * i + e] = __uint_as_float(v[e] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                even[i] = 2 * i < valid ? bf16_bits_to_float(p[2 * i]) : 0.0f;
+                odd[i] = 2 * i + 1 < valid ? bf16_bits_to_float(p[2 * i + 1]) : 0.0f;
+            }
+        }
+    } else {
+        const float *p = (const float *)a.q + at + d;
+        if (valid >= 32 && is_aligned16(p)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 w = ((const float4 *)p)[i];
+                even[2 * i] = w.x, odd[2 * i] = w.y, even[2 * i + 1] = w.z, odd[2 * i + 1] = w.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                even[i] = 2 * i < valid ? p[2 * i] : 0.0f;
+                odd[i] = 2 * i + 1 < valid ? p[2 * i + 1] : 0.0f;
+            }
+        }
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store_result(const AttendArgs &a, long long at, float y) {
+    if (BF16) ((uint16_t *)a.out)[at] = float_to_bf16_bits(y);
+    else ((float *)a.out)[at] = y;
+}
+
+// Few queries per sequence: generation.  A workgroup takes one piece of a row of tiles, its four waves every fourth tile of it.
+//
+// Scores are computed transposed, K Q^T by v_mfma_scale_f32_16x16x128: a lane holds those of query lane % 16 and the tokens 16 t + 4 (lane
+// / 16) + i (t < 8, i < 4) -- 32 of the 128 tokens of a tile, which is just what it has to hold of the weights for O^T = V^T P^T, so weights
+// never leave their lane.  Keys go from memory straight to registers (16 lanes' rows of 64 bytes side by side); values pass through an area
+// of LDS that belongs to the wave, to be read transposed (ds_read_b64_tr_b4: sixteen tokens of one element a lane) in the order of
+// tokens that the weights have.  DP: head_dim rounded up to 64, 128 or 256; UNITS: 1, or DP / 64 where a vector has several scales
+// (each 64 elements then have scores and weights of their own).
+template <int DP, int UNITS, bool BF16>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(const AttendArgs a) {
+    constexpr int kPieces = BF16 ? 3 : 5;
+    constexpr int kHalves = DP == 256 ? 2 : 1;              // 16-byte chunks of a row that a lane holds
+    constexpr int kLoads = DP == 64 ? 4 : 8;                // loads of sixteen tokens by all lanes (thirty-two for rows of 32 bytes)
+    constexpr int kStride = DP / 2 + 8;                     // bytes between rows of values in LDS: tr reads without bank conflicts
+    constexpr int kDTiles = DP / 16;
+    constexpr int kWaveBytes = kTile * kStride + 2 * UNITS * kTile * 4;
+    static_assert(kRows * (DP + 4) * 4 <= kTile * kStride, "a wave's results take the place of its values");
+    __shared__ __attribute__((aligned(16))) uint8_t s_area[4][kWaveBytes];
+    __shared__ float s_best[4][kRows], s_sum[4][kRows];
+
+    Work w;
+    if (!find_work<true>(a, blockIdx.x, w)) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
+    const SequenceView v = view_sequence(a, w.b);
+    const int rows = min(kRows, v.count * a.group - w.row_tile * kRows);
+    const int first_row = w.row_tile * kRows;
+    uint8_t *s_values = s_area[wave];
+    float *s_key_scale = (float *)(s_area[wave] + kTile * kStride), *s_value_scale = s_key_scale + UNITS * kTile;
+
+    // the queries of this lane's column, in pieces
+    const int my_row = first_row + min(column, rows - 1);
+    const int my_token = v.start + my_row / a.group, my_head = w.head * a.group + my_row % a.group;
+    const int position = v.first_position + my_row / a.group;
+    const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;       // last token behind the window
+    u32x6 query[kHalves][kPieces];
+    int query_scale[kHalves][kPieces];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+        f32x16 even, odd;
+        const int chunk = DP == 64 ? g & 1 : g + 4 * h;
+        load_query<BF16>(a, my_token * a.q_token + my_head * a.q_head, 32 * chunk, column < rows, even, odd);
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = max(top, max(__float_as_uint(even[i]) & 0x7fffffffu, __float_as_uint(odd[i]) & 0x7fffffffu));
+        split_fp6<kPieces>(even, odd, top, query[h], query_scale[h]);
+    }
+    const int lowest = v.first_position + first_row / a.group, highest = v.first_position + (first_row + rows - 1) / a.group;
+
+    const int tile_from = w.piece * w.per_piece, tile_to = min(tile_from + w.per_piece, v.tiles);
+    const int *table = a.at.table + (long long)w.b * a.at.table_stride;
+    const int page_mask = (1 << a.shape.page_shift) - 1, chunks = a.shape.row_bytes >> 4;
+
+    auto tile_at = [&](int k) { return (k < v.sink_tiles ? k : v.first_tile + k - v.sink_tiles) * kTile; };
+    // pages of a tile's tokens lane and 64 + lane, -1 where there is none
+    auto load_pages = [&](int k, int *page) {
+        const int base = tile_at(k);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int j = base + 64 * i + lane;
+            page[i] = j < v.end ? table[j >> a.shape.page_shift] : -1;
+        }
+    };
+    i32x4 keys[kHalves][kLoads], values[kHalves][kLoads];
+    float key_scale[UNITS][2], value_scale[UNITS][2];
+    unsigned long long valid[2];
+    auto load_tile = [&](int k, const int *page) {
+        const int base = tile_at(k);
+        int safe[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool there = (unsigned)page[i] < (unsigned)a.shape.pages;
+            safe[i] = there ? page[i] : 0;
+            valid[i] = __ballot(there);
+            const long long line = ((long long)safe[i] * a.shape.kv_heads + w.head) << a.shape.page_shift;
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) {
+                const int segment = min((u * 64) >> a.shape.segment_shift, a.shape.segments - 1);
+                const long long at = line * a.shape.segments + ((long long)segment << a.shape.page_shift) + ((base + lane) & page_mask);
+                const long long where = i == 0 ? at : line * a.shape.segments + ((long long)segment << a.shape.page_shift) + ((base + 64 + lane) & page_mask);
+                key_scale[u][i] = a.scales[0][where];
+                value_scale[u][i] = a.scales[1][where];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < kLoads; ++t) {
+            long long row;
+            if (DP == 64) {
+                const int token = base + 32 * t + (lane >> 5) * 16;
+                const int p0 = __builtin_amdgcn_readlane(safe[t >> 1], 32 * (t & 1)), p1 = __builtin_amdgcn_readlane(safe[t >> 1], 32 * (t & 1) + 16);
+                row = (((long long)(lane < 32 ? p0 : p1) * a.shape.kv_heads + w.head) << a.shape.page_shift) + (token & page_mask);
+            } else {
+                const int p = __builtin_amdgcn_readlane(safe[t >> 2], 16 * (t & 3));
+                row = (((long long)p * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 16 * t) & page_mask);
+            }
+            const long long at = (row + column) * a.shape.row_bytes;
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                // (behind the end of a row the last chunk again: queries are zero there, and results are not stored)
+                const int chunk = min(DP == 64 ? g & 1 : g + 4 * h, chunks - 1);
+                keys[h][t] = *(const i32x4 *)(a.codes[0] + at + 16 * chunk);
+                values[h][t] = *(const i32x4 *)(a.codes[1] + at + 16 * chunk);
+            }
+        }
+    };
+
+    f32x4 result[kDTiles];
+#pragma unroll
+    for (int d = 0; d < kDTiles; ++d) result[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float best = -__builtin_inff(), sum = 0.0f;
+    int page[2];
+    int k = tile_from + wave;
+    if (k < tile_to) {
+        load_pages(k, page);
+        load_tile(k, page);
+        if (k + 4 < tile_to) load_pages(k + 4, page);
+    }
+    for (; k < tile_to; k += 4) {
+        const int base = tile_at(k);
+        const unsigned long long here[2] = {valid[0], valid[1]};
+        // values and scales to LDS; what no page holds has scale 0
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+            for (int t = 0; t < kLoads; ++t) {
+                const int token = DP == 64 ? 32 * t + (lane >> 5) * 16 + column : 16 * t + column;
+                const int chunk = DP == 64 ? g & 1 : g + 4 * h;
+                uint8_t *to = s_values + token * kStride + 16 * chunk;
+                *(i32x2 *)to = (i32x2){values[h][t][0], values[h][t][1]};
+                *(i32x2 *)(to + 8) = (i32x2){values[h][t][2], values[h][t][3]};
+            }
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int byte = lane + 64 * i;
-                if (byte >= a.shape.row_bytes) continue;
-                const float w = s_p[wave][t][(2 * byte) >> a.shape.segment_shift];
-                const cache_f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4((uint32_t)a.codes[1][here * a.shape.row_bytes + byte], 1.0f, 0);
-                acc[i][0] += w * e.x;
-                acc[i][1] += w * e.y;
+                const bool there = (here[i] >> lane) & 1;
+                s_key_scale[u * kTile + 64 * i + lane] = there ? key_scale[u][i] * a.factor : 0.0f;
+                s_value_scale[u * kTile + 64 * i + lane] = there ? value_scale[u][i] : 0.0f;
             }
+        wave_lds_sync();
+        __builtin_amdgcn_sched_barrier(0);
+
+        // scores
+        f32x4 score[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            if constexpr (UNITS == 1) {
+                f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+                    for (int i = kPieces - 1; i >= 0; --i) {
+                        // (rows of 32 bytes: a load holds two times sixteen tokens, of which the scale of 2^-127 takes one away)
+                        const int by = DP == 64 ? ((lane >> 5) == (t & 1) ? query_scale[h][i] : 0) : query_scale[h][i];
+                        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(keys[h][DP == 64 ? t >> 1 : t]), as_operand(query[h][i]), c, kFp4, kFp6,
+                                                                             0, kOne, 0, by);
+                    }
+                score[t] = c * *(const f32x4 *)(s_key_scale + 16 * t + 4 * g);
+            } else {
+                score[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < UNITS; ++u) {
+                    f32x4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = kPieces - 1; i >= 0; --i) {
+                        const int by = (lane >> 5) == (u & 1) ? query_scale[u >> 1][i] : 0;
+                        c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(keys[u >> 1][t]), as_operand(query[u >> 1][i]), c, kFp4, kFp6, 0, kOne,
+                                                                             0, by);
+                    }
+                    score[t] += c * *(const f32x4 *)(s_key_scale + u * kTile + 16 * t + 4 * g);
+                }
+            }
+            if (t & 1) __builtin_amdgcn_sched_barrier(0);
+        }
+        // (done here, so that the keys' registers are free for the next tile)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) asm volatile("" : "+v"(score[t]));
+        __builtin_amdgcn_sched_barrier(0);
+        if (k + 4 < tile_to) {
+            load_tile(k + 4, page);
+            if (k + 8 < tile_to) load_pages(k + 8, page);
+        }
+
+        __builtin_amdgcn_sched_barrier(0);
+        // which of the lane's tokens its query sees
+        const bool full = base + kTile - 1 <= lowest && (!a.window || highest - base < a.window || base + kTile <= a.sinks) && !~here[0] && !~here[1];
+        uint32_t see = 0xffffffffu;
+        if (!full) {
+            see = 0;
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = base + 16 * t + 4 * g + i;
+                    const uint32_t seen = (uint32_t)(j <= position) & ((uint32_t)(j > behind) | (uint32_t)(j < a.sinks)) &
+                                          ((uint32_t)(here[t >> 2] >> (16 * (t & 3) + 4 * g + i)) & 1u);
+                    see |= seen << (4 * t + i);
+                    score[t][i] = seen ? score[t][i] : -__builtin_inff();
+                }
+        }
+        float top = best;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) top = fmaxf(fmaxf(fmaxf(top, score[t][0]), fmaxf(score[t][1], score[t][2])), score[t][3]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float zero = top == -__builtin_inff() ? 0.0f : top;
+        if (__ballot(top != best)) {
+            const float fade = __builtin_amdgcn_exp2f(best - zero);
+            sum *= fade;
+#pragma unroll
+            for (int d = 0; d < kDTiles; ++d) result[d] *= fade;
+            best = top;
+        }
+        f32x4 weight[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                weight[t][i] = __builtin_amdgcn_exp2f(score[t][i] - zero);
+                sum += weight[t][i];
+            }
+
+        __builtin_amdgcn_sched_barrier(0);
+        // their values: weights times scales in pieces, element by element of the values' rows
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) {
+            f32x16 early, late;
+            uint32_t most = 0;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const f32x4 by = *(const f32x4 *)(s_value_scale + u * kTile + 16 * t + 4 * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = weight[t][i] * by[i];
+                    if (!full) x = (see >> (4 * t + i)) & 1 ? x : 0.0f;         // (whatever its scale is)
+                    most = max(most, __float_as_uint(x));
+                    if (t < 4) early[4 * t + i] = x;
+                    else late[4 * (t - 4) + i] = x;
+                }
+                if (t == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+            u32x6 piece[kPieces];
+            int by[kPieces];
+            split_fp6<kPieces>(early, late, most, piece, by);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int d = 0; d < kDTiles / UNITS; ++d) {
+                const int dt = u * (kDTiles / UNITS) + d;
+                i32x4 rows_of_v;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    // position 16 h + j of the weights is register (16 h + j) / 2 of the first or (odd) the second sixteen
+                    const int n = 8 * h + (column >> 1), token = 16 * (n >> 2) + 4 * g + (n & 3) + 64 * (column & 1);
+                    const i32x2 part = __builtin_amdgcn_ds_read_tr4_b64_v2i32((QT_LDS i32x2 *)(s_values + token * kStride + 8 * dt));
+                    rows_of_v[2 * h] = part[0], rows_of_v[2 * h + 1] = part[1];
+                }
+#pragma unroll
+                for (int i = kPieces - 1; i >= 0; --i)
+                    result[dt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(rows_of_v), as_operand(piece[i]), result[dt], kFp4, kFp6, 0, kOne, 0,
+                                                                                  by[i]);
+                if (d & 1) __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
         wave_lds_sync();
-        first += 64;
-        if (a.window && first >= a.sinks) first = max(first, (position + 1 - a.window) & ~63);
     }
-    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+
+    // the four waves' results, joined
+    if (lane < kRows) s_best[wave][lane] = best, s_sum[wave][lane] = sum;
+    float *s_result = (float *)s_area[wave];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int d = 0; d < kDTiles; ++d) *(f32x4 *)(s_result + column * (DP + 4) + 16 * d + 4 * g) = result[d];
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * DP; e += 256) {
+        const int r = e / DP, d = e % DP;
+        float top = s_best[0][r];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int d = 2 * (lane + 64 * i) + e;
-            if (d >= dim) continue;
-            const long long at = token * a.out_token + head * a.out_head + d;
-            const float y = sum == 0.0f ? 0.0f : acc[i][e] * by;
-            if (BF16) ((uint16_t *)a.out)[at] = float_to_bf16_bits(y);
-            else ((float *)a.out)[at] = y;
+        for (int i = 1; i < 4; ++i) top = fmaxf(top, s_best[i][r]);
+        const float zero = top == -__builtin_inff() ? 0.0f : top;
+        float total = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float fade = __builtin_amdgcn_exp2f(s_best[i][r] - zero);
+            total += s_sum[i][r] * fade;
+            y += ((const float *)s_area[i])[r * (DP + 4) + d] * fade;
         }
+        if (w.pieces > 1) {
+            float *part = a.partial + (long long)(w.slot + w.piece) * kRows * (DP + 2) + r * (DP + 2);
+            part[2 + d] = y;
+            if (d == 0) part[0] = top, part[1] = total;
+        } else if (d < a.shape.head_dim) {
+            const int row = first_row + r;
+            store_result<BF16>(a, (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head + d,
+                               total == 0.0f ? 0.0f : y / total);
+        }
+    }
+}
+
+// Joins the pieces of every row of tiles that was cut.
+template <int DP, bool BF16>
+__global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
+    Work w;
+    if (!find_work<false>(a, blockIdx.x, w) || w.pieces == 1) return;
+    const SequenceView v = view_sequence(a, w.b);
+    const int first_row = w.row_tile * kRows, rows = min(kRows, v.count * a.group - first_row);
+    for (int e = threadIdx.x; e < rows * DP; e += 256) {
+        const int r = e / DP, d = e % DP;
+        if (d >= a.shape.head_dim) continue;
+        const float *part = a.partial + (long long)w.slot * kRows * (DP + 2) + r * (DP + 2);
+        constexpr int kNext = kRows * (DP + 2);
+        float top = -__builtin_inff();
+        for (int i = 0; i < w.pieces; ++i) top = fmaxf(top, part[(long long)i * kNext]);
+        const float zero = top == -__builtin_inff() ? 0.0f : top;
+        float total = 0.0f, y = 0.0f;
+        for (int i = 0; i < w.pieces; ++i) {
+            const float *p = part + (long long)i * kNext;
+            const float fade = __builtin_amdgcn_exp2f(p[0] - zero);
+            total += p[1] * fade;
+            y += p[2 + d] * fade;
+        }
+        const int row = first_row + r;
+        store_result<BF16>(a, (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head + d,
+                           total == 0.0f ? 0.0f : y / total);
+    }
+}
+
+int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+int slots_of(int dim) { return compute_units() * (dim == 256 ? 1 : 2); }
+
+template <int DP, bool BF16>
+void launch_attend(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream) {
+    const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u));
+    if (DP == 64 || a.shape.segments == 1) hipLaunchKernelGGL((attend_few_kernel<DP, 1, BF16>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attend_few_kernel<DP, DP / 64, BF16>), grid, dim3(256), 0, stream, a);
+    if (may_cut) hipLaunchKernelGGL((attend_join_kernel<DP, BF16>), dim3(rows_of_tiles), dim3(256), 0, stream, a);
 }
 
 }  // namespace
 }  // namespace qt
 
+extern "C" long long qtensor_hip_cache_attend_workspace(const qtensor_cache *cache) {
+    using namespace qt;
+    clear_error();
+    CacheShape shape;
+    if (!cache_shape("cache_attend_workspace", cache, shape)) return 0;
+    const int dim = padded_dim(shape.head_dim);
+    return 2LL * slots_of(dim) * kRows * (dim + 2) * (long long)sizeof(float);
+}
+
 extern "C" void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *q,
-                                         const qtensor_cache_vectors *out, int heads, float scale, int window, int sinks, void *stream) {
+                                         const qtensor_cache_vectors *out, int heads, float scale, int window, int sinks, void *workspace,
+                                         long long workspace_bytes, void *stream_v) {
     using namespace qt;
     clear_error();
     AttendArgs a;
     if (!cache_shape("cache_attend", cache, a.shape) || !cache_places("cache_attend", places, a.at)) return;
     if (!q || !out || (a.at.tokens > 0 && (!q->base || !out->base))) { set_error(kNullPointer, "cache_attend: null queries or result"); return; }
-    if (heads < 1 || heads > 65535 || heads % a.shape.kv_heads || window < 0 || sinks < 0 || !(scale - scale == 0.0f) || q->is_bf16 != out->is_bf16) {
+    if (heads < 1 || heads > 32767 || heads % a.shape.kv_heads || window < 0 || sinks < 0 || !(scale - scale == 0.0f) || q->is_bf16 != out->is_bf16) {
         set_error(kBadArgument, "cache_attend: needs query heads that are a multiple of the cache's, a finite scale, window and sinks of at least 0 and a "
                                 "result of the queries' type (got %d heads of %d, scale %g, window %d, sinks %d)", heads, a.shape.kv_heads, scale, window, sinks);
         return;
@@ -148,8 +519,23 @@ extern "C" void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtens
     a.heads = heads, a.group = heads / a.shape.kv_heads;
     a.factor = scale * 1.4426950408889634f;
     a.window = window, a.sinks = sinks;
-    const dim3 grid(a.at.tokens, (heads + 3) / 4);
-    if (q->is_bf16) hipLaunchKernelGGL(attend_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(attend_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, a);
+    const int dim = padded_dim(a.shape.head_dim);
+    a.slots = slots_of(dim);
+    a.partial = (float *)workspace;
+    // rows of tiles: at most one more per sequence than full ones
+    const long long rows = (long long)a.at.tokens * a.group;
+    const long long rows_of_tiles = a.shape.kv_heads * (a.at.starts ? rows / kRows + a.at.batch : a.at.batch * (long long)((a.group + kRows - 1) / kRows));
+    if (rows >= (1LL << 31) || rows_of_tiles >= (1LL << 30)) { set_error(kBadArgument, "cache_attend: %d tokens are too many for one call", a.at.tokens); return; }
+    const bool may_cut = ((long long)a.at.table_pages << a.shape.page_shift) > kLeastTiles * kTile;
+    if (may_cut && (!workspace || !is_aligned(workspace, 16) || workspace_bytes < 2LL * a.slots * kRows * (dim + 2) * (long long)sizeof(float))) {
+        set_error(kBadArgument, "cache_attend: the workspace is smaller than qtensor_hip_cache_attend_workspace says");
+        return;
+    }
+    const hipStream_t stream = (hipStream_t)stream_v;
+    const unsigned n = (unsigned)rows_of_tiles;
+    auto launch = dim == 64 ? (q->is_bf16 ? launch_attend<64, true> : launch_attend<64, false>)
+                : dim == 128 ? (q->is_bf16 ? launch_attend<128, true> : launch_attend<128, false>)
+                             : (q->is_bf16 ? launch_attend<256, true> : launch_attend<256, false>);
+    launch(a, n, may_cut, stream);
     launch_ok("cache_attend");
 }

@@ -48,7 +48,9 @@ if F.lib is not None:
         getattr(F.lib, _name).argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.POINTER(_Vectors), ct.POINTER(_Vectors), ct.c_void_p]
     F.lib.qtensor_hip_cache_attend.restype = None
     F.lib.qtensor_hip_cache_attend.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.POINTER(_Vectors), ct.POINTER(_Vectors), ct.c_int,
-                                               ct.c_float, ct.c_int, ct.c_int, ct.c_void_p]
+                                               ct.c_float, ct.c_int, ct.c_int, ct.c_void_p, ct.c_longlong, ct.c_void_p]
+    F.lib.qtensor_hip_cache_attend_workspace.restype = ct.c_longlong
+    F.lib.qtensor_hip_cache_attend_workspace.argtypes = [ct.POINTER(_Cache)]
 
 
 class QTensorCache:
@@ -140,8 +142,12 @@ class QTensorCache:
         else:
             self._check_vectors(out, "out", (tokens, heads, self.head_dim), q.dtype)
         places = self._places(table, lengths, starts, tokens)
+        # scratch for the pieces of long sequences: taken for the call, as that of the products is
+        with torch.cuda.device(q.device):
+            size = F.lib.qtensor_hip_cache_attend_workspace(self._ref())
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
         F._call(F.lib.qtensor_hip_cache_attend, q.device, self._ref(), places, _vectors(q), _vectors(out), heads, scale,
-                window or 0, sinks)
+                window or 0, sinks, scratch.data_ptr(), size)
         return out
 
     # ---- checks and descriptions
