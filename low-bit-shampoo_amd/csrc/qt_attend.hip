@@ -100,6 +100,12 @@ __device__ __forceinline__ bool find_work(const AttendArgs &a, unsigned index, W
     return s_found != 0;
 }
 
+// Of the tokens 16 t + i of a lane (t < 8, i < 4; bit 4 t + i), those up to x.
+__device__ __forceinline__ uint32_t tokens_up_to(int x) {
+    const int bits = 4 * (x >> 4) + min(x & 15, 3) + 1;
+    return x < 0 ? 0u : x >= 115 ? 0xffffffffu : (1u << (bits & 31)) - 1u;
+}
+
 // 32 consecutive elements of a query from element d on, zeros behind its end.
 template <bool BF16>
 __device__ __forceinline__ void load_query(const AttendArgs &a, long long at, int d, bool there, f32x16 &even, f32x16 &odd) {
@@ -145,6 +151,8 @@ __device__ __forceinline__ void store_result(const AttendArgs &a, long long at, 
     else ((float *)a.out)[at] = y;
 }
 
+constexpr int few_waves(int dim, int units, bool bf16) { return dim == 64 || (dim == 128 && units == 1 && bf16) ? 2 : 1; }
+
 // Few queries per sequence: generation.  A workgroup takes one piece of a row of tiles, its four waves every fourth tile of it.
 //
 // Scores are computed transposed, K Q^T by v_mfma_scale_f32_16x16x128: a lane holds those of query lane % 16 and the tokens 16 t + 4 (lane
@@ -154,7 +162,7 @@ __device__ __forceinline__ void store_result(const AttendArgs &a, long long at, 
 // tokens that the weights have.  DP: head_dim rounded up to 64, 128 or 256; UNITS: 1, or DP / 64 where a vector has several scales
 // (each 64 elements then have scores and weights of their own).
 template <int DP, int UNITS, bool BF16>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(const AttendArgs a) {
+__global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_kernel(const AttendArgs a) {
     constexpr int kPieces = BF16 ? 3 : 5;
     constexpr int kHalves = DP == 256 ? 2 : 1;              // 16-byte chunks of a row that a lane holds
     constexpr int kLoads = DP == 64 ? 4 : 8;                // loads of sixteen tokens by all lanes (thirty-two for rows of 32 bytes)
@@ -167,7 +175,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
 
     Work w;
     if (!find_work<true>(a, blockIdx.x, w)) return;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
+    w.b = __builtin_amdgcn_readfirstlane(w.b);
+    w.head = __builtin_amdgcn_readfirstlane(w.head);
+    w.row_tile = __builtin_amdgcn_readfirstlane(w.row_tile);
+    w.piece = __builtin_amdgcn_readfirstlane(w.piece);
+    w.per_piece = __builtin_amdgcn_readfirstlane(w.per_piece);
     const SequenceView v = view_sequence(a, w.b);
     const int rows = min(kRows, v.count * a.group - w.row_tile * kRows);
     const int first_row = w.row_tile * kRows;
@@ -208,6 +221,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
         }
     };
     i32x4 keys[kHalves][kLoads], values[kHalves][kLoads];
+    uint32_t inside[kHalves];           // this lane's 16 bytes among sixteen rows; behind the end of a row the last chunk again (queries are
+                                        // zero there, and results are not stored)
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) inside[h] = column * a.shape.row_bytes + 16 * min(DP == 64 ? g & 1 : g + 4 * h, chunks - 1);
     float key_scale[UNITS][2], value_scale[UNITS][2];
     unsigned long long valid[2];
     auto load_tile = [&](int k, const int *page) {
@@ -228,24 +245,23 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
                 value_scale[u][i] = a.scales[1][where];
             }
         }
+        // (one base per sixteen tokens in scalar registers, the lane's place among them in one vector register for all loads)
 #pragma unroll
         for (int t = 0; t < kLoads; ++t) {
-            long long row;
+            long long at;
             if (DP == 64) {
-                const int token = base + 32 * t + (lane >> 5) * 16;
                 const int p0 = __builtin_amdgcn_readlane(safe[t >> 1], 32 * (t & 1)), p1 = __builtin_amdgcn_readlane(safe[t >> 1], 32 * (t & 1) + 16);
-                row = (((long long)(lane < 32 ? p0 : p1) * a.shape.kv_heads + w.head) << a.shape.page_shift) + (token & page_mask);
+                const long long at0 = ((((long long)p0 * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 32 * t) & page_mask)) * a.shape.row_bytes;
+                const long long at1 = ((((long long)p1 * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 32 * t + 16) & page_mask)) * a.shape.row_bytes;
+                at = lane < 32 ? at0 : at1;
             } else {
                 const int p = __builtin_amdgcn_readlane(safe[t >> 2], 16 * (t & 3));
-                row = (((long long)p * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 16 * t) & page_mask);
+                at = ((((long long)p * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 16 * t) & page_mask)) * a.shape.row_bytes;
             }
-            const long long at = (row + column) * a.shape.row_bytes;
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
-                // (behind the end of a row the last chunk again: queries are zero there, and results are not stored)
-                const int chunk = min(DP == 64 ? g & 1 : g + 4 * h, chunks - 1);
-                keys[h][t] = *(const i32x4 *)(a.codes[0] + at + 16 * chunk);
-                values[h][t] = *(const i32x4 *)(a.codes[1] + at + 16 * chunk);
+                keys[h][t] = *(const i32x4 *)(a.codes[0] + at + inside[h]);
+                values[h][t] = *(const i32x4 *)(a.codes[1] + at + inside[h]);
             }
         }
     };
@@ -283,6 +299,11 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
                 s_key_scale[u * kTile + 64 * i + lane] = there ? key_scale[u][i] * a.factor : 0.0f;
                 s_value_scale[u * kTile + 64 * i + lane] = there ? value_scale[u][i] : 0.0f;
             }
+        // (a weight of zero times a scale that is not finite is not zero: only then such weights are looked for)
+        float odd_scale = 0.0f;
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) odd_scale += 0.0f * value_scale[u][0] + 0.0f * value_scale[u][1];
+        const bool odd = __ballot(odd_scale != 0.0f) != 0;
         wave_lds_sync();
         __builtin_amdgcn_sched_barrier(0);
 
@@ -303,7 +324,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
                     }
                 score[t] = c * *(const f32x4 *)(s_key_scale + 16 * t + 4 * g);
             } else {
-                score[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
                     f32x4 c = {0.f, 0.f, 0.f, 0.f};
@@ -313,7 +333,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
                         c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(keys[u >> 1][t]), as_operand(query[u >> 1][i]), c, kFp4, kFp6, 0, kOne,
                                                                              0, by);
                     }
-                    score[t] += c * *(const f32x4 *)(s_key_scale + u * kTile + 16 * t + 4 * g);
+                    c *= *(const f32x4 *)(s_key_scale + u * kTile + 16 * t + 4 * g);
+                    score[t] = u == 0 ? c : score[t] + c;
                 }
             }
             if (t & 1) __builtin_amdgcn_sched_barrier(0);
@@ -328,21 +349,21 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
         }
 
         __builtin_amdgcn_sched_barrier(0);
-        // which of the lane's tokens its query sees
-        const bool full = base + kTile - 1 <= lowest && (!a.window || highest - base < a.window || base + kTile <= a.sinks) && !~here[0] && !~here[1];
+        // which of the lane's tokens its query sees: bit 4 t + i of `see` (tokens past the end are past every position)
+        const bool whole = !(~here[0] | ~here[1]);
+        const bool full = base + kTile - 1 <= lowest && (!a.window || highest - base < a.window || base + kTile <= a.sinks) && whole;
         uint32_t see = 0xffffffffu;
         if (!full) {
-            see = 0;
+            see = tokens_up_to(position - base - 4 * g);
+            if (a.window) see &= ~tokens_up_to(behind - base - 4 * g) | tokens_up_to(a.sinks - 1 - base - 4 * g);
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < 8; ++t) see &= ~(15u << (4 * t)) | (((uint32_t)(here[t >> 2] >> (16 * (t & 3) + 4 * g)) & 15u) << (4 * t));
+            }
 #pragma unroll
             for (int t = 0; t < 8; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int j = base + 16 * t + 4 * g + i;
-                    const uint32_t seen = (uint32_t)(j <= position) & ((uint32_t)(j > behind) | (uint32_t)(j < a.sinks)) &
-                                          ((uint32_t)(here[t >> 2] >> (16 * (t & 3) + 4 * g + i)) & 1u);
-                    see |= seen << (4 * t + i);
-                    score[t][i] = seen ? score[t][i] : -__builtin_inff();
-                }
+                for (int i = 0; i < 4; ++i) score[t][i] = see & (1u << (4 * t + i)) ? score[t][i] : -__builtin_inff();
         }
         float top = best;
 #pragma unroll
@@ -377,13 +398,21 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
                 const f32x4 by = *(const f32x4 *)(s_value_scale + u * kTile + 16 * t + 4 * g);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float x = weight[t][i] * by[i];
-                    if (!full) x = (see >> (4 * t + i)) & 1 ? x : 0.0f;         // (whatever its scale is)
+                    const float x = weight[t][i] * by[i];
                     most = max(most, __float_as_uint(x));
                     if (t < 4) early[4 * t + i] = x;
                     else late[4 * (t - 4) + i] = x;
                 }
                 if (t == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+            if (__builtin_expect(odd, 0)) {
+                most = 0;
+#pragma unroll
+                for (int n = 0; n < 16; ++n) {
+                    early[n] = see & (1u << n) ? early[n] : 0.0f;
+                    late[n] = see & (1u << (16 + n)) ? late[n] : 0.0f;
+                    most = max(most, max(__float_as_uint(early[n]), __float_as_uint(late[n])));
+                }
             }
             u32x6 piece[kPieces];
             int by[kPieces];
@@ -444,32 +473,64 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_few_kernel(cons
     }
 }
 
-// Joins the pieces of every row of tiles that was cut.
+// Joins the pieces of every row of tiles that was cut, a workgroup for each of its rows: what the pieces count for first, then a
+// share of them per group of DP / 4 threads.
 template <int DP, bool BF16>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
+    constexpr int kGroups = 1024 / DP;
+    __shared__ float s_share[256];
+    __shared__ float s_reduce[4], s_total[4];
+    __shared__ f32x4 s_part[256];
     Work w;
     if (!find_work<false>(a, blockIdx.x, w) || w.pieces == 1) return;
     const SequenceView v = view_sequence(a, w.b);
-    const int first_row = w.row_tile * kRows, rows = min(kRows, v.count * a.group - first_row);
-    for (int e = threadIdx.x; e < rows * DP; e += 256) {
-        const int r = e / DP, d = e % DP;
-        if (d >= a.shape.head_dim) continue;
-        const float *part = a.partial + (long long)w.slot * kRows * (DP + 2) + r * (DP + 2);
-        constexpr int kNext = kRows * (DP + 2);
-        float top = -__builtin_inff();
-        for (int i = 0; i < w.pieces; ++i) top = fmaxf(top, part[(long long)i * kNext]);
-        const float zero = top == -__builtin_inff() ? 0.0f : top;
-        float total = 0.0f, y = 0.0f;
-        for (int i = 0; i < w.pieces; ++i) {
-            const float *p = part + (long long)i * kNext;
-            const float fade = __builtin_amdgcn_exp2f(p[0] - zero);
-            total += p[1] * fade;
-            y += p[2 + d] * fade;
+    const int row = w.row_tile * kRows + blockIdx.y;
+    if (row >= v.count * a.group) return;
+    constexpr int kNext = kRows * (DP + 2);
+    const float *part = a.partial + (long long)w.slot * kNext + blockIdx.y * (DP + 2);
+    const int wave = threadIdx.x >> 6;
+    float top = -__builtin_inff();
+    for (int i = threadIdx.x; i < w.pieces; i += 256) top = fmaxf(top, part[(long long)i * kNext]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    if ((threadIdx.x & 63) == 0) s_reduce[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_reduce[0], s_reduce[1]), fmaxf(s_reduce[2], s_reduce[3]));
+    const float zero = top == -__builtin_inff() ? 0.0f : top;
+    const int group = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+    float total = 0.0f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first < w.pieces; first += 256) {
+        const int i = first + (int)threadIdx.x, count = min(256, w.pieces - first);
+        __syncthreads();
+        float share = 0.0f;
+        if (i < w.pieces) {
+            share = __builtin_amdgcn_exp2f(part[(long long)i * kNext] - zero);
+            total += part[(long long)i * kNext + 1] * share;
         }
-        const int row = first_row + r;
-        store_result<BF16>(a, (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head + d,
-                           total == 0.0f ? 0.0f : y / total);
+        s_share[threadIdx.x] = share;
+        __syncthreads();
+#pragma unroll 4
+        for (int j = group; j < count; j += kGroups) {
+            const float2 *p = (const float2 *)(part + (long long)(first + j) * kNext + 2 + d);
+            const float2 u = p[0], v2 = p[1];
+            const float by = s_share[j];
+            y += (f32x4){u.x * by, u.y * by, v2.x * by, v2.y * by};
+        }
     }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    if ((threadIdx.x & 63) == 0) s_total[wave] = total;
+    s_part[threadIdx.x] = y;
+    __syncthreads();
+    total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
+    if (group != 0) return;
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) y += s_part[threadIdx.x + i * (DP / 4)];
+    const long long at = (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (d + e < a.shape.head_dim) store_result<BF16>(a, at + d + e, total == 0.0f ? 0.0f : y[e] / total);
 }
 
 int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -480,7 +541,7 @@ void launch_attend(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hi
     const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u));
     if (DP == 64 || a.shape.segments == 1) hipLaunchKernelGGL((attend_few_kernel<DP, 1, BF16>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((attend_few_kernel<DP, DP / 64, BF16>), grid, dim3(256), 0, stream, a);
-    if (may_cut) hipLaunchKernelGGL((attend_join_kernel<DP, BF16>), dim3(rows_of_tiles), dim3(256), 0, stream, a);
+    if (may_cut) hipLaunchKernelGGL((attend_join_kernel<DP, BF16>), dim3(rows_of_tiles, a.at.starts ? kRows : min(kRows, a.group)), dim3(256), 0, stream, a);
 }
 
 }  // namespace
