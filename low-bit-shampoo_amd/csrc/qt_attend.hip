@@ -6,6 +6,8 @@
 // values the weights before they are split.
 #include "qt_attend.h"
 
+#include <type_traits>
+
 namespace qt {
 namespace {
 
@@ -75,7 +77,7 @@ __device__ __forceinline__ bool find_work(const AttendArgs &a, unsigned index, W
             const SequenceView v = view_sequence(a, b);
             items = row_tiles(a, v) * a.shape.kv_heads;
             tiles = v.tiles;
-            pieces = max(1, (tiles + most - 1) / most);
+            pieces = max(1, (tiles + most / 2) / most);       // (of up to one and a half times as many tiles: half a piece is not worth a join)
             mine = ((unsigned long long)(unsigned)(BY_PIECE ? items * pieces : items) << 32) + (unsigned)(pieces > 1 ? items * pieces : 0);
         }
         const unsigned long long upto = before + block_scan(mine, total, s_sums), from = upto - mine;
@@ -104,6 +106,20 @@ __device__ __forceinline__ bool find_work(const AttendArgs &a, unsigned index, W
 __device__ __forceinline__ uint32_t tokens_up_to(int x) {
     const int bits = 4 * (x >> 4) + min(x & 15, 3) + 1;
     return x < 0 ? 0u : x >= 115 ? 0xffffffffu : (1u << (bits & 31)) - 1u;
+}
+
+// x times what lanes 4 t ... 4 t + 3 of the lane's row of sixteen hold.
+template <int LANE>
+__device__ __forceinline__ float of_row(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x150 + LANE, 0xf, 0xf, false));
+}
+__device__ __forceinline__ f32x4 times_row(f32x4 x, float by, int t) {
+    switch (t) {
+    case 0: return (f32x4){x[0] * of_row<0>(by), x[1] * of_row<1>(by), x[2] * of_row<2>(by), x[3] * of_row<3>(by)};
+    case 1: return (f32x4){x[0] * of_row<4>(by), x[1] * of_row<5>(by), x[2] * of_row<6>(by), x[3] * of_row<7>(by)};
+    case 2: return (f32x4){x[0] * of_row<8>(by), x[1] * of_row<9>(by), x[2] * of_row<10>(by), x[3] * of_row<11>(by)};
+    default: return (f32x4){x[0] * of_row<12>(by), x[1] * of_row<13>(by), x[2] * of_row<14>(by), x[3] * of_row<15>(by)};
+    }
 }
 
 // 32 consecutive elements of a query from element d on, zeros behind its end.
@@ -151,7 +167,16 @@ __device__ __forceinline__ void store_result(const AttendArgs &a, long long at, 
     else ((float *)a.out)[at] = y;
 }
 
+constexpr int kWaitLds = 0xc07f;        // s_waitcnt lgkmcnt(0), nothing else
+
 constexpr int few_waves(int dim, int units, bool bf16) { return dim == 64 || (dim == 128 && units == 1 && bf16) ? 2 : 1; }
+
+// Order of the 16-byte chunks of row `row` of values in LDS: chunk c stands at c ^ swap.  Of the 64 rows that a transposed read takes eight
+// bytes each from, four share a bank then, as few as 512 bytes can.
+template <int DP>
+__device__ __forceinline__ int swap_of(int row) {
+    return DP == 64 ? (row >> 3) & 1 : DP == 128 ? (row >> 2) & 3 : (row >> 1) & 7;
+}
 
 // Few queries per sequence: generation.  A workgroup takes one piece of a row of tiles, its four waves every fourth tile of it.
 //
@@ -166,11 +191,12 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     constexpr int kPieces = BF16 ? 3 : 5;
     constexpr int kHalves = DP == 256 ? 2 : 1;              // 16-byte chunks of a row that a lane holds
     constexpr int kLoads = DP == 64 ? 4 : 8;                // loads of sixteen tokens by all lanes (thirty-two for rows of 32 bytes)
-    constexpr int kStride = DP / 2 + 8;                     // bytes between rows of values in LDS: tr reads without bank conflicts
+    constexpr int kRowBytes = DP / 2;                       // of a token's values in LDS; the 16-byte chunks of a row stand in an order of
+                                                            // its own (swap), so that transposed reads fall on all banks
+    constexpr int kValueLoads = kTile * kRowBytes / 1024;
     constexpr int kDTiles = DP / 16;
-    constexpr int kWaveBytes = kTile * kStride + 2 * UNITS * kTile * 4;
-    static_assert(kRows * (DP + 4) * 4 <= kTile * kStride, "a wave's results take the place of its values");
-    __shared__ __attribute__((aligned(16))) uint8_t s_area[4][kWaveBytes];
+    constexpr int kArea = kTile * kRowBytes > kRows * (DP + 4) * 4 ? kTile * kRowBytes : kRows * (DP + 4) * 4;      // a wave's results take the place of its values
+    __shared__ __attribute__((aligned(16))) uint8_t s_area[4][kArea];
     __shared__ float s_best[4][kRows], s_sum[4][kRows];
 
     Work w;
@@ -185,7 +211,6 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     const int rows = min(kRows, v.count * a.group - w.row_tile * kRows);
     const int first_row = w.row_tile * kRows;
     uint8_t *s_values = s_area[wave];
-    float *s_key_scale = (float *)(s_area[wave] + kTile * kStride), *s_value_scale = s_key_scale + UNITS * kTile;
 
     // the queries of this lane's column, in pieces
     const int my_row = first_row + min(column, rows - 1);
@@ -211,58 +236,68 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     const int page_mask = (1 << a.shape.page_shift) - 1, chunks = a.shape.row_bytes >> 4;
 
     auto tile_at = [&](int k) { return (k < v.sink_tiles ? k : v.first_tile + k - v.sink_tiles) * kTile; };
-    // pages of a tile's tokens lane and 64 + lane, -1 where there is none
+    // The token whose page and scales this lane looks up, and 64 further on: those that its row of 16 lanes has scores of, one each, so that
+    // they reach the others of the row as operands of its multiplications (row_newbcast)
+    const int own_token = 16 * (column >> 2) + 4 * g + (column & 3);
     auto load_pages = [&](int k, int *page) {
-        const int base = tile_at(k);
+        const int base = tile_at(k) + own_token;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int j = base + 64 * i + lane;
-            page[i] = j < v.end ? table[j >> a.shape.page_shift] : -1;
-        }
+        for (int i = 0; i < 2; ++i) page[i] = table[min(base + 64 * i, v.end - 1) >> a.shape.page_shift];
     };
-    i32x4 keys[kHalves][kLoads], values[kHalves][kLoads];
+    i32x4 keys[kHalves][kLoads];
     uint32_t inside[kHalves];           // this lane's 16 bytes among sixteen rows; behind the end of a row the last chunk again (queries are
                                         // zero there, and results are not stored)
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) inside[h] = column * a.shape.row_bytes + 16 * min(DP == 64 ? g & 1 : g + 4 * h, chunks - 1);
     float key_scale[UNITS][2], value_scale[UNITS][2];
     unsigned long long valid[2];
+    uint32_t value_inside[DP == 256 ? 2 : 1];       // what the same lane loads of the values: chunk (lane's place) ^ swap of its row
+#pragma unroll
+    for (int i = 0; i < (DP == 256 ? 2 : 1); ++i) {
+        constexpr int kChunks = DP / 32;
+        const int row = DP == 64 ? (lane >> 1) & 15 : DP == 128 ? lane >> 2 : 8 * i + (lane >> 3);
+        value_inside[i] = row * a.shape.row_bytes + 16 * min((lane & (kChunks - 1)) ^ swap_of<DP>(row), chunks - 1);
+    }
+    // sixteen tokens from 16 t of a tile on: where their rows begin
+    auto line_of = [&](const int *safe, int base, int t) {
+        const int p = __builtin_amdgcn_readlane(safe[t >> 2], 4 * (t & 3));
+        return ((((long long)p * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 16 * t) & page_mask)) * a.shape.row_bytes;
+    };
+    int safe[2];
     auto load_tile = [&](int k, const int *page) {
         const int base = tile_at(k);
-        int safe[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const bool there = (unsigned)page[i] < (unsigned)a.shape.pages;
+            const bool there = (unsigned)page[i] < (unsigned)a.shape.pages && base + 64 * i + own_token < v.end;
             safe[i] = there ? page[i] : 0;
             valid[i] = __ballot(there);
             const long long line = ((long long)safe[i] * a.shape.kv_heads + w.head) << a.shape.page_shift;
 #pragma unroll
             for (int u = 0; u < UNITS; ++u) {
                 const int segment = min((u * 64) >> a.shape.segment_shift, a.shape.segments - 1);
-                const long long at = line * a.shape.segments + ((long long)segment << a.shape.page_shift) + ((base + lane) & page_mask);
-                const long long where = i == 0 ? at : line * a.shape.segments + ((long long)segment << a.shape.page_shift) + ((base + 64 + lane) & page_mask);
-                key_scale[u][i] = a.scales[0][where];
-                value_scale[u][i] = a.scales[1][where];
+                const long long at = line * a.shape.segments + ((long long)segment << a.shape.page_shift) + ((base + 64 * i + own_token) & page_mask);
+                key_scale[u][i] = a.scales[0][at];
+                value_scale[u][i] = a.scales[1][at];
             }
         }
         // (one base per sixteen tokens in scalar registers, the lane's place among them in one vector register for all loads)
 #pragma unroll
         for (int t = 0; t < kLoads; ++t) {
-            long long at;
-            if (DP == 64) {
-                const int p0 = __builtin_amdgcn_readlane(safe[t >> 1], 32 * (t & 1)), p1 = __builtin_amdgcn_readlane(safe[t >> 1], 32 * (t & 1) + 16);
-                const long long at0 = ((((long long)p0 * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 32 * t) & page_mask)) * a.shape.row_bytes;
-                const long long at1 = ((((long long)p1 * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 32 * t + 16) & page_mask)) * a.shape.row_bytes;
-                at = lane < 32 ? at0 : at1;
-            } else {
-                const int p = __builtin_amdgcn_readlane(safe[t >> 2], 16 * (t & 3));
-                at = ((((long long)p * a.shape.kv_heads + w.head) << a.shape.page_shift) + ((base + 16 * t) & page_mask)) * a.shape.row_bytes;
-            }
+            const long long at = DP == 64 ? (lane < 32 ? line_of(safe, base, 2 * t) : line_of(safe, base, 2 * t + 1)) : line_of(safe, base, t);
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) {
-                keys[h][t] = *(const i32x4 *)(a.codes[0] + at + inside[h]);
-                values[h][t] = *(const i32x4 *)(a.codes[1] + at + inside[h]);
-            }
+            for (int h = 0; h < kHalves; ++h) keys[h][t] = *(const i32x4 *)(a.codes[0] + at + inside[h]);
+        }
+    };
+    // values of a tile whose pages `safe` has, from memory to LDS: lane i of a load fills bytes 16 i of a kilobyte
+    auto load_values = [&](int k, const int *safe) {
+        const int base = tile_at(k);
+#pragma unroll
+        for (int t = 0; t < kValueLoads; ++t) {
+            const uint8_t *from;
+            if (DP == 64) from = a.codes[1] + (lane < 32 ? line_of(safe, base, 2 * t) : line_of(safe, base, 2 * t + 1)) + value_inside[0];
+            else if (DP == 128) from = a.codes[1] + line_of(safe, base, t) + value_inside[0];
+            else from = a.codes[1] + line_of(safe, base, t >> 1) + value_inside[t & 1];
+            __builtin_amdgcn_global_load_lds((const QT_GLOBAL void *)from, (QT_LDS void *)(s_values + 1024 * t), 16, 0, 0);
         }
     };
 
@@ -271,41 +306,22 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     for (int d = 0; d < kDTiles; ++d) result[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float best = -__builtin_inff(), sum = 0.0f;
     int page[2];
-    int k = tile_from + wave;
-    if (k < tile_to) {
-        load_pages(k, page);
-        load_tile(k, page);
-        if (k + 4 < tile_to) load_pages(k + 4, page);
-    }
-    for (; k < tile_to; k += 4) {
+    // one tile; `more`: the wave has another one, which is asked for on the way (without a branch: waits count loads)
+    auto step = [&](int k, auto more) {
         const int base = tile_at(k);
         const unsigned long long here[2] = {valid[0], valid[1]};
-        // values and scales to LDS; what no page holds has scale 0
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h)
-#pragma unroll
-            for (int t = 0; t < kLoads; ++t) {
-                const int token = DP == 64 ? 32 * t + (lane >> 5) * 16 + column : 16 * t + column;
-                const int chunk = DP == 64 ? g & 1 : g + 4 * h;
-                uint8_t *to = s_values + token * kStride + 16 * chunk;
-                *(i32x2 *)to = (i32x2){values[h][t][0], values[h][t][1]};
-                *(i32x2 *)(to + 8) = (i32x2){values[h][t][2], values[h][t][3]};
-            }
+        // what no page holds has scale 0; a weight of zero times a scale that is not finite is not zero: only then such weights are looked for
+        float by_key[UNITS][2], by_value[UNITS][2], odd_scale = 0.0f;
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const bool there = (here[i] >> lane) & 1;
-                s_key_scale[u * kTile + 64 * i + lane] = there ? key_scale[u][i] * a.factor : 0.0f;
-                s_value_scale[u * kTile + 64 * i + lane] = there ? value_scale[u][i] : 0.0f;
+                by_key[u][i] = there ? key_scale[u][i] * a.factor : 0.0f;
+                by_value[u][i] = there ? value_scale[u][i] : 0.0f;
+                odd_scale += 0.0f * by_value[u][i];
             }
-        // (a weight of zero times a scale that is not finite is not zero: only then such weights are looked for)
-        float odd_scale = 0.0f;
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) odd_scale += 0.0f * value_scale[u][0] + 0.0f * value_scale[u][1];
         const bool odd = __ballot(odd_scale != 0.0f) != 0;
-        wave_lds_sync();
-        __builtin_amdgcn_sched_barrier(0);
 
         // scores
         f32x4 score[8];
@@ -322,7 +338,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
                         c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(keys[h][DP == 64 ? t >> 1 : t]), as_operand(query[h][i]), c, kFp4, kFp6,
                                                                              0, kOne, 0, by);
                     }
-                score[t] = c * *(const f32x4 *)(s_key_scale + 16 * t + 4 * g);
+                score[t] = times_row(c, by_key[0][t >> 2], t & 3);
             } else {
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
@@ -333,22 +349,15 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
                         c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(keys[u >> 1][t]), as_operand(query[u >> 1][i]), c, kFp4, kFp6, 0, kOne,
                                                                              0, by);
                     }
-                    c *= *(const f32x4 *)(s_key_scale + u * kTile + 16 * t + 4 * g);
+                    c = times_row(c, by_key[u][t >> 2], t & 3);
                     score[t] = u == 0 ? c : score[t] + c;
                 }
             }
-            if (t & 1) __builtin_amdgcn_sched_barrier(0);
         }
-        // (done here, so that the keys' registers are free for the next tile)
 #pragma unroll
-        for (int t = 0; t < 8; ++t) asm volatile("" : "+v"(score[t]));
+        for (int t = 0; t < 8; ++t) asm volatile("" : "+v"(score[t]));      // (done here: the keys' registers are free)
         __builtin_amdgcn_sched_barrier(0);
-        if (k + 4 < tile_to) {
-            load_tile(k + 4, page);
-            if (k + 8 < tile_to) load_pages(k + 8, page);
-        }
 
-        __builtin_amdgcn_sched_barrier(0);
         // which of the lane's tokens its query sees: bit 4 t + i of `see` (tokens past the end are past every position)
         const bool whole = !(~here[0] | ~here[1]);
         const bool full = base + kTile - 1 <= lowest && (!a.window || highest - base < a.window || base + kTile <= a.sinks) && whole;
@@ -357,8 +366,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
             see = tokens_up_to(position - base - 4 * g);
             if (a.window) see &= ~tokens_up_to(behind - base - 4 * g) | tokens_up_to(a.sinks - 1 - base - 4 * g);
             if (!whole) {
-#pragma unroll
-                for (int t = 0; t < 8; ++t) see &= ~(15u << (4 * t)) | (((uint32_t)(here[t >> 2] >> (16 * (t & 3) + 4 * g)) & 15u) << (4 * t));
+                see &= ((uint32_t)(here[0] >> (16 * g)) & 0xffffu) | ((uint32_t)(here[1] >> (16 * g)) << 16);
             }
 #pragma unroll
             for (int t = 0; t < 8; ++t)
@@ -395,10 +403,10 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
             uint32_t most = 0;
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                const f32x4 by = *(const f32x4 *)(s_value_scale + u * kTile + 16 * t + 4 * g);
+                const f32x4 scaled = times_row(weight[t], by_value[u][t >> 2], t & 3);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float x = weight[t][i] * by[i];
+                    const float x = scaled[i];
                     most = max(most, __float_as_uint(x));
                     if (t < 4) early[4 * t + i] = x;
                     else late[4 * (t - 4) + i] = x;
@@ -418,26 +426,48 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
             int by[kPieces];
             split_fp6<kPieces>(early, late, most, piece, by);
             __builtin_amdgcn_sched_barrier(0);
+            constexpr int kMine = kDTiles / UNITS;
+            i32x4 rows_of_v[kMine];
 #pragma unroll
-            for (int d = 0; d < kDTiles / UNITS; ++d) {
-                const int dt = u * (kDTiles / UNITS) + d;
-                i32x4 rows_of_v;
+            for (int d = 0; d < kMine; ++d)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     // position 16 h + j of the weights is register (16 h + j) / 2 of the first or (odd) the second sixteen
-                    const int n = 8 * h + (column >> 1), token = 16 * (n >> 2) + 4 * g + (n & 3) + 64 * (column & 1);
-                    const i32x2 part = __builtin_amdgcn_ds_read_tr4_b64_v2i32((QT_LDS i32x2 *)(s_values + token * kStride + 8 * dt));
-                    rows_of_v[2 * h] = part[0], rows_of_v[2 * h + 1] = part[1];
+                    const int dt = u * kMine + d, n = 8 * h + (column >> 1), token = 16 * (n >> 2) + 4 * g + (n & 3) + 64 * (column & 1);
+                    const i32x2 part = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+                        (QT_LDS i32x2 *)(s_values + token * kRowBytes + 16 * ((dt >> 1) ^ swap_of<DP>(token)) + 8 * (dt & 1)));
+                    rows_of_v[d][2 * h] = part[0], rows_of_v[d][2 * h + 1] = part[1];
                 }
-#pragma unroll
-                for (int i = kPieces - 1; i >= 0; --i)
-                    result[dt] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(rows_of_v), as_operand(piece[i]), result[dt], kFp4, kFp6, 0, kOne, 0,
-                                                                                  by[i]);
-                if (d & 1) __builtin_amdgcn_sched_barrier(0);
+            if constexpr (decltype(more)::value) {
+                if (u == UNITS - 1) {
+                    // the next tile, as soon as nothing of this one is read any more: keys into registers that were free while the
+                    // weights were split, values to LDS, where the reads above have to be through
+                    __builtin_amdgcn_sched_barrier(0);
+                    __builtin_amdgcn_s_waitcnt(kWaitLds);
+                    wave_lds_sync();
+                    load_tile(k + 4, page);
+                    load_values(k + 4, safe);
+                    load_pages(min(k + 8, tile_to - 1), page);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
             }
+#pragma unroll
+            for (int i = kPieces - 1; i >= 0; --i)
+#pragma unroll
+                for (int d = 0; d < kMine; ++d)
+                    result[u * kMine + d] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(rows_of_v[d]), as_operand(piece[i]), result[u * kMine + d],
+                                                                                             kFp4, kFp6, 0, kOne, 0, by[i]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        wave_lds_sync();
+    };
+    int k = tile_from + wave;
+    if (k < tile_to) {
+        load_pages(k, page);
+        load_tile(k, page);
+        load_values(k, safe);
+        load_pages(min(k + 4, tile_to - 1), page);
+        for (; k + 4 < tile_to; k += 4) step(k, std::true_type());
+        step(k, std::false_type());
     }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
