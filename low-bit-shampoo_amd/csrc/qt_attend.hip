@@ -20,86 +20,74 @@ struct Work {
     int per_piece;                                   // tiles of one piece
 };
 
-__device__ __forceinline__ unsigned long long wave_scan(unsigned long long x) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const unsigned long long y = __shfl_up(x, off, 64);
-        if (lane >= off) x += y;
-    }
-    return x;
+// Sum over the lanes up to this one (64 lanes), additions inside rows of sixteen and of their last lanes without LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
 }
-
-// Sum over the workgroup (total) and inclusive sum up to this thread, of 256 threads.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long x, unsigned long long &total, unsigned long long *s) {
-    x = wave_scan(x);
-    const int wave = threadIdx.x >> 6;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) s[wave] = x;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        if (w < wave) x += s[w];
-        total += s[w];
-    }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += dpp_or_zero<0x111, 0xf>(x);        // row_shr 1, 2, 4, 8
+    x += dpp_or_zero<0x112, 0xf>(x);
+    x += dpp_or_zero<0x114, 0xf>(x);
+    x += dpp_or_zero<0x118, 0xf>(x);
+    x += dpp_or_zero<0x142, 0xa>(x);        // row_bcast 15: into rows 1 and 3
+    x += dpp_or_zero<0x143, 0xc>(x);        // row_bcast 31: into rows 2 and 3
     return x;
 }
 
 __device__ __forceinline__ int row_tiles(const AttendArgs &a, const SequenceView &v) { return (v.count * a.group + kRows - 1) / kRows; }
 
 // How a call is cut: a row of tiles (a sequence, a head of the cache, sixteen queries) into pieces of about as many tiles as all the work
-// has per slot.  Finds the `index`th piece (BY_PIECE) or the first piece of the `index`th row of tiles; false beyond the last.
+// has per slot (of up to one and a half times as many: half a piece is not worth a join).  Finds the `index`th piece (BY_PIECE) or the
+// first piece of the `index`th row of tiles; false beyond the last.  Every wave works it out for itself, a sequence per lane.
+//
+// Pieces behind the first of a row are at most tiles / most, so there are no more than slots of them, and rows that are cut have at most 4/3 slots
+// pieces in all; `most` may round below the exact quotient by a few 2^-24 (a sum in fp32), and a row whose partial results would lie
+// behind the workspace's 2 slots places is refused below, whatever the lengths say.
 template <bool BY_PIECE>
-__device__ __forceinline__ bool find_work(const AttendArgs &a, unsigned index, Work &w) {
-    __shared__ unsigned long long s_sums[4];
-    __shared__ Work s_work;
-    __shared__ int s_found;
-    unsigned long long all = 0;
-    for (int first = 0; first < a.at.batch; first += 256) {
-        const int b = first + (int)threadIdx.x;
-        unsigned long long mine = 0, total;
+__device__ __forceinline__ bool find_work(const AttendArgs &a, uint32_t index, Work &w) {
+    const int lane = threadIdx.x & 63;
+    float all = 0.0f;
+    for (int first = 0; first < a.at.batch; first += 64) {
+        const int b = first + lane;
         if (b < a.at.batch) {
             const SequenceView v = view_sequence(a, b);
-            mine = (unsigned long long)row_tiles(a, v) * a.shape.kv_heads * v.tiles;
+            all += (float)(row_tiles(a, v) * a.shape.kv_heads) * (float)v.tiles;
         }
-        block_scan(mine, total, s_sums);
-        all += total;
     }
-    const int most = (int)max((unsigned long long)kLeastTiles, (all + a.slots - 1) / a.slots);
-    if (threadIdx.x == 0) s_found = 0;
-    unsigned long long before = 0;          // pieces or rows of tiles (high half) and partial results (low half) of the sequences before
-    for (int first = 0; first < a.at.batch; first += 256) {
-        const int b = first + (int)threadIdx.x;
-        unsigned long long mine = 0, total;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
+    const int most = max(kLeastTiles, (int)min(ceilf(all / (float)a.slots), 1.0e9f));
+    uint32_t before = 0, partial = 0;           // pieces or rows of tiles, and partial results, of the sequences before
+    for (int first = 0; first < a.at.batch; first += 64) {
+        const int b = first + lane;
         int items = 0, pieces = 1, tiles = 0;
         if (b < a.at.batch) {
             const SequenceView v = view_sequence(a, b);
             items = row_tiles(a, v) * a.shape.kv_heads;
             tiles = v.tiles;
-            pieces = max(1, (tiles + most / 2) / most);       // (of up to one and a half times as many tiles: half a piece is not worth a join)
-            mine = ((unsigned long long)(unsigned)(BY_PIECE ? items * pieces : items) << 32) + (unsigned)(pieces > 1 ? items * pieces : 0);
+            pieces = max(1, (tiles + most / 2) / most);
         }
-        const unsigned long long upto = before + block_scan(mine, total, s_sums), from = upto - mine;
-        if (index >= (unsigned)(from >> 32) && index < (unsigned)(upto >> 32)) {
-            const int local = (int)(index - (unsigned)(from >> 32)), item = BY_PIECE ? local / pieces : local;
-            Work found;
-            found.b = b;
-            found.head = item % a.shape.kv_heads;
-            found.row_tile = item / a.shape.kv_heads;
-            found.piece = BY_PIECE ? local - item * pieces : 0;
-            found.pieces = pieces;
-            found.slot = (int)(unsigned)from + item * pieces;
-            found.per_piece = (tiles + pieces - 1) / pieces;
-            s_work = found;
-            s_found = 1;
+        const uint32_t mine = (uint32_t)(BY_PIECE ? items * pieces : items), parts = pieces > 1 ? (uint32_t)(items * pieces) : 0u;
+        const uint32_t upto = before + wave_scan(mine), parts_upto = partial + wave_scan(parts);
+        const unsigned long long at = __ballot(index < upto);
+        if (at) {
+            const int found = __builtin_ctzll(at);
+            const uint32_t from = __builtin_amdgcn_readlane(upto - mine, found);
+            w.b = first + found;
+            w.pieces = __builtin_amdgcn_readlane(pieces, found);
+            const int total_tiles = __builtin_amdgcn_readlane(tiles, found), local = (int)(index - from), item = BY_PIECE ? local / w.pieces : local;
+            w.row_tile = item / a.shape.kv_heads;
+            w.head = item - w.row_tile * a.shape.kv_heads;
+            w.piece = BY_PIECE ? local - item * w.pieces : 0;
+            w.slot = (int)__builtin_amdgcn_readlane(parts_upto - parts, found) + item * w.pieces;
+            w.per_piece = (total_tiles + w.pieces - 1) / w.pieces;
+            return w.pieces == 1 || (w.slot >= 0 && w.slot + w.pieces <= 2 * a.slots);
         }
-        before += total;
-        if (index < (unsigned)(before >> 32)) break;
+        before = __builtin_amdgcn_readlane(upto, 63);
+        partial = __builtin_amdgcn_readlane(parts_upto, 63);
     }
-    __syncthreads();
-    w = s_work;
-    return s_found != 0;
+    return false;
 }
 
 // Of the tokens 16 t + i of a lane (t < 8, i < 4; bit 4 t + i), those up to x.
@@ -122,41 +110,42 @@ __device__ __forceinline__ f32x4 times_row(f32x4 x, float by, int t) {
     }
 }
 
-// 32 consecutive elements of a query from element d on, zeros behind its end.
+// 32 consecutive elements of a query from element d on, zeros behind its end: as they lie in memory, and as fp32 numbers of even and odd place.
 template <bool BF16>
-__device__ __forceinline__ void load_query(const AttendArgs &a, long long at, int d, bool there, f32x16 &even, f32x16 &odd) {
+__device__ __forceinline__ void load_query(const AttendArgs &a, long long at, int d, bool there, uint4 *raw) {
     const int valid = there ? a.shape.head_dim - d : 0;
-    if (BF16) {
-        const uint16_t *p = (const uint16_t *)a.q + at + d;
-        if (valid >= 32 && is_aligned16(p)) {
+    constexpr int kWords = BF16 ? 4 : 8;
+    const uint8_t *p = (const uint8_t *)a.q + (at + d) * (BF16 ? 2 : 4);
+    if (valid >= 32 && is_aligned16(p)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint4 w = ((const uint4 *)p)[i];
-                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) even[4 * i + e] = __uint_as_float(v[e] << 16), odd[4 * i + e] = __uint_as_float(v[e] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                even[i] = 2 * i < valid ? bf16_bits_to_float(p[2 * i]) : 0.0f;
-                odd[i] = 2 * i + 1 < valid ? bf16_bits_to_float(p[2 * i + 1]) : 0.0f;
-            }
-        }
+        for (int i = 0; i < kWords; ++i) raw[i] = ((const uint4 *)p)[i];
     } else {
-        const float *p = (const float *)a.q + at + d;
-        if (valid >= 32 && is_aligned16(p)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 w = ((const float4 *)p)[i];
-                even[2 * i] = w.x, odd[2 * i] = w.y, even[2 * i + 1] = w.z, odd[2 * i + 1] = w.w;
+        for (int i = 0; i < kWords; ++i) {
+            uint32_t word[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = 4 * i + e;
+                if (BF16)
+                    word[e] = (2 * n < valid ? ((const uint16_t *)p)[2 * n] : 0u) | ((2 * n + 1 < valid ? ((const uint16_t *)p)[2 * n + 1] : 0u) << 16);
+                else
+                    word[e] = n < valid ? ((const uint32_t *)p)[n] : 0u;
             }
+            raw[i] = make_uint4(word[0], word[1], word[2], word[3]);
+        }
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack_query(const uint4 *raw, f32x16 &even, f32x16 &odd) {
+#pragma unroll
+    for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+        const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        if (BF16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) even[4 * i + e] = __uint_as_float(word[e] << 16), odd[4 * i + e] = __uint_as_float(word[e] & 0xffff0000u);
         } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                even[i] = 2 * i < valid ? p[2 * i] : 0.0f;
-                odd[i] = 2 * i + 1 < valid ? p[2 * i + 1] : 0.0f;
-            }
+            even[2 * i] = __uint_as_float(word[0]), odd[2 * i] = __uint_as_float(word[1]);
+            even[2 * i + 1] = __uint_as_float(word[2]), odd[2 * i + 1] = __uint_as_float(word[3]);
         }
     }
 }
@@ -202,33 +191,16 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     Work w;
     if (!find_work<true>(a, blockIdx.x, w)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
-    w.b = __builtin_amdgcn_readfirstlane(w.b);
-    w.head = __builtin_amdgcn_readfirstlane(w.head);
-    w.row_tile = __builtin_amdgcn_readfirstlane(w.row_tile);
-    w.piece = __builtin_amdgcn_readfirstlane(w.piece);
-    w.per_piece = __builtin_amdgcn_readfirstlane(w.per_piece);
     const SequenceView v = view_sequence(a, w.b);
     const int rows = min(kRows, v.count * a.group - w.row_tile * kRows);
     const int first_row = w.row_tile * kRows;
     uint8_t *s_values = s_area[wave];
 
-    // the queries of this lane's column, in pieces
+    // the query of this lane's column
     const int my_row = first_row + min(column, rows - 1);
     const int my_token = v.start + my_row / a.group, my_head = w.head * a.group + my_row % a.group;
     const int position = v.first_position + my_row / a.group;
     const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;       // last token behind the window
-    u32x6 query[kHalves][kPieces];
-    int query_scale[kHalves][kPieces];
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-        f32x16 even, odd;
-        const int chunk = DP == 64 ? g & 1 : g + 4 * h;
-        load_query<BF16>(a, my_token * a.q_token + my_head * a.q_head, 32 * chunk, column < rows, even, odd);
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = max(top, max(__float_as_uint(even[i]) & 0x7fffffffu, __float_as_uint(odd[i]) & 0x7fffffffu));
-        split_fp6<kPieces>(even, odd, top, query[h], query_scale[h]);
-    }
     const int lowest = v.first_position + first_row / a.group, highest = v.first_position + (first_row + rows - 1) / a.group;
 
     const int tile_from = w.piece * w.per_piece, tile_to = min(tile_from + w.per_piece, v.tiles);
@@ -305,6 +277,8 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
 #pragma unroll
     for (int d = 0; d < kDTiles; ++d) result[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float best = -__builtin_inff(), sum = 0.0f;
+    u32x6 query[kHalves][kPieces];
+    int query_scale[kHalves][kPieces];
     int page[2];
     // one tile; `more`: the wave has another one, which is asked for on the way (without a branch: waits count loads)
     auto step = [&](int k, auto more) {
@@ -460,12 +434,26 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // pages, queries and the first tile are asked for before any of them is waited for
     int k = tile_from + wave;
+    uint4 raw[kHalves][BF16 ? 4 : 8];
+    if (k < tile_to) load_pages(k, page);
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h)
+        load_query<BF16>(a, my_token * a.q_token + my_head * a.q_head, 32 * (DP == 64 ? g & 1 : g + 4 * h), column < rows, raw[h]);
     if (k < tile_to) {
-        load_pages(k, page);
         load_tile(k, page);
         load_values(k, safe);
         load_pages(min(k + 4, tile_to - 1), page);
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+            f32x16 even, odd;
+            unpack_query<BF16>(raw[h], even, odd);
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max(top, max(__float_as_uint(even[i]) & 0x7fffffffu, __float_as_uint(odd[i]) & 0x7fffffffu));
+            split_fp6<kPieces>(even, odd, top, query[h], query_scale[h]);
+        }
         for (; k + 4 < tile_to; k += 4) step(k, std::true_type());
         step(k, std::false_type());
     }
