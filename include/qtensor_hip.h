@@ -510,9 +510,9 @@ void qtensor_hip_cache_read(const qtensor_cache *cache, const qtensor_cache_plac
  * sequence up to itself; with window > 0 only the last `window` of them (itself included) and the first `sinks` of the sequence.
  * heads is a multiple of kv_heads, query head h reads head h / (heads / kv_heads).  A token that sees nothing gets zeros.
  * workspace: scratch for long sequences, whose pieces are joined at the end; 16-byte aligned, as many bytes as
- * qtensor_hip_cache_attend_workspace says (for a cache of this shape on the current device); may be null where the table holds
- * no more than 1024 tokens of a sequence. */
-long long qtensor_hip_cache_attend_workspace(const qtensor_cache *cache);
+ * qtensor_hip_cache_attend_workspace says (for a cache of this shape, queries of this type, with or without starts, on the
+ * current device: it does not depend on the call's tokens). */
+long long qtensor_hip_cache_attend_workspace(const qtensor_cache *cache, int heads, int is_bf16, int has_starts);
 void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *q,
                               const qtensor_cache_vectors *out, int heads, float scale, int window, int sinks, void *workspace,
                               long long workspace_bytes, qtensor_stream_t stream);

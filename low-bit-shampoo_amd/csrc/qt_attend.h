@@ -17,9 +17,22 @@ struct AttendArgs {
     int heads, group;
     float factor;           // scale * log2 e
     int window, sinks;      // window 0: no window
-    int slots;              // workgroups that a call is cut for
-    float *partial;         // 2 * slots pieces of (16 rows x (DP + 2)) floats
+    int few_rows;           // sequences with up to so many queries (times heads that share one of the cache) go to the kernel for few, others to
+                            // the one for many
+    int slots;              // workgroups that the kernel's work is cut for
+    int least;              // tiles below which a piece is not worth having
+    float *partial;         // attend_places(slots) pieces of (rows x (DP + 2)) floats
 };
+
+// Pieces of rows of tiles that were cut, at most (see find_work).
+constexpr int attend_places(int slots) { return slots + slots / 2; }
+
+constexpr int attend_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+constexpr int kRowsOfMany = 128;    // queries that a workgroup of the kernel for many takes
+int attend_many_slots(int dim);
+// Launches the kernel for sequences of many queries (and what joins its pieces): `rows_of_tiles` at most.
+void launch_attend_many(AttendArgs a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream);
 
 #if defined(__HIPCC__)
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -77,13 +90,25 @@ __device__ __forceinline__ i32x8 as_operand(const u32x6 &p) {
 __device__ __forceinline__ i32x8 as_operand(const i32x4 &p) { return (i32x8){p[0], p[1], p[2], p[3], 0, 0, 0, 0}; }
 
 // The tokens that the new ones of a sequence see: all of it up to them, or with a window its first `sinks` and the window of the
-// first of them, in tiles of 128: `sink_tiles` from token 0, then those from `first_tile` on.
+// first of them, in tiles of 2^SHIFT: `sink_tiles` from token 0, then those from `first_tile` on.
 struct SequenceView {
     int start, count;                   // its rows of the call
     int first_position, end;            // position of the first; tokens of the sequence that its table can hold
     int sink_tiles, first_tile, tiles;
 };
 
+// Tiles of what queries from `first` on see of the tokens before `end`.
+template <int SHIFT>
+__device__ __forceinline__ void view_tokens(const AttendArgs &a, SequenceView &v, int first, int end) {
+    constexpr int kRound = (1 << SHIFT) - 1;
+    int low = 0;
+    if (a.window) low = min(end, max(0, max(first, 0) - (a.window - 1)));
+    v.first_tile = low >> SHIFT;
+    v.sink_tiles = min((int)(((long long)min(a.sinks, low) + kRound) >> SHIFT), v.first_tile);
+    v.tiles = v.sink_tiles + ((end + kRound) >> SHIFT) - v.first_tile;
+}
+
+template <int SHIFT>
 __device__ __forceinline__ SequenceView view_sequence(const AttendArgs &a, int b) {
     SequenceView v;
     const int length = a.at.lengths[b];
@@ -93,13 +118,213 @@ __device__ __forceinline__ SequenceView view_sequence(const AttendArgs &a, int b
     v.first_position = length - v.count;
     const long long covered = (long long)a.at.table_pages << a.shape.page_shift;
     v.end = (int)min((long long)max(length, 0), min(covered, 0x7fffff00LL));
-    int low = 0;
-    if (a.window) low = min(v.end, max(0, max(v.first_position, 0) - (a.window - 1)));
-    v.first_tile = low >> 7;
-    v.sink_tiles = min((int)(((long long)min(a.sinks, low) + 127) >> 7), v.first_tile);
-    v.tiles = v.sink_tiles + ((v.end + 127) >> 7) - v.first_tile;
+    view_tokens<SHIFT>(a, v, v.first_position, v.end);
     return v;
 }
+struct AttendWork {
+    int b, head, row_tile, piece, pieces, slot;      // slot: first partial result of this row of tiles
+    int per_piece;                                   // tiles of one piece
+};
+
+// Sum over the lanes up to this one (64 lanes), additions inside rows of sixteen and of their last lanes without LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += dpp_or_zero<0x111, 0xf>(x);        // row_shr 1, 2, 4, 8
+    x += dpp_or_zero<0x112, 0xf>(x);
+    x += dpp_or_zero<0x114, 0xf>(x);
+    x += dpp_or_zero<0x118, 0xf>(x);
+    x += dpp_or_zero<0x142, 0xa>(x);        // row_bcast 15: into rows 1 and 3
+    x += dpp_or_zero<0x143, 0xc>(x);        // row_bcast 31: into rows 2 and 3
+    return x;
+}
+
+// Rows of tiles of a sequence's queries; none if the sequence is the other kernel's.
+template <int ROWS>
+__device__ __forceinline__ int row_tiles(const AttendArgs &a, const SequenceView &v) {
+    const int rows = v.count * a.group;
+    return (rows > a.few_rows) == (ROWS == kRowsOfMany) ? (rows + ROWS - 1) / ROWS : 0;
+}
+
+// First row of a row of tiles: of many, the last ones first, as they see most.
+template <int ROWS>
+__device__ __forceinline__ int first_row_of(int rows, int row_tile) {
+    return (ROWS == kRowsOfMany ? (rows + ROWS - 1) / ROWS - 1 - row_tile : row_tile) * ROWS;
+}
+
+// How a kernel's work is cut: a row of tiles (a sequence, a head of the cache, ROWS queries) into pieces of about as many tiles as all the work
+// has per slot (of up to one and a half times as many: half a piece is not worth a join).  Finds the `index`th piece (BY_PIECE) or the
+// first piece of the `index`th row of tiles; false beyond the last.  Every wave works it out for itself, a sequence per lane.
+//
+// Pieces behind the first of a row are at most tiles / most, so there are no more than slots of them, and rows that are cut have at most 4/3 slots
+// pieces in all; `most` may round below the exact quotient by a few 2^-24 (a sum in fp32), and a row whose partial results would lie
+// behind the workspace's places (slots and a half) is refused below, whatever the lengths say.
+template <int ROWS, int SHIFT, bool BY_PIECE>
+__device__ __forceinline__ bool find_work(const AttendArgs &a, uint32_t index, AttendWork &w) {
+    const int lane = threadIdx.x & 63;
+    float all = 0.0f;
+    for (int first = 0; first < a.at.batch; first += 64) {
+        const int b = first + lane;
+        if (b < a.at.batch) {
+            const SequenceView v = view_sequence<SHIFT>(a, b);
+            all += (float)(row_tiles<ROWS>(a, v) * a.shape.kv_heads) * (float)v.tiles;
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
+    const int most = max(a.least, (int)min(ceilf(all / (float)a.slots), 1.0e9f));
+    uint32_t before = 0, partial = 0;           // pieces or rows of tiles, and partial results, of the sequences before
+    for (int first = 0; first < a.at.batch; first += 64) {
+        const int b = first + lane;
+        int items = 0, pieces = 1, tiles = 0;
+        if (b < a.at.batch) {
+            const SequenceView v = view_sequence<SHIFT>(a, b);
+            items = row_tiles<ROWS>(a, v) * a.shape.kv_heads;
+            tiles = v.tiles;
+            pieces = max(1, (tiles + most / 2) / most);
+        }
+        const uint32_t mine = (uint32_t)(BY_PIECE ? items * pieces : items), parts = pieces > 1 ? (uint32_t)(items * pieces) : 0u;
+        const uint32_t upto = before + wave_scan(mine), parts_upto = partial + wave_scan(parts);
+        const unsigned long long at = __ballot(index < upto);
+        if (at) {
+            const int found = __builtin_ctzll(at);
+            const uint32_t from = __builtin_amdgcn_readlane(upto - mine, found);
+            w.b = first + found;
+            w.pieces = __builtin_amdgcn_readlane(pieces, found);
+            const int total_tiles = __builtin_amdgcn_readlane(tiles, found), local = (int)(index - from), item = BY_PIECE ? local / w.pieces : local;
+            w.row_tile = item / a.shape.kv_heads;
+            w.head = item - w.row_tile * a.shape.kv_heads;
+            w.piece = BY_PIECE ? local - item * w.pieces : 0;
+            w.slot = (int)__builtin_amdgcn_readlane(parts_upto - parts, found) + item * w.pieces;
+            w.per_piece = (total_tiles + w.pieces - 1) / w.pieces;
+            return w.pieces == 1 || (w.slot >= 0 && w.slot + w.pieces <= attend_places(a.slots));
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+        partial = __builtin_amdgcn_readlane(parts_upto, 63);
+    }
+    return false;
+}
+
+// What lane LANE of the lane's row of sixteen holds: an operand of the instruction that takes it.
+template <int LANE>
+__device__ __forceinline__ float of_row(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x150 + LANE, 0xf, 0xf, false));
+}
+// 32 consecutive elements of a query from element d on, zeros behind its end: as they lie in memory, and as fp32 numbers of even and odd place.
+template <bool BF16>
+__device__ __forceinline__ void load_query(const AttendArgs &a, long long at, int d, bool there, uint4 *raw) {
+    const int valid = there ? a.shape.head_dim - d : 0;
+    constexpr int kWords = BF16 ? 4 : 8;
+    const uint8_t *p = (const uint8_t *)a.q + (at + d) * (BF16 ? 2 : 4);
+    if (valid >= 32 && is_aligned16(p)) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) raw[i] = ((const uint4 *)p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            uint32_t word[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = 4 * i + e;
+                if (BF16)
+                    word[e] = (2 * n < valid ? ((const uint16_t *)p)[2 * n] : 0u) | ((2 * n + 1 < valid ? ((const uint16_t *)p)[2 * n + 1] : 0u) << 16);
+                else
+                    word[e] = n < valid ? ((const uint32_t *)p)[n] : 0u;
+            }
+            raw[i] = make_uint4(word[0], word[1], word[2], word[3]);
+        }
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack_query(const uint4 *raw, f32x16 &even, f32x16 &odd) {
+#pragma unroll
+    for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
+        const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        if (BF16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) even[4 * i + e] = __uint_as_float(word[e] << 16), odd[4 * i + e] = __uint_as_float(word[e] & 0xffff0000u);
+        } else {
+            even[2 * i] = __uint_as_float(word[0]), odd[2 * i] = __uint_as_float(word[1]);
+            even[2 * i + 1] = __uint_as_float(word[2]), odd[2 * i + 1] = __uint_as_float(word[3]);
+        }
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ void store_result(const AttendArgs &a, long long at, float y) {
+    if (BF16) ((uint16_t *)a.out)[at] = float_to_bf16_bits(y);
+    else ((float *)a.out)[at] = y;
+}
+
+// Order of the 16-byte chunks of row `row` of a tile's codes in LDS: chunk c stands at c ^ swap.  Sixteen rows' chunks of one place fall on all
+// banks then, and of the 64 rows that a transposed read takes eight bytes each from, four share a bank, as few as 512 bytes can.
+template <int DP>
+__device__ __forceinline__ int swap_of(int row) {
+    return DP == 64 ? (row >> 3) & 1 : DP == 128 ? (row >> 2) & 3 : (row >> 1) & 7;
+}
+
+// Joins the pieces of every row of tiles that was cut, a workgroup for each of its rows: what the pieces count for first, then a
+// share of them per group of DP / 4 threads.
+template <int ROWS, int SHIFT, int DP, bool BF16>
+__global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
+    constexpr int kGroups = 1024 / DP;
+    __shared__ float s_share[256];
+    __shared__ float s_reduce[4], s_total[4];
+    __shared__ f32x4 s_part[256];
+    AttendWork w;
+    if (!find_work<ROWS, SHIFT, false>(a, blockIdx.x, w) || w.pieces == 1) return;
+    const SequenceView v = view_sequence<SHIFT>(a, w.b);
+    const int rows = v.count * a.group, row = first_row_of<ROWS>(rows, w.row_tile) + blockIdx.y;
+    if (row >= rows) return;
+    constexpr int kNext = ROWS * (DP + 2);
+    const float *part = a.partial + (long long)w.slot * kNext + blockIdx.y * (DP + 2);
+    const int wave = threadIdx.x >> 6;
+    float top = -__builtin_inff();
+    for (int i = threadIdx.x; i < w.pieces; i += 256) top = fmaxf(top, part[(long long)i * kNext]);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    if ((threadIdx.x & 63) == 0) s_reduce[wave] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_reduce[0], s_reduce[1]), fmaxf(s_reduce[2], s_reduce[3]));
+    const float zero = top == -__builtin_inff() ? 0.0f : top;
+    const int group = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
+    float total = 0.0f;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+    for (int first = 0; first < w.pieces; first += 256) {
+        const int i = first + (int)threadIdx.x, count = min(256, w.pieces - first);
+        __syncthreads();
+        float share = 0.0f;
+        if (i < w.pieces) {
+            share = __builtin_amdgcn_exp2f(part[(long long)i * kNext] - zero);
+            total += part[(long long)i * kNext + 1] * share;
+        }
+        s_share[threadIdx.x] = share;
+        __syncthreads();
+#pragma unroll 4
+        for (int j = group; j < count; j += kGroups) {
+            const float2 *p = (const float2 *)(part + (long long)(first + j) * kNext + 2 + d);
+            const float2 u = p[0], v2 = p[1];
+            const float by = s_share[j];
+            y += (f32x4){u.x * by, u.y * by, v2.x * by, v2.y * by};
+        }
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    if ((threadIdx.x & 63) == 0) s_total[wave] = total;
+    s_part[threadIdx.x] = y;
+    __syncthreads();
+    total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
+    if (group != 0) return;
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) y += s_part[threadIdx.x + i * (DP / 4)];
+    const long long at = (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (d + e < a.shape.head_dim) store_result<BF16>(a, at + d + e, total == 0.0f ? 0.0f : y[e] / total);
+}
+
 #endif  // __HIPCC__
 
 }  // namespace qt

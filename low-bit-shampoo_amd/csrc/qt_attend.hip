@@ -13,82 +13,10 @@ namespace {
 
 constexpr int kTile = 128;              // tokens a wave takes at a time: one step of k of a matrix instruction with the weights
 constexpr int kRows = 16;               // queries (of all heads that share a head of the cache) in a tile of rows
-constexpr int kLeastTiles = 8;          // tiles below which a row of tiles is not cut: two for each wave
-
-struct Work {
-    int b, head, row_tile, piece, pieces, slot;      // slot: first partial result of this row of tiles
-    int per_piece;                                   // tiles of one piece
-};
-
-// Sum over the lanes up to this one (64 lanes), additions inside rows of sixteen and of their last lanes without LDS.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_or_zero(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-    x += dpp_or_zero<0x111, 0xf>(x);        // row_shr 1, 2, 4, 8
-    x += dpp_or_zero<0x112, 0xf>(x);
-    x += dpp_or_zero<0x114, 0xf>(x);
-    x += dpp_or_zero<0x118, 0xf>(x);
-    x += dpp_or_zero<0x142, 0xa>(x);        // row_bcast 15: into rows 1 and 3
-    x += dpp_or_zero<0x143, 0xc>(x);        // row_bcast 31: into rows 2 and 3
-    return x;
-}
-
-__device__ __forceinline__ int row_tiles(const AttendArgs &a, const SequenceView &v) { return (v.count * a.group + kRows - 1) / kRows; }
-
-// How a call is cut: a row of tiles (a sequence, a head of the cache, sixteen queries) into pieces of about as many tiles as all the work
-// has per slot (of up to one and a half times as many: half a piece is not worth a join).  Finds the `index`th piece (BY_PIECE) or the
-// first piece of the `index`th row of tiles; false beyond the last.  Every wave works it out for itself, a sequence per lane.
-//
-// Pieces behind the first of a row are at most tiles / most, so there are no more than slots of them, and rows that are cut have at most 4/3 slots
-// pieces in all; `most` may round below the exact quotient by a few 2^-24 (a sum in fp32), and a row whose partial results would lie
-// behind the workspace's 2 slots places is refused below, whatever the lengths say.
-template <bool BY_PIECE>
-__device__ __forceinline__ bool find_work(const AttendArgs &a, uint32_t index, Work &w) {
-    const int lane = threadIdx.x & 63;
-    float all = 0.0f;
-    for (int first = 0; first < a.at.batch; first += 64) {
-        const int b = first + lane;
-        if (b < a.at.batch) {
-            const SequenceView v = view_sequence(a, b);
-            all += (float)(row_tiles(a, v) * a.shape.kv_heads) * (float)v.tiles;
-        }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
-    const int most = max(kLeastTiles, (int)min(ceilf(all / (float)a.slots), 1.0e9f));
-    uint32_t before = 0, partial = 0;           // pieces or rows of tiles, and partial results, of the sequences before
-    for (int first = 0; first < a.at.batch; first += 64) {
-        const int b = first + lane;
-        int items = 0, pieces = 1, tiles = 0;
-        if (b < a.at.batch) {
-            const SequenceView v = view_sequence(a, b);
-            items = row_tiles(a, v) * a.shape.kv_heads;
-            tiles = v.tiles;
-            pieces = max(1, (tiles + most / 2) / most);
-        }
-        const uint32_t mine = (uint32_t)(BY_PIECE ? items * pieces : items), parts = pieces > 1 ? (uint32_t)(items * pieces) : 0u;
-        const uint32_t upto = before + wave_scan(mine), parts_upto = partial + wave_scan(parts);
-        const unsigned long long at = __ballot(index < upto);
-        if (at) {
-            const int found = __builtin_ctzll(at);
-            const uint32_t from = __builtin_amdgcn_readlane(upto - mine, found);
-            w.b = first + found;
-            w.pieces = __builtin_amdgcn_readlane(pieces, found);
-            const int total_tiles = __builtin_amdgcn_readlane(tiles, found), local = (int)(index - from), item = BY_PIECE ? local / w.pieces : local;
-            w.row_tile = item / a.shape.kv_heads;
-            w.head = item - w.row_tile * a.shape.kv_heads;
-            w.piece = BY_PIECE ? local - item * w.pieces : 0;
-            w.slot = (int)__builtin_amdgcn_readlane(parts_upto - parts, found) + item * w.pieces;
-            w.per_piece = (total_tiles + w.pieces - 1) / w.pieces;
-            return w.pieces == 1 || (w.slot >= 0 && w.slot + w.pieces <= 2 * a.slots);
-        }
-        before = __builtin_amdgcn_readlane(upto, 63);
-        partial = __builtin_amdgcn_readlane(parts_upto, 63);
-    }
-    return false;
-}
+constexpr int kFewRows = 32;            // queries of a sequence that are still few: two rows of tiles
+constexpr int kLeastTiles = 4;          // tiles of a piece: one for each wave
+constexpr int kWholeTiles = 12;         // a call whose sequences have no more tiles than that is not cut: three rounds of the waves take less
+                                        // time than two and a launch that joins pieces
 
 // Of the tokens 16 t + i of a lane (t < 8, i < 4; bit 4 t + i), those up to x.
 __device__ __forceinline__ uint32_t tokens_up_to(int x) {
@@ -97,10 +25,6 @@ __device__ __forceinline__ uint32_t tokens_up_to(int x) {
 }
 
 // x times what lanes 4 t ... 4 t + 3 of the lane's row of sixteen hold.
-template <int LANE>
-__device__ __forceinline__ float of_row(float x) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x150 + LANE, 0xf, 0xf, false));
-}
 __device__ __forceinline__ f32x4 times_row(f32x4 x, float by, int t) {
     switch (t) {
     case 0: return (f32x4){x[0] * of_row<0>(by), x[1] * of_row<1>(by), x[2] * of_row<2>(by), x[3] * of_row<3>(by)};
@@ -110,62 +34,9 @@ __device__ __forceinline__ f32x4 times_row(f32x4 x, float by, int t) {
     }
 }
 
-// 32 consecutive elements of a query from element d on, zeros behind its end: as they lie in memory, and as fp32 numbers of even and odd place.
-template <bool BF16>
-__device__ __forceinline__ void load_query(const AttendArgs &a, long long at, int d, bool there, uint4 *raw) {
-    const int valid = there ? a.shape.head_dim - d : 0;
-    constexpr int kWords = BF16 ? 4 : 8;
-    const uint8_t *p = (const uint8_t *)a.q + (at + d) * (BF16 ? 2 : 4);
-    if (valid >= 32 && is_aligned16(p)) {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) raw[i] = ((const uint4 *)p)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            uint32_t word[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = 4 * i + e;
-                if (BF16)
-                    word[e] = (2 * n < valid ? ((const uint16_t *)p)[2 * n] : 0u) | ((2 * n + 1 < valid ? ((const uint16_t *)p)[2 * n + 1] : 0u) << 16);
-                else
-                    word[e] = n < valid ? ((const uint32_t *)p)[n] : 0u;
-            }
-            raw[i] = make_uint4(word[0], word[1], word[2], word[3]);
-        }
-    }
-}
-template <bool BF16>
-__device__ __forceinline__ void unpack_query(const uint4 *raw, f32x16 &even, f32x16 &odd) {
-#pragma unroll
-    for (int i = 0; i < (BF16 ? 4 : 8); ++i) {
-        const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        if (BF16) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) even[4 * i + e] = __uint_as_float(word[e] << 16), odd[4 * i + e] = __uint_as_float(word[e] & 0xffff0000u);
-        } else {
-            even[2 * i] = __uint_as_float(word[0]), odd[2 * i] = __uint_as_float(word[1]);
-            even[2 * i + 1] = __uint_as_float(word[2]), odd[2 * i + 1] = __uint_as_float(word[3]);
-        }
-    }
-}
-
-template <bool BF16>
-__device__ __forceinline__ void store_result(const AttendArgs &a, long long at, float y) {
-    if (BF16) ((uint16_t *)a.out)[at] = float_to_bf16_bits(y);
-    else ((float *)a.out)[at] = y;
-}
-
 constexpr int kWaitLds = 0xc07f;        // s_waitcnt lgkmcnt(0), nothing else
 
-constexpr int few_waves(int dim, int units, bool bf16) { return dim == 64 || (dim == 128 && units == 1 && bf16) ? 2 : 1; }
-
-// Order of the 16-byte chunks of row `row` of values in LDS: chunk c stands at c ^ swap.  Of the 64 rows that a transposed read takes eight
-// bytes each from, four share a bank then, as few as 512 bytes can.
-template <int DP>
-__device__ __forceinline__ int swap_of(int row) {
-    return DP == 64 ? (row >> 3) & 1 : DP == 128 ? (row >> 2) & 3 : (row >> 1) & 7;
-}
+constexpr int few_waves(int dim, int units, bool bf16) { return dim == 256 || (units > 1 && !bf16) ? 1 : 2; }
 
 // Few queries per sequence: generation.  A workgroup takes one piece of a row of tiles, its four waves every fourth tile of it.
 //
@@ -188,12 +59,12 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     __shared__ __attribute__((aligned(16))) uint8_t s_area[4][kArea];
     __shared__ float s_best[4][kRows], s_sum[4][kRows];
 
-    Work w;
-    if (!find_work<true>(a, blockIdx.x, w)) return;
+    AttendWork w;
+    if (!find_work<kRows, 7, true>(a, blockIdx.x, w)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
-    const SequenceView v = view_sequence(a, w.b);
+    const SequenceView v = view_sequence<7>(a, w.b);
     const int rows = min(kRows, v.count * a.group - w.row_tile * kRows);
-    const int first_row = w.row_tile * kRows;
+    const int first_row = first_row_of<kRows>(0, w.row_tile);
     uint8_t *s_values = s_area[wave];
 
     // the query of this lane's column
@@ -203,7 +74,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;       // last token behind the window
     const int lowest = v.first_position + first_row / a.group, highest = v.first_position + (first_row + rows - 1) / a.group;
 
-    const int tile_from = w.piece * w.per_piece, tile_to = min(tile_from + w.per_piece, v.tiles);
+    const int tile_from = min(w.piece * w.per_piece, v.tiles), tile_to = min(tile_from + w.per_piece, v.tiles);
     const int *table = a.at.table + (long long)w.b * a.at.table_stride;
     const int page_mask = (1 << a.shape.page_shift) - 1, chunks = a.shape.row_bytes >> 4;
 
@@ -491,87 +362,34 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     }
 }
 
-// Joins the pieces of every row of tiles that was cut, a workgroup for each of its rows: what the pieces count for first, then a
-// share of them per group of DP / 4 threads.
-template <int DP, bool BF16>
-__global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
-    constexpr int kGroups = 1024 / DP;
-    __shared__ float s_share[256];
-    __shared__ float s_reduce[4], s_total[4];
-    __shared__ f32x4 s_part[256];
-    Work w;
-    if (!find_work<false>(a, blockIdx.x, w) || w.pieces == 1) return;
-    const SequenceView v = view_sequence(a, w.b);
-    const int row = w.row_tile * kRows + blockIdx.y;
-    if (row >= v.count * a.group) return;
-    constexpr int kNext = kRows * (DP + 2);
-    const float *part = a.partial + (long long)w.slot * kNext + blockIdx.y * (DP + 2);
-    const int wave = threadIdx.x >> 6;
-    float top = -__builtin_inff();
-    for (int i = threadIdx.x; i < w.pieces; i += 256) top = fmaxf(top, part[(long long)i * kNext]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    if ((threadIdx.x & 63) == 0) s_reduce[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_reduce[0], s_reduce[1]), fmaxf(s_reduce[2], s_reduce[3]));
-    const float zero = top == -__builtin_inff() ? 0.0f : top;
-    const int group = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
-    float total = 0.0f;
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first < w.pieces; first += 256) {
-        const int i = first + (int)threadIdx.x, count = min(256, w.pieces - first);
-        __syncthreads();
-        float share = 0.0f;
-        if (i < w.pieces) {
-            share = __builtin_amdgcn_exp2f(part[(long long)i * kNext] - zero);
-            total += part[(long long)i * kNext + 1] * share;
-        }
-        s_share[threadIdx.x] = share;
-        __syncthreads();
-#pragma unroll 4
-        for (int j = group; j < count; j += kGroups) {
-            const float2 *p = (const float2 *)(part + (long long)(first + j) * kNext + 2 + d);
-            const float2 u = p[0], v2 = p[1];
-            const float by = s_share[j];
-            y += (f32x4){u.x * by, u.y * by, v2.x * by, v2.y * by};
-        }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-    if ((threadIdx.x & 63) == 0) s_total[wave] = total;
-    s_part[threadIdx.x] = y;
-    __syncthreads();
-    total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
-    if (group != 0) return;
-#pragma unroll
-    for (int i = 1; i < kGroups; ++i) y += s_part[threadIdx.x + i * (DP / 4)];
-    const long long at = (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (d + e < a.shape.head_dim) store_result<BF16>(a, at + d + e, total == 0.0f ? 0.0f : y[e] / total);
-}
-
-int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
-int slots_of(int dim) { return compute_units() * (dim == 256 ? 1 : 2); }
+// Workgroups that the device holds of the kernel for few.
+int few_slots(int dim, int segments, bool bf16) { return compute_units() * few_waves(dim, dim == 64 || segments == 1 ? 1 : dim / 64, bf16); }
 
 template <int DP, bool BF16>
-void launch_attend(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream) {
+void launch_few(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream) {
     const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u));
     if (DP == 64 || a.shape.segments == 1) hipLaunchKernelGGL((attend_few_kernel<DP, 1, BF16>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((attend_few_kernel<DP, DP / 64, BF16>), grid, dim3(256), 0, stream, a);
-    if (may_cut) hipLaunchKernelGGL((attend_join_kernel<DP, BF16>), dim3(rows_of_tiles, a.at.starts ? kRows : min(kRows, a.group)), dim3(256), 0, stream, a);
+    if (may_cut)
+        hipLaunchKernelGGL((attend_join_kernel<kRows, 7, DP, BF16>), dim3(rows_of_tiles, a.at.starts ? kRows : min(kRows, a.group)), dim3(256), 0, stream, a);
+}
+
+long long workspace_of(const CacheShape &shape, int group, bool bf16, bool ragged) {
+    const int dim = attend_dim(shape.head_dim);
+    const long long few = (long long)attend_places(few_slots(dim, shape.segments, bf16)) * kRows;
+    const long long many = bf16 && (ragged || group > kFewRows) ? (long long)attend_places(attend_many_slots(dim)) * kRowsOfMany : 0;
+    return (few > many ? few : many) * (dim + 2) * (long long)sizeof(float);
 }
 
 }  // namespace
 }  // namespace qt
 
-extern "C" long long qtensor_hip_cache_attend_workspace(const qtensor_cache *cache) {
+extern "C" long long qtensor_hip_cache_attend_workspace(const qtensor_cache *cache, int heads, int is_bf16, int has_starts) {
     using namespace qt;
     clear_error();
     CacheShape shape;
     if (!cache_shape("cache_attend_workspace", cache, shape)) return 0;
-    const int dim = padded_dim(shape.head_dim);
-    return 2LL * slots_of(dim) * kRows * (dim + 2) * (long long)sizeof(float);
+    return workspace_of(shape, heads / shape.kv_heads, is_bf16 != 0, has_starts != 0);
 }
 
 extern "C" void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *q,
@@ -598,23 +416,45 @@ extern "C" void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtens
     a.heads = heads, a.group = heads / a.shape.kv_heads;
     a.factor = scale * 1.4426950408889634f;
     a.window = window, a.sinks = sinks;
-    const int dim = padded_dim(a.shape.head_dim);
-    a.slots = slots_of(dim);
     a.partial = (float *)workspace;
-    // rows of tiles: at most one more per sequence than full ones
-    const long long rows = (long long)a.at.tokens * a.group;
-    const long long rows_of_tiles = a.shape.kv_heads * (a.at.starts ? rows / kRows + a.at.batch : a.at.batch * (long long)((a.group + kRows - 1) / kRows));
-    if (rows >= (1LL << 31) || rows_of_tiles >= (1LL << 30)) { set_error(kBadArgument, "cache_attend: %d tokens are too many for one call", a.at.tokens); return; }
-    const bool may_cut = ((long long)a.at.table_pages << a.shape.page_shift) > kLeastTiles * kTile;
-    if (may_cut && (!workspace || !is_aligned(workspace, 16) || workspace_bytes < 2LL * a.slots * kRows * (dim + 2) * (long long)sizeof(float))) {
+    const bool bf16 = q->is_bf16 != 0, ragged = a.at.starts != nullptr;
+    const int dim = attend_dim(a.shape.head_dim);
+    // queries in 32 bits are all the kernel for few's: it has pieces enough for them
+    a.few_rows = bf16 ? kFewRows : 0x7fffffff;
+    const long long rows = (long long)a.at.tokens * a.group, batch = a.at.batch;
+    if (rows >= (1LL << 31) || (rows / kRows + batch) * a.shape.kv_heads >= (1LL << 30)) {
+        set_error(kBadArgument, "cache_attend: %d tokens are too many for one call", a.at.tokens);
+        return;
+    }
+    if (!workspace || !is_aligned(workspace, 16) || workspace_bytes < workspace_of(a.shape, a.group, bf16, ragged)) {
         set_error(kBadArgument, "cache_attend: the workspace is smaller than qtensor_hip_cache_attend_workspace says");
         return;
     }
     const hipStream_t stream = (hipStream_t)stream_v;
-    const unsigned n = (unsigned)rows_of_tiles;
-    auto launch = dim == 64 ? (q->is_bf16 ? launch_attend<64, true> : launch_attend<64, false>)
-                : dim == 128 ? (q->is_bf16 ? launch_attend<128, true> : launch_attend<128, false>)
-                             : (q->is_bf16 ? launch_attend<256, true> : launch_attend<256, false>);
-    launch(a, n, may_cut, stream);
+    const long long held = (long long)a.at.table_pages << a.shape.page_shift;        // most tokens of a sequence
+    if (bf16 && (ragged ? rows : (long long)a.group) > kFewRows) {
+        const long long rows_of_tiles = a.shape.kv_heads * (ragged ? rows / kRowsOfMany + batch : batch * ((a.group + kRowsOfMany - 1) / kRowsOfMany));
+        AttendArgs many = a;
+        many.slots = attend_many_slots(dim);
+        launch_attend_many(many, (unsigned)rows_of_tiles, held > 1024 && rows_of_tiles < 4LL * many.slots, stream);
+    }
+    if (!bf16 || ragged || a.group <= kFewRows) {
+        // rows of tiles: at most one more per sequence than full ones, and no more per sequence than few queries have
+        long long rows_of_tiles = ragged ? rows / kRows + batch : batch * ((a.group + kRows - 1) / kRows);
+        if (bf16) rows_of_tiles = rows_of_tiles < batch * (kFewRows / kRows) ? rows_of_tiles : batch * (kFewRows / kRows);
+        long long tiles = (held + kTile - 1) / kTile;
+        if (window) {
+            const long long seen = ((long long)window + (ragged ? kFewRows : 1) + kTile - 2) / kTile + 1 + ((long long)sinks + kTile - 1) / kTile;
+            if ((bf16 || !ragged) && seen < tiles) tiles = seen;
+        }
+        const bool may_cut = tiles > kWholeTiles;
+        a.slots = few_slots(dim, a.shape.segments, bf16);
+        a.least = may_cut ? kLeastTiles : 1 << 28;
+        const unsigned n = (unsigned)(rows_of_tiles * a.shape.kv_heads);
+        auto launch = dim == 64 ? (bf16 ? launch_few<64, true> : launch_few<64, false>)
+                    : dim == 128 ? (bf16 ? launch_few<128, true> : launch_few<128, false>)
+                                 : (bf16 ? launch_few<256, true> : launch_few<256, false>);
+        launch(a, n, may_cut, stream);
+    }
     launch_ok("cache_attend");
 }

@@ -50,7 +50,7 @@ if F.lib is not None:
     F.lib.qtensor_hip_cache_attend.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.POINTER(_Vectors), ct.POINTER(_Vectors), ct.c_int,
                                                ct.c_float, ct.c_int, ct.c_int, ct.c_void_p, ct.c_longlong, ct.c_void_p]
     F.lib.qtensor_hip_cache_attend_workspace.restype = ct.c_longlong
-    F.lib.qtensor_hip_cache_attend_workspace.argtypes = [ct.POINTER(_Cache)]
+    F.lib.qtensor_hip_cache_attend_workspace.argtypes = [ct.POINTER(_Cache), ct.c_int, ct.c_int, ct.c_int]
 
 
 class QTensorCache:
@@ -144,7 +144,7 @@ class QTensorCache:
         places = self._places(table, lengths, starts, tokens)
         # scratch for the pieces of long sequences: taken for the call, as that of the products is
         with torch.cuda.device(q.device):
-            size = F.lib.qtensor_hip_cache_attend_workspace(self._ref())
+            size = F.lib.qtensor_hip_cache_attend_workspace(self._ref(), heads, q.dtype == torch.bfloat16, starts is not None)
         scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
         F._call(F.lib.qtensor_hip_cache_attend, q.device, self._ref(), places, _vectors(q), _vectors(out), heads, scale,
                 window or 0, sinks, scratch.data_ptr(), size)
