@@ -54,7 +54,7 @@ struct CacheCopy {
     uint8_t *codes[2];
     float *scales[2];
     int lanes, segment_lanes;       // lanes of eight elements per vector and per segment
-    uint32_t items;                 // lanes of all vectors of keys (of values as many)
+    uint32_t items;                 // lanes of all vectors of keys, which take those of the values too
     FastDiv by_lanes, by_heads;
 };
 
@@ -69,31 +69,39 @@ __device__ __forceinline__ int token_position(const CachePlaces &at, int token, 
     return at.lengths[b] - (at.starts[b + 1] - token);
 }
 
+// Eight elements as they lie in memory (16 bytes of bf16, 32 of fp32), zeros behind the end of a vector.
 template <bool BF16>
-__device__ __forceinline__ void load_eight(const void *base, long long at, int valid, float *x) {
-    if (BF16) {
-        const uint16_t *p = (const uint16_t *)base + at;
-        if (valid >= 8 && is_aligned16(p)) {
-            const uint4 w = *(const uint4 *)p;
-            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void load_eight(const void *base, long long at, int valid, uint4 *raw) {
+    constexpr int kWords = BF16 ? 1 : 2;
+    const uint8_t *p = (const uint8_t *)base + at * (BF16 ? 2 : 4);
+    if (valid >= 8 && is_aligned16(p)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[2 * i] = __uint_as_float(v[i] << 16);
-                x[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = i < valid ? bf16_bits_to_float(p[i]) : 0.0f;
-        }
+        for (int i = 0; i < kWords; ++i) raw[i] = load_u32x4<true>(p + 16 * i);
     } else {
-        const float *p = (const float *)base + at;
-        if (valid >= 8 && is_aligned16(p)) {
-            const float4 u = *(const float4 *)p, v = *(const float4 *)(p + 4);
-            x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-            x[4] = v.x; x[5] = v.y; x[6] = v.z; x[7] = v.w;
-        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = i < valid ? p[i] : 0.0f;
+        for (int i = 0; i < kWords; ++i) {
+            uint32_t word[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = 4 * i + e;
+                if (BF16)
+                    word[e] = (2 * n < valid ? ((const uint16_t *)p)[2 * n] : 0u) | ((2 * n + 1 < valid ? ((const uint16_t *)p)[2 * n + 1] : 0u) << 16);
+                else
+                    word[e] = n < valid ? ((const uint32_t *)p)[n] : 0u;
+            }
+            raw[i] = make_uint4(word[0], word[1], word[2], word[3]);
+        }
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ void unpack_eight(const uint4 *raw, float *x) {
+#pragma unroll
+    for (int i = 0; i < (BF16 ? 1 : 2); ++i) {
+        const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (BF16) x[2 * e] = __uint_as_float(word[e] << 16), x[2 * e + 1] = __uint_as_float(word[e] & 0xffff0000u);
+            else x[4 * i + e] = __uint_as_float(word[e]);
         }
     }
 }
@@ -123,73 +131,135 @@ __device__ __forceinline__ void store_eight(void *base, long long at, int valid,
     }
 }
 
+// What a lane works on: eight elements of the keys and the values of one head of one token.
+struct CacheItem {
+    int valid;          // elements of the vector from here on; 0: nothing
+    uint32_t lane, token, head;
+};
+__device__ __forceinline__ CacheItem cache_item(const CacheCopy &a, uint32_t item) {
+    CacheItem it;
+    const bool there = item < a.items;
+    const uint32_t vector = fastdiv(there ? item : 0, a.by_lanes);
+    it.lane = (there ? item : 0) - vector * a.lanes;
+    it.token = fastdiv(vector, a.by_heads);
+    it.head = vector - it.token * a.shape.kv_heads;
+    it.valid = there ? max(0, a.shape.head_dim - (int)it.lane * 8) : 0;
+    return it;
+}
+
 // A lane takes eight elements of a vector; a segment is 8, 16 or 32 lanes side by side.  Largest magnitude by integer maximum of
 // the magnitudes' bits (NaN above infinity, so that a segment with a NaN gets a NaN for its scale and reads as NaN),
-// scale and quotients by correctly rounded division, nearest number (ties to the even code, beyond 6 to 6) by the conversion
-// instruction.
-template <bool BF16>
+// scale and quotients by correctly rounded division (qt_divide.h; quotients below 2^-40, which it may round otherwise, are code 0),
+// nearest number (ties to the even code, beyond 6 to 6) by the conversion instruction.
+template <bool BF16, int ITEMS>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheCopy a) {
-    const uint32_t item = blockIdx.x * kCacheThreads + threadIdx.x;
-    const int which = blockIdx.y;
-    int b = 0;
-    const uint32_t first_vector = fastdiv(blockIdx.x * kCacheThreads, a.by_lanes);
-    if (a.at.starts) b = sequence_of_block(a.at, (int)fastdiv(first_vector, a.by_heads));
-    const bool there = item < a.items;
-    const uint32_t vector = fastdiv(there ? item : 0, a.by_lanes), lane = (there ? item : 0) - vector * a.lanes;
-    const uint32_t token = fastdiv(vector, a.by_heads), head = vector - token * a.shape.kv_heads;
-    const int position = there ? token_position(a.at, (int)token, b) : -1;
-    const long long row = position < 0 ? -1 : cache_row(a.shape, a.at, b, position, (int)head);
-    const int valid = row < 0 ? 0 : a.shape.head_dim - (int)lane * 8;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (valid > 0)
-        load_eight<BF16>(a.vectors.base[which], token * a.vectors.token_stride[which] + head * a.vectors.head_stride[which] + lane * 8, valid, x);
-    uint32_t top = 0;
+    const uint32_t first = blockIdx.x * (kCacheThreads * ITEMS);
+    CacheItem it[ITEMS];
+    uint4 raw[ITEMS][2][BF16 ? 1 : 2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    top = group_max_u32<8>(top);
-    if (a.segment_lanes >= 16) top = max(top, dpp_u32<0x140>(top));
-    if (a.segment_lanes >= 32) top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-    if (row < 0) return;
-    const float scale = __uint_as_float(top) / 6.0f;
-    const float by = scale == 0.0f ? 1.0f : scale;
-    uint32_t word = 0;
-    if (top != 0 && top < 0x7f800000u) {      // (zeroes times a scale that is not finite are NaN)
-        word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[0] / by, x[1] / by, 1.0f, 0);
-        word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[2] / by, x[3] / by, 1.0f, 1);
-        word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[4] / by, x[5] / by, 1.0f, 2);
-        word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, x[6] / by, x[7] / by, 1.0f, 3);
+    for (int n = 0; n < ITEMS; ++n) {
+        it[n] = cache_item(a, first + n * kCacheThreads + threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            load_eight<BF16>(a.vectors.base[i], it[n].token * a.vectors.token_stride[i] + it[n].head * a.vectors.head_stride[i] + it[n].lane * 8,
+                             it[n].valid, raw[n][i]);
     }
-    if ((int)lane * 4 < a.shape.row_bytes) *(uint32_t *)(a.codes[which] + row * a.shape.row_bytes + lane * 4) = word;
-    const int segment = (int)(lane * 8) >> a.shape.segment_shift;
-    if ((lane & (a.segment_lanes - 1)) == 0) a.scales[which][cache_scale_at(a.shape, row) + ((long long)segment << a.shape.page_shift)] = scale;
+    int b = 0;
+    if (a.at.starts) b = sequence_of_block(a.at, (int)fastdiv(fastdiv(first, a.by_lanes), a.by_heads));
+#pragma unroll
+    for (int n = 0; n < ITEMS; ++n) {
+        const int position = first + n * kCacheThreads + threadIdx.x < a.items ? token_position(a.at, (int)it[n].token, b) : -1;
+        const long long row = position < 0 ? -1 : cache_row(a.shape, a.at, b, position, (int)it[n].head);
+        const int segment = (int)(it[n].lane * 8) >> a.shape.segment_shift;
+        const long long scale_at = cache_scale_at(a.shape, row) + ((long long)segment << a.shape.page_shift);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float x[8];
+            unpack_eight<BF16>(raw[n][i], x);
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+            top = group_max_u32<8>(top);
+            if (a.segment_lanes >= 16) top = max(top, dpp_u32<0x140>(top));
+            if (a.segment_lanes >= 32) top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+            const float scale = __uint_as_float(top) / 6.0f;
+            float y[8];
+            const uint32_t bits = __float_as_uint(scale);
+            if (bits >= kFastDivLo && bits <= kFastDivHi) {
+                const float r = exact_reciprocal(scale);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = quotient(x[e], scale, r);
+            } else {
+                // (zeroes times a scale that is not finite are NaN)
+                const bool zero = bits == 0 || top >= 0x7f800000u;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = zero ? 0.0f : x[e] / scale;
+            }
+            uint32_t word = 0;
+            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[0], y[1], 1.0f, 0);
+            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[2], y[3], 1.0f, 1);
+            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[4], y[5], 1.0f, 2);
+            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[6], y[7], 1.0f, 3);
+            if (row >= 0 && (int)it[n].lane * 4 < a.shape.row_bytes) *(uint32_t *)(a.codes[i] + row * a.shape.row_bytes + it[n].lane * 4) = word;
+            if (row >= 0 && (it[n].lane & (a.segment_lanes - 1)) == 0) a.scales[i][scale_at] = scale;
+        }
+    }
 }
 
 // The reverse, eight elements a lane; tokens that the cache does not have come out as zeros.
-template <bool BF16>
+template <bool BF16, int ITEMS>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCopy a) {
-    const uint32_t item = blockIdx.x * kCacheThreads + threadIdx.x;
-    const int which = blockIdx.y;
+    const uint32_t first = blockIdx.x * (kCacheThreads * ITEMS);
     int b = 0;
-    const uint32_t first_vector = fastdiv(blockIdx.x * kCacheThreads, a.by_lanes);
-    if (a.at.starts) b = sequence_of_block(a.at, (int)fastdiv(first_vector, a.by_heads));
-    if (item >= a.items) return;
-    const uint32_t vector = fastdiv(item, a.by_lanes), lane = item - vector * a.lanes;
-    const uint32_t token = fastdiv(vector, a.by_heads), head = vector - token * a.shape.kv_heads;
-    const int position = token_position(a.at, (int)token, b);
-    const long long row = position < 0 ? -1 : cache_row(a.shape, a.at, b, position, (int)head);
-    const int valid = a.shape.head_dim - (int)lane * 8;
-    if (valid <= 0) return;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (row >= 0) {
-        const uint32_t word = *(const uint32_t *)(a.codes[which] + row * a.shape.row_bytes + lane * 4);
-        const int segment = (int)(lane * 8) >> a.shape.segment_shift;
-        const float scale = a.scales[which][cache_scale_at(a.shape, row) + ((long long)segment << a.shape.page_shift)];
-        const cache_f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 0), q = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 1),
-                          r = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 2), s = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word, 1.0f, 3);
-        x[0] = p.x * scale; x[1] = p.y * scale; x[2] = q.x * scale; x[3] = q.y * scale;
-        x[4] = r.x * scale; x[5] = r.y * scale; x[6] = s.x * scale; x[7] = s.y * scale;
+    if (a.at.starts) b = sequence_of_block(a.at, (int)fastdiv(fastdiv(first, a.by_lanes), a.by_heads));
+    CacheItem it[ITEMS];
+    bool there[ITEMS];
+    uint32_t word[ITEMS][2];
+    float scale[ITEMS][2];
+#pragma unroll
+    for (int n = 0; n < ITEMS; ++n) {
+        it[n] = cache_item(a, first + n * kCacheThreads + threadIdx.x);
+        const int position = it[n].valid > 0 ? token_position(a.at, (int)it[n].token, b) : -1;
+        const long long row = position < 0 ? -1 : cache_row(a.shape, a.at, b, position, (int)it[n].head);
+        there[n] = row >= 0;
+        const long long from = there[n] ? row : 0;       // (every cache has a row 0)
+        const int segment = (int)(it[n].lane * 8) >> a.shape.segment_shift;
+        const long long scale_at = cache_scale_at(a.shape, from) + ((long long)(there[n] ? segment : 0) << a.shape.page_shift);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            word[n][i] = *(const uint32_t *)(a.codes[i] + from * a.shape.row_bytes + (there[n] ? it[n].lane * 4 : 0));
+            scale[n][i] = a.scales[i][scale_at];
+        }
     }
-    store_eight<BF16>(a.vectors.base[which], token * a.vectors.token_stride[which] + head * a.vectors.head_stride[which] + lane * 8, valid, x);
+#pragma unroll
+    for (int n = 0; n < ITEMS; ++n) {
+        if (it[n].valid <= 0) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float x[8];
+#define QT_EACH(e)                                                                                             \
+    {                                                                                                          \
+        const cache_f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[n][i], 1.0f, e);                    \
+        x[2 * e] = there[n] ? p.x * scale[n][i] : 0.0f, x[2 * e + 1] = there[n] ? p.y * scale[n][i] : 0.0f;     \
+    }
+            QT_EACH(0) QT_EACH(1) QT_EACH(2) QT_EACH(3)
+#undef QT_EACH
+            store_eight<BF16>(a.vectors.base[i], it[n].token * a.vectors.token_stride[i] + it[n].head * a.vectors.head_stride[i] + it[n].lane * 8,
+                              it[n].valid, x);
+        }
+    }
+}
+
+template <bool BF16>
+void launch_copy(bool write, const CacheCopy &a, hipStream_t stream) {
+    // several items a thread where there are workgroups enough for every unit: their loads wait together
+    const bool large = a.items >= 1u << 21;
+    const int items = !large ? 1 : write ? 2 : 4;
+    const dim3 grid((a.items + kCacheThreads * items - 1) / (kCacheThreads * items));
+    if (write && large) hipLaunchKernelGGL((cache_write_kernel<BF16, 2>), grid, dim3(kCacheThreads), 0, stream, a);
+    else if (write) hipLaunchKernelGGL((cache_write_kernel<BF16, 1>), grid, dim3(kCacheThreads), 0, stream, a);
+    else if (large) hipLaunchKernelGGL((cache_read_kernel<BF16, 4>), grid, dim3(kCacheThreads), 0, stream, a);
+    else hipLaunchKernelGGL((cache_read_kernel<BF16, 1>), grid, dim3(kCacheThreads), 0, stream, a);
 }
 
 void copy_cache(const char *what, bool write, const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *keys,
@@ -221,10 +291,8 @@ void copy_cache(const char *what, bool write, const qtensor_cache *cache, const 
     a.items = (uint32_t)items;
     a.by_lanes = make_fastdiv((uint32_t)a.lanes);
     a.by_heads = make_fastdiv((uint32_t)a.shape.kv_heads);
-    const dim3 grid((a.items + kCacheThreads - 1) / kCacheThreads, 2);
-    auto kernel = write ? (keys->is_bf16 ? cache_write_kernel<true> : cache_write_kernel<false>)
-                        : (keys->is_bf16 ? cache_read_kernel<true> : cache_read_kernel<false>);
-    hipLaunchKernelGGL(kernel, grid, dim3(kCacheThreads), 0, stream, a);
+    if (keys->is_bf16) launch_copy<true>(write, a, stream);
+    else launch_copy<false>(write, a, stream);
     launch_ok(what);
 }
 
