@@ -54,8 +54,8 @@ struct CacheCopy {
     uint8_t *codes[2];
     float *scales[2];
     int lanes, segment_lanes;       // lanes of eight elements per vector and per segment
-    uint32_t items;                 // lanes of all vectors of keys, which take those of the values too
-    FastDiv by_lanes, by_heads;
+    int block_tokens;               // tokens of a workgroup
+    FastDiv by_lanes;
 };
 
 // Sequence of `token` and its position there; -1 for a token that is of no sequence.
@@ -106,13 +106,15 @@ __device__ __forceinline__ void unpack_eight(const uint4 *raw, float *x) {
     }
 }
 
-template <bool BF16>
+template <bool BF16, bool STREAM>
 __device__ __forceinline__ void store_eight(void *base, long long at, int valid, const float *x) {
     if (BF16) {
         uint16_t *p = (uint16_t *)base + at;
         if (valid >= 8 && is_aligned16(p)) {
-            *(uint4 *)p = make_uint4(floats_to_bf16_pair(x[0], x[1]), floats_to_bf16_pair(x[2], x[3]), floats_to_bf16_pair(x[4], x[5]),
-                                     floats_to_bf16_pair(x[6], x[7]));
+            const qt_u32x4 y = {floats_to_bf16_pair(x[0], x[1]), floats_to_bf16_pair(x[2], x[3]), floats_to_bf16_pair(x[4], x[5]),
+                                floats_to_bf16_pair(x[6], x[7])};
+            if (STREAM) __builtin_nontemporal_store(y, (qt_u32x4 *)p);
+            else *(qt_u32x4 *)p = y;
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -121,8 +123,8 @@ __device__ __forceinline__ void store_eight(void *base, long long at, int valid,
     } else {
         float *p = (float *)base + at;
         if (valid >= 8 && is_aligned16(p)) {
-            *(float4 *)p = make_float4(x[0], x[1], x[2], x[3]);
-            *(float4 *)(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            store_f32x4<STREAM>(p, make_float4(x[0], x[1], x[2], x[3]));
+            store_f32x4<STREAM>(p + 4, make_float4(x[4], x[5], x[6], x[7]));
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -131,47 +133,59 @@ __device__ __forceinline__ void store_eight(void *base, long long at, int valid,
     }
 }
 
-// What a lane works on: eight elements of the keys and the values of one head of one token.
-struct CacheItem {
-    int valid;          // elements of the vector from here on; 0: nothing
-    uint32_t lane, token, head;
+// A thread's place: eight elements from `lane` * 8 on of the vectors of one token, whose heads it goes through.  A workgroup takes some
+// sixteen tokens of a few heads: codes and scales of a head's consecutive tokens lie side by side, and where the token
+// lies is looked up once for all of them.
+struct CacheThread {
+    int valid;                  // elements of a vector from here on; 0: nothing
+    int lane, token;
+    long long line, inside;     // first row of head 0 of the token's page, and the token's row among that; line < 0: it has no page
 };
-__device__ __forceinline__ CacheItem cache_item(const CacheCopy &a, uint32_t item) {
-    CacheItem it;
-    const bool there = item < a.items;
-    const uint32_t vector = fastdiv(there ? item : 0, a.by_lanes);
-    it.lane = (there ? item : 0) - vector * a.lanes;
-    it.token = fastdiv(vector, a.by_heads);
-    it.head = vector - it.token * a.shape.kv_heads;
-    it.valid = there ? max(0, a.shape.head_dim - (int)it.lane * 8) : 0;
-    return it;
+__device__ __forceinline__ CacheThread cache_thread(const CacheCopy &a) {
+    CacheThread t;
+    const int nth = (int)fastdiv(threadIdx.x, a.by_lanes);
+    t.lane = (int)threadIdx.x - nth * a.lanes;
+    t.token = (int)blockIdx.x * a.block_tokens + nth;
+    const bool there = nth < a.block_tokens && t.token < a.at.tokens;
+    t.valid = there ? max(0, a.shape.head_dim - t.lane * 8) : 0;
+    t.token = there ? t.token : 0;
+    return t;
+}
+__device__ __forceinline__ void cache_look_up(const CacheCopy &a, CacheThread &t) {
+    int b = 0;
+    if (a.at.starts) b = sequence_of_block(a.at, (int)blockIdx.x * a.block_tokens);
+    t.line = -1, t.inside = 0;
+    const int position = t.valid > 0 ? token_position(a.at, t.token, b) : -1;
+    const int nth = position >> a.shape.page_shift;
+    if (position < 0 || nth >= a.at.table_pages) return;
+    const int page = a.at.table[b * a.at.table_stride + nth];
+    if ((unsigned)page >= (unsigned)a.shape.pages) return;
+    t.line = ((long long)page * a.shape.kv_heads) << a.shape.page_shift;
+    t.inside = position & ((1 << a.shape.page_shift) - 1);
 }
 
 // A lane takes eight elements of a vector; a segment is 8, 16 or 32 lanes side by side.  Largest magnitude by integer maximum of
 // the magnitudes' bits (NaN above infinity, so that a segment with a NaN gets a NaN for its scale and reads as NaN),
 // scale and quotients by correctly rounded division (qt_divide.h; quotients below 2^-40, which it may round otherwise, are code 0),
 // nearest number (ties to the even code, beyond 6 to 6) by the conversion instruction.
-template <bool BF16, int ITEMS>
+template <bool BF16, int HEADS>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheCopy a) {
-    const uint32_t first = blockIdx.x * (kCacheThreads * ITEMS);
-    CacheItem it[ITEMS];
-    uint4 raw[ITEMS][2][BF16 ? 1 : 2];
+    CacheThread t = cache_thread(a);
+    const int first_head = blockIdx.y * HEADS;
+    uint4 raw[HEADS][2][BF16 ? 1 : 2];
 #pragma unroll
-    for (int n = 0; n < ITEMS; ++n) {
-        it[n] = cache_item(a, first + n * kCacheThreads + threadIdx.x);
+    for (int n = 0; n < HEADS; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            load_eight<BF16>(a.vectors.base[i], it[n].token * a.vectors.token_stride[i] + it[n].head * a.vectors.head_stride[i] + it[n].lane * 8,
-                             it[n].valid, raw[n][i]);
-    }
-    int b = 0;
-    if (a.at.starts) b = sequence_of_block(a.at, (int)fastdiv(fastdiv(first, a.by_lanes), a.by_heads));
+            load_eight<BF16>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.lane * 8,
+                             first_head + n < a.shape.kv_heads ? t.valid : 0, raw[n][i]);
+    cache_look_up(a, t);
+    const int segment = (t.lane * 8) >> a.shape.segment_shift;
 #pragma unroll
-    for (int n = 0; n < ITEMS; ++n) {
-        const int position = first + n * kCacheThreads + threadIdx.x < a.items ? token_position(a.at, (int)it[n].token, b) : -1;
-        const long long row = position < 0 ? -1 : cache_row(a.shape, a.at, b, position, (int)it[n].head);
-        const int segment = (int)(it[n].lane * 8) >> a.shape.segment_shift;
-        const long long scale_at = cache_scale_at(a.shape, row) + ((long long)segment << a.shape.page_shift);
+    for (int n = 0; n < HEADS; ++n) {
+        const bool there = t.line >= 0 && first_head + n < a.shape.kv_heads;
+        const long long line = t.line + ((long long)(first_head + n) << a.shape.page_shift);
+        const long long scale_at = line * a.shape.segments + ((long long)segment << a.shape.page_shift) + t.inside;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float x[8];
@@ -200,66 +214,65 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheC
             word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[2], y[3], 1.0f, 1);
             word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[4], y[5], 1.0f, 2);
             word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[6], y[7], 1.0f, 3);
-            if (row >= 0 && (int)it[n].lane * 4 < a.shape.row_bytes) *(uint32_t *)(a.codes[i] + row * a.shape.row_bytes + it[n].lane * 4) = word;
-            if (row >= 0 && (it[n].lane & (a.segment_lanes - 1)) == 0) a.scales[i][scale_at] = scale;
+            if (there && t.lane * 4 < a.shape.row_bytes) *(uint32_t *)(a.codes[i] + (line + t.inside) * a.shape.row_bytes + t.lane * 4) = word;
+            if (there && (t.lane & (a.segment_lanes - 1)) == 0) a.scales[i][scale_at] = scale;
         }
     }
 }
 
-// The reverse, eight elements a lane; tokens that the cache does not have come out as zeros.
-template <bool BF16, int ITEMS>
+// The reverse, eight elements a lane; tokens that the cache does not have come out as zeros.  STREAM: the result is more than the caches
+// hold and goes past them.
+template <bool BF16, int HEADS, bool STREAM>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCopy a) {
-    const uint32_t first = blockIdx.x * (kCacheThreads * ITEMS);
-    int b = 0;
-    if (a.at.starts) b = sequence_of_block(a.at, (int)fastdiv(fastdiv(first, a.by_lanes), a.by_heads));
-    CacheItem it[ITEMS];
-    bool there[ITEMS];
-    uint32_t word[ITEMS][2];
-    float scale[ITEMS][2];
+    CacheThread t = cache_thread(a);
+    const int first_head = blockIdx.y * HEADS;
+    cache_look_up(a, t);
+    const bool there = t.line >= 0;
+    const int segment = there ? (t.lane * 8) >> a.shape.segment_shift : 0;
+    uint32_t word[HEADS][2];
+    float scale[HEADS][2];
 #pragma unroll
-    for (int n = 0; n < ITEMS; ++n) {
-        it[n] = cache_item(a, first + n * kCacheThreads + threadIdx.x);
-        const int position = it[n].valid > 0 ? token_position(a.at, (int)it[n].token, b) : -1;
-        const long long row = position < 0 ? -1 : cache_row(a.shape, a.at, b, position, (int)it[n].head);
-        there[n] = row >= 0;
-        const long long from = there[n] ? row : 0;       // (every cache has a row 0)
-        const int segment = (int)(it[n].lane * 8) >> a.shape.segment_shift;
-        const long long scale_at = cache_scale_at(a.shape, from) + ((long long)(there[n] ? segment : 0) << a.shape.page_shift);
+    for (int n = 0; n < HEADS; ++n) {
+        // (what is not there is read from row 0, which every cache has)
+        const long long line = there ? t.line + ((long long)min(first_head + n, a.shape.kv_heads - 1) << a.shape.page_shift) : 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            word[n][i] = *(const uint32_t *)(a.codes[i] + from * a.shape.row_bytes + (there[n] ? it[n].lane * 4 : 0));
-            scale[n][i] = a.scales[i][scale_at];
+            word[n][i] = *(const uint32_t *)(a.codes[i] + (line + t.inside) * a.shape.row_bytes + (there ? t.lane * 4 : 0));
+            scale[n][i] = a.scales[i][line * a.shape.segments + ((long long)segment << a.shape.page_shift) + t.inside];
         }
     }
+    if (t.valid <= 0) return;
 #pragma unroll
-    for (int n = 0; n < ITEMS; ++n) {
-        if (it[n].valid <= 0) continue;
+    for (int n = 0; n < HEADS; ++n) {
+        if (first_head + n >= a.shape.kv_heads) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float x[8];
-#define QT_EACH(e)                                                                                             \
-    {                                                                                                          \
-        const cache_f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[n][i], 1.0f, e);                    \
-        x[2 * e] = there[n] ? p.x * scale[n][i] : 0.0f, x[2 * e + 1] = there[n] ? p.y * scale[n][i] : 0.0f;     \
+#define QT_EACH(e)                                                                                     \
+    {                                                                                                  \
+        const cache_f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[n][i], 1.0f, e);            \
+        x[2 * e] = there ? p.x * scale[n][i] : 0.0f, x[2 * e + 1] = there ? p.y * scale[n][i] : 0.0f;   \
     }
             QT_EACH(0) QT_EACH(1) QT_EACH(2) QT_EACH(3)
 #undef QT_EACH
-            store_eight<BF16>(a.vectors.base[i], it[n].token * a.vectors.token_stride[i] + it[n].head * a.vectors.head_stride[i] + it[n].lane * 8,
-                              it[n].valid, x);
+            store_eight<BF16, STREAM>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.lane * 8,
+                                      t.valid, x);
         }
     }
 }
 
 template <bool BF16>
 void launch_copy(bool write, const CacheCopy &a, hipStream_t stream) {
-    // several items a thread where there are workgroups enough for every unit: their loads wait together
-    const bool large = a.items >= 1u << 21;
-    const int items = !large ? 1 : write ? 2 : 4;
-    const dim3 grid((a.items + kCacheThreads * items - 1) / (kCacheThreads * items));
-    if (write && large) hipLaunchKernelGGL((cache_write_kernel<BF16, 2>), grid, dim3(kCacheThreads), 0, stream, a);
-    else if (write) hipLaunchKernelGGL((cache_write_kernel<BF16, 1>), grid, dim3(kCacheThreads), 0, stream, a);
-    else if (large) hipLaunchKernelGGL((cache_read_kernel<BF16, 4>), grid, dim3(kCacheThreads), 0, stream, a);
-    else hipLaunchKernelGGL((cache_read_kernel<BF16, 1>), grid, dim3(kCacheThreads), 0, stream, a);
+    // several heads a thread where there are workgroups enough for every unit: their loads wait together
+    const long long elements = (long long)a.at.tokens * a.shape.kv_heads * a.shape.head_dim;
+    const bool large = elements >= 1 << 22;
+    const unsigned blocks = (unsigned)((a.at.tokens + a.block_tokens - 1) / a.block_tokens), heads = (unsigned)a.shape.kv_heads;
+    const dim3 one(blocks, heads), few(blocks, (heads + 3) / 4);
+    if (write && large) hipLaunchKernelGGL((cache_write_kernel<BF16, 4>), few, dim3(kCacheThreads), 0, stream, a);
+    else if (write) hipLaunchKernelGGL((cache_write_kernel<BF16, 1>), one, dim3(kCacheThreads), 0, stream, a);
+    else if (elements >= 1 << 25) hipLaunchKernelGGL((cache_read_kernel<BF16, 4, true>), few, dim3(kCacheThreads), 0, stream, a);
+    else if (large) hipLaunchKernelGGL((cache_read_kernel<BF16, 4, false>), few, dim3(kCacheThreads), 0, stream, a);
+    else hipLaunchKernelGGL((cache_read_kernel<BF16, 1, false>), one, dim3(kCacheThreads), 0, stream, a);
 }
 
 void copy_cache(const char *what, bool write, const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *keys,
@@ -286,11 +299,8 @@ void copy_cache(const char *what, bool write, const qtensor_cache *cache, const 
     while (segment > 64 && segment / 2 >= cache->head_dim) segment /= 2;
     a.segment_lanes = segment / 8;
     a.lanes = a.segment_lanes * a.shape.segments;
-    const long long items = (long long)a.at.tokens * a.shape.kv_heads * a.lanes;
-    if (items >= (1LL << 29)) { set_error(kBadArgument, "%s: %d tokens are too many for one call", what, a.at.tokens); return; }
-    a.items = (uint32_t)items;
+    a.block_tokens = kCacheThreads / a.lanes;
     a.by_lanes = make_fastdiv((uint32_t)a.lanes);
-    a.by_heads = make_fastdiv((uint32_t)a.shape.kv_heads);
     if (keys->is_bf16) launch_copy<true>(write, a, stream);
     else launch_copy<false>(write, a, stream);
     launch_ok(what);
