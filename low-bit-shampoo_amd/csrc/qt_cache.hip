@@ -53,7 +53,7 @@ struct CacheCopy {
     CacheVectors vectors;
     uint8_t *codes[2];
     float *scales[2];
-    int lanes, segment_lanes;       // lanes of eight elements per vector and per segment
+    int lanes, segment_lanes;       // lanes per vector and per segment
     int block_tokens;               // tokens of a workgroup
     FastDiv by_lanes;
 };
@@ -69,85 +69,75 @@ __device__ __forceinline__ int token_position(const CachePlaces &at, int token, 
     return at.lengths[b] - (at.starts[b + 1] - token);
 }
 
-// Eight elements as they lie in memory (16 bytes of bf16, 32 of fp32), zeros behind the end of a vector.
+// A lane takes sixteen bytes of a vector: eight elements of bf16, four of fp32.
 template <bool BF16>
-__device__ __forceinline__ void load_eight(const void *base, long long at, int valid, uint4 *raw) {
-    constexpr int kWords = BF16 ? 1 : 2;
+constexpr int kLaneElements = BF16 ? 8 : 4;
+
+// As they lie in memory, zeros behind the end of a vector.
+template <bool BF16>
+__device__ __forceinline__ uint4 load_lane(const void *base, long long at, int valid) {
     const uint8_t *p = (const uint8_t *)base + at * (BF16 ? 2 : 4);
-    if (valid >= 8 && is_aligned16(p)) {
+    if (valid >= kLaneElements<BF16> && is_aligned16(p)) return load_u32x4<true>(p);
+    uint32_t word[4];
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) raw[i] = load_u32x4<true>(p + 16 * i);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            uint32_t word[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = 4 * i + e;
-                if (BF16)
-                    word[e] = (2 * n < valid ? ((const uint16_t *)p)[2 * n] : 0u) | ((2 * n + 1 < valid ? ((const uint16_t *)p)[2 * n + 1] : 0u) << 16);
-                else
-                    word[e] = n < valid ? ((const uint32_t *)p)[n] : 0u;
-            }
-            raw[i] = make_uint4(word[0], word[1], word[2], word[3]);
-        }
+    for (int e = 0; e < 4; ++e) {
+        if (BF16) word[e] = (2 * e < valid ? ((const uint16_t *)p)[2 * e] : 0u) | ((2 * e + 1 < valid ? ((const uint16_t *)p)[2 * e + 1] : 0u) << 16);
+        else word[e] = e < valid ? ((const uint32_t *)p)[e] : 0u;
     }
+    return make_uint4(word[0], word[1], word[2], word[3]);
 }
 template <bool BF16>
-__device__ __forceinline__ void unpack_eight(const uint4 *raw, float *x) {
+__device__ __forceinline__ void unpack_lane(uint4 raw, float *x) {
+    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < (BF16 ? 1 : 2); ++i) {
-        const uint32_t word[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (BF16) x[2 * e] = __uint_as_float(word[e] << 16), x[2 * e + 1] = __uint_as_float(word[e] & 0xffff0000u);
-            else x[4 * i + e] = __uint_as_float(word[e]);
-        }
+    for (int e = 0; e < 4; ++e) {
+        if (BF16) x[2 * e] = __uint_as_float(word[e] << 16), x[2 * e + 1] = __uint_as_float(word[e] & 0xffff0000u);
+        else x[e] = __uint_as_float(word[e]);
     }
 }
-
 template <bool BF16, bool STREAM>
-__device__ __forceinline__ void store_eight(void *base, long long at, int valid, const float *x) {
-    if (BF16) {
-        uint16_t *p = (uint16_t *)base + at;
-        if (valid >= 8 && is_aligned16(p)) {
-            const qt_u32x4 y = {floats_to_bf16_pair(x[0], x[1]), floats_to_bf16_pair(x[2], x[3]), floats_to_bf16_pair(x[4], x[5]),
-                                floats_to_bf16_pair(x[6], x[7])};
-            if (STREAM) __builtin_nontemporal_store(y, (qt_u32x4 *)p);
-            else *(qt_u32x4 *)p = y;
-        } else {
+__device__ __forceinline__ void store_lane(void *base, long long at, int valid, const float *x) {
+    uint8_t *p = (uint8_t *)base + at * (BF16 ? 2 : 4);
+    if (valid >= kLaneElements<BF16> && is_aligned16(p)) {
+        qt_u32x4 y;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < valid) p[i] = float_to_bf16_bits(x[i]);
-        }
+        for (int e = 0; e < 4; ++e) y[e] = BF16 ? floats_to_bf16_pair(x[2 * e], x[2 * e + 1]) : __float_as_uint(x[e]);
+        if (STREAM) __builtin_nontemporal_store(y, (qt_u32x4 *)p);
+        else *(qt_u32x4 *)p = y;
     } else {
-        float *p = (float *)base + at;
-        if (valid >= 8 && is_aligned16(p)) {
-            store_f32x4<STREAM>(p, make_float4(x[0], x[1], x[2], x[3]));
-            store_f32x4<STREAM>(p + 4, make_float4(x[4], x[5], x[6], x[7]));
-        } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i < valid) p[i] = x[i];
+        for (int e = 0; e < kLaneElements<BF16>; ++e) {
+            if (e >= valid) continue;
+            if (BF16) ((uint16_t *)p)[e] = float_to_bf16_bits(x[e]);
+            else ((float *)p)[e] = x[e];
         }
     }
 }
+// Its codes: four bytes, or two.
+template <bool BF16>
+__device__ __forceinline__ uint32_t load_codes(const uint8_t *p) { return BF16 ? *(const uint32_t *)p : *(const uint16_t *)p; }
+template <bool BF16>
+__device__ __forceinline__ void store_codes(uint8_t *p, uint32_t word) {
+    if (BF16) *(uint32_t *)p = word;
+    else *(uint16_t *)p = (uint16_t)word;
+}
 
-// A thread's place: eight elements from `lane` * 8 on of the vectors of one token, whose heads it goes through.  A workgroup takes some
+// A thread's place: a lane's elements of the vectors of one token, whose heads it goes through.  A workgroup takes some
 // sixteen tokens of a few heads: codes and scales of a head's consecutive tokens lie side by side, and where the token
 // lies is looked up once for all of them.
 struct CacheThread {
-    int valid;                  // elements of a vector from here on; 0: nothing
-    int lane, token;
+    int valid;                  // elements of a vector from `first` on; 0: nothing
+    int first, token;
     long long line, inside;     // first row of head 0 of the token's page, and the token's row among that; line < 0: it has no page
 };
+template <bool BF16>
 __device__ __forceinline__ CacheThread cache_thread(const CacheCopy &a) {
     CacheThread t;
     const int nth = (int)fastdiv(threadIdx.x, a.by_lanes);
-    t.lane = (int)threadIdx.x - nth * a.lanes;
+    t.first = ((int)threadIdx.x - nth * a.lanes) * kLaneElements<BF16>;
     t.token = (int)blockIdx.x * a.block_tokens + nth;
     const bool there = nth < a.block_tokens && t.token < a.at.tokens;
-    t.valid = there ? max(0, a.shape.head_dim - t.lane * 8) : 0;
+    t.valid = there ? max(0, a.shape.head_dim - t.first) : 0;
     t.token = there ? t.token : 0;
     return t;
 }
@@ -164,23 +154,23 @@ __device__ __forceinline__ void cache_look_up(const CacheCopy &a, CacheThread &t
     t.inside = position & ((1 << a.shape.page_shift) - 1);
 }
 
-// A lane takes eight elements of a vector; a segment is 8, 16 or 32 lanes side by side.  Largest magnitude by integer maximum of
+// A segment is 8, 16 or 32 lanes side by side in bf16, twice as many in fp32.  Largest magnitude by integer maximum of
 // the magnitudes' bits (NaN above infinity, so that a segment with a NaN gets a NaN for its scale and reads as NaN),
 // scale and quotients by correctly rounded division (qt_divide.h; quotients below 2^-40, which it may round otherwise, are code 0),
 // nearest number (ties to the even code, beyond 6 to 6) by the conversion instruction.
 template <bool BF16, int HEADS>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheCopy a) {
-    CacheThread t = cache_thread(a);
+    CacheThread t = cache_thread<BF16>(a);
     const int first_head = blockIdx.y * HEADS;
-    uint4 raw[HEADS][2][BF16 ? 1 : 2];
+    uint4 raw[HEADS][2];
 #pragma unroll
     for (int n = 0; n < HEADS; ++n)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            load_eight<BF16>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.lane * 8,
-                             first_head + n < a.shape.kv_heads ? t.valid : 0, raw[n][i]);
+            raw[n][i] = load_lane<BF16>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.first,
+                                        first_head + n < a.shape.kv_heads ? t.valid : 0);
     cache_look_up(a, t);
-    const int segment = (t.lane * 8) >> a.shape.segment_shift;
+    const int segment = t.first >> a.shape.segment_shift;
 #pragma unroll
     for (int n = 0; n < HEADS; ++n) {
         const bool there = t.line >= 0 && first_head + n < a.shape.kv_heads;
@@ -188,47 +178,50 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheC
         const long long scale_at = line * a.shape.segments + ((long long)segment << a.shape.page_shift) + t.inside;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float x[8];
-            unpack_eight<BF16>(raw[n][i], x);
+            constexpr int kEach = kLaneElements<BF16>;
+            float x[kEach], y[kEach];
+            unpack_lane<BF16>(raw[n][i], x);
             uint32_t top = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+            for (int e = 0; e < kEach; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
             top = group_max_u32<8>(top);
             if (a.segment_lanes >= 16) top = max(top, dpp_u32<0x140>(top));
             if (a.segment_lanes >= 32) top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+            if (a.segment_lanes >= 64) top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
             const float scale = __uint_as_float(top) / 6.0f;
-            float y[8];
             const uint32_t bits = __float_as_uint(scale);
             if (bits >= kFastDivLo && bits <= kFastDivHi) {
                 const float r = exact_reciprocal(scale);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = quotient(x[e], scale, r);
+                for (int e = 0; e < kEach; ++e) y[e] = quotient(x[e], scale, r);
             } else {
                 // (zeroes times a scale that is not finite are NaN)
                 const bool zero = bits == 0 || top >= 0x7f800000u;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = zero ? 0.0f : x[e] / scale;
+                for (int e = 0; e < kEach; ++e) y[e] = zero ? 0.0f : x[e] / scale;
             }
             uint32_t word = 0;
             word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[0], y[1], 1.0f, 0);
             word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[2], y[3], 1.0f, 1);
-            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[4], y[5], 1.0f, 2);
-            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[6], y[7], 1.0f, 3);
-            if (there && t.lane * 4 < a.shape.row_bytes) *(uint32_t *)(a.codes[i] + (line + t.inside) * a.shape.row_bytes + t.lane * 4) = word;
-            if (there && (t.lane & (a.segment_lanes - 1)) == 0) a.scales[i][scale_at] = scale;
+            if constexpr (BF16) {
+                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[4], y[5], 1.0f, 2);
+                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[6], y[7], 1.0f, 3);
+            }
+            if (there && t.first < 2 * a.shape.row_bytes) store_codes<BF16>(a.codes[i] + (line + t.inside) * a.shape.row_bytes + t.first / 2, word);
+            if (there && (t.first & ((1 << a.shape.segment_shift) - 1)) == 0) a.scales[i][scale_at] = scale;
         }
     }
 }
 
-// The reverse, eight elements a lane; tokens that the cache does not have come out as zeros.  STREAM: the result is more than the caches
+// The reverse; tokens that the cache does not have come out as zeros.  STREAM: the result is more than the caches
 // hold and goes past them.
 template <bool BF16, int HEADS, bool STREAM>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCopy a) {
-    CacheThread t = cache_thread(a);
+    CacheThread t = cache_thread<BF16>(a);
     const int first_head = blockIdx.y * HEADS;
     cache_look_up(a, t);
     const bool there = t.line >= 0;
-    const int segment = there ? (t.lane * 8) >> a.shape.segment_shift : 0;
+    const int segment = there ? t.first >> a.shape.segment_shift : 0;
     uint32_t word[HEADS][2];
     float scale[HEADS][2];
 #pragma unroll
@@ -237,7 +230,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCo
         const long long line = there ? t.line + ((long long)min(first_head + n, a.shape.kv_heads - 1) << a.shape.page_shift) : 0;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            word[n][i] = *(const uint32_t *)(a.codes[i] + (line + t.inside) * a.shape.row_bytes + (there ? t.lane * 4 : 0));
+            word[n][i] = load_codes<BF16>(a.codes[i] + (line + t.inside) * a.shape.row_bytes + (there ? t.first / 2 : 0));
             scale[n][i] = a.scales[i][line * a.shape.segments + ((long long)segment << a.shape.page_shift) + t.inside];
         }
     }
@@ -247,16 +240,17 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCo
         if (first_head + n >= a.shape.kv_heads) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float x[8];
+            float x[kLaneElements<BF16>];
 #define QT_EACH(e)                                                                                     \
     {                                                                                                  \
         const cache_f32x2 p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[n][i], 1.0f, e);            \
         x[2 * e] = there ? p.x * scale[n][i] : 0.0f, x[2 * e + 1] = there ? p.y * scale[n][i] : 0.0f;   \
     }
-            QT_EACH(0) QT_EACH(1) QT_EACH(2) QT_EACH(3)
+            QT_EACH(0) QT_EACH(1)
+            if constexpr (BF16) { QT_EACH(2) QT_EACH(3) }
 #undef QT_EACH
-            store_eight<BF16, STREAM>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.lane * 8,
-                                      t.valid, x);
+            store_lane<BF16, STREAM>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.first,
+                                     t.valid, x);
         }
     }
 }
@@ -297,7 +291,7 @@ void copy_cache(const char *what, bool write, const qtensor_cache *cache, const 
     // a segment is no longer than the vector, rounded up to a power of two
     int segment = cache->blocksize;
     while (segment > 64 && segment / 2 >= cache->head_dim) segment /= 2;
-    a.segment_lanes = segment / 8;
+    a.segment_lanes = segment / (keys->is_bf16 ? 8 : 4);
     a.lanes = a.segment_lanes * a.shape.segments;
     a.block_tokens = kCacheThreads / a.lanes;
     a.by_lanes = make_fastdiv((uint32_t)a.lanes);
