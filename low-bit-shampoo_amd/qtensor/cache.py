@@ -52,6 +52,14 @@ if F.lib is not None:
     F.lib.qtensor_hip_cache_attend_workspace.restype = ct.c_longlong
     F.lib.qtensor_hip_cache_attend_workspace.argtypes = [ct.POINTER(_Cache), ct.c_int, ct.c_int, ct.c_int]
 
+    # the same calls with their host side in native code (csrc/direct_call.cpp): what it does not take goes the way below
+    _native = F._direct
+    if _native is not None:
+        _native.bind_cache([ct.cast(getattr(F.lib, "qtensor_hip_cache_" + n), ct.c_void_p).value
+                            for n in ("write", "read", "attend", "attend_workspace")])
+else:
+    _native = None
+
 
 class QTensorCache:
     """The cache of one layer: `pages` pages of `page_size` tokens (a power of two from 16 to 4096), kv_heads heads of head_dim
@@ -93,6 +101,9 @@ class QTensorCache:
     # ---- the calls
     def write(self, keys: Tensor, values: Tensor, table: Tensor, lengths: Tensor, starts: Optional[Tensor] = None) -> None:
         """Encodes keys and values [tokens, kv_heads, head_dim] (fp32 or bf16, the last dimension contiguous) of the new tokens."""
+        if _native is not None and _native.cache_write(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize,
+                                                       keys, values, table, lengths, starts):
+            return
         F._require_gpu(self.codes, "QTensorCache.write")
         F._dtype_slot(keys.dtype, "keys")
         tokens = keys.shape[0] if keys.dim() == 3 else -1
@@ -106,12 +117,17 @@ class QTensorCache:
         """(keys, values) [tokens, kv_heads, head_dim] as the cache holds them, of the same tokens that `write` would take; with
         starts up to the lengths of whole sequences, everything.  tokens: how many (starts[-1], which only the GPU knows);
         one of each sequence without starts."""
-        F._require_gpu(self.codes, "QTensorCache.read")
-        F._dtype_slot(dtype, "the result")
         if tokens is None:
             if starts is not None:
                 raise ValueError("read with starts needs the number of tokens")
             tokens = lengths.numel()
+        if _native is not None:
+            done = _native.cache_read(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, table, lengths,
+                                      starts, tokens, dtype)
+            if done is not None:
+                return done
+        F._require_gpu(self.codes, "QTensorCache.read")
+        F._dtype_slot(dtype, "the result")
         places = self._places(table, lengths, starts, tokens)
         keys, values = (torch.empty(tokens, self.kv_heads, self.head_dim, dtype=dtype, device=self.codes.device) for _ in range(2))
         F._call(F.lib.qtensor_hip_cache_read, self.codes.device, self._ref(), places, _vectors(keys), _vectors(values))
@@ -124,6 +140,11 @@ class QTensorCache:
         sequence up to itself; with a window only the last `window` tokens of that, itself included, and the first `sinks`
         of the sequence.  scale: 1 / sqrt(head_dim) unless given.  A token that sees nothing gets zeros.  out: optional result of the
         shape and type of q."""
+        if _native is not None:
+            done = _native.cache_attend(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, q, table, lengths,
+                                        starts, scale, window, sinks, out)
+            if done is not None:
+                return done
         F._require_gpu(self.codes, "QTensorCache.attend")
         F._dtype_slot(q.dtype, "q")
         tokens, heads = (q.shape[0], q.shape[1]) if q.dim() == 3 else (-1, -1)

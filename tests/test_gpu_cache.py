@@ -425,3 +425,38 @@ def test_refusals(Cache):
         cache.attend(q.clone().requires_grad_(), *good)
     torch.cuda.synchronize()
     assert torch.equal(cache.codes, before)
+
+
+def test_the_host_side_in_python_does_the_same(Cache, monkeypatch):
+    """Calls that native code does not take (or all of them, without it) have the same bits."""
+    import qtensor.cache as C
+    assert C._native is not None
+    cache, table, lens, _ = made(Cache, [70, 0, 300], None, 2, 96, 16, 64)
+    starts = torch.tensor([0, 30, 30, 41], dtype=torch.int32).cuda()
+    k, v, q = (tokens(41, h, 96, torch.bfloat16, 120 + h).cuda() for h in (2, 3, 6))
+    v = v[:, :2]
+
+    def everything():
+        cache.codes.zero_(), cache.scales.zero_()
+        cache.write(k, v, table, lens, starts)
+        cache.write(k[:3], v[:3], table, lens)
+        out = torch.zeros(41, 6, 96, dtype=torch.bfloat16, device="cuda")
+        given = cache.attend(q, table, lens, starts, scale=0.3, window=50, sinks=3, out=out)
+        assert given is out
+        return [*cache.read(table, lens, starts, tokens=41, dtype=torch.bfloat16), *cache.read(table, lens), out, cache.attend(q[:3], table, lens),
+                cache.attend(q, table, lens, starts, window=7)]
+
+    native = everything()
+    calls = []
+
+    class Spy:
+        def __getattr__(self, name):
+            return lambda *a: calls.append((name, getattr(real, name)(*a))) or calls[-1][1]
+
+    real = C._native
+    monkeypatch.setattr(C, "_native", Spy())
+    everything()
+    assert len(calls) == 7 and all(done is not None for _, done in calls)
+    monkeypatch.setattr(C, "_native", None)
+    for a, b in zip(native, everything()):
+        assert a.dtype == b.dtype and torch.equal(a, b)
