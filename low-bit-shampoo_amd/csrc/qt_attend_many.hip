@@ -33,7 +33,7 @@ __device__ __forceinline__ uint32_t tokens_up_to(int x) {
 template <bool ADD>
 __device__ __forceinline__ f32x16 times_row(const f32x16 &x, float by, const f32x16 &to) {
     f32x16 y;
-#define QT_EACH(i) y[i] = ADD ? to[i] + x[i] * of_row<i>(by) : x[i] * of_row<i>(by);
+#define QT_EACH(i) y[i] = ADD ? __builtin_fmaf(x[i], of_row<i>(by), to[i]) : x[i] * of_row<i>(by);
     QT_EACH(0) QT_EACH(1) QT_EACH(2) QT_EACH(3) QT_EACH(4) QT_EACH(5) QT_EACH(6) QT_EACH(7)
     QT_EACH(8) QT_EACH(9) QT_EACH(10) QT_EACH(11) QT_EACH(12) QT_EACH(13) QT_EACH(14) QT_EACH(15)
 #undef QT_EACH
@@ -224,16 +224,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                 for (int h = 0; h < kSteps; ++h) {
                     const int row = 32 * t + column;
                     const i32x4 keys = *(const i32x4 *)(s_keys[buffer] + row * kRowBytes + 16 * ((2 * h + half) ^ swap_of<DP>(row)));
-                    if (h == 0 || UNITS > 1)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) c[i] = 0.0f;
-#pragma unroll
-                    for (int i = kPieces - 1; i >= 0; --i)
-                        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(as_operand(keys), as_operand(query[h][i]), c, kFp4, kFp6, 0, kOne, 0, query_scale[h][i]);
+                    for (int i = kPieces - 1; i >= 0; --i) {
+                        const f32x16 none = {};
+                        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(as_operand(keys), as_operand(query[h][i]),
+                                                                            i == kPieces - 1 && (h == 0 || UNITS > 1) ? none : c, kFp4, kFp6, 0, kOne, 0,
+                                                                            query_scale[h][i]);
+                    }
                     if constexpr (UNITS > 1) score[t] = h == 0 ? times_row<false>(c, by_key[h][t], c) : times_row<true>(c, by_key[h][t], score[t]);
                 }
                 if constexpr (UNITS == 1) score[t] = times_row<false>(c, by_key[0][t], c);
             }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(score[t]));      // (here, in one block with what they are made of)
+            __builtin_amdgcn_sched_barrier(0);
             const bool whole = !(~here[0] | ~here[1]);
             const bool full = base + kManyTile - 1 <= lowest && (!a.window || highest - base < a.window || base + kManyTile <= a.sinks) && whole;
             uint32_t see = 0xffffffffu;
@@ -277,8 +281,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
                     const float p = __builtin_amdgcn_exp2f(score[t][i] - zero), q = __builtin_amdgcn_exp2f(score[t][i + 1] - zero);
-                    sum += p + q;
-                    const f16x2 both = __builtin_convertvector((cache_f32x2){p, q}, f16x2);
+                    const f16x2 both = __builtin_convertvector((cache_f32x2){p, q}, f16x2), ones = {(_Float16)1.0f, (_Float16)1.0f};
+                    sum = __builtin_amdgcn_fdot2(both, ones, sum, false);       // of the weights as they are multiplied, in fp32
                     weight[2 * t + (i >> 3)][i & 7] = both[0];
                     weight[2 * t + (i >> 3)][(i & 7) + 1] = both[1];
                 }
