@@ -15,6 +15,7 @@ struct AttendArgs {
     void *out;
     long long q_token, q_head, out_token, out_head;
     int heads, group;
+    int q_in_eights;        // not 0: eight elements of a query from a multiple of eight on are there together, and aligned to 16 bytes
     float factor;           // scale * log2 e
     int window, sinks;      // window 0: no window
     int few_rows;           // sequences with up to so many queries (times heads that share one of the cache) go to the kernel for few, others to

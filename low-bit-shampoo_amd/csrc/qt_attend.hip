@@ -414,6 +414,7 @@ extern "C" void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtens
     a.q = q->base, a.q_token = q->token_stride, a.q_head = q->head_stride;
     a.out = out->base, a.out_token = out->token_stride, a.out_head = out->head_stride;
     a.heads = heads, a.group = heads / a.shape.kv_heads;
+    a.q_in_eights = q->is_bf16 && is_aligned(q->base, 16) && q->token_stride % 8 == 0 && q->head_stride % 8 == 0 && a.shape.head_dim % 8 == 0;
     a.factor = scale * 1.4426950408889634f;
     a.window = window, a.sinks = sinks;
     a.partial = (float *)workspace;

@@ -1,12 +1,14 @@
 // Attention over a 4-bit cache for sequences of many queries: prompts, or many heads that share one of the cache (qt_attend.h).
 //
 // A workgroup takes 128 queries (of all heads that share a head of the cache), thirty-two for each of its four waves, and goes through the
-// tokens they see in tiles of 64.  Scores as in the kernel for few queries, but by v_mfma_scale_f32_32x32x64: the codes of the keys are
-// multiplied as they are with the queries' three 6-bit pieces, and scaled afterwards.  The weights' products are bound by the vector
-// unit rather than by matrix instructions when weights are split, so here the values are expanded, once for all 128 queries: a thread turns 16
-// bytes of codes into 32 fp16 numbers times their scale (two roundings of 2^-12, against 2^-9 of the result's type) in LDS, and weights
-// are rounded to fp16 (2^-12).  fp16 has no range to spare: weights are 2^11 times what they are, and scales relative to a power of two that
-// follows the largest scale of the tiles so far, so that a value loses bits only 2^25 below the largest.
+// tokens they see in tiles of 64.  Products of that many queries are bound by what the vector unit does between them, so the codes
+// are expanded here, once for all 128: a thread turns 16 bytes of codes into 32 fp16 numbers times their scale in LDS, and the
+// scores come out of v_mfma_f32_32x32x16_f16 as exponents, the running maximum already taken off (it is what the sums begin with).
+//
+// Roundings: keys and values to fp16 (two of 2^-12: the scale and the product), queries times the scale of the scores to fp16, weights to fp16
+// (2^-12 each), all against 2^-9 of the result's type; sums, maxima and results in fp32.  fp16 has no range to spare, so keys and values
+// are held relative to powers of two that follow the largest scales of the tiles so far (queries and results are corrected when one grows):
+// a key or value loses bits only 2^16 below the largest of its head.  Weights are 2^11 times what they are, which keeps those of 2^-25.
 #include "qt_attend.h"
 
 namespace qt {
@@ -17,6 +19,9 @@ constexpr int kManyShift = 6;
 constexpr int kManyLeast = 8;           // tiles of a piece, at least
 constexpr float kWeightBits = 11.0f;    // weights are kept times 2^11 ...
 constexpr float kSlack = 4.0f;          // ... and the running maximum may lag behind by 4: below 2^15 in fp16
+// Keys and values whose scale has the largest exponent so far are held times 2^3; larger ones of up to 2^9 times that still fit (6 * 2 *
+// 2^(3 + 9) < 65504) before the power of two has to follow.
+constexpr int kHeldBits = 3, kHeadroom = 9;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -29,37 +34,59 @@ __device__ __forceinline__ uint32_t tokens_up_to(int x) {
     return x < 0 ? 0u : x >= 27 ? 0xffffu : (1u << (bits & 31)) - 1u;
 }
 
-// Sixteen scores times what the lanes of the lane's row of sixteen hold, one each.
-template <bool ADD>
-__device__ __forceinline__ f32x16 times_row(const f32x16 &x, float by, const f32x16 &to) {
-    f32x16 y;
-#define QT_EACH(i) y[i] = ADD ? __builtin_fmaf(x[i], of_row<i>(by), to[i]) : x[i] * of_row<i>(by);
-    QT_EACH(0) QT_EACH(1) QT_EACH(2) QT_EACH(3) QT_EACH(4) QT_EACH(5) QT_EACH(6) QT_EACH(7)
-    QT_EACH(8) QT_EACH(9) QT_EACH(10) QT_EACH(11) QT_EACH(12) QT_EACH(13) QT_EACH(14) QT_EACH(15)
-#undef QT_EACH
-    return y;
-}
-__device__ __forceinline__ uint32_t rows_not_finite(float by) {
-    uint32_t y = 0;
-#define QT_EACH(i) y |= (uint32_t)((__float_as_uint(of_row<i>(by)) & 0x7f800000u) == 0x7f800000u) << i;
-    QT_EACH(0) QT_EACH(1) QT_EACH(2) QT_EACH(3) QT_EACH(4) QT_EACH(5) QT_EACH(6) QT_EACH(7)
-    QT_EACH(8) QT_EACH(9) QT_EACH(10) QT_EACH(11) QT_EACH(12) QT_EACH(13) QT_EACH(14) QT_EACH(15)
-#undef QT_EACH
-    return y;
-}
-
-// Bytes of row `row` of expanded values in LDS are moved by this (exclusive or), so that the eight rows of 64 bytes that a transposed
-// read takes lie in different banks two by two.
+// Place of 16-byte chunk `chunk` of row `row` of expanded codes in LDS.  Chunks of one place of sixteen rows (reads of keys), four chunks of each
+// of four rows (a quarter of what a wave writes at a time), and the 64 bytes of each of four rows that half a transposed read takes are
+// all on different banks.
 template <int DP>
-__device__ __forceinline__ int value_swap(int row) { return (DP == 64 ? (row >> 1) & 1 : row & 3) << 6; }
+__device__ __forceinline__ int held_place(int row, int chunk) {
+    if (DP == 64) return chunk ^ (((row >> 1) & 3) | ((((row >> 1) ^ (row >> 3)) & 1) << 2));
+    const int a = row & 3, j = (row >> 2) & 3;
+    return chunk ^ ((a << 2) | (a ^ j)) ^ (DP == 256 ? ((chunk >> 4) & 1) << 1 : 0);
+}
 
-template <int DP, int UNITS>
+// Which of a lane's tokens of a tile have a page (bit 16 t + i: token 32 t + 8 (i / 4) + 4 half + i % 4).
+__device__ __forceinline__ uint32_t pages_there(const AttendArgs &a, const int *table, int end, int base) {
+    uint32_t see = 0;
+#pragma unroll 1
+    for (int group = 0; group < kManyTile / 16; ++group) {
+        const int token = base + 16 * group;
+        if (token >= end) break;
+        // eight of a lane's tokens lie in every group of sixteen, and none past the end is before a query
+        if ((unsigned)table[token >> a.shape.page_shift] < (unsigned)a.shape.pages) see |= 0xffu << (8 * group);
+    }
+    return see;
+}
+// A bit for every 64 elements of values in whose scale there is a NaN or an infinity, over the tokens `first` to `end` that a query at
+// `position` sees.
+__device__ __forceinline__ uint32_t values_not_finite(const AttendArgs &a, const int *table, int first, int end, int position, int head) {
+    uint32_t found = 0;
+#pragma unroll 1
+    for (int token = first; token < min(end, position + 1); ++token) {
+        if (a.window && position - token >= a.window && token >= a.sinks) continue;
+        const int page = table[token >> a.shape.page_shift];
+        if ((unsigned)page >= (unsigned)a.shape.pages) continue;
+        const long long line = ((long long)page * a.shape.kv_heads + head) << a.shape.page_shift;
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+            const int segment = (64 * u) >> a.shape.segment_shift;
+            if (segment >= a.shape.segments) break;
+            const float by = a.scales[1][line * a.shape.segments + ((long long)segment << a.shape.page_shift) + (token & ((1 << a.shape.page_shift) - 1))];
+            if (!(by - by == 0.0f)) found |= 1u << u;
+        }
+    }
+    return found;
+}
+
+template <int DP>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const AttendArgs a) {
-    constexpr int kPieces = 3, kSteps = DP / 64, kDTiles = DP / 32, kChunks = DP / 32;
-    constexpr int kKeyBytes = kManyTile * DP / 2, kRowBytes = DP / 2, kValueRow = DP * 2;
-    constexpr int kEach = kManyTile * kChunks > 256 ? kManyTile * kChunks / 256 : 1;        // 16-byte chunks of a tile's codes per thread
-    __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][kKeyBytes];
-    __shared__ __attribute__((aligned(16))) uint8_t s_values[2][kManyTile * kValueRow];
+    constexpr int kSteps = DP / 16, kDTiles = DP / 32, kChunks = DP / 32, kRow = DP * 2;
+    constexpr int kEach = DP == 256 ? 2 : 1;            // chunks of keys and of values a thread stages (heads of 64: of one of the two)
+    constexpr int kKinds = DP == 64 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][kManyTile * kRow];
+    __shared__ __attribute__((aligned(16))) uint8_t s_values[2][kManyTile * kRow];
+    __shared__ int s_exponent[2];                       // largest exponents of a scale of keys and values so far
+    __shared__ int s_event[3];                          // of three tiles in turn: bit 0: an exponent has outgrown what is held; bit 1: a
+                                                        // scale of a value is not finite; bit 2: a token's page is not there
 
     AttendWork w;
     if (!find_work<kRowsOfMany, kManyShift, true>(a, blockIdx.x, w)) return;
@@ -74,7 +101,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;
     // positions of this wave's queries and of all of the workgroup's
     const int lowest = v.first_position + min(first_row + 32 * wave, all_rows - 1) / a.group;
-    const int highest = first_row + 32 * wave < all_rows ? v.first_position + min(first_row + 32 * wave + 31, all_rows - 1) / a.group : -1;
+    const int highest = v.first_position + min(first_row + 32 * wave + 31, all_rows - 1) / a.group;
     {
         const int last = v.first_position + min(first_row + kRowsOfMany - 1, all_rows - 1) / a.group;
         v.end = max(0, min(v.end, last + 1));
@@ -85,161 +112,259 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
 
     const int *table = a.at.table + (long long)w.b * a.at.table_stride;
     const int page_mask = (1 << a.shape.page_shift) - 1, chunks = a.shape.row_bytes >> 4;
-    auto tile_at = [&](int k) { return (k < v.sink_tiles ? k : v.first_tile + k - v.sink_tiles) * kManyTile; };
+    auto tile_at = [&](int k) __attribute__((always_inline)) { return (k < v.sink_tiles ? k : v.first_tile + k - v.sink_tiles) * kManyTile; };
 
-    // what this thread stages of a tile: chunk id % kChunks of token id / kChunks
-    const int own_token = 8 * ((lane & 15) >> 2) + 4 * half + (lane & 3);       // ... and whose scales its row of lanes needs: this + 32 i
-    i32x4 key_chunk[kEach], value_chunk[kEach];
-    float chunk_scale[kEach], key_scale[UNITS][2], value_scale[UNITS][2];
-    unsigned long long valid[2];
-    int page[kEach + 2];
-    auto load_pages = [&](int k) {
+    // What this thread stages of a tile: chunk `my_chunk` of the tokens stage_row(i).  A wave's tokens lie in one group of sixteen, so in one
+    // page (heads of 64: in two; the first two waves stage keys, the others values).
+    const int my_chunk = lane & (kChunks - 1);
+    auto stage_row = [&](int i) __attribute__((always_inline)) { return DP == 64 ? 32 * (wave & 1) + (lane >> 1) : DP == 128 ? 16 * wave + (lane >> 2) : 32 * i + 8 * wave + (lane >> 3); };
+    constexpr int kPages = DP == 64 ? 2 : kEach;
+    const int chunk_byte = 16 * min(my_chunk, chunks - 1), segment = min((32 * my_chunk) >> a.shape.segment_shift, a.shape.segments - 1) << a.shape.page_shift;
+    int page[kPages];
+    auto load_pages = [&](int k) __attribute__((always_inline)) {
         const int base = tile_at(k);
 #pragma unroll
-        for (int i = 0; i < kEach + 2; ++i) {
-            const int token = base + (i < kEach ? (threadIdx.x + 256 * i) / kChunks % kManyTile : own_token + 32 * (i - kEach));
+        for (int i = 0; i < kPages; ++i) {
+            const int token = base + (DP == 64 ? 32 * (wave & 1) + 16 * i : DP == 128 ? 16 * wave : 32 * i + 8 * wave);
             page[i] = table[min(token, v.end - 1) >> a.shape.page_shift];
         }
     };
-    auto load_tile = [&](int k) {
+    i32x4 chunk[kKinds][kEach];
+    float scale[kKinds][kEach];
+    bool there[kEach], hole[kEach];
+    auto load_tile = [&](int k) __attribute__((always_inline)) {
         const int base = tile_at(k);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const int id = threadIdx.x + 256 * i, inside = id / kChunks % kManyTile, token = base + inside;
-            const bool there = (unsigned)page[i] < (unsigned)a.shape.pages && token < v.end;
-            const long long line = ((long long)(there ? page[i] : 0) * a.shape.kv_heads + w.head) << a.shape.page_shift;
-            const int chunk = min(id % kChunks, chunks - 1), in_page = token & page_mask;
-            const long long at = (line + in_page) * a.shape.row_bytes + 16 * chunk;
-            key_chunk[i] = *(const i32x4 *)(a.codes[0] + at);
-            value_chunk[i] = *(const i32x4 *)(a.codes[1] + at);
-            const int segment = min((32 * chunk) >> a.shape.segment_shift, a.shape.segments - 1);
-            chunk_scale[i] = a.scales[1][line * a.shape.segments + ((long long)segment << a.shape.page_shift) + in_page];
-            if (!there) page[i] = -1;
-        }
+            const int token = base + stage_row(i);
+            int p = __builtin_amdgcn_readfirstlane(page[i]);
+            if (DP == 64) p = lane < 32 ? p : __builtin_amdgcn_readfirstlane(page[kPages - 1]);
+            there[i] = (unsigned)p < (unsigned)a.shape.pages && token < v.end;
+            hole[i] = (unsigned)p >= (unsigned)a.shape.pages && token < v.end;
+            const long long line = ((long long)((unsigned)p < (unsigned)a.shape.pages ? p : 0) * a.shape.kv_heads + w.head) << a.shape.page_shift;
+            const long long code_at = line * a.shape.row_bytes, scale_at = line * a.shape.segments;
+            const uint32_t in_page = token & page_mask;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int token = base + own_token + 32 * i;
-            const bool there = (unsigned)page[kEach + i] < (unsigned)a.shape.pages && token < v.end;
-            valid[i] = __ballot(there);
-            const long long line = ((long long)(there ? page[kEach + i] : 0) * a.shape.kv_heads + w.head) << a.shape.page_shift;
-#pragma unroll
-            for (int u = 0; u < UNITS; ++u) {
-                const int segment = min((u * 64) >> a.shape.segment_shift, a.shape.segments - 1);
-                const long long at = line * a.shape.segments + ((long long)segment << a.shape.page_shift) + (token & page_mask);
-                key_scale[u][i] = a.scales[0][at];
-                value_scale[u][i] = a.scales[1][at];
+            for (int n = 0; n < kKinds; ++n) {
+                const int kind = DP == 64 ? wave >> 1 : n;
+                chunk[n][i] = *(const i32x4 *)((kind == 0 ? a.codes[0] : a.codes[1]) + code_at + (in_page * (uint32_t)a.shape.row_bytes + chunk_byte));
+                scale[n][i] = *((kind == 0 ? a.scales[0] : a.scales[1]) + scale_at + (in_page + segment));
             }
         }
     };
 
-    u32x6 query[kSteps][kPieces];
-    int query_scale[kSteps][kPieces];
-    f32x16 result[kDTiles];
+    // places in LDS: of this lane's first operands and of what it stages (held_place: other chunks and rows differ by constants)
+    const int value_row = 4 * half + ((lane & 15) >> 2);
+    const uint32_t key_place = column * kRow + 16 * held_place<DP>(column, half);
+    const uint32_t value_place = value_row * kRow + 16 * held_place<DP>(value_row, 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) + 8 * (lane & 1);
+    const uint32_t stage_place = stage_row(0) * kRow + 16 * held_place<DP>(stage_row(0), 4 * my_chunk);
+
+    f16x8 query[kSteps];
+    f32x16 result[kDTiles] = {}, below;         // below: what the sums of the scores begin with, minus the running maximum
+    float best = -__builtin_inff(), sum = 0.0f;
+    int odd = 0;                                // not 0: somewhere a scale of a value is not finite
+    int exponent[2] = {1, 1};                   // of the largest scales of keys and values that are held
+
+    // This lane's eight elements of every sixteen of its query, zeros behind its end.
+    const uint16_t *my_query = (const uint16_t *)a.q + my_token * a.q_token + my_head * a.q_head;
+    auto load_query_chunks = [&](uint4 *raw) __attribute__((always_inline)) {
+        const int last = a.shape.head_dim - 1;
+        if (a.q_in_eights) {
+#pragma unroll
+            for (int h = 0; h < kSteps; ++h) {
+                const int d = 16 * h + 8 * half;
+                raw[h] = *(const uint4 *)(my_query + (d <= last ? d : 0));
+                if (d > last) raw[h] = make_uint4(0, 0, 0, 0);
+            }
+        } else {
+            int from = 8 * half;
+            asm volatile("" : "+v"(from));          // (nothing of this is worked out ahead for the other way)
+#pragma unroll
+            for (int h = 0; h < kSteps; ++h) {
+                uint32_t word[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = 16 * h + from + 2 * e;
+                    const uint32_t x = my_query[min(d, last)], y = my_query[min(d + 1, last)];
+                    word[e] = (d <= last ? x : 0u) | ((d + 1 <= last ? y : 0u) << 16);
+                }
+                raw[h] = make_uint4(word[0], word[1], word[2], word[3]);
+            }
+        }
+    };
+    auto take_query = [&](const uint4 *raw) __attribute__((always_inline)) {
+        const int up = exponent[0] - 127 - kHeldBits;
+#pragma unroll
+        for (int h = 0; h < kSteps; ++h) {
+            const uint32_t word[4] = {raw[h].x, raw[h].y, raw[h].z, raw[h].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                query[h][2 * e] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(word[e] << 16) * a.factor, up);
+                query[h][2 * e + 1] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(word[e] & 0xffff0000u) * a.factor, up);
+            }
+        }
+    };
+
+    // Expands this thread's chunks into `buffer`, a word (eight elements) of a chunk at a time: kSteps of them.  Before them: notes in
+    // s_event[slot] what the workgroup has to know.
+    _Float16 scaled[kKinds][kEach];
+    auto stage_scales = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < kKinds; ++n)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                const int kind = DP == 64 ? wave >> 1 : n;
+                float by = there[i] ? scale[n][i] : 0.0f;
+                const int bits = (int)((__float_as_uint(by) >> 23) & 0xff), held = kind == 0 ? exponent[0] : exponent[1];
+                if (__builtin_expect((bits > min(held + kHeadroom, 254)) | hole[i], 0)) {
+                    if (hole[i]) {
+                        atomicOr(&s_event[slot], 4);
+                    } else if (bits < 255) {
+                        atomicMax(&s_exponent[kind], bits);
+                        atomicOr(&s_event[slot], 1);
+                    } else if (kind == 1) {
+                        atomicOr(&s_event[slot], 2);
+                        by = 0.0f;
+                    }
+                }
+                scaled[n][i] = (_Float16)__builtin_amdgcn_ldexpf(by, 127 + kHeldBits - held);
+            }
+    };
+    auto stage_word = [&](int buffer, int piece) __attribute__((always_inline)) {
+        const int n = piece / (4 * kEach), i = piece / 4 % kEach, e = piece % 4, kind = DP == 64 ? wave >> 1 : n;
+        const f16x2 times = {scaled[n][i], scaled[n][i]};
+        const uint32_t word = (uint32_t)chunk[n][i][e];
+        const f16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 0) * times, x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 1) * times,
+                    x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 2) * times, x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 3) * times;
+        QT_LDS uint8_t *area = kind == 0 ? (QT_LDS uint8_t *)s_keys[0] : (QT_LDS uint8_t *)s_values[0];
+        *(QT_LDS f16x8 *)(area + buffer * (kManyTile * kRow) + (stage_place ^ (16 * e)) + 32 * i * kRow) =
+            (f16x8){x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+    };
+    auto stage_all = [&](int buffer, int slot) __attribute__((always_inline)) {
+        stage_scales(slot);
+#pragma unroll
+        for (int piece = 0; piece < kSteps; ++piece) stage_word(buffer, piece);
+    };
+    if (threadIdx.x < 2) s_exponent[threadIdx.x] = 1;
+    // (A later tile may hold scales that have outgrown what the first ones set: the workgroup begins again then, with the exponents that it has
+    // found, which is rare and keeps the loop free of everything that would have to be corrected.)
+    bool again = tile_from < tile_to;
+    while (again) {
+    again = false;
 #pragma unroll
     for (int d = 0; d < kDTiles; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) result[d][i] = 0.0f;
-    float best = -__builtin_inff(), sum = 0.0f, poison[UNITS];
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) poison[u] = 0.0f;
-    int exponent = 1;                       // of the largest scale of a value so far: values are kept times 2^(138 - exponent)
-
-    // scales of the tile that is worked on; writes of the next tile's codes
-    float by_key[UNITS][2], by_value[UNITS][2];
-    unsigned long long here[2];
-    bool odd = false;                       // a scale of its values is not finite
-    auto stage = [&](int buffer) {
-        uint32_t top = 0;
-        bool bad = false;
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const bool there = (valid[i] >> lane) & 1;
-                by_key[u][i] = there ? key_scale[u][i] * a.factor : 0.0f;
-                by_value[u][i] = there ? value_scale[u][i] : 0.0f;
-                const uint32_t bits = __float_as_uint(by_value[u][i]) & 0x7fffffffu;
-                bad |= bits >= 0x7f800000u;
-                if (bits < 0x7f800000u) top = max(top, bits);
-            }
-        here[0] = valid[0], here[1] = valid[1];
-        odd = __ballot(bad) != 0;
-        top = group_max_u32<64>(top);
-        const int larger = max(exponent, (int)(top >> 23));
-        if (larger != exponent) {
-            const float fade = __builtin_amdgcn_ldexpf(1.0f, exponent - larger);
-#pragma unroll
-            for (int d = 0; d < kDTiles; ++d) result[d] *= fade;
-            exponent = larger;
-        }
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int id = threadIdx.x + 256 * i, row = id / kChunks, chunk = id % kChunks;
-            if (kManyTile * kChunks < 256 && row >= kManyTile) break;
-            *(i32x4 *)(s_keys[buffer] + row * kRowBytes + 16 * (chunk ^ swap_of<DP>(row))) = key_chunk[i];
-            const float scale = page[i] < 0 || (__float_as_uint(chunk_scale[i]) & 0x7fffffffu) >= 0x7f800000u ? 0.0f : chunk_scale[i];
-            const _Float16 scaled = (_Float16)__builtin_amdgcn_ldexpf(scale, 138 - exponent);
-            const f16x2 by = {scaled, scaled};
-            uint8_t *to = s_values[buffer] + row * kValueRow + ((64 * chunk) ^ value_swap<DP>(row));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t word = (uint32_t)value_chunk[i][e];
-                const f16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 0) * by, x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 1) * by,
-                            x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 2) * by, x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 3) * by;
-                *(f16x8 *)(to + 16 * e) = (f16x8){x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-            }
-        }
-    };
-
-    if (tile_from < tile_to) {
-        uint4 raw[kSteps][4];
+    for (int i = 0; i < 16; ++i) below[i] = 0.0f;
+    best = -__builtin_inff(), sum = 0.0f, odd = 0;
+    int event = 0;
+    {
+        __syncthreads();
+        if (threadIdx.x < 3) s_event[threadIdx.x] = 0;
+        uint4 raw[kSteps];
         load_pages(tile_from);
-#pragma unroll
-        for (int h = 0; h < kSteps; ++h) load_query<true>(a, my_token * a.q_token + my_head * a.q_head, 64 * h + 32 * half, mine, raw[h]);
+        load_query_chunks(raw);
         load_tile(tile_from);
-#pragma unroll
-        for (int h = 0; h < kSteps; ++h) {
-            f32x16 even, odd_places;
-            unpack_query<true>(raw[h], even, odd_places);
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = max(top, max(__float_as_uint(even[i]) & 0x7fffffffu, __float_as_uint(odd_places[i]) & 0x7fffffffu));
-            split_fp6<kPieces>(even, odd_places, top, query[h], query_scale[h]);
-        }
-        stage(0);
         load_pages(min(tile_from + 1, tile_to - 1));
         __syncthreads();
-    }
-    for (int k = tile_from; k < tile_to; ++k) {
-        const int base = tile_at(k), buffer = (k - tile_from) & 1;
-        const bool more = k + 1 < tile_to;
-        if (more) load_tile(k + 1);
-        // (a wave whose queries see nothing of the tile only stages the next one)
-        if (base <= highest && (!a.window || base + kManyTile - 1 > lowest - a.window || base < a.sinks)) {
-            f32x16 score[2];
+        // the first tile sets the exponents
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                f32x16 c;
+        for (int n = 0; n < kKinds; ++n) {
+            uint32_t top = 0;
 #pragma unroll
-                for (int h = 0; h < kSteps; ++h) {
-                    const int row = 32 * t + column;
-                    const i32x4 keys = *(const i32x4 *)(s_keys[buffer] + row * kRowBytes + 16 * ((2 * h + half) ^ swap_of<DP>(row)));
-#pragma unroll
-                    for (int i = kPieces - 1; i >= 0; --i) {
-                        const f32x16 none = {};
-                        c = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(as_operand(keys), as_operand(query[h][i]),
-                                                                            i == kPieces - 1 && (h == 0 || UNITS > 1) ? none : c, kFp4, kFp6, 0, kOne, 0,
-                                                                            query_scale[h][i]);
-                    }
-                    if constexpr (UNITS > 1) score[t] = h == 0 ? times_row<false>(c, by_key[h][t], c) : times_row<true>(c, by_key[h][t], score[t]);
-                }
-                if constexpr (UNITS == 1) score[t] = times_row<false>(c, by_key[0][t], c);
+            for (int i = 0; i < kEach; ++i) {
+                const uint32_t bits = there[i] ? (__float_as_uint(scale[n][i]) >> 23) & 0xff : 0u;
+                if (bits < 255) top = max(top, bits);
             }
+            top = group_max_u32<64>(top);
+            if (lane == 0) atomicMax(&s_exponent[DP == 64 ? wave >> 1 : n], (int)top);
+        }
+        __syncthreads();
+        exponent[0] = s_exponent[0], exponent[1] = s_exponent[1];
+        take_query(raw);
+        stage_all(0, 0);
+        __syncthreads();
+        event = s_event[0];
+    }
+    // The running maximum follows where a score is more than 2^4 above it (scores are relative to it and to 2^-11), in both halves of a
+    // column; `done`: weights of the tile that are not in the result yet.
+    f16x8 weight[4];
+    auto follow = [&](float top, f32x16 &score, int done) __attribute__((always_inline)) {
+        const bool first = best == -__builtin_inff();
+        if (!__ballot(top > (first ? -__builtin_inff() : kWeightBits + kSlack))) return;
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float up = first ? top : fmaxf(top - kWeightBits, 0.0f);          // what the maximum rises by
+        const bool rises = up != -__builtin_inff();
+        const float fade = first ? 0.0f : __builtin_amdgcn_exp2f(-up), shift = rises ? (first ? up - kWeightBits : up) : 0.0f;
+        if (rises) best = first ? up : best + up;
+        sum *= fade;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) asm volatile("" : "+v"(score[t]));      // (here, in one block with what they are made of)
-            __builtin_amdgcn_sched_barrier(0);
-            const bool whole = !(~here[0] | ~here[1]);
-            const bool full = base + kManyTile - 1 <= lowest && (!a.window || highest - base < a.window || base + kManyTile <= a.sinks) && whole;
+        for (int d = 0; d < kDTiles; ++d) result[d] *= fade;
+        const _Float16 fade16 = (_Float16)fade;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+            if (n < done) weight[n] *= fade16;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) score[i] -= shift;
+        const float under = best == -__builtin_inff() ? 0.0f : kWeightBits - best;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) below[i] = under;
+    };
+    // weights of scores 2 j and 2 j + 1 of half a tile
+    auto weigh = [&](const f32x16 &score, int t, int j) __attribute__((always_inline)) {
+        const float p = __builtin_amdgcn_exp2f(score[2 * j]), q = __builtin_amdgcn_exp2f(score[2 * j + 1]);
+        const f16x2 both = __builtin_convertvector((cache_f32x2){p, q}, f16x2), ones = {(_Float16)1.0f, (_Float16)1.0f};
+        sum = __builtin_amdgcn_fdot2(both, ones, sum, false);       // of the weights as they are multiplied, in fp32
+        weight[2 * t + (j >> 2)][2 * j & 7] = both[0];
+        weight[2 * t + (j >> 2)][(2 * j & 7) + 1] = both[1];
+    };
+    auto largest = [&](const f32x16 &score) __attribute__((always_inline)) {
+        float top = score[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, score[i]);
+        return top;
+    };
+
+    // Half a tile's products are interleaved with vector work of the other half or of the next tile: scores of the second half with the weights
+    // of the first, values of the first with the weights of the second, values of the second with expanding the next tile.  kSteps matrix instructions
+    // each, and as much vector work as fits beside them.
+    int slot = 0;
+    for (int k = tile_from; k < tile_to; ++k) {
+        const int base = tile_at(k), buffer = (k - tile_from) & 1, next_slot = slot == 2 ? 0 : slot + 1;
+        const bool more = k + 1 < tile_to;
+        if (threadIdx.x == 0) s_event[next_slot == 2 ? 0 : next_slot + 1] = 0;      // (the tile before's, which all have read)
+        if (more) {
+            load_tile(k + 1);
+            load_pages(min(k + 2, tile_to - 1));
+        }
+        {
+            const bool full = (base + kManyTile - 1 <= lowest) & (!a.window | (highest - base < a.window) | (base + kManyTile <= a.sinks)) & !(event & 4);
+            f32x16 score[2];
+            f16x8 ahead[2][4];
+            // Operands are read from LDS four matrix instructions ahead of those that take them.  A lane's places differ by constants: by exclusive
+            // ors where chunks do, by offsets where rows do (each kept as one register and worked out anew for every tile: kept apart, the
+            // places would take more registers than there are).
+            uint32_t key_at = buffer * (kManyTile * kRow) + key_place, value_at = buffer * (kManyTile * kRow) + value_place;
+            asm volatile("" : "+v"(key_at), "+v"(value_at));
+            auto read_keys = [&](int t, int first, f16x8 *to) __attribute__((always_inline)) {
+#pragma unroll
+                for (int h = first; h < first + 4; ++h)
+                    to[h - first] = *(const QT_LDS f16x8 *)((const QT_LDS uint8_t *)s_keys[0] + (key_at ^ (32 * h ^ (h >= 8 ? 32 : 0))) + 32 * t * kRow);
+            };
+            auto read_values = [&](int t, int first, f16x8 *to) __attribute__((always_inline)) {
+#pragma unroll
+                for (int f = first; f < first + 4; ++f)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int n = 2 * t + f / kDTiles, d = f % kDTiles;
+                        const uint32_t at = (value_at ^ (64 * d ^ (d >= 4 ? 32 : 0) ^ (DP == 64 ? 64 * e : 32 * e))) + (16 * n + 8 * e) * kRow;
+                        const i16x4 part = __builtin_amdgcn_ds_read_tr16_b64_v4i16((QT_LDS i16x4 *)((QT_LDS uint8_t *)s_values[0] + at));
+                        const f16x4 four = __builtin_bit_cast(f16x4, part);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) to[f - first][4 * e + x] = four[x];
+                    }
+            };
             uint32_t see = 0xffffffffu;
             if (!full) {
                 const int x = position - base - 4 * half;
@@ -248,71 +373,92 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                     const int y = behind - base - 4 * half, z = a.sinks - 1 - base - 4 * half;
                     see &= ~(tokens_up_to(y) | (tokens_up_to(y - 32) << 16)) | (tokens_up_to(z) | (tokens_up_to(z - 32) << 16));
                 }
-                if (!whole) see &= ((uint32_t)(here[0] >> (32 * half)) & 0xffffu) | ((uint32_t)(here[1] >> (32 * half)) << 16);
+                if (event & 4) see &= pages_there(a, table, v.end, base);
+            }
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+                if (t == 0) read_keys(0, 0, ahead[0]);
+#pragma unroll
+                for (int m = 0; m < kSteps; ++m) {
+                    if (m % 4 == 0) {
+                        if (m + 4 < kSteps) read_keys(t, m + 4, ahead[(m >> 2 & 1) ^ 1]);
+                        else if (t == 0) read_keys(1, 0, ahead[(m >> 2 & 1) ^ 1]);
+                        else read_values(0, 0, ahead[(m >> 2 & 1) ^ 1]);
+                    }
+                    score[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[(m >> 2) & 1][m & 3], query[m], m == 0 ? below : score[t], 0, 0, 0);
+                    if (t == 1) {
+#pragma unroll
+                        for (int j = 8 * m / kSteps; j < 8 * (m + 1) / kSteps; ++j) weigh(score[0], 0, j);
+                        __builtin_amdgcn_sched_barrier(0);
+                    } else if (m % 4 == 3) {
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                if (t == 1) asm volatile("" : "+v"(weight[0]), "+v"(weight[1]), "+v"(sum));      // (made here, beside the products)
+                __builtin_amdgcn_s_setprio(0);
+                // (the number of groups of four is even or, for heads of 64, one: what is read ahead across the turn lies in the other four registers)
+                if constexpr (kSteps == 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ahead[0][e] = ahead[1][e];
+                }
+                if (!full) {
+                    asm volatile("" : "+v"(see));           // (tested here, not ahead of the products)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) score[t][i] = see & (1u << (16 * t + i)) ? score[t][i] : -__builtin_inff();
-            }
-            if (__builtin_expect(odd, 0)) {
-#pragma unroll
-                for (int u = 0; u < UNITS; ++u)
-                    if (see & (rows_not_finite(by_value[u][0]) | (rows_not_finite(by_value[u][1]) << 16))) poison[u] = __builtin_nanf("");
-            }
-            float top = -__builtin_inff();
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, score[t][i]);
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__ballot(top > best + kSlack)) {
-                // (-inf + 4 is -inf: the first token that is seen sets the maximum)
-                const float next = fmaxf(best, top);
-                const float fade = next == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(best - next);
-                sum *= fade;
-#pragma unroll
-                for (int d = 0; d < kDTiles; ++d) result[d] *= fade;
-                best = next;
-            }
-            const float zero = best == -__builtin_inff() ? 0.0f : best - kWeightBits;
-            f16x8 weight[4];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float p = __builtin_amdgcn_exp2f(score[t][i] - zero), q = __builtin_amdgcn_exp2f(score[t][i + 1] - zero);
-                    const f16x2 both = __builtin_convertvector((cache_f32x2){p, q}, f16x2), ones = {(_Float16)1.0f, (_Float16)1.0f};
-                    sum = __builtin_amdgcn_fdot2(both, ones, sum, false);       // of the weights as they are multiplied, in fp32
-                    weight[2 * t + (i >> 3)][i & 7] = both[0];
-                    weight[2 * t + (i >> 3)][(i & 7) + 1] = both[1];
                 }
+                follow(largest(score[t]), score[t], 2 * t);
+            }
+            if (more) stage_scales(next_slot);
 #pragma unroll
-            for (int d = 0; d < kDTiles; ++d)
+            for (int t = 0; t < 2; ++t) {
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    f16x8 rows;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int token = 16 * n + 8 * e + 4 * half + ((lane & 15) >> 2), byte = 64 * d + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-                        const i16x4 part = __builtin_amdgcn_ds_read_tr16_b64_v4i16((QT_LDS i16x4 *)(s_values[buffer] + token * kValueRow + (byte ^ value_swap<DP>(token))));
-                        const f16x4 four = __builtin_bit_cast(f16x4, part);
-                        rows[4 * e] = four[0], rows[4 * e + 1] = four[1], rows[4 * e + 2] = four[2], rows[4 * e + 3] = four[3];
+                for (int m = 0; m < kSteps; ++m) {
+                    if (m % 4 == 0) {
+                        if (m + 4 < kSteps) read_values(t, m + 4, ahead[(m >> 2 & 1) ^ 1]);
+                        else if (t == 0) read_values(1, 0, ahead[(m >> 2 & 1) ^ 1]);
                     }
-                    result[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(rows, weight[n], result[d], 0, 0, 0);
+                    result[m % kDTiles] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ahead[(m >> 2) & 1][m & 3], weight[2 * t + m / kDTiles], result[m % kDTiles], 0, 0, 0);
+                    if (t == 0) {
+#pragma unroll
+                        for (int j = 8 * m / kSteps; j < 8 * (m + 1) / kSteps; ++j) weigh(score[1], 1, j);
+                    } else {
+                        stage_word(buffer ^ 1, m);      // (without a next tile: of this one once more, which nobody reads)
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-        }
-        if (more) {
-            stage(buffer ^ 1);
-            load_pages(min(k + 2, tile_to - 1));
+                __builtin_amdgcn_s_setprio(0);
+                if constexpr (kSteps == 4) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) ahead[0][e] = ahead[1][e];
+                }
+            }
         }
         __syncthreads();
+        odd |= event & 2;
+        if (more) event = s_event[next_slot];
+        slot = next_slot;
+        if (event & 1) {
+            again = true;
+            break;
+        }
+    }
     }
     sum += __shfl_xor(sum, 32, 64);
-#pragma unroll
-    for (int u = 0; u < UNITS; ++u) poison[u] += __shfl_xor(poison[u], 32, 64);
     if (!mine) return;
+    // values that are not finite were staged as zeros: what is multiplied with one that it sees is NaN.  (Looked for here, once more over
+    // all of this piece's tokens, only where there was one at all.)
+    uint32_t poison = 0;
+    if (__builtin_expect(odd, 0)) {
+#pragma unroll 1
+        for (int k = tile_from; k < tile_to; ++k) poison |= values_not_finite(a, table, tile_at(k), min(v.end, tile_at(k) + kManyTile), position, w.head);
+    }
     // four consecutive elements of a result at a time
-    const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int from_held = exponent[1] - 127 - kHeldBits;
+    const float by = w.pieces > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     float *part = a.partial + ((long long)(w.slot + w.piece) * kRowsOfMany + 32 * wave + column) * (DP + 2);
     const long long at = (long long)my_token * a.out_token + (long long)my_head * a.out_head;
     if (w.pieces > 1 && half == 0) part[0] = best, part[1] = sum;
@@ -323,8 +469,10 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
             const int element = 32 * d + 2 * i + 4 * half;
             float y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                y[e] = __builtin_amdgcn_ldexpf(w.pieces > 1 ? result[d][i + e] : result[d][i + e] * by, exponent - 138) + poison[UNITS == 1 ? 0 : d / 2];
+            for (int e = 0; e < 4; ++e) {
+                y[e] = __builtin_amdgcn_ldexpf(result[d][i + e] * by, from_held);
+                if (poison >> (d / 2) & 1) y[e] = __builtin_nanf("");
+            }
             if (w.pieces > 1) {
                 *(float2 *)(part + 2 + element) = make_float2(y[0], y[1]);
                 *(float2 *)(part + 4 + element) = make_float2(y[2], y[3]);
@@ -344,8 +492,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
 template <int DP>
 void launch_many(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream) {
     const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u));
-    if (DP == 64 || a.shape.segments == 1) hipLaunchKernelGGL((attend_many_kernel<DP, 1>), grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attend_many_kernel<DP, DP / 64>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(attend_many_kernel<DP>, grid, dim3(256), 0, stream, a);
     if (may_cut)
         hipLaunchKernelGGL((attend_join_kernel<kRowsOfMany, kManyShift, DP, true>), dim3(rows_of_tiles, kRowsOfMany), dim3(256), 0, stream, a);
 }
