@@ -266,66 +266,6 @@ __device__ __forceinline__ int swap_of(int row) {
     return DP == 64 ? (row >> 3) & 1 : DP == 128 ? (row >> 2) & 3 : (row >> 1) & 7;
 }
 
-// Joins the pieces of every row of tiles that was cut, a workgroup for each of its rows: what the pieces count for first, then a
-// share of them per group of DP / 4 threads.
-template <int ROWS, int SHIFT, int DP, bool BF16>
-__global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
-    constexpr int kGroups = 1024 / DP;
-    __shared__ float s_share[256];
-    __shared__ float s_reduce[4], s_total[4];
-    __shared__ f32x4 s_part[256];
-    AttendWork w;
-    if (!find_work<ROWS, SHIFT, false>(a, blockIdx.x, w) || w.pieces == 1) return;
-    const SequenceView v = view_sequence<SHIFT>(a, w.b);
-    const int rows = v.count * a.group, row = first_row_of<ROWS>(rows, w.row_tile) + blockIdx.y;
-    if (row >= rows) return;
-    constexpr int kNext = ROWS * (DP + 2);
-    const float *part = a.partial + (long long)w.slot * kNext + blockIdx.y * (DP + 2);
-    const int wave = threadIdx.x >> 6;
-    float top = -__builtin_inff();
-    for (int i = threadIdx.x; i < w.pieces; i += 256) top = fmaxf(top, part[(long long)i * kNext]);
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    if ((threadIdx.x & 63) == 0) s_reduce[wave] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_reduce[0], s_reduce[1]), fmaxf(s_reduce[2], s_reduce[3]));
-    const float zero = top == -__builtin_inff() ? 0.0f : top;
-    const int group = threadIdx.x / (DP / 4), d = threadIdx.x % (DP / 4) * 4;
-    float total = 0.0f;
-    f32x4 y = {0.f, 0.f, 0.f, 0.f};
-    for (int first = 0; first < w.pieces; first += 256) {
-        const int i = first + (int)threadIdx.x, count = min(256, w.pieces - first);
-        __syncthreads();
-        float share = 0.0f;
-        if (i < w.pieces) {
-            share = __builtin_amdgcn_exp2f(part[(long long)i * kNext] - zero);
-            total += part[(long long)i * kNext + 1] * share;
-        }
-        s_share[threadIdx.x] = share;
-        __syncthreads();
-#pragma unroll 4
-        for (int j = group; j < count; j += kGroups) {
-            const float2 *p = (const float2 *)(part + (long long)(first + j) * kNext + 2 + d);
-            const float2 u = p[0], v2 = p[1];
-            const float by = s_share[j];
-            y += (f32x4){u.x * by, u.y * by, v2.x * by, v2.y * by};
-        }
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-    if ((threadIdx.x & 63) == 0) s_total[wave] = total;
-    s_part[threadIdx.x] = y;
-    __syncthreads();
-    total = (s_total[0] + s_total[1]) + (s_total[2] + s_total[3]);
-    if (group != 0) return;
-#pragma unroll
-    for (int i = 1; i < kGroups; ++i) y += s_part[threadIdx.x + i * (DP / 4)];
-    const long long at = (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (d + e < a.shape.head_dim) store_result<BF16>(a, at + d + e, total == 0.0f ? 0.0f : y[e] / total);
-}
-
 #endif  // __HIPCC__
 
 }  // namespace qt

@@ -489,12 +489,48 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         }
 }
 
+// Joins the pieces of every row of tiles that was cut: a wave per query, eight of them one after the other.
+constexpr int kJoinRows = 32;
+template <int DP>
+__global__ __launch_bounds__(256) void attend_join_many_kernel(const AttendArgs a) {
+    AttendWork w;
+    if (!find_work<kRowsOfMany, kManyShift, false>(a, blockIdx.x, w) || w.pieces == 1) return;
+    const SequenceView v = view_sequence<kManyShift>(a, w.b);
+    const int rows = v.count * a.group, first = first_row_of<kRowsOfMany>(rows, w.row_tile) + kJoinRows * blockIdx.y;
+    const int d = (threadIdx.x & 63) * 4;
+    constexpr int kNext = kRowsOfMany * (DP + 2);
+    for (int r = threadIdx.x >> 6; r < kJoinRows && first + r < rows; r += 4) {
+        const float *part = a.partial + (long long)w.slot * kNext + (kJoinRows * blockIdx.y + r) * (DP + 2);
+        float top = -__builtin_inff();
+#pragma unroll 4
+        for (int i = 0; i < w.pieces; ++i) top = fmaxf(top, part[(long long)i * kNext]);
+        const float zero = top == -__builtin_inff() ? 0.0f : top;
+        float total = 0.0f;
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+        for (int i = 0; i < w.pieces; ++i) {
+            const float *p = part + (long long)i * kNext;
+            const float by = __builtin_amdgcn_exp2f(p[0] - zero);
+            total += p[1] * by;
+            if (d < DP) {
+                const float2 low = *(const float2 *)(p + 2 + d), high = *(const float2 *)(p + 4 + d);
+                y += (f32x4){low.x * by, low.y * by, high.x * by, high.y * by};
+            }
+        }
+        const int row = first + r;
+        const long long at = (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < a.shape.head_dim) store_result<true>(a, at + d + e, total == 0.0f ? 0.0f : y[e] / total);
+    }
+}
+
 template <int DP>
 void launch_many(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream) {
     const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u));
     hipLaunchKernelGGL(attend_many_kernel<DP>, grid, dim3(256), 0, stream, a);
     if (may_cut)
-        hipLaunchKernelGGL((attend_join_kernel<kRowsOfMany, kManyShift, DP, true>), dim3(rows_of_tiles, kRowsOfMany), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL(attend_join_many_kernel<DP>, dim3(rows_of_tiles, kRowsOfMany / kJoinRows), dim3(256), 0, stream, a);
 }
 
 }  // namespace
