@@ -49,6 +49,9 @@ constexpr int few_waves(int dim, int units, bool bf16) { return dim == 256 || (u
 template <int DP, int UNITS, bool BF16>
 __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_kernel(const AttendArgs a) {
     constexpr int kPieces = BF16 ? 3 : 5;
+    // One or two rows of tiles read the cache: past the L2 (two sequences of 131072 tokens 58.8 -> 52.9 us).  Queries in 32 bits come in any number
+    // and read it again for every sixteen (4 x 2048 of them 1669 us, 1719 past the L2).
+    constexpr bool kOnce = BF16;
     constexpr int kHalves = DP == 256 ? 2 : 1;              // 16-byte chunks of a row that a lane holds
     constexpr int kLoads = DP == 64 ? 4 : 8;                // loads of sixteen tokens by all lanes (thirty-two for rows of 32 bytes)
     constexpr int kRowBytes = DP / 2;                       // of a token's values in LDS; the 16-byte chunks of a row stand in an order of
@@ -128,7 +131,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
         for (int t = 0; t < kLoads; ++t) {
             const long long at = DP == 64 ? (lane < 32 ? line_of(safe, base, 2 * t) : line_of(safe, base, 2 * t + 1)) : line_of(safe, base, t);
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) keys[h][t] = *(const i32x4 *)(a.codes[0] + at + inside[h]);
+            for (int h = 0; h < kHalves; ++h) keys[h][t] = kOnce ? __builtin_nontemporal_load((const i32x4 *)(a.codes[0] + at + inside[h])) : *(const i32x4 *)(a.codes[0] + at + inside[h]);
         }
     };
     // values of a tile whose pages `safe` has, from memory to LDS: lane i of a load fills bytes 16 i of a kilobyte
@@ -140,7 +143,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
             if (DP == 64) from = a.codes[1] + (lane < 32 ? line_of(safe, base, 2 * t) : line_of(safe, base, 2 * t + 1)) + value_inside[0];
             else if (DP == 128) from = a.codes[1] + line_of(safe, base, t) + value_inside[0];
             else from = a.codes[1] + line_of(safe, base, t >> 1) + value_inside[t & 1];
-            __builtin_amdgcn_global_load_lds((const QT_GLOBAL void *)from, (QT_LDS void *)(s_values + 1024 * t), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const QT_GLOBAL void *)from, (QT_LDS void *)(s_values + 1024 * t), 16, 0, kOnce ? 2 : 0);
         }
     };
 
