@@ -26,7 +26,7 @@ struct AttendArgs {
 };
 
 // Pieces of rows of tiles that were cut, at most (see find_work).
-constexpr int attend_places(int slots) { return slots + slots / 2; }
+constexpr int attend_places(int slots) { return 2 * slots; }
 
 constexpr int attend_dim(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 
@@ -155,22 +155,27 @@ __device__ __forceinline__ int first_row_of(int rows, int row_tile) {
     return (ROWS == kRowsOfMany ? (rows + ROWS - 1) / ROWS - 1 - row_tile : row_tile) * ROWS;
 }
 
+// Pieces of a row of `tiles` tiles: of up to one and a half times `most`, as half a piece is not worth its part in the join; but where
+// units would stay idle (`most` is the least), of no more than that.
+__device__ __forceinline__ int pieces_of(const AttendArgs &a, int tiles, int most) { return max(1, (tiles + (most > a.least ? most / 2 : most - 1)) / most); }
+
 // How a kernel's work is cut: a row of tiles (a sequence, a head of the cache, ROWS queries) into pieces of about as many tiles as all the work
-// has per slot (of up to one and a half times as many: half a piece is not worth a join).  Finds the `index`th piece (BY_PIECE) or the
-// first piece of the `index`th row of tiles; false beyond the last.  Every wave works it out for itself, a sequence per lane.
+// has per slot.  Finds the `index`th piece (BY_PIECE) or the first piece of the `index`th row of tiles; false beyond the last.  Every wave
+// works it out for itself, a sequence per lane.
 //
-// Pieces behind the first of a row are at most tiles / most, so there are no more than slots of them, and rows that are cut have at most 4/3 slots
-// pieces in all; `most` may round below the exact quotient by a few 2^-24 (a sum in fp32), and a row whose partial results would lie
-// behind the workspace's places (slots and a half) is refused below, whatever the lengths say.
+// Pieces behind the first of a row are at most tiles / most, so there are no more than slots of them; and rows that are cut have fewer than 2 tiles /
+// most pieces each, fewer than 2 slots in all.  `most` may round below the exact quotient by a few 2^-24 (a sum in fp32): a row whose
+// partial results would lie behind the workspace's places (two per slot) is refused below, whatever the lengths say.
 template <int ROWS, int SHIFT, bool BY_PIECE>
-__device__ __forceinline__ bool find_work(const AttendArgs &a, uint32_t index, AttendWork &w) {
+__device__ __forceinline__ bool find_work(const AttendArgs &a, uint32_t index, AttendWork &w, SequenceView &v) {
     const int lane = threadIdx.x & 63;
+    const bool few = a.at.batch <= 64;          // (every lane keeps its only sequence)
+    SequenceView mine = {};
     float all = 0.0f;
     for (int first = 0; first < a.at.batch; first += 64) {
-        const int b = first + lane;
-        if (b < a.at.batch) {
-            const SequenceView v = view_sequence<SHIFT>(a, b);
-            all += (float)(row_tiles<ROWS>(a, v) * a.shape.kv_heads) * (float)v.tiles;
+        if (first + lane < a.at.batch) {
+            mine = view_sequence<SHIFT>(a, first + lane);
+            all += (float)(row_tiles<ROWS>(a, mine) * a.shape.kv_heads) * (float)mine.tiles;
         }
     }
 #pragma unroll
@@ -178,28 +183,30 @@ __device__ __forceinline__ bool find_work(const AttendArgs &a, uint32_t index, A
     const int most = max(a.least, (int)min(ceilf(all / (float)a.slots), 1.0e9f));
     uint32_t before = 0, partial = 0;           // pieces or rows of tiles, and partial results, of the sequences before
     for (int first = 0; first < a.at.batch; first += 64) {
-        const int b = first + lane;
-        int items = 0, pieces = 1, tiles = 0;
-        if (b < a.at.batch) {
-            const SequenceView v = view_sequence<SHIFT>(a, b);
-            items = row_tiles<ROWS>(a, v) * a.shape.kv_heads;
-            tiles = v.tiles;
-            pieces = max(1, (tiles + most / 2) / most);
+        int items = 0, pieces = 1;
+        if (first + lane < a.at.batch) {
+            if (!few) mine = view_sequence<SHIFT>(a, first + lane);
+            items = row_tiles<ROWS>(a, mine) * a.shape.kv_heads;
+            pieces = pieces_of(a, mine.tiles, most);
         }
-        const uint32_t mine = (uint32_t)(BY_PIECE ? items * pieces : items), parts = pieces > 1 ? (uint32_t)(items * pieces) : 0u;
-        const uint32_t upto = before + wave_scan(mine), parts_upto = partial + wave_scan(parts);
+        const uint32_t here = (uint32_t)(BY_PIECE ? items * pieces : items), parts = pieces > 1 ? (uint32_t)(items * pieces) : 0u;
+        const uint32_t upto = before + wave_scan(here), parts_upto = partial + wave_scan(parts);
         const unsigned long long at = __ballot(index < upto);
         if (at) {
             const int found = __builtin_ctzll(at);
-            const uint32_t from = __builtin_amdgcn_readlane(upto - mine, found);
+            const uint32_t from = __builtin_amdgcn_readlane(upto - here, found);
+            v.start = __builtin_amdgcn_readlane(mine.start, found), v.count = __builtin_amdgcn_readlane(mine.count, found);
+            v.first_position = __builtin_amdgcn_readlane(mine.first_position, found), v.end = __builtin_amdgcn_readlane(mine.end, found);
+            v.sink_tiles = __builtin_amdgcn_readlane(mine.sink_tiles, found), v.first_tile = __builtin_amdgcn_readlane(mine.first_tile, found);
+            v.tiles = __builtin_amdgcn_readlane(mine.tiles, found);
             w.b = first + found;
             w.pieces = __builtin_amdgcn_readlane(pieces, found);
-            const int total_tiles = __builtin_amdgcn_readlane(tiles, found), local = (int)(index - from), item = BY_PIECE ? local / w.pieces : local;
+            const int local = (int)(index - from), item = BY_PIECE ? local / w.pieces : local;
             w.row_tile = item / a.shape.kv_heads;
             w.head = item - w.row_tile * a.shape.kv_heads;
             w.piece = BY_PIECE ? local - item * w.pieces : 0;
             w.slot = (int)__builtin_amdgcn_readlane(parts_upto - parts, found) + item * w.pieces;
-            w.per_piece = (total_tiles + w.pieces - 1) / w.pieces;
+            w.per_piece = (v.tiles + w.pieces - 1) / w.pieces;
             return w.pieces == 1 || (w.slot >= 0 && w.slot + w.pieces <= attend_places(a.slots));
         }
         before = __builtin_amdgcn_readlane(upto, 63);

@@ -63,9 +63,9 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     __shared__ float s_best[4][kRows], s_sum[4][kRows];
 
     AttendWork w;
-    if (!find_work<kRows, 7, true>(a, blockIdx.x, w)) return;
+    SequenceView v;
+    if (!find_work<kRows, 7, true>(a, blockIdx.x, w, v)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
-    const SequenceView v = view_sequence<7>(a, w.b);
     const int rows = min(kRows, v.count * a.group - w.row_tile * kRows);
     const int first_row = first_row_of<kRows>(0, w.row_tile);
     uint8_t *s_values = s_area[wave];
@@ -374,8 +374,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
     __shared__ float s_reduce[4], s_total[4];
     __shared__ f32x4 s_part[256];
     AttendWork w;
-    if (!find_work<kRows, 7, false>(a, blockIdx.x, w) || w.pieces == 1) return;
-    const SequenceView v = view_sequence<7>(a, w.b);
+    SequenceView v;
+    if (!find_work<kRows, 7, false>(a, blockIdx.x, w, v) || w.pieces == 1) return;
     const int rows = v.count * a.group, row = first_row_of<kRows>(rows, w.row_tile) + blockIdx.y;
     if (row >= rows) return;
     constexpr int kNext = kRows * (DP + 2);

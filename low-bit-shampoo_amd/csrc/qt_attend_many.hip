@@ -89,9 +89,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                                                         // scale of a value is not finite; bit 2: a token's page is not there
 
     AttendWork w;
-    if (!find_work<kRowsOfMany, kManyShift, true>(a, blockIdx.x, w)) return;
+    SequenceView v;
+    if (!find_work<kRowsOfMany, kManyShift, true>(a, blockIdx.x, w, v)) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
-    SequenceView v = view_sequence<kManyShift>(a, w.b);
     const int all_rows = v.count * a.group;
     const int first_row = first_row_of<kRowsOfMany>(all_rows, w.row_tile);
     const int my_row = min(first_row + 32 * wave + column, all_rows - 1);
@@ -494,8 +494,8 @@ constexpr int kJoinRows = 32;
 template <int DP>
 __global__ __launch_bounds__(256) void attend_join_many_kernel(const AttendArgs a) {
     AttendWork w;
-    if (!find_work<kRowsOfMany, kManyShift, false>(a, blockIdx.x, w) || w.pieces == 1) return;
-    const SequenceView v = view_sequence<kManyShift>(a, w.b);
+    SequenceView v;
+    if (!find_work<kRowsOfMany, kManyShift, false>(a, blockIdx.x, w, v) || w.pieces == 1) return;
     const int rows = v.count * a.group, first = first_row_of<kRowsOfMany>(rows, w.row_tile) + kJoinRows * blockIdx.y;
     const int d = (threadIdx.x & 63) * 4;
     constexpr int kNext = kRowsOfMany * (DP + 2);
