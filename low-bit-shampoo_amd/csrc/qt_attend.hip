@@ -158,6 +158,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     auto step = [&](int k, auto more) {
         const int base = tile_at(k);
         const unsigned long long here[2] = {valid[0], valid[1]};
+        // (a scale that is not finite makes every score NaN: the sums are zero only to 2^-127 of another token's where a load holds two)
         // what no page holds has scale 0; a weight of zero times a scale that is not finite is not zero: only then such weights are looked for
         float by_key[UNITS][2], by_value[UNITS][2], odd_scale = 0.0f;
 #pragma unroll
@@ -165,7 +166,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const bool there = (here[i] >> lane) & 1;
-                by_key[u][i] = there ? key_scale[u][i] * a.factor : 0.0f;
+                by_key[u][i] = there ? __builtin_fmaf(key_scale[u][i], 0.0f, key_scale[u][i] * a.factor) : 0.0f;
                 by_value[u][i] = there ? value_scale[u][i] : 0.0f;
                 odd_scale += 0.0f * by_value[u][i];
             }

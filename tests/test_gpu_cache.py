@@ -277,6 +277,25 @@ def test_nan_in_a_token_that_is_seen_reaches_only_its_head(Cache):
     assert torch.equal(after[0, :2], before[0, :2]) and torch.equal(after[1], before[1])
 
 
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (33, 64), (128, 64), (128, 128), (256, 64), (256, 256)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_infinite_keys_are_nan_to_every_query_that_sees_them(Cache, dim, blocksize, dtype):
+    """A key's segment with an infinity stands for NaN, whatever the tokens beside it hold."""
+    cache, table, lens, _ = made(Cache, [50], None, 1, dim, 16, blocksize)
+    (k, v), = fill(cache, table, lens, dtype, 98)
+    k[::7, 0, 0], starts = math.inf, torch.tensor([0, 50], dtype=torch.int32).cuda()
+    cache.write(k.cuda(), v.cuda(), table, lens, starts)
+    for new in (1, 8):
+        for seed in range(5):
+            q = tokens(new, 2, dim, dtype, 200 + seed).cuda()
+            at = torch.tensor([0, new], dtype=torch.int32).cuda()
+            assert torch.isnan(cache.attend(q, table, lens, at)).all()
+            see = cache.attend(q[-1:], table, lens, window=1)
+            assert torch.isnan(see).all() if 49 % 7 == 0 else torch.isfinite(see).all()
+    lens -= 1
+    assert torch.isfinite(cache.attend(q[-1:], table, lens, window=6)).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_pages_that_are_not_there(Cache, dtype):
     """Pages marked -1 or beyond the cache, and lengths beyond the table: not written, zeros, not seen."""
