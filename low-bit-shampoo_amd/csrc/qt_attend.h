@@ -14,7 +14,7 @@ struct AttendArgs {
     const void *q;
     void *out;
     long long q_token, q_head, out_token, out_head;
-    int heads, group;
+    int group;              // query heads that share one of the cache
     int q_in_eights;        // not 0: eight elements of a query from a multiple of eight on are there together, and aligned to 16 bytes
     float factor;           // scale * log2 e
     int window, sinks;      // window 0: no window

@@ -13,10 +13,17 @@ namespace {
 
 constexpr int kTile = 128;              // tokens a wave takes at a time: one step of k of a matrix instruction with the weights
 constexpr int kRows = 16;               // queries (of all heads that share a head of the cache) in a tile of rows
-constexpr int kFewRows = 32;            // queries of a sequence that are still few: two rows of tiles
-constexpr int kLeastTiles = 4;          // tiles of a piece: one for each wave
-constexpr int kWholeTiles = 12;         // a call whose sequences have no more tiles than that is not cut: three rounds of the waves take less
-                                        // time than two and a launch that joins pieces
+// Queries of a sequence that are still few: two rows of tiles.  (32 sequences of 4000 tokens and 4 heads of the cache, 32 / 64 / 96 queries
+// each: 47 / 63 / 91 us here, 74 / 66 / 69 by the kernel for many.)
+constexpr int kFewRows = 32;
+// Pairs of a query and a token (of a head of the cache) up to which all of a call is taken to be few: 8 sequences of 2000 tokens, 4 heads and
+// 32 queries each (2 * 10^6) 16 us, 22 with the kernel for many launched beside it; 1 of 16000 with 64 (4 * 10^6) 12 and 35; 32 of 500 with
+// 256 (16 * 10^6) 39 and 26.
+constexpr double kFewWork = 8388608.0;
+constexpr int kLeastTiles = 4;          // tiles of a piece: one for each wave (4 sequences of 2500 tokens 13.2 us; in pieces of 8 15.8)
+// A call whose sequences have no more tiles than that is not cut: three rounds of the waves take less time than two and a launch that joins
+// pieces (32 sequences of 1500 tokens 14.7 us, 16.8 if they are cut; of 1700 17.9 and 16.7).
+constexpr int kWholeTiles = 12;
 
 // Of the tokens 16 t + i of a lane (t < 8, i < 4; bit 4 t + i), those up to x.
 __device__ __forceinline__ uint32_t tokens_up_to(int x) {
@@ -477,15 +484,13 @@ extern "C" void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtens
     for (int i = 0; i < 2; ++i) a.codes[i] = cache->codes[i], a.scales[i] = cache->scales[i];
     a.q = q->base, a.q_token = q->token_stride, a.q_head = q->head_stride;
     a.out = out->base, a.out_token = out->token_stride, a.out_head = out->head_stride;
-    a.heads = heads, a.group = heads / a.shape.kv_heads;
+    a.group = heads / a.shape.kv_heads;
     a.q_in_eights = q->is_bf16 && is_aligned(q->base, 16) && q->token_stride % 8 == 0 && q->head_stride % 8 == 0 && a.shape.head_dim % 8 == 0;
     a.factor = scale * 1.4426950408889634f;
     a.window = window, a.sinks = sinks;
     a.partial = (float *)workspace;
     const bool bf16 = q->is_bf16 != 0, ragged = a.at.starts != nullptr;
     const int dim = attend_dim(a.shape.head_dim);
-    // queries in 32 bits are all the kernel for few's: it has pieces enough for them
-    a.few_rows = bf16 ? kFewRows : 0x7fffffff;
     const long long rows = (long long)a.at.tokens * a.group, batch = a.at.batch;
     if (rows >= (1LL << 31) || (rows / kRows + batch) * a.shape.kv_heads >= (1LL << 30)) {
         set_error(kBadArgument, "cache_attend: %d tokens are too many for one call", a.at.tokens);
@@ -497,20 +502,26 @@ extern "C" void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtens
     }
     const hipStream_t stream = (hipStream_t)stream_v;
     const long long held = (long long)a.at.table_pages << a.shape.page_shift;        // most tokens of a sequence
-    if (bf16 && (ragged ? rows : (long long)a.group) > kFewRows) {
+    // Queries in 32 bits are all the kernel for few's, which has pieces enough for them; and all of a call that is too little work for a second
+    // pair of launches (kFewWork).
+    const bool few_alone = !bf16 || (double)rows * a.shape.kv_heads * (double)held <= kFewWork;
+    a.few_rows = few_alone ? 0x7fffffff : kFewRows;
+    if (!few_alone && (ragged ? rows : (long long)a.group) > kFewRows) {
         const long long rows_of_tiles = a.shape.kv_heads * (ragged ? rows / kRowsOfMany + batch : batch * ((a.group + kRowsOfMany - 1) / kRowsOfMany));
         AttendArgs many = a;
         many.slots = attend_many_slots(dim);
-        launch_attend_many(many, (unsigned)rows_of_tiles, held > 1024 && rows_of_tiles < 4LL * many.slots, stream);
+        // (not cut where whole rows of tiles keep every unit busy: 4 sequences of 4000 tokens, 4 heads, 4000 queries of each, 147 us, 151 with the
+        // launch that joins; nor short ones: 32 of 700 tokens with 256 queries 31 us, cut 51)
+        launch_attend_many(many, (unsigned)rows_of_tiles, held > 1024 && rows_of_tiles < many.slots, stream);
     }
-    if (!bf16 || ragged || a.group <= kFewRows) {
+    if (few_alone || ragged || a.group <= kFewRows) {
         // rows of tiles: at most one more per sequence than full ones, and no more per sequence than few queries have
         long long rows_of_tiles = ragged ? rows / kRows + batch : batch * ((a.group + kRows - 1) / kRows);
-        if (bf16) rows_of_tiles = rows_of_tiles < batch * (kFewRows / kRows) ? rows_of_tiles : batch * (kFewRows / kRows);
+        if (!few_alone) rows_of_tiles = rows_of_tiles < batch * (kFewRows / kRows) ? rows_of_tiles : batch * (kFewRows / kRows);
         long long tiles = (held + kTile - 1) / kTile;
         if (window) {
             const long long seen = ((long long)window + (ragged ? kFewRows : 1) + kTile - 2) / kTile + 1 + ((long long)sinks + kTile - 1) / kTile;
-            if ((bf16 || !ragged) && seen < tiles) tiles = seen;
+            if ((!few_alone || !ragged) && seen < tiles) tiles = seen;
         }
         const bool may_cut = tiles > kWholeTiles;
         a.slots = few_slots(dim, a.shape.segments, bf16);

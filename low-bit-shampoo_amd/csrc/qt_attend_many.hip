@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kManyTile = 64;
 constexpr int kManyShift = 6;
-constexpr int kManyLeast = 8;           // tiles of a piece, at least
+constexpr int kManyLeast = 4;           // tiles of a piece, at least
 constexpr float kWeightBits = 11.0f;    // weights are kept times 2^11 ...
 constexpr float kSlack = 4.0f;          // ... and the running maximum may lag behind by 4: below 2^15 in fp16
 // Keys and values whose scale has the largest exponent so far are held times 2^3; larger ones of up to 2^9 times that still fit (6 * 2 *
@@ -100,6 +100,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const int position = v.first_position + my_row / a.group;
     const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;
     // positions of this wave's queries and of all of the workgroup's
+    const int seen_from = a.window ? max(0, v.first_position + first_row / a.group - (a.window - 1)) : 0;        // (by any, sinks aside)
     const int lowest = v.first_position + min(first_row + 32 * wave, all_rows - 1) / a.group;
     const int highest = v.first_position + min(first_row + 32 * wave + 31, all_rows - 1) / a.group;
     {
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
             const int token = base + stage_row(i);
             int p = __builtin_amdgcn_readfirstlane(page[i]);
             if (DP == 64) p = lane < 32 ? p : __builtin_amdgcn_readfirstlane(page[kPages - 1]);
-            there[i] = (unsigned)p < (unsigned)a.shape.pages && token < v.end;
+            there[i] = (unsigned)p < (unsigned)a.shape.pages && token < v.end && (token >= seen_from || token < a.sinks);
             hole[i] = (unsigned)p >= (unsigned)a.shape.pages && token < v.end;
             const long long line = ((long long)((unsigned)p < (unsigned)a.shape.pages ? p : 0) * a.shape.kv_heads + w.head) << a.shape.page_shift;
             const long long code_at = line * a.shape.row_bytes, scale_at = line * a.shape.segments;
@@ -489,34 +490,48 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         }
 }
 
-// Joins the pieces of every row of tiles that was cut: a wave per query, eight of them one after the other.
-constexpr int kJoinRows = 32;
+// Joins the pieces of every row of tiles that was cut, a wave per query: what the pieces count for first, a piece per lane, then a share of
+// them per group of DP / 4 lanes.  Reads each partial result once; bound by the latency of dependent loads, so the queries of a row
+// of tiles are spread over as many workgroups (gridDim.y) as fill the device, each of which has to find its work first.
 template <int DP>
 __global__ __launch_bounds__(256) void attend_join_many_kernel(const AttendArgs a) {
+    constexpr int kGroups = 256 / DP, kNext = kRowsOfMany * (DP + 2);
     AttendWork w;
     SequenceView v;
     if (!find_work<kRowsOfMany, kManyShift, false>(a, blockIdx.x, w, v) || w.pieces == 1) return;
-    const int rows = v.count * a.group, first = first_row_of<kRowsOfMany>(rows, w.row_tile) + kJoinRows * blockIdx.y;
-    const int d = (threadIdx.x & 63) * 4;
-    constexpr int kNext = kRowsOfMany * (DP + 2);
-    for (int r = threadIdx.x >> 6; r < kJoinRows && first + r < rows; r += 4) {
-        const float *part = a.partial + (long long)w.slot * kNext + (kJoinRows * blockIdx.y + r) * (DP + 2);
-        float top = -__builtin_inff();
-#pragma unroll 4
-        for (int i = 0; i < w.pieces; ++i) top = fmaxf(top, part[(long long)i * kNext]);
+    const int rows = v.count * a.group, first = first_row_of<kRowsOfMany>(rows, w.row_tile), each = kRowsOfMany / gridDim.y;
+    const int lane = threadIdx.x & 63, group = lane / (DP / 4), d = lane % (DP / 4) * 4;
+    for (int r = blockIdx.y * each + (threadIdx.x >> 6); r < (int)(blockIdx.y + 1) * each && first + r < rows; r += 4) {
+        const float *part = a.partial + (long long)w.slot * kNext + r * (DP + 2);
+        float top = -__builtin_inff(), total = 0.0f;
+        for (int i = lane; i < w.pieces; i += 64) top = fmaxf(top, part[(long long)i * kNext]);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
         const float zero = top == -__builtin_inff() ? 0.0f : top;
-        float total = 0.0f;
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int i = 0; i < w.pieces; ++i) {
-            const float *p = part + (long long)i * kNext;
-            const float by = __builtin_amdgcn_exp2f(p[0] - zero);
-            total += p[1] * by;
-            if (d < DP) {
-                const float2 low = *(const float2 *)(p + 2 + d), high = *(const float2 *)(p + 4 + d);
-                y += (f32x4){low.x * by, low.y * by, high.x * by, high.y * by};
+        for (int from = 0; from < w.pieces; from += 64) {
+            const int count = min(64, w.pieces - from);
+            float share = 0.0f;
+            if (lane < count) {
+                const float *p = part + (long long)(from + lane) * kNext;
+                share = __builtin_amdgcn_exp2f(p[0] - zero);
+                total += p[1] * share;
+            }
+            for (int i = 0; i < count; i += kGroups) {
+                const int piece = min(i + group, count - 1);
+                const float by = __shfl(share, i + group, 64);
+                const float2 *p = (const float2 *)(part + (long long)(from + piece) * kNext + 2 + d);
+                const float2 low = p[0], high = p[1];
+                if (i + group < count) y += (f32x4){low.x * by, low.y * by, high.x * by, high.y * by};
             }
         }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+#pragma unroll
+        for (int off = DP / 4; off < 64; off <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += __shfl_xor(y[e], off, 64);
+        if (group != 0) continue;
         const int row = first + r;
         const long long at = (long long)(v.start + row / a.group) * a.out_token + (long long)(w.head * a.group + row % a.group) * a.out_head;
 #pragma unroll
@@ -529,8 +544,10 @@ template <int DP>
 void launch_many(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream) {
     const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u));
     hipLaunchKernelGGL(attend_many_kernel<DP>, grid, dim3(256), 0, stream, a);
-    if (may_cut)
-        hipLaunchKernelGGL(attend_join_many_kernel<DP>, dim3(rows_of_tiles, kRowsOfMany / kJoinRows), dim3(256), 0, stream, a);
+    if (!may_cut) return;
+    unsigned parts = 32;                // a workgroup per four queries, or fewer where there are rows of tiles enough
+    while (parts > 4 && rows_of_tiles * parts > 2048) parts /= 2;
+    hipLaunchKernelGGL(attend_join_many_kernel<DP>, dim3(rows_of_tiles, parts), dim3(256), 0, stream, a);
 }
 
 }  // namespace

@@ -46,21 +46,6 @@ __device__ __forceinline__ int sequence_of_block(const CachePlaces &at, int toke
     }
     return b;
 }
-
-// Row of `position` of sequence b among all rows of one head (page * page_size + offset), or -1 where the table has no page for it.
-__device__ __forceinline__ long long cache_row(const CacheShape &s, const CachePlaces &at, int b, int position, int head) {
-    const int nth = position >> s.page_shift;
-    if (position < 0 || nth >= at.table_pages) return -1;
-    const int page = at.table[b * at.table_stride + nth];
-    if ((unsigned)page >= (unsigned)s.pages) return -1;
-    return ((((long long)page * s.kv_heads + head) << s.page_shift)) + (position & ((1 << s.page_shift) - 1));
-}
-
-// Where the scale of segment 0 of that row lies; segment i is i << page_shift further on.
-__device__ __forceinline__ long long cache_scale_at(const CacheShape &s, long long row) {
-    const long long inside = row & ((1 << s.page_shift) - 1);
-    return (row - inside) * s.segments + inside;
-}
 #endif  // __HIPCC__
 
 }  // namespace qt

@@ -213,9 +213,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheC
     }
 }
 
-// The reverse; tokens that the cache does not have come out as zeros.  STREAM: the result is more than the caches
-// hold and goes past them.
-template <bool BF16, int HEADS, bool STREAM>
+// The reverse; tokens that the cache does not have come out as zeros.  Large results (of four heads a thread) go past the caches.
+template <bool BF16, int HEADS>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCopy a) {
     CacheThread t = cache_thread<BF16>(a);
     const int first_head = blockIdx.y * HEADS;
@@ -249,7 +248,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCo
             QT_EACH(0) QT_EACH(1)
             if constexpr (BF16) { QT_EACH(2) QT_EACH(3) }
 #undef QT_EACH
-            store_lane<BF16, STREAM>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.first,
+            store_lane<BF16, (HEADS > 1)>(a.vectors.base[i], t.token * a.vectors.token_stride[i] + (first_head + n) * a.vectors.head_stride[i] + t.first,
                                      t.valid, x);
         }
     }
@@ -257,16 +256,17 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(const CacheCo
 
 template <bool BF16>
 void launch_copy(bool write, const CacheCopy &a, hipStream_t stream) {
-    // several heads a thread where there are workgroups enough for every unit: their loads wait together
+    // Several heads a thread where there are workgroups enough for every unit: their loads wait together.  Keys of 2^22 / 2^23 / 2^26 elements
+    // in bf16: one head 7.2 / 12.7 / 82 us written, 7.6 / 11.7 / 115 read; four 7.7 / 11.5 / 66 and, results past the caches, 7.1 /
+    // 8.6 / 54 (of 2^21, read: 5.6 with one, 6.9 with four).
     const long long elements = (long long)a.at.tokens * a.shape.kv_heads * a.shape.head_dim;
-    const bool large = elements >= 1 << 22;
+    const bool large = elements >= (write ? 1 << 23 : 1 << 22);
     const unsigned blocks = (unsigned)((a.at.tokens + a.block_tokens - 1) / a.block_tokens), heads = (unsigned)a.shape.kv_heads;
     const dim3 one(blocks, heads), few(blocks, (heads + 3) / 4);
     if (write && large) hipLaunchKernelGGL((cache_write_kernel<BF16, 4>), few, dim3(kCacheThreads), 0, stream, a);
     else if (write) hipLaunchKernelGGL((cache_write_kernel<BF16, 1>), one, dim3(kCacheThreads), 0, stream, a);
-    else if (elements >= 1 << 25) hipLaunchKernelGGL((cache_read_kernel<BF16, 4, true>), few, dim3(kCacheThreads), 0, stream, a);
-    else if (large) hipLaunchKernelGGL((cache_read_kernel<BF16, 4, false>), few, dim3(kCacheThreads), 0, stream, a);
-    else hipLaunchKernelGGL((cache_read_kernel<BF16, 1, false>), one, dim3(kCacheThreads), 0, stream, a);
+    else if (large) hipLaunchKernelGGL((cache_read_kernel<BF16, 4>), few, dim3(kCacheThreads), 0, stream, a);
+    else hipLaunchKernelGGL((cache_read_kernel<BF16, 1>), one, dim3(kCacheThreads), 0, stream, a);
 }
 
 void copy_cache(const char *what, bool write, const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *keys,

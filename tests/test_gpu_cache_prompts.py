@@ -22,6 +22,18 @@ def Cache():
     return QTensorCache
 
 
+@pytest.fixture(params=["little", "much"], autouse=True)
+def room(request):
+    """How calls are taken depends on the tokens that the table has room for: with much of it, many queries go their own way."""
+    prepared.room = 0 if request.param == "little" else 1 << 23
+
+
+def widened(table, page_size):
+    """Pages that are not there behind a sequence's, which change nothing."""
+    more = max(0, prepared.room // page_size - table.shape[1])
+    return torch.cat([table, torch.full((table.shape[0], more), -1, dtype=torch.int32, device=table.device)], 1)
+
+
 def prepared(cache_type, keys, values, page_size=16, blocksize=64):
     """A cache of one sequence in pages of random order: (cache, table, lengths)."""
     n, kv_heads, dim = keys.shape
@@ -30,21 +42,21 @@ def prepared(cache_type, keys, values, page_size=16, blocksize=64):
     cache = cache_type(width + 2, kv_heads, dim, page_size=page_size, blocksize=blocksize)
     lengths, starts = torch.tensor([n], dtype=torch.int32).cuda(), torch.tensor([0, n], dtype=torch.int32).cuda()
     cache.write(keys.cuda(), values.cuda(), table, lengths, starts)
-    return cache, table, lengths
+    return cache, widened(table, page_size), lengths
 
 
 def normal(seed, *shape):
     return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
 
 
-def compare(out, q, new, keys, values, blocksize, scale=None, window=None, sinks=0):
+def compare(out, q, new, keys, values, blocksize, scale=None, window=None, sinks=0, there=None):
     """Finite elements within the bound, the others NaN where the formula has NaN."""
     n = keys.shape[0]
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
     k, v = R.held(keys, blocksize), R.held(values, blocksize)
     positions = range(n - new, n)
-    want, _, _ = R.attend(q, positions, k, v, scale, window, sinks)
-    _, size, spread = R.attend(q, positions, torch.nan_to_num(k), torch.nan_to_num(v), scale, window, sinks)
+    want, _, _ = R.attend(q, positions, k, v, scale, window, sinks, there)
+    _, size, spread = R.attend(q, positions, torch.nan_to_num(k), torch.nan_to_num(v), scale, window, sinks, there)
     out = out.cpu().double()
     assert torch.equal(torch.isnan(out), torch.isnan(want))
     off = torch.nan_to_num((out - want).abs())
@@ -146,6 +158,32 @@ def test_pieces_of_different_sizes_are_joined(Cache, bad):
     compare(attend(cache, table, lengths, q), q, new, k, v, 64)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (50, 0), (50, 20), (1, 1)])
+def test_pages_that_are_not_there_and_tokens_that_are_not_seen(Cache, dim, window, sinks):
+    """Missing pages are not seen; NaN behind the window of every query and behind the last token change no bit."""
+    n, new = 330, 90
+    k, v, q = normal(27, n, 2, dim).bfloat16(), normal(28, n, 2, dim).bfloat16(), normal(29, new, 4, dim).bfloat16()
+    cache, table, lengths = prepared(Cache, k, v, 16, 64)
+    lengths -= 10
+    clean = attend(cache, table, lengths, q, window=window, sinks=sinks)
+    compare(clean, q, new, k[:-10], v[:-10], 64, window=window, sinks=sinks)
+    bad = [t.clone() for t in (k, v)]
+    for t in bad:
+        t[-10:] = math.nan
+        if window is not None:
+            t[sinks:n - 10 - new - window + 1] = math.nan
+    lengths += 10
+    cache.write(*(t.cuda() for t in bad), table, lengths, torch.tensor([0, n], dtype=torch.int32).cuda())
+    lengths -= 10
+    assert torch.equal(attend(cache, table, lengths, q, window=window, sinks=sinks), clean)
+    cache, table, lengths = prepared(Cache, k, v, 16, 64)
+    table[0, 1], table[0, 17], table[0, 19] = -1, cache.pages, -7
+    there = torch.ones(n, dtype=torch.bool)
+    there[16:32], there[272:288], there[304:320] = False, False, False
+    compare(attend(cache, table, lengths, q, window=window, sinks=sinks), q, new, k, v, 64, window=window, sinks=sinks, there=there)
+
+
 @pytest.mark.parametrize("n", [1, 5, 700, 3000])
 @pytest.mark.parametrize("group", [33, 64, 150])
 def test_one_token_of_many_heads_that_share_one(Cache, n, group):
@@ -165,6 +203,7 @@ def test_sequences_of_few_and_many_new_tokens_in_one_call_and_more_than_a_wave_h
     table = torch.randperm(150 * width, generator=torch.Generator().manual_seed(1)).view(150, width).to(torch.int32).cuda()
     cache = Cache(150 * width, 1, 64, page_size=16)
     lengths = torch.tensor(lens, dtype=torch.int32).cuda()
+    table = widened(table, 16)
     at = [[sum(x[:b]) for b in range(151)] for x in (lens, news)]
     cache.write(k.cuda(), v.cuda(), table, lengths, torch.tensor(at[0], dtype=torch.int32).cuda())
     keys, values = cache.read(table, lengths, torch.tensor(at[0], dtype=torch.int32).cuda(), tokens=total)
