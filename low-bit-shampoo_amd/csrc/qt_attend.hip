@@ -51,8 +51,16 @@ constexpr int few_waves(int dim, int units, bool bf16) { return dim == 256 || (u
 // / 16) + i (t < 8, i < 4) -- 32 of the 128 tokens of a tile, which is just what it has to hold of the weights for O^T = V^T P^T, so weights
 // never leave their lane.  Keys go from memory straight to registers (16 lanes' rows of 64 bytes side by side); values pass through an area
 // of LDS that belongs to the wave, to be read transposed (ds_read_b64_tr_b4: sixteen tokens of one element a lane) in the order of
-// tokens that the weights have.  DP: head_dim rounded up to 64, 128 or 256; UNITS: 1, or DP / 64 where a vector has several scales
-// (each 64 elements then have scores and weights of their own).
+// tokens that the weights have.
+//
+// The running maximum and sum of the softmax are kept per wave and joined at the end, so the cache is read once.  Bound by memory where
+// sequences are long (2 of up to 131072 tokens, 8 heads of 128 in one segment, 8 queries each: 52.7 us, 4.8 TB/s with the join), otherwise
+// by latency: about 5 us of finding work and asking for the first tile, 2.5 to 3.6 us a tile, of which the split of the weights (conversions of
+// 32 numbers that take 73 cycles each) is the longest part, and 5 us of a second launch where pieces are joined (32 sequences of up to 8000
+// tokens, 4 queries per head, segments of 64: 44 us, 3.4 TB/s).  Splitting by value scale, not expanding the values, keeps the products exact in
+// the cache's numbers; four waves to a piece share nothing but the join, so no barrier stands in the loop.  DP: head_dim
+// rounded up to 64, 128 or 256; UNITS: 1, or DP / 64 where a vector has several scales (each 64 elements then have scores and weights of
+// their own).
 template <int DP, int UNITS, bool BF16>
 __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_kernel(const AttendArgs a) {
     constexpr int kPieces = BF16 ? 3 : 5;
@@ -138,7 +146,10 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
         for (int t = 0; t < kLoads; ++t) {
             const long long at = DP == 64 ? (lane < 32 ? line_of(safe, base, 2 * t) : line_of(safe, base, 2 * t + 1)) : line_of(safe, base, t);
 #pragma unroll
-            for (int h = 0; h < kHalves; ++h) keys[h][t] = kOnce ? __builtin_nontemporal_load((const i32x4 *)(a.codes[0] + at + inside[h])) : *(const i32x4 *)(a.codes[0] + at + inside[h]);
+            for (int h = 0; h < kHalves; ++h) {
+                const i32x4 *from = (const i32x4 *)(a.codes[0] + at + inside[h]);
+                keys[h][t] = kOnce ? __builtin_nontemporal_load(from) : *from;
+            }
         }
     };
     // values of a tile whose pages `safe` has, from memory to LDS: lane i of a load fills bytes 16 i of a kilobyte
@@ -374,7 +385,8 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
 }
 
 // Joins the pieces of every row of tiles that was cut, a workgroup for each of its rows: what the pieces count for first, then a
-// share of them per group of DP / 4 threads.
+// share of them per group of DP / 4 threads.  Sums in a fixed order.  Bound by latency (about 5 us with its launch, of any number of pieces up
+// to some hundred); an atomic end in the first kernel would save the launch, at the price of results that depend on the order.
 template <int DP, bool BF16>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
     constexpr int kGroups = 1024 / DP;
