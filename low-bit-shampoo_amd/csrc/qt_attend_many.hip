@@ -57,7 +57,7 @@ __device__ __forceinline__ uint32_t pages_there(const AttendArgs &a, const int *
     for (int group = 0; group < kManyTile / 16; ++group) {
         const int token = base + 16 * group;
         if (token >= end) break;
-        // eight of a lane's tokens lie in every group of sixteen, and none past the end is before a query
+        // eight of a lane's tokens lie in every group of sixteen, and past the end no query sees any
         if ((unsigned)table[token >> a.shape.page_shift] < (unsigned)a.shape.pages) see |= 0xffu << (8 * group);
     }
     return see;
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const int my_token = v.start + my_row / a.group, my_head = w.head * a.group + my_row % a.group;
     const int position = v.first_position + my_row / a.group;
     const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;
-    // positions of this wave's queries and of all of the workgroup's
+    // positions of this wave's queries and of all of the workgroup's; a query may stand behind all tokens that the table has pages for
     const int seen_from = a.window ? max(0, v.first_position + first_row / a.group - (a.window - 1)) : 0;        // (by any, sinks aside)
     const int lowest = v.first_position + min(first_row + 32 * wave, all_rows - 1) / a.group;
     const int highest = v.first_position + min(first_row + 32 * wave + 31, all_rows - 1) / a.group;
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
             load_pages(min(k + 2, tile_to - 1));
         }
         {
-            const bool full = (base + kManyTile - 1 <= lowest) & (!a.window | (highest - base < a.window) | (base + kManyTile <= a.sinks)) & !(event & 4);
+            const bool full = (base + kManyTile - 1 <= min(lowest, v.end - 1)) & (!a.window | (highest - base < a.window) | (base + kManyTile <= a.sinks)) & !(event & 4);
             f32x16 score[2];
             f16x8 ahead[2][4];
             // Operands are read from LDS four matrix instructions ahead of those that take them.  A lane's places differ by constants: by exclusive
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
             };
             uint32_t see = 0xffffffffu;
             if (!full) {
-                const int x = position - base - 4 * half;
+                const int x = min(position, v.end - 1) - base - 4 * half;
                 see = tokens_up_to(x) | (tokens_up_to(x - 32) << 16);
                 if (a.window) {
                     const int y = behind - base - 4 * half, z = a.sinks - 1 - base - 4 * half;

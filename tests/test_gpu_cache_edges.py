@@ -1,0 +1,97 @@
+"""The 4-bit attention cache where calls end and where their numbers are far apart.  Against the definition in 64 bits.
+
+The bound on the route of many queries, in units of `size` = sum_j p_j max |v_j| over the tokens that a query sees itself: keys are rounded
+twice to 2^-12 (scale and product), so a score is off by 2 * 2^-12 of `sharp` = max_j scale sum_d |q_d k_jd|; elements of a query below fp16's
+normal numbers by 2^-25 against keys of at most 768 there, dim * 768 * 2^-25 in exponents of 2; a weight by the factor exp of twice that.  Weights
+and values round to 2^-11 each, the result to 2^-9: 2^-8 of `size` holds these."""
+import math
+
+import pytest
+import torch
+
+from oracle import cache_ref as R
+
+pytestmark = pytest.mark.gpu
+
+MUCH = 1 << 23                          # with so much room in the table, sequences of many queries go their own way
+
+
+@pytest.fixture(scope="module")
+def Cache():
+    from qtensor.cache import QTensorCache
+    import qtensor.functional as F
+    assert torch.cuda.is_available() and F.lib is not None
+    return QTensorCache
+
+
+def normal(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def ints(*x):
+    return torch.tensor(x, dtype=torch.int32).cuda()
+
+
+def one_sequence(cache_type, k, v, blocksize=64, page_size=16, pages=None, room=0):
+    """(cache, table, lengths): one sequence in pages of random order, of which the table has `pages`, and -1 up to `room` tokens."""
+    n, kv_heads, dim = k.shape
+    width = -(-n // page_size) if pages is None else pages
+    table = torch.randperm(width + 2, generator=torch.Generator().manual_seed(n))[:width].view(1, width).to(torch.int32)
+    table = torch.cat([table, torch.full((1, max(0, room // page_size - width)), -1, dtype=torch.int32)], 1).cuda()
+    cache = cache_type(width + 2, kv_heads, dim, page_size=page_size, blocksize=blocksize)
+    cache.write(k.cuda(), v.cuda(), table, ints(n), ints(0, n))
+    return cache, table, ints(n)
+
+
+def expected(q, first, k, v, blocksize, scale=None, window=None, sinks=0, there=None):
+    """(result, size, sharp) of queries at `first` and on, all fp64."""
+    new, heads, dim = q.shape
+    count, kv_heads, _ = k.shape
+    scale = dim ** -0.5 if scale is None else scale
+    K, V = R.held(k, blocksize), R.held(v, blocksize)
+    i, j = torch.arange(first, first + new)[:, None], torch.arange(count)[None, :]
+    see = j <= i
+    if window is not None:
+        see = see & ((i - j < window) | (j < sinks))
+    if there is not None:
+        see = see & there[None, :]
+    out, size, sharp = torch.zeros(new, heads, dim).double(), torch.zeros(new, heads, 1).double(), torch.zeros(new, heads, 1).double()
+    any_seen = see.any(1)
+    for h in range(heads):
+        kh, vh, qh = K[:, h // (heads // kv_heads)], V[:, h // (heads // kv_heads)], q[:, h].double()
+        # (what a query does not see is left out of its sums, so that what it holds does not matter)
+        s = (scale * (qh @ torch.nan_to_num(kh).T)).masked_fill(~see, -math.inf)
+        nan = (see & ~torch.isfinite(kh).all(1)[None, :]).any(1) | ~torch.isfinite(qh).all(1)
+        p = torch.nan_to_num(torch.softmax(torch.nan_to_num(s, nan=0.0, neginf=-math.inf), 1))
+        out[:, h] = p @ vh
+        out[nan & any_seen, h] = math.nan
+        size[:, h, 0] = p @ vh.abs().amax(1)
+        sharp[:, h, 0] = (abs(scale) * (torch.nan_to_num(qh).abs() @ torch.nan_to_num(kh).abs().T)).masked_fill(~see, 0.0).amax(1)
+    out[~any_seen] = 0.0
+    return out, size, sharp
+
+
+def compare_many(out, q, first, k, v, blocksize, **how):
+    want, size, sharp = expected(q, first, k, v, blocksize, **how)
+    dim = q.shape[-1]
+    out = out.cpu().double()
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    off = torch.nan_to_num((out - want).abs())
+    limit = size * (2 * (2 * 2.0 ** -12 * sharp + math.log(2) * dim * 768 * 2.0 ** -25) + 2.0 ** -8) + 2.0 ** -8 * torch.nan_to_num(want).abs()
+    assert (off <= limit).all(), (int((off > limit).sum()), float((off / size.clamp(min=1e-300)).max()), float(sharp.max()))
+
+
+# ------------------------------------------------------------------------------------------------ tables that end inside a tile
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page_size", [16, 32])
+@pytest.mark.parametrize("cut", [False, True])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (200, 5)])
+def test_tokens_behind_the_table_are_not_seen(Cache, dim, page_size, cut, window, sinks):
+    """Queries on both sides of the last token that the table has a page for, which is inside a tile of 64."""
+    kv_heads, covered = (2, 3600 if page_size == 16 else 3616) if cut else (8, 1008 if page_size == 16 else 992)
+    assert covered % 64 and 1200 * kv_heads * covered > MUCH
+    n, new, group = covered + 40, 300, 4
+    k, v, q = normal(1, n, kv_heads, dim).bfloat16(), normal(2, n, kv_heads, dim).bfloat16(), normal(3, new, kv_heads * group, dim).bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, page_size=page_size, pages=covered // page_size)
+    out = cache.attend(q.cuda(), table, lengths, ints(0, new), window=window, sinks=sinks)
+    compare_many(out, q, n - new, k, v, 64, window=window, sinks=sinks, there=torch.arange(n) < covered)
