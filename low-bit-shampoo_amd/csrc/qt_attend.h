@@ -46,6 +46,7 @@ typedef unsigned u32x6 __attribute__((ext_vector_type(6)));
 
 #define QT_LDS __attribute__((address_space(3)))
 #define QT_GLOBAL __attribute__((address_space(1)))
+#define QT_CONSTANT __attribute__((address_space(4)))
 
 constexpr int kFp4 = 4, kFp6 = 2;               // operand formats of the scaled matrix instructions
 constexpr int kOne = 0x7f7f7f7f;                // scale bytes that stand for 2^0

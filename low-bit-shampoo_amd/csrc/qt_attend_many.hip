@@ -28,6 +28,14 @@ constexpr float kSlack = 4.0f;          // ... and the running maximum may lag b
 // Keys and values whose scale has the largest exponent so far are held times 2^3; larger ones of up to 2^9 times that still fit (6 * 2 *
 // 2^(3 + 9) < 65504) before the power of two has to follow.
 constexpr int kHeldBits = 3, kHeadroom = 9;
+constexpr float kLargest = 65504.0f;    // of fp16
+
+enum Event {
+    kOutgrown = 1,          // an exponent has outgrown what is held
+    kOddValue = 2,          // a scale of a value is not finite
+    kHole = 4,              // a token's page is not there
+    kUnfit = 8              // fp16 does not hold a query: the workgroup's part is computed in fp32 (attend_in_fp32)
+};
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -83,6 +91,102 @@ __device__ __forceinline__ uint32_t values_not_finite(const AttendArgs &a, const
     return found;
 }
 
+// A workgroup's part of the work: a piece of the tokens that 128 queries see.
+struct ManyPart {
+    AttendWork w;
+    SequenceView v;                     // of these queries
+    int all_rows, first_row;
+    int tile_from, tile_to;
+};
+__device__ __forceinline__ bool find_part(const AttendArgs &a, uint32_t index, ManyPart &p) {
+    if (!find_work<kRowsOfMany, kManyShift, true>(a, index, p.w, p.v)) return false;
+    p.all_rows = p.v.count * a.group;
+    p.first_row = first_row_of<kRowsOfMany>(p.all_rows, p.w.row_tile);
+    const int last = p.v.first_position + min(p.first_row + kRowsOfMany - 1, p.all_rows - 1) / a.group;
+    p.v.end = max(0, min(p.v.end, last + 1));
+    view_tokens<kManyShift>(a, p.v, p.v.first_position + p.first_row / a.group, p.v.end);
+    const int per_piece = (p.v.tiles + p.w.pieces - 1) / p.w.pieces;
+    p.tile_from = min(p.w.piece * per_piece, p.v.tiles), p.tile_to = min(p.tile_from + per_piece, p.v.tiles);
+    return true;
+}
+
+// What a workgroup does whose numbers fp16 does not hold: its queries one by one, a wave for each, in fp32 from the cache as it is.  Scores
+// with a token per lane, results with DP / 64 elements per lane.  About a hundred times slower, for inputs that are rare: queries times keys
+// beyond 2^21 in different channels.  A function of its own that finds its work once more, so
+// that nothing of this takes registers in the loop before it (inlined: 1.2 % of whole prompts).
+template <int DP>
+__device__ __attribute__((noinline)) void attend_in_fp32(const AttendArgs QT_CONSTANT *arguments, uint32_t index) {
+    const AttendArgs &a = *(const AttendArgs *)arguments;
+    ManyPart p;
+    if (!find_part(a, __builtin_amdgcn_readfirstlane(index), p)) return;
+    const AttendWork &w = p.w;
+    const SequenceView &v = p.v;
+    const int first_row = p.first_row;
+    constexpr int kEach = DP / 64;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, d = lane * kEach, page_mask = (1 << a.shape.page_shift) - 1;
+    const int *table = a.at.table + (long long)w.b * a.at.table_stride;
+#pragma unroll 1
+    for (int nth = 32 * wave; nth < min(32 * wave + 32, p.all_rows - first_row); ++nth) {
+        const int row = first_row + nth, token = v.start + row / a.group, head = w.head * a.group + row % a.group;
+        const int position = v.first_position + row / a.group;
+        const uint16_t *query = (const uint16_t *)a.q + token * a.q_token + head * a.q_head;
+        float best = -__builtin_inff(), sum = 0.0f, y[kEach] = {};
+#pragma unroll 1
+        for (int k = p.tile_from; k < p.tile_to; ++k) {
+            const int base = (k < v.sink_tiles ? k : v.first_tile + k - v.sink_tiles) * kManyTile, mine = base + lane;
+            const int page = mine < v.end ? table[mine >> a.shape.page_shift] : -1;
+            const bool see = (unsigned)page < (unsigned)a.shape.pages && mine <= position && (!a.window || position - mine < a.window || mine < a.sinks);
+            float score = -__builtin_inff();
+            if (see) {
+                const long long line = ((long long)page * a.shape.kv_heads + w.head) << a.shape.page_shift;
+                const int inside = mine & page_mask;
+                score = 0.0f;
+#pragma unroll 1
+                for (int e = 0; e < a.shape.head_dim; e += 2) {
+                    const float by = a.scales[0][line * a.shape.segments + ((long long)(e >> a.shape.segment_shift) << a.shape.page_shift) + inside];
+                    const cache_f32x2 two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a.codes[0][(line + inside) * a.shape.row_bytes + e / 2], 1.0f, 0);
+                    score = __builtin_fmaf(__uint_as_float((uint32_t)query[e] << 16), two.x * by, score);
+                    if (e + 1 < a.shape.head_dim) score = __builtin_fmaf(__uint_as_float((uint32_t)query[e + 1] << 16), two.y * by, score);
+                }
+                score *= a.factor;
+            }
+            float top = fmaxf(best, score);
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+            const float zero = top == -__builtin_inff() ? 0.0f : top, fade = __builtin_amdgcn_exp2f(best - zero);
+            const float weight = see ? __builtin_amdgcn_exp2f(score - zero) : 0.0f;
+            float all = weight;
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) all += __shfl_xor(all, off, 64);
+            sum = __builtin_fmaf(sum, fade, all), best = top;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) y[e] *= fade;
+#pragma unroll 1
+            for (unsigned long long left = __ballot(see); left; left &= left - 1) {
+                const int from = __builtin_ctzll(left), inside = (base + from) & page_mask;
+                const float by = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), from));
+                const long long line = ((long long)(int)__builtin_amdgcn_readlane(page, from) * a.shape.kv_heads + w.head) << a.shape.page_shift;
+                if (d >= a.shape.head_dim) continue;
+                const float scale = a.scales[1][line * a.shape.segments + ((long long)(d >> a.shape.segment_shift) << a.shape.page_shift) + inside];
+                const uint8_t *codes = a.codes[1] + (line + inside) * a.shape.row_bytes + d / 2;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    const cache_f32x2 two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[e / 2], 1.0f, 0);
+                    y[e] = __builtin_fmaf(by, ((d + e) & 1 ? two.y : two.x) * scale, y[e]);
+                }
+            }
+        }
+        float *part = a.partial + ((long long)(w.slot + w.piece) * kRowsOfMany + nth) * (DP + 2);
+        if (w.pieces > 1 && lane == 0) part[0] = best, part[1] = sum;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (w.pieces > 1) part[2 + d + e] = y[e];
+            else if (d + e < a.shape.head_dim)
+                store_result<true>(a, token * a.out_token + head * a.out_head + d + e, sum == 0.0f ? 0.0f : y[e] / sum);
+        }
+    }
+}
+
 template <int DP>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(const AttendArgs a) {
     constexpr int kSteps = DP / 16, kDTiles = DP / 32, kChunks = DP / 32, kRow = DP * 2;
@@ -91,15 +195,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     __shared__ __attribute__((aligned(16))) uint8_t s_keys[2][kManyTile * kRow];
     __shared__ __attribute__((aligned(16))) uint8_t s_values[2][kManyTile * kRow];
     __shared__ int s_exponent[2];                       // largest exponents of a scale of keys and values so far
-    __shared__ int s_event[3];                          // of three tiles in turn: bit 0: an exponent has outgrown what is held; bit 1: a
-                                                        // scale of a value is not finite; bit 2: a token's page is not there
+    __shared__ int s_event[3];                          // of three tiles in turn, what has been met (Event)
 
-    AttendWork w;
-    SequenceView v;
-    if (!find_work<kRowsOfMany, kManyShift, true>(a, blockIdx.x, w, v)) return;
+    ManyPart p;
+    if (!find_part(a, blockIdx.x, p)) return;
+    const AttendWork &w = p.w;
+    const SequenceView &v = p.v;
+    const int all_rows = p.all_rows, first_row = p.first_row, tile_from = p.tile_from, tile_to = p.tile_to;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
-    const int all_rows = v.count * a.group;
-    const int first_row = first_row_of<kRowsOfMany>(all_rows, w.row_tile);
     const int my_row = min(first_row + 32 * wave + column, all_rows - 1);
     const bool mine = first_row + 32 * wave + column < all_rows;
     const int my_token = v.start + my_row / a.group, my_head = w.head * a.group + my_row % a.group;
@@ -109,14 +212,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const int seen_from = a.window ? max(0, v.first_position + first_row / a.group - (a.window - 1)) : 0;        // (by any, sinks aside)
     const int lowest = v.first_position + min(first_row + 32 * wave, all_rows - 1) / a.group;
     const int highest = v.first_position + min(first_row + 32 * wave + 31, all_rows - 1) / a.group;
-    {
-        const int last = v.first_position + min(first_row + kRowsOfMany - 1, all_rows - 1) / a.group;
-        v.end = max(0, min(v.end, last + 1));
-        view_tokens<kManyShift>(a, v, v.first_position + first_row / a.group, v.end);
-    }
-    const int per_piece = (v.tiles + w.pieces - 1) / w.pieces;
-    const int tile_from = min(w.piece * per_piece, v.tiles), tile_to = min(tile_from + per_piece, v.tiles);
-
     const int *table = a.at.table + (long long)w.b * a.at.table_stride;
     const int page_mask = (1 << a.shape.page_shift) - 1, chunks = a.shape.row_bytes >> 4;
     auto tile_at = [&](int k) __attribute__((always_inline)) { return (k < v.sink_tiles ? k : v.first_tile + k - v.sink_tiles) * kManyTile; };
@@ -169,7 +264,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     f16x8 query[kSteps];
     f32x16 result[kDTiles] = {}, below;         // below: what the sums of the scores begin with, minus the running maximum
     float best = -__builtin_inff(), sum = 0.0f;
-    int odd = 0;                                // not 0: somewhere a scale of a value is not finite
+    int met = 0;                                // events of all tiles so far
     int exponent[2] = {1, 1};                   // of the largest scales of keys and values that are held
 
     // This lane's eight elements of every sixteen of its query, zeros behind its end.
@@ -201,15 +296,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     };
     auto take_query = [&](const uint4 *raw) __attribute__((always_inline)) {
         const int up = exponent[0] - 127 - kHeldBits;
+        float top = 0.0f;
 #pragma unroll
         for (int h = 0; h < kSteps; ++h) {
             const uint32_t word[4] = {raw[h].x, raw[h].y, raw[h].z, raw[h].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                query[h][2 * e] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(word[e] << 16) * a.factor, up);
-                query[h][2 * e + 1] = (_Float16)__builtin_amdgcn_ldexpf(__uint_as_float(word[e] & 0xffff0000u) * a.factor, up);
+                const float x = __builtin_amdgcn_ldexpf(__uint_as_float(word[e] << 16) * a.factor, up);
+                const float y = __builtin_amdgcn_ldexpf(__uint_as_float(word[e] & 0xffff0000u) * a.factor, up);
+                top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
+                query[h][2 * e] = (_Float16)x, query[h][2 * e + 1] = (_Float16)y;
             }
         }
+        if (__builtin_expect(top > kLargest, 0)) atomicOr(&s_event[0], kUnfit);
     };
 
     // Expands this thread's chunks into `buffer`, a word (eight elements) of a chunk at a time: kSteps of them.  Before them: notes in
@@ -225,12 +324,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                 const int bits = (int)((__float_as_uint(by) >> 23) & 0xff), held = kind == 0 ? exponent[0] : exponent[1];
                 if (__builtin_expect((bits > min(held + kHeadroom, 254)) | hole[i], 0)) {
                     if (hole[i]) {
-                        atomicOr(&s_event[slot], 4);
+                        atomicOr(&s_event[slot], kHole);
                     } else if (bits < 255) {
                         atomicMax(&s_exponent[kind], bits);
-                        atomicOr(&s_event[slot], 1);
+                        atomicOr(&s_event[slot], kOutgrown);
                     } else if (kind == 1) {
-                        atomicOr(&s_event[slot], 2);
+                        atomicOr(&s_event[slot], kOddValue);
                         by = 0.0f;
                     }
                 }
@@ -256,6 +355,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     // (A later tile may hold scales that have outgrown what the first ones set: the workgroup begins again then, with the exponents that it has
     // found, which is rare and keeps the loop free of everything that would have to be corrected.)
     bool again = tile_from < tile_to;
+    int event = 0;
     while (again) {
     again = false;
 #pragma unroll
@@ -264,8 +364,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         for (int i = 0; i < 16; ++i) result[d][i] = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) below[i] = 0.0f;
-    best = -__builtin_inff(), sum = 0.0f, odd = 0;
-    int event = 0;
+    best = -__builtin_inff(), sum = 0.0f;
     {
         __syncthreads();
         if (threadIdx.x < 3) s_event[threadIdx.x] = 0;
@@ -292,8 +391,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         take_query(raw);
         stage_all(0, 0);
         __syncthreads();
-        event = s_event[0];
+        met = event = __builtin_amdgcn_readfirstlane(s_event[0]);
     }
+    if (event & kUnfit) break;
     // The running maximum follows where a score is more than 2^4 above it (scores are relative to it and to 2^-11), in both halves of a
     // column; `done`: weights of the tile that are not in the result yet.
     f16x8 weight[4];
@@ -346,7 +446,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
             load_pages(min(k + 2, tile_to - 1));
         }
         {
-            const bool full = (base + kManyTile - 1 <= min(lowest, v.end - 1)) & (!a.window | (highest - base < a.window) | (base + kManyTile <= a.sinks)) & !(event & 4);
+            const bool full = (base + kManyTile - 1 <= min(lowest, v.end - 1)) & (!a.window | (highest - base < a.window) | (base + kManyTile <= a.sinks)) & !(event & kHole);
             f32x16 score[2];
             f16x8 ahead[2][4];
             // Operands are read from LDS four matrix instructions ahead of those that take them.  A lane's places differ by constants: by exclusive
@@ -380,7 +480,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                     const int y = behind - base - 4 * half, z = a.sinks - 1 - base - 4 * half;
                     see &= ~(tokens_up_to(y) | (tokens_up_to(y - 32) << 16)) | (tokens_up_to(z) | (tokens_up_to(z - 32) << 16));
                 }
-                if (event & 4) see &= pages_there(a, table, v.end, base);
+                if (event & kHole) see &= pages_there(a, table, v.end, base);
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -445,30 +545,34 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
             }
         }
         __syncthreads();
-        odd |= event & 2;
-        if (more) event = s_event[next_slot];
+        if (more) event = __builtin_amdgcn_readfirstlane(s_event[next_slot]);
+        met |= event;
         slot = next_slot;
-        if (event & 1) {
+        if (event & kOutgrown) {
             again = true;
             break;
         }
     }
+    }
+    if (__builtin_expect(met & kUnfit, 0)) {
+        attend_in_fp32<DP>((const AttendArgs QT_CONSTANT *)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x);        // (`a`, the kernel's only argument)
+        return;
     }
     sum += __shfl_xor(sum, 32, 64);
     if (!mine) return;
     // values that are not finite were staged as zeros: what is multiplied with one that it sees is NaN.  (Looked for here, once more over
     // all of this piece's tokens, only where there was one at all.)
     uint32_t poison = 0;
-    if (__builtin_expect(odd, 0)) {
+    if (__builtin_expect(met & kOddValue, 0)) {
 #pragma unroll 1
         for (int k = tile_from; k < tile_to; ++k) poison |= values_not_finite(a, table, tile_at(k), min(v.end, tile_at(k) + kManyTile), position, w.head);
     }
-    // four consecutive elements of a result at a time
+    // four consecutive elements of a result at a time (of a piece: without the 2^11 of its weights)
     const int from_held = exponent[1] - 127 - kHeldBits;
-    const float by = w.pieces > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float one = __builtin_amdgcn_exp2f(-kWeightBits), by = w.pieces > 1 ? one : sum == 0.0f ? 0.0f : 1.0f / sum;
     float *part = a.partial + ((long long)(w.slot + w.piece) * kRowsOfMany + 32 * wave + column) * (DP + 2);
     const long long at = (long long)my_token * a.out_token + (long long)my_head * a.out_head;
-    if (w.pieces > 1 && half == 0) part[0] = best, part[1] = sum;
+    if (w.pieces > 1 && half == 0) part[0] = best, part[1] = sum * one;
 #pragma unroll
     for (int d = 0; d < kDTiles; ++d)
 #pragma unroll

@@ -66,7 +66,7 @@ def expected(q, first, k, v, blocksize, scale=None, window=None, sinks=0, there=
         out[:, h] = p @ vh
         out[nan & any_seen, h] = math.nan
         size[:, h, 0] = p @ vh.abs().amax(1)
-        sharp[:, h, 0] = (abs(scale) * (torch.nan_to_num(qh).abs() @ torch.nan_to_num(kh).abs().T)).masked_fill(~see, 0.0).amax(1)
+        sharp[:, h, 0] = (abs(scale) * (torch.nan_to_num(qh, 0.0, 0.0, 0.0).abs() @ torch.nan_to_num(kh).abs().T)).masked_fill(~see, 0.0).amax(1)
     out[~any_seen] = 0.0
     return out, size, sharp
 
@@ -95,3 +95,19 @@ def test_tokens_behind_the_table_are_not_seen(Cache, dim, page_size, cut, window
     cache, table, lengths = one_sequence(Cache, k, v, page_size=page_size, pages=covered // page_size)
     out = cache.attend(q.cuda(), table, lengths, ints(0, new), window=window, sinks=sinks)
     compare_many(out, q, n - new, k, v, 64, window=window, sinks=sinks, there=torch.arange(n) < covered)
+
+
+# ------------------------------------------------------------------------------------------------ numbers that are far apart
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (128, 64), (128, 128), (256, 64)])
+@pytest.mark.parametrize("large", [8000.0, 1.0e6])
+def test_large_queries_and_keys_in_different_channels(Cache, dim, blocksize, large):
+    """Products of their largest elements are beyond fp16, the scores are not; the large keys are later than some of the queries."""
+    n, new = 300, 260
+    k, v, q = normal(4, n, 2, dim), normal(5, n, 2, dim).bfloat16(), normal(6, new, 4, dim)
+    k[200:, :, 5], q[:, :, 5] = large, 0.0
+    q[::3, :, dim - 2], k[:, :, dim - 2] = large, 0.0
+    k, q = k.bfloat16(), q.bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize, room=MUCH)
+    out = cache.attend(q.cuda(), table, lengths, ints(0, new))
+    assert torch.isfinite(out).all()
+    compare_many(out, q, n - new, k, v, blocksize)
