@@ -91,6 +91,10 @@ __device__ __forceinline__ uint32_t values_not_finite(const AttendArgs &a, const
     return found;
 }
 
+// Scores of an infinite query are infinities of either sign or NaN, and the formula's weights NaN; minus infinities alone would pass for tokens that
+// are not seen.
+__device__ __forceinline__ float nan_if_infinite(float x) { return __builtin_fmaf(x, 0.0f, x); }
+
 // A workgroup's part of the work: a piece of the tokens that 128 queries see.
 struct ManyPart {
     AttendWork w;
@@ -302,8 +306,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
             const uint32_t word[4] = {raw[h].x, raw[h].y, raw[h].z, raw[h].w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float x = __builtin_amdgcn_ldexpf(__uint_as_float(word[e] << 16) * a.factor, up);
-                const float y = __builtin_amdgcn_ldexpf(__uint_as_float(word[e] & 0xffff0000u) * a.factor, up);
+                const float x = __builtin_amdgcn_ldexpf(nan_if_infinite(__uint_as_float(word[e] << 16)) * a.factor, up);
+                const float y = __builtin_amdgcn_ldexpf(nan_if_infinite(__uint_as_float(word[e] & 0xffff0000u)) * a.factor, up);
                 top = fmaxf(top, fmaxf(fabsf(x), fabsf(y)));
                 query[h][2 * e] = (_Float16)x, query[h][2 * e + 1] = (_Float16)y;
             }

@@ -111,3 +111,17 @@ def test_large_queries_and_keys_in_different_channels(Cache, dim, blocksize, lar
     out = cache.attend(q.cuda(), table, lengths, ints(0, new))
     assert torch.isfinite(out).all()
     compare_many(out, q, n - new, k, v, blocksize)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192])
+@pytest.mark.parametrize("n,new", [(300, 260), (4000, 48)])
+def test_queries_that_are_not_finite(Cache, dim, n, new):
+    """An infinite element makes every product infinite or NaN, whatever its sign and that of the keys: the formula has NaN."""
+    k, v, q = normal(7, n, 2, dim), normal(8, n, 2, dim).bfloat16(), normal(9, new, 4, dim).bfloat16()
+    k[:, :, 7] = k[:, :, 7].abs() + 0.5
+    k = k.bfloat16()
+    q[3, 0, 7], q[20, 1, 7], q[21, 3, 1], q[30, 2, 7] = -math.inf, math.inf, math.nan, -math.inf
+    cache, table, lengths = one_sequence(Cache, k, v, 64, 64, room=MUCH)
+    out = cache.attend(q.cuda(), table, lengths, ints(0, new))
+    assert torch.isnan(out[3, 0]).all() and torch.isnan(out[30, 2]).all() and int(torch.isnan(out).sum()) == 4 * dim
+    compare_many(out, q, n - new, k, v, 64)
