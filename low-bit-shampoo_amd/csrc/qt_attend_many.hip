@@ -7,8 +7,8 @@
 //
 // Roundings: keys and values to fp16 (two of 2^-12: the scale and the product), queries times the scale of the scores to fp16, weights to fp16
 // (2^-12 each), all against 2^-9 of the result's type; sums, maxima and results in fp32.  fp16 has no range to spare, so keys and values
-// are held relative to powers of two that follow the largest scales of the tiles so far (where one outgrows them the workgroup begins again):
-// a key or value loses bits only 2^16 below the largest of its head.  Weights are 2^11 times what they are, which keeps those of 2^-25.
+// are held relative to powers of two that follow the largest scales of the tiles so far (where one outgrows them the workgroup begins again);
+// what does not fit beside the largest of its head is computed in fp32 (kUnfit).  Weights are 2^11 times what they are, which keeps those of 2^-25.
 //
 // 4 prompts of 1500 to 8192 tokens, 8 heads of 128 with 4 queries each: 1190 to 1255 us, 840 to 885 TFLOP/s, where a large product of the library
 // reaches 1155 in fp16.  Bound by power (the clock falls to 1.8 GHz) and by two waves per unit of four matrix pipes having to wait at a barrier a
@@ -25,17 +25,24 @@ constexpr int kManyShift = 6;
 constexpr int kManyLeast = 4;           // tiles of a piece, at least
 constexpr float kWeightBits = 11.0f;    // weights are kept times 2^11 ...
 constexpr float kSlack = 4.0f;          // ... and the running maximum may lag behind by 4: below 2^15 in fp16
-// Keys and values whose scale has the largest exponent so far are held times 2^3; larger ones of up to 2^9 times that still fit (6 * 2 *
-// 2^(3 + 9) < 65504) before the power of two has to follow.
-constexpr int kHeldBits = 3, kHeadroom = 9;
+// Keys and values whose scale has the largest exponent so far are held times 2^3; values of up to 2^9 times that still fit (6 * 2 * 2^(3 + 9) <
+// 65504) before the power of two has to follow, keys of up to 2^3 times: what queries lose below fp16's normal numbers, 2^-25, is
+// multiplied with keys of at most 6 * 2 * 2^(3 + 3) then, 0.006 of an exponent over 256 elements at the very most.
+constexpr int kHeldBits = 3, kKeyHeadroom = 3, kValueHeadroom = 9;
+// Scales down to 2^-16 of that keep all their bits (1/2 * 2^(3 - 16) is fp16's least normal number).  Smaller values are not left to it, nor are smaller
+// keys beside queries of more than 2^6, whose products with the 2^-25 that such keys lose could reach 2^-11.
+constexpr int kSpan = 16;
+constexpr float kLargeQuery = 64.0f;
 constexpr float kLargest = 65504.0f;    // of fp16
 
 enum Event {
     kOutgrown = 1,          // an exponent has outgrown what is held
     kOddValue = 2,          // a scale of a value is not finite
     kHole = 4,              // a token's page is not there
-    kUnfit = 8              // fp16 does not hold a query: the workgroup's part is computed in fp32 (attend_in_fp32)
+    kUnfit = 8,             // fp16 does not hold a query or a value: the workgroup's part is computed in fp32 (attend_in_fp32)
+    kQueryIsLarge = 16, kKeyIsSmall = 32        // nor both together
 };
+__device__ __forceinline__ bool is_unfit(int met) { return (met & kUnfit) || (met & (kQueryIsLarge | kKeyIsSmall)) == (kQueryIsLarge | kKeyIsSmall); }
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
@@ -115,8 +122,9 @@ __device__ __forceinline__ bool find_part(const AttendArgs &a, uint32_t index, M
 }
 
 // What a workgroup does whose numbers fp16 does not hold: its queries one by one, a wave for each, in fp32 from the cache as it is.  Scores
-// with a token per lane, results with DP / 64 elements per lane.  About a hundred times slower, for inputs that are rare: queries times keys
-// beyond 2^21 in different channels.  A function of its own that finds its work once more, so
+// with a token per lane, results with DP / 64 elements per lane.  160 to 200 times slower (a prompt of 4096 tokens, 8 heads with 4 queries each, of 64 /
+// 128 / 256 elements: 23, 36 and 113 ms, otherwise 0.14, 0.19 and 0.56), for inputs that are rare: largest elements of queries and keys that multiply
+// to more than 2^21, values 2^16 below the largest of their head.  A function of its own that finds its work once more, so
 // that nothing of this takes registers in the loop before it (inlined: 1.2 % of whole prompts).
 template <int DP>
 __device__ __attribute__((noinline)) void attend_in_fp32(const AttendArgs QT_CONSTANT *arguments, uint32_t index) {
@@ -134,26 +142,34 @@ __device__ __attribute__((noinline)) void attend_in_fp32(const AttendArgs QT_CON
         const int row = first_row + nth, token = v.start + row / a.group, head = w.head * a.group + row % a.group;
         const int position = v.first_position + row / a.group;
         const uint16_t *query = (const uint16_t *)a.q + token * a.q_token + head * a.q_head;
-        float best = -__builtin_inff(), sum = 0.0f, y[kEach] = {};
+        float best = -__builtin_inff(), sum = 0.0f, y[kEach] = {}, q[kEach];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) q[e] = d + e < a.shape.head_dim ? __uint_as_float((uint32_t)query[d + e] << 16) : 0.0f;
 #pragma unroll 1
         for (int k = p.tile_from; k < p.tile_to; ++k) {
             const int base = (k < v.sink_tiles ? k : v.first_tile + k - v.sink_tiles) * kManyTile, mine = base + lane;
             const int page = mine < v.end ? table[mine >> a.shape.page_shift] : -1;
             const bool see = (unsigned)page < (unsigned)a.shape.pages && mine <= position && (!a.window || position - mine < a.window || mine < a.sinks);
-            float score = -__builtin_inff();
-            if (see) {
-                const long long line = ((long long)page * a.shape.kv_heads + w.head) << a.shape.page_shift;
-                const int inside = mine & page_mask;
-                score = 0.0f;
+            const long long line = ((long long)(see ? page : 0) * a.shape.kv_heads + w.head) << a.shape.page_shift;
+            float score = 0.0f;
 #pragma unroll 1
-                for (int e = 0; e < a.shape.head_dim; e += 2) {
-                    const float by = a.scales[0][line * a.shape.segments + ((long long)(e >> a.shape.segment_shift) << a.shape.page_shift) + inside];
-                    const cache_f32x2 two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(a.codes[0][(line + inside) * a.shape.row_bytes + e / 2], 1.0f, 0);
-                    score = __builtin_fmaf(__uint_as_float((uint32_t)query[e] << 16), two.x * by, score);
-                    if (e + 1 < a.shape.head_dim) score = __builtin_fmaf(__uint_as_float((uint32_t)query[e + 1] << 16), two.y * by, score);
+            for (int from = 0; from < a.shape.head_dim; from += 32) {
+                const uint4 codes = *(const uint4 *)(a.codes[0] + (line + (mine & page_mask)) * a.shape.row_bytes + from / 2);
+                const float by = a.scales[0][line * a.shape.segments + ((long long)(from >> a.shape.segment_shift) << a.shape.page_shift) + (mine & page_mask)];
+                const uint32_t word[4] = {codes.x, codes.y, codes.z, codes.w};
+                const int lanes = from / kEach;         // who has these elements of the query
+                auto add = [&](cache_f32x2 two, int e) __attribute__((always_inline)) {
+                    const float one = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q[e % kEach]), lanes + e / kEach));
+                    const float next = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q[(e + 1) % kEach]), lanes + (e + 1) / kEach));
+                    score = __builtin_fmaf(one, two.x * by, score), score = __builtin_fmaf(next, two.y * by, score);
+                };
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    add(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[i], 1.0f, 0), 8 * i), add(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[i], 1.0f, 1), 8 * i + 2);
+                    add(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[i], 1.0f, 2), 8 * i + 4), add(__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(word[i], 1.0f, 3), 8 * i + 6);
                 }
-                score *= a.factor;
             }
+            score = see ? score * a.factor : -__builtin_inff();
             float top = fmaxf(best, score);
 #pragma unroll
             for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
@@ -165,18 +181,21 @@ __device__ __attribute__((noinline)) void attend_in_fp32(const AttendArgs QT_CON
             sum = __builtin_fmaf(sum, fade, all), best = top;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) y[e] *= fade;
-#pragma unroll 1
-            for (unsigned long long left = __ballot(see); left; left &= left - 1) {
-                const int from = __builtin_ctzll(left), inside = (base + from) & page_mask;
+            const unsigned long long seen = __ballot(see);
+            const int segment = min(d, a.shape.head_dim - 1) >> a.shape.segment_shift, byte = min(d, 2 * a.shape.row_bytes - kEach) / 2;
+#pragma unroll 8
+            for (int from = 0; from < kManyTile; ++from) {
+                const bool here = (seen >> from) & 1;
+                const int inside = (base + from) & page_mask;
                 const float by = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(weight), from));
-                const long long line = ((long long)(int)__builtin_amdgcn_readlane(page, from) * a.shape.kv_heads + w.head) << a.shape.page_shift;
-                if (d >= a.shape.head_dim) continue;
-                const float scale = a.scales[1][line * a.shape.segments + ((long long)(d >> a.shape.segment_shift) << a.shape.page_shift) + inside];
-                const uint8_t *codes = a.codes[1] + (line + inside) * a.shape.row_bytes + d / 2;
+                const long long at = ((long long)(here ? (int)__builtin_amdgcn_readlane(page, from) : 0) * a.shape.kv_heads + w.head) << a.shape.page_shift;
+                const float scale = a.scales[1][at * a.shape.segments + ((long long)segment << a.shape.page_shift) + inside];
+                const uint8_t *codes = a.codes[1] + (at + inside) * a.shape.row_bytes + byte;
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) {
                     const cache_f32x2 two = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes[e / 2], 1.0f, 0);
-                    y[e] = __builtin_fmaf(by, ((d + e) & 1 ? two.y : two.x) * scale, y[e]);
+                    const float more = __builtin_fmaf(by, ((d + e) & 1 ? two.y : two.x) * scale, y[e]);
+                    y[e] = here ? more : y[e];
                 }
             }
         }
@@ -312,7 +331,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                 query[h][2 * e] = (_Float16)x, query[h][2 * e + 1] = (_Float16)y;
             }
         }
-        if (__builtin_expect(top > kLargest, 0)) atomicOr(&s_event[0], kUnfit);
+        if (__builtin_expect(top > kLargeQuery, 0)) atomicOr(&s_event[0], top > kLargest ? kUnfit : kQueryIsLarge);
     };
 
     // Expands this thread's chunks into `buffer`, a word (eight elements) of a chunk at a time: kSteps of them.  Before them: notes in
@@ -326,15 +345,21 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
                 const int kind = DP == 64 ? wave >> 1 : n;
                 float by = there[i] ? scale[n][i] : 0.0f;
                 const int bits = (int)((__float_as_uint(by) >> 23) & 0xff), held = kind == 0 ? exponent[0] : exponent[1];
-                if (__builtin_expect((bits > min(held + kHeadroom, 254)) | hole[i], 0)) {
+                const int least = max(held - kSpan, 0);
+                // (what is within, but for zeros, is so by one comparison)
+                if (__builtin_expect(((uint32_t)(bits - least) > (uint32_t)(min(held + (kind == 0 ? kKeyHeadroom : kValueHeadroom), 254) - least)) | hole[i], 0)) {
                     if (hole[i]) {
                         atomicOr(&s_event[slot], kHole);
-                    } else if (bits < 255) {
+                    } else if (bits == 255) {
+                        if (kind == 1) {
+                            atomicOr(&s_event[slot], kOddValue);
+                            by = 0.0f;
+                        }
+                    } else if (bits > held) {
                         atomicMax(&s_exponent[kind], bits);
                         atomicOr(&s_event[slot], kOutgrown);
-                    } else if (kind == 1) {
-                        atomicOr(&s_event[slot], kOddValue);
-                        by = 0.0f;
+                    } else if (by != 0.0f) {
+                        atomicOr(&s_event[slot], kind == 0 ? kKeyIsSmall : kUnfit);
                     }
                 }
                 scaled[n][i] = (_Float16)__builtin_amdgcn_ldexpf(by, 127 + kHeldBits - held);
@@ -397,7 +422,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         __syncthreads();
         met = event = __builtin_amdgcn_readfirstlane(s_event[0]);
     }
-    if (event & kUnfit) break;
+    if (is_unfit(met)) break;
     // The running maximum follows where a score is more than 2^4 above it (scores are relative to it and to 2^-11), in both halves of a
     // column; `done`: weights of the tile that are not in the result yet.
     f16x8 weight[4];
@@ -552,13 +577,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
         if (more) event = __builtin_amdgcn_readfirstlane(s_event[next_slot]);
         met |= event;
         slot = next_slot;
+        if (is_unfit(met)) break;
         if (event & kOutgrown) {
             again = true;
             break;
         }
     }
     }
-    if (__builtin_expect(met & kUnfit, 0)) {
+    if (__builtin_expect(is_unfit(met), 0)) {
         attend_in_fp32<DP>((const AttendArgs QT_CONSTANT *)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x);        // (`a`, the kernel's only argument)
         return;
     }

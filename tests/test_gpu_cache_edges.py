@@ -125,3 +125,73 @@ def test_queries_that_are_not_finite(Cache, dim, n, new):
     out = cache.attend(q.cuda(), table, lengths, ints(0, new))
     assert torch.isnan(out[3, 0]).all() and torch.isnan(out[30, 2]).all() and int(torch.isnan(out).sum()) == 4 * dim
     compare_many(out, q, n - new, k, v, 64)
+
+
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (128, 64), (128, 128), (256, 256), (1, 64), (33, 64), (100, 64), (200, 128), (224, 64), (255, 64)])
+@pytest.mark.parametrize("exponent", [-10, -18, -30, -90])
+def test_values_much_smaller_than_those_of_later_tokens(Cache, dim, blocksize, exponent):
+    """The first queries see only the small ones: what comes later must not take their bits."""
+    n = 330
+    k, v, q = normal(10, n, 2, dim).bfloat16(), normal(11, n, 2, dim), normal(12, n, 4, dim).bfloat16()
+    v[:100] *= 2.0 ** exponent
+    v = v.bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize, room=MUCH)
+    compare_many(cache.attend(q.cuda(), table, lengths, ints(0, n)), q, 0, k, v, blocksize)
+    # and larger ones that the window has left behind, in the first tiles of the same workgroup
+    k, v = k.flip(0), v.flip(0)
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize, room=MUCH)
+    compare_many(cache.attend(q.cuda(), table, lengths, ints(0, n), window=20), q, 0, k, v, blocksize, window=20)
+
+
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (128, 128)])
+def test_values_far_apart_in_pieces(Cache, dim, blocksize):
+    n, new = 4000, 48
+    k, v, q = normal(13, n, 1, dim).bfloat16(), normal(14, n, 1, dim), normal(15, new, 2, dim).bfloat16()
+    v[:3970] = v[:3970].abs() * 2.0 ** -40
+    v = v.bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize, 64, room=MUCH)
+    compare_many(cache.attend(q.cuda(), table, lengths, ints(0, new)), q, n - new, k, v, blocksize)
+
+
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (128, 64), (256, 64)])
+@pytest.mark.parametrize("grown,query", [(2.0 ** 8, 2.0 ** -6), (2.0 ** 30, 2.0 ** -18), (2.0 ** 20, 2.0 ** 12), (1.0, 2.0 ** -40), (1.0, 2.0 ** 14)])
+def test_keys_that_grow_and_queries_of_any_size(Cache, dim, blocksize, grown, query):
+    """Scores of a few: of large keys and small queries, or the reverse; the first tokens' keys are smaller yet."""
+    n, new = 300, 230
+    k, v, q = normal(16, n, 2, dim), normal(17, n, 2, dim).bfloat16(), (query * normal(18, new, 4, dim)).bfloat16()
+    k[64:] *= grown
+    k = (k * 4.0 / (query * grown)).bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize, room=MUCH)
+    compare_many(cache.attend(q.cuda(), table, lengths, ints(0, new)), q, n - new, k, v, blocksize)
+
+
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (128, 64), (128, 128), (256, 64)])
+def test_queries_below_what_fp16_holds_with_keys_that_grow(Cache, dim, blocksize):
+    """All elements alike, so that what they lose adds up: keys of 6 and then of +-6 * 2^9, queries that make 2^-25 more or less of one another."""
+    n, new = 200, 130
+    k, v = torch.full((n, 1, dim), 6.0), torch.ones(n, 1, dim)
+    k[64:] *= 2.0 ** 9
+    k[65::2] *= -1.0
+    v[65::2] *= -1.0
+    q = torch.full((new, 2, dim), 1.5 * 2.0 ** -21)
+    q[1::2] *= 5.0 / 3.0
+    k, v, q = k.bfloat16(), v.bfloat16(), q.bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize, room=MUCH)
+    scale = math.log(2.0)
+    compare_many(cache.attend(q.cuda(), table, lengths, ints(0, new), scale=scale), q, n - new, k, v, blocksize, scale=scale)
+
+
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (128, 64), (128, 128), (256, 64)])
+def test_keys_below_what_fp16_holds_with_large_queries(Cache, dim, blocksize):
+    """All elements alike again: small keys that differ by less than a step of fp16 beside large ones, in a channel where queries are zero."""
+    n, new = 260, 150
+    k, v = torch.full((n, 1, dim), 6.0 * 2.0 ** -26), torch.ones(n, 1, dim)
+    k[1::2] *= 1.125
+    v[1::2] *= -1.0
+    k[130:, :, 3] = 6.0
+    q = torch.full((new, 2, dim), 2.0 ** 27 / (6.75 * dim))
+    q[:, :, 3] = 0.0
+    k, v, q = k.bfloat16(), v.bfloat16(), q.bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize, room=MUCH)
+    scale = math.log(2.0)
+    compare_many(cache.attend(q.cuda(), table, lengths, ints(0, new), scale=scale), q, n - new, k, v, blocksize, scale=scale)
