@@ -26,6 +26,7 @@ from torch import Tensor
 import qtensor.functional as F
 
 _BLOCKSIZES = (64, 128, 256)
+_MOST = 2 ** 31 - 1                                 # of anything that is counted: the library's numbers have 32 bits
 
 
 class _Cache(ct.Structure):
@@ -168,7 +169,7 @@ class QTensorCache:
             size = F.lib.qtensor_hip_cache_attend_workspace(self._ref(), heads, q.dtype == torch.bfloat16, starts is not None)
         scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
         F._call(F.lib.qtensor_hip_cache_attend, q.device, self._ref(), places, _vectors(q), _vectors(out), heads, scale,
-                window or 0, sinks, scratch.data_ptr(), size)
+                min(window or 0, _MOST), min(sinks, _MOST), scratch.data_ptr(), size)
         return out
 
     # ---- checks and descriptions
@@ -199,6 +200,8 @@ class QTensorCache:
             raise ValueError("the rows of table must be contiguous.")
         if batch < 1 or table.shape[1] < 1:
             raise ValueError("need at least one sequence and one page in the table.")
+        if tokens > _MOST:
+            raise ValueError(f"{tokens} tokens are too many for one call.")
         if starts is not None:
             F._check_buffer(starts, "starts", batch + 1, torch.int32, self.codes.device)
         elif tokens != batch:

@@ -195,3 +195,33 @@ def test_keys_below_what_fp16_holds_with_large_queries(Cache, dim, blocksize):
     cache, table, lengths = one_sequence(Cache, k, v, blocksize, room=MUCH)
     scale = math.log(2.0)
     compare_many(cache.attend(q.cuda(), table, lengths, ints(0, new), scale=scale), q, n - new, k, v, blocksize, scale=scale)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0e-30, 3.0])
+def test_scales_of_scores_of_any_sign_and_size(Cache, scale):
+    n, new = 300, 230
+    k, v, q = normal(19, n, 2, 64).bfloat16(), normal(20, n, 2, 64).bfloat16(), normal(21, new, 4, 64).bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, room=MUCH)
+    compare_many(cache.attend(q.cuda(), table, lengths, ints(0, new), scale=scale), q, n - new, k, v, 64, scale=scale)
+
+
+# ------------------------------------------------------------------------------------------------ windows beyond every length
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("window,sinks", [(2 ** 31 - 1, 0), (2 ** 31, 0), (2 ** 32, 7), (2 ** 32 + 5, 0), (10, 2 ** 31), (10, 2 ** 32 + 1)])
+def test_windows_and_sinks_beyond_32_bits_are_all_tokens(Cache, monkeypatch, native, window, sinks):
+    import qtensor.cache as C
+    if not native:
+        monkeypatch.setattr(C, "_native", None)
+    k, v, q = normal(22, 200, 2, 64), normal(23, 200, 2, 64), normal(24, 9, 4, 64)
+    cache, table, lengths = one_sequence(Cache, k, v)
+    out = cache.attend(q.cuda(), table, lengths, ints(0, 9), window=window, sinks=sinks).cpu().double()
+    want, size, spread = R.attend(q, range(191, 200), R.held(k, 64), R.held(v, 64), 0.125)
+    assert ((out - want).abs() <= R.bounds(torch.float32, want, size, spread, 64)).all()
+
+
+def test_more_tokens_than_the_library_counts_are_refused(Cache):
+    k = normal(34, 20, 1, 64)
+    cache, table, lengths = one_sequence(Cache, k, k)
+    for tokens in (2 ** 31, 2 ** 32 + 20):
+        with pytest.raises(ValueError):
+            cache.read(table, lengths, ints(0, 20), tokens=tokens)
