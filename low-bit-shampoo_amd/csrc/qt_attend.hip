@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
     const int my_row = first_row + min(column, rows - 1);
     const int my_token = v.start + my_row / a.group, my_head = w.head * a.group + my_row % a.group;
     const int position = v.first_position + my_row / a.group;
-    const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;       // last token behind the window
+    const int behind = a.window ? max(max(position, 0) - a.window, -1) : -1;         // last token behind the window
     const int lowest = v.first_position + first_row / a.group, highest = v.first_position + (first_row + rows - 1) / a.group;
 
     const int tile_from = min(w.piece * w.per_piece, v.tiles), tile_to = min(tile_from + w.per_piece, v.tiles);

@@ -230,9 +230,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attend_many_kernel(con
     const bool mine = first_row + 32 * wave + column < all_rows;
     const int my_token = v.start + my_row / a.group, my_head = w.head * a.group + my_row % a.group;
     const int position = v.first_position + my_row / a.group;
-    const int behind = a.window && position >= 0 ? position - a.window : -0x7fffffff;
+    const int behind = a.window ? max(max(position, 0) - a.window, -1) : -1;         // last token behind the window
     // positions of this wave's queries and of all of the workgroup's; a query may stand behind all tokens that the table has pages for
-    const int seen_from = a.window ? max(0, v.first_position + first_row / a.group - (a.window - 1)) : 0;        // (by any, sinks aside)
+    const int seen_from = a.window ? max(0, max(0, v.first_position + first_row / a.group) - (a.window - 1)) : 0;        // (by any, sinks aside)
     const int lowest = v.first_position + min(first_row + 32 * wave, all_rows - 1) / a.group;
     const int highest = v.first_position + min(first_row + 32 * wave + 31, all_rows - 1) / a.group;
     const int *table = a.at.table + (long long)w.b * a.at.table_stride;

@@ -225,3 +225,16 @@ def test_more_tokens_than_the_library_counts_are_refused(Cache):
     for tokens in (2 ** 31, 2 ** 32 + 20):
         with pytest.raises(ValueError):
             cache.read(table, lengths, ints(0, 20), tokens=tokens)
+
+
+@pytest.mark.parametrize("room", [0, MUCH])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 200])
+def test_the_largest_windows_of_a_sequence_shorter_than_its_part(Cache, room, dtype, window):
+    """Its first rows have negative positions and see nothing; the others see all up to themselves."""
+    n, new = 100, 300
+    k, v, q = normal(25, n, 2, 64).to(dtype), normal(26, n, 2, 64).to(dtype), normal(27, new, 4, 64).to(dtype)
+    cache, table, lengths = one_sequence(Cache, k, v, room=room)
+    out = cache.attend(q.cuda(), table, lengths, ints(0, new), window=window)
+    assert not out[:200].any()
+    compare_many(out[200:], q[200:], 0, k, v, 64)
