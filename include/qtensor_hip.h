@@ -486,9 +486,10 @@ typedef struct {
 } qtensor_cache;
 /* Which tokens a call is about.  Sequence b has lengths[b] tokens, token t in page table[b * table_stride + t / page_size];
  * the call's tokens are the last starts[b + 1] - starts[b] of each sequence, packed end to end (starts[0] = 0, ascending,
- * starts[batch] = tokens), or with starts == NULL the last one of each (tokens = batch).  All arrays on the device.  A token
+ * starts[batch] <= tokens), or with starts == NULL the last one of each (tokens = batch).  All arrays on the device.  A token
  * of a negative position (a sequence shorter than its part of the call) or without a page (beyond table_pages, or a page
- * number outside the cache) is not written, reads as zeros and is not seen. */
+ * number outside the cache) is not written, reads as zeros and is not seen.  Tokens behind starts[batch] are of no sequence: they are not
+ * written, read as zeros and get zeros from attend. */
 typedef struct {
     const int *table, *lengths, *starts;
     long long table_stride;

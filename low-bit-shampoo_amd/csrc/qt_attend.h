@@ -161,8 +161,8 @@ __device__ __forceinline__ int first_row_of(int rows, int row_tile) {
 __device__ __forceinline__ int pieces_of(const AttendArgs &a, int tiles, int most) { return max(1, (tiles + (most > a.least ? most / 2 : most - 1)) / most); }
 
 // How a kernel's work is cut: a row of tiles (a sequence, a head of the cache, ROWS queries) into pieces of about as many tiles as all the work
-// has per slot.  Finds the `index`th piece (BY_PIECE) or the first piece of the `index`th row of tiles; false beyond the last.  Every wave
-// works it out for itself, a sequence per lane.
+// has per slot.  Finds the `index`th piece (BY_PIECE) or the first piece of the `index`th row of tiles; false beyond the last, where w.piece says by how
+// many and w.pieces is 0.  Every wave works it out for itself, a sequence per lane.
 //
 // Pieces behind the first of a row are at most tiles / most, so there are no more than slots of them; and rows that are cut have fewer than 2 tiles /
 // most pieces each, fewer than 2 slots in all.  `most` may round below the exact quotient by a few 2^-24 (a sum in fp32): a row whose
@@ -213,6 +213,7 @@ __device__ __forceinline__ bool find_work(const AttendArgs &a, uint32_t index, A
         before = __builtin_amdgcn_readlane(upto, 63);
         partial = __builtin_amdgcn_readlane(parts_upto, 63);
     }
+    w.piece = (int)(index - before), w.pieces = 0;
     return false;
 }
 

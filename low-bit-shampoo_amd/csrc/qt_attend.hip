@@ -45,6 +45,21 @@ constexpr int kWaitLds = 0xc07f;        // s_waitcnt lgkmcnt(0), nothing else
 
 constexpr int few_waves(int dim, int units, bool bf16) { return dim == 256 || (units > 1 && !bf16) ? 1 : 2; }
 
+// Zeros for rows of the call that are of no sequence (a step captured with room for more tokens than there are), from the `nth` of them on every `each`th.
+template <bool BF16>
+__device__ __forceinline__ void clear_rows_of_none(const AttendArgs &a, int nth, int each) {
+    int end = 0;                            // of the last sequence whose rows are all there
+    for (int b = threadIdx.x & 63; b < a.at.batch; b += 64) {
+        const int from = a.at.starts[b], to = a.at.starts[b + 1];
+        if (from >= 0 && from <= to && to <= a.at.tokens) end = max(end, to);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) end = max(end, __shfl_xor(end, off, 64));
+    for (int row = end + nth; row < a.at.tokens; row += each)
+        for (int e = threadIdx.x; e < a.group * a.shape.kv_heads * a.shape.head_dim; e += 256)
+            store_result<BF16>(a, row * a.out_token + e / a.shape.head_dim * a.out_head + e % a.shape.head_dim, 0.0f);
+}
+
 // Few queries per sequence: generation.  A workgroup takes one piece of a row of tiles, its four waves every fourth tile of it.
 //
 // Scores are computed transposed, K Q^T by v_mfma_scale_f32_16x16x128: a lane holds those of query lane % 16 and the tokens 16 t + 4 (lane
@@ -79,7 +94,10 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
 
     AttendWork w;
     SequenceView v;
-    if (!find_work<kRows, 7, true>(a, blockIdx.x, w, v)) return;
+    if (!find_work<kRows, 7, true>(a, blockIdx.x, w, v)) {
+        if (a.at.starts && w.pieces == 0) clear_rows_of_none<BF16>(a, w.piece, (int)gridDim.x - ((int)blockIdx.x - w.piece));
+        return;
+    }
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
     const int rows = min(kRows, v.count * a.group - w.row_tile * kRows);
     const int first_row = first_row_of<kRows>(0, w.row_tile);
@@ -450,7 +468,8 @@ int few_slots(int dim, int segments, bool bf16) { return compute_units() * few_w
 
 template <int DP, bool BF16>
 void launch_few(const AttendArgs &a, unsigned rows_of_tiles, bool may_cut, hipStream_t stream) {
-    const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u));
+    // (with starts some workgroups more than there can be work for: they see to the rows of no sequence)
+    const dim3 grid(rows_of_tiles + (may_cut ? (unsigned)a.slots : 0u) + (a.at.starts ? (unsigned)(a.at.tokens < 1024 ? (a.at.tokens + 15) / 16 : 64) : 0u));
     if (DP == 64 || a.shape.segments == 1) hipLaunchKernelGGL((attend_few_kernel<DP, 1, BF16>), grid, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((attend_few_kernel<DP, DP / 64, BF16>), grid, dim3(256), 0, stream, a);
     if (may_cut)

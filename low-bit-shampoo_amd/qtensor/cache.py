@@ -12,7 +12,8 @@ cache.  Everything runs on the GPU through libqtensor_hip.so, on torch's current
 `table` int32 [batch, n]: the pages of every sequence in order; `lengths` int32 [batch]: its tokens, the new ones included;
 `starts` int32 [batch + 1]: where the new tokens of each sequence begin in the packed tensors (the first 0, the last their
 number), or None where every sequence has one.  All three live on the GPU and no call waits for it, so a step of generation can be
-captured in a graph and replayed with other contents.  A token of a negative position or without a page (beyond the table, or a
+captured in a graph and replayed with other contents; tensors may have room for more tokens than starts says: those are of no
+sequence, are not written, read as zeros and get zeros from `attend`.  A token of a negative position or without a page (beyond the table, or a
 number that is not a page of the cache) is not written, reads as zeros and is not seen: pages that a window has left behind may
 be handed back and marked -1.
 """

@@ -238,3 +238,45 @@ def test_the_largest_windows_of_a_sequence_shorter_than_its_part(Cache, room, dt
     out = cache.attend(q.cuda(), table, lengths, ints(0, new), window=window)
     assert not out[:200].any()
     compare_many(out[200:], q[200:], 0, k, v, 64)
+
+
+# ------------------------------------------------------------------------------------------------ rows of no sequence
+@pytest.mark.parametrize("room", [0, MUCH])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 80, 256])
+@pytest.mark.parametrize("tokens", [41, 42, 48, 300])
+def test_rows_behind_the_last_start_are_zeros(Cache, room, dtype, dim, tokens):
+    """A step captured with room for more tokens than there are."""
+    k, v = normal(28, 90, 2, dim).to(dtype), normal(29, 90, 2, dim).to(dtype)
+    cache, table, _ = one_sequence(Cache, k, v, room=room)
+    table, lengths, starts = table.repeat(3, 1), ints(90, 0, 50), ints(0, 40, 40, 41)
+    q = normal(30, tokens, 6, dim).to(dtype).cuda()
+    for stride in (1, 2):
+        whole = torch.full((tokens, 6 * stride, dim), math.nan, dtype=dtype, device="cuda")
+        out = cache.attend(q, table, lengths, starts, out=whole[:, ::stride])
+        assert torch.equal(out[:41], cache.attend(q[:41].contiguous(), table, lengths, starts)) and not out[41:].any()
+        assert stride == 1 or torch.isnan(whole[:, 1::2]).all()
+    # no tokens at all, and starts that promise more than there are
+    nothing = torch.full_like(q, math.nan)
+    assert not cache.attend(q, table, lengths, ints(0, 0, 0, 0), out=nothing).any()
+    out = cache.attend(q, table, lengths, ints(0, 40, 40, tokens + 1), out=torch.full_like(q, math.nan))
+    assert torch.equal(out[:40], cache.attend(q[:40].contiguous(), table[:1], lengths[:1], ints(0, 40))) and not out[40:].any()
+
+
+def test_a_captured_step_with_fewer_tokens_at_a_replay(Cache):
+    k, v = normal(31, 90, 2, 64).bfloat16(), normal(32, 90, 2, 64).bfloat16()
+    cache, table, _ = one_sequence(Cache, k, v)
+    table, lengths, starts = table.repeat(2, 1), ints(90, 60), ints(0, 20, 24)
+    q, out = normal(33, 24, 4, 64).bfloat16().cuda(), torch.empty(24, 4, 64, dtype=torch.bfloat16, device="cuda")
+    cache.attend(q, table, lengths, starts, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(q, table, lengths, starts, out=out)
+    for counts in ((0, 20, 24), (0, 3, 5), (0, 0, 0), (0, 24, 24), (0, 0, 1)):
+        starts.copy_(torch.tensor(counts, dtype=torch.int32))
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = out.clone()
+        assert torch.equal(replayed, cache.attend(q, table, lengths, starts)) and not replayed[counts[2]:].any()
+        assert torch.isfinite(replayed).all()
