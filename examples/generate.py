@@ -124,10 +124,14 @@ class Server:
     @torch.no_grad()
     def generate(self, sequences, new, captured=True):
         """`new` tokens behind each prompt, the likeliest each time: [batch, new]."""
+        shortest, longest = min(len(s) for s in sequences), max(len(s) for s in sequences)
+        if new < 1 or shortest < 1 or longest + new - 1 > LONGEST:
+            raise ValueError(f"{new} tokens behind prompts of {shortest} to {longest}: at least one of each, and {LONGEST} with all but the last new one")
         token = self.prompts(sequences).argmax(-1)
         out = [token.clone()]
-        token = self.step(token).argmax(-1)
-        out.append(token.clone())
+        if new > 1:
+            token = self.step(token).argmax(-1)
+            out.append(token.clone())
         if captured and new > 2:
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):           # (recorded, not run)
