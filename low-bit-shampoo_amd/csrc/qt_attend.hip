@@ -78,7 +78,7 @@ __device__ __forceinline__ void clear_rows_of_none(const AttendArgs &a, int nth,
 // their own).
 template <int DP, int UNITS, bool BF16>
 __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_kernel(const AttendArgs a) {
-    constexpr int kPieces = BF16 ? 3 : 5;
+    constexpr int kPieces = BF16 ? 3 : 5, kQueryPieces = 5;         // of weights, and of queries (of bf16 queries the last two only where they matter)
     // One or two rows of tiles read the cache: past the L2 (two sequences of 131072 tokens 58.8 -> 52.9 us).  Queries in 32 bits come in any number
     // and read it again for every sixteen (4 x 2048 of them 1669 us, 1719 past the L2).
     constexpr bool kOnce = BF16;
@@ -187,8 +187,9 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
 #pragma unroll
     for (int d = 0; d < kDTiles; ++d) result[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float best = -__builtin_inff(), sum = 0.0f;
-    u32x6 query[kHalves][kPieces];
-    int query_scale[kHalves][kPieces];
+    u32x6 query[kHalves][kQueryPieces];
+    int query_scale[kHalves][kQueryPieces];
+    float matters = 0.0f;               // scale of a key (times that of the scores) above which what kPieces pieces leave of the queries matters
     int page[2];
     // one tile; `more`: the wave has another one, which is asked for on the way (without a branch: waits count loads)
     auto step = [&](int k, auto more) {
@@ -207,36 +208,52 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
                 odd_scale += 0.0f * by_value[u][i];
             }
         const bool odd = __ballot(odd_scale != 0.0f) != 0;
+        bool rest = false;
+        if constexpr (kQueryPieces > kPieces) {
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) rest |= fmaxf(fabsf(by_key[u][0]), fabsf(by_key[u][1])) > matters;
+            rest = __ballot(rest) != 0;
+        }
 
         // scores
         f32x4 score[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
+        // (pieces from `to` - 1 down to `from`)
+        auto products = [&](int t, int from, int to) __attribute__((always_inline)) {
+            f32x4 all;
             if constexpr (UNITS == 1) {
                 f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-                    for (int i = kPieces - 1; i >= 0; --i) {
+                    for (int i = to - 1; i >= from; --i) {
                         // (rows of 32 bytes: a load holds two times sixteen tokens, of which the scale of 2^-127 takes one away)
                         const int by = DP == 64 ? ((lane >> 5) == (t & 1) ? query_scale[h][i] : 0) : query_scale[h][i];
                         c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(keys[h][DP == 64 ? t >> 1 : t]), as_operand(query[h][i]), c, kFp4, kFp6,
                                                                              0, kOne, 0, by);
                     }
-                score[t] = times_row(c, by_key[0][t >> 2], t & 3);
+                all = times_row(c, by_key[0][t >> 2], t & 3);
             } else {
 #pragma unroll
                 for (int u = 0; u < UNITS; ++u) {
                     f32x4 c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int i = kPieces - 1; i >= 0; --i) {
+                    for (int i = to - 1; i >= from; --i) {
                         const int by = (lane >> 5) == (u & 1) ? query_scale[u >> 1][i] : 0;
                         c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(as_operand(keys[u >> 1][t]), as_operand(query[u >> 1][i]), c, kFp4, kFp6, 0, kOne,
                                                                              0, by);
                     }
                     c = times_row(c, by_key[u][t >> 2], t & 3);
-                    score[t] = u == 0 ? c : score[t] + c;
+                    all = u == 0 ? c : all + c;
                 }
+            }
+            return all;
+        };
+#pragma unroll
+        for (int t = 0; t < 8; ++t) score[t] = products(t, 0, kPieces);
+        if constexpr (kQueryPieces > kPieces) {
+            if (rest) {
+#pragma unroll
+                for (int t = 0; t < 8; ++t) score[t] += products(t, kPieces, kQueryPieces);
             }
         }
 #pragma unroll
@@ -356,6 +373,7 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
         load_tile(k, page);
         load_values(k, safe);
         load_pages(min(k + 4, tile_to - 1), page);
+        uint32_t largest = 0;
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
             f32x16 even, odd;
@@ -363,7 +381,15 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = max(top, max(__float_as_uint(even[i]) & 0x7fffffffu, __float_as_uint(odd[i]) & 0x7fffffffu));
-            split_fp6<kPieces>(even, odd, top, query[h], query_scale[h]);
+            split_fp6<kQueryPieces>(even, odd, top, query[h], query_scale[h]);
+            largest = max(largest, top);
+        }
+        if constexpr (kQueryPieces > kPieces) {
+            // An element of a query is off by 2^-14 of the largest of them at most, with even odds anywhere below; a score by this over sqrt(3) times
+            // sqrt(DP) elements of keys, which are some two times their scale.  Up to 2^-9 of an exponent of 2 are left.
+            constexpr float kLeft = 0.001953125f * 1.7320508f / 2.0f / (DP == 64 ? 8.0f : DP == 128 ? 11.3137085f : 16.0f);
+            const int exponent = (int)(group_max_u32<64>(largest) >> 23);
+            matters = __builtin_amdgcn_ldexpf(kLeft, 127 + 14 - exponent);
         }
         for (; k + 4 < tile_to; k += 4) step(k, std::true_type());
         step(k, std::false_type());

@@ -280,3 +280,23 @@ def test_a_captured_step_with_fewer_tokens_at_a_replay(Cache):
         replayed = out.clone()
         assert torch.equal(replayed, cache.attend(q, table, lengths, starts)) and not replayed[counts[2]:].any()
         assert torch.isfinite(replayed).all()
+
+
+# ------------------------------------------------------------------------------------------------ few queries beside outliers
+@pytest.mark.parametrize("dim,blocksize", [(64, 64), (64, 128), (128, 64), (128, 128), (96, 64), (256, 64), (256, 256)])
+@pytest.mark.parametrize("outlier", [1.0, 30.0, 300.0, 1000.0])
+@pytest.mark.parametrize("n,new,group", [(700, 1, 4), (60, 12, 2), (5000, 3, 1)])
+def test_bf16_queries_beside_outliers(Cache, dim, blocksize, outlier, n, new, group):
+    """Large elements of queries and keys in different channels of the same 32: the scores are ordinary, and no bits of the small elements may be
+    lost to the large ones.  What a score may be off by: 2^-7 of an exponent of 2, four times the 2^-9 that the kernel leaves on average; weights and
+    values 2^-8 of `size`, the result's rounding 2^-9."""
+    k, v, q = normal(35, n, 2, dim), normal(36, n, 2, dim).bfloat16(), normal(37, new, 2 * group, dim)
+    k[:, :, 9], k[:, :, 20] = 0.0, outlier * k[:, :, 20].sign()
+    q[:, :, 9], q[:, :, 20] = outlier, q[:, :, 20] / outlier
+    k, q = k.bfloat16(), q.bfloat16()
+    cache, table, lengths = one_sequence(Cache, k, v, blocksize)
+    out = cache.attend(q.cuda(), table, lengths, ints(0, new))
+    want, size, _ = expected(q, n - new, k, v, blocksize)
+    off = (out.cpu().double() - want).abs()
+    limit = size * (2 * math.log(2) * 2.0 ** -7 + 2.0 ** -8) + 2.0 ** -8 * want.abs()
+    assert (off <= limit).all(), (int((off > limit).sum()), float((off / size).max()))
