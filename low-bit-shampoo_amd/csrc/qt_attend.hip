@@ -69,18 +69,20 @@ __device__ __forceinline__ void clear_rows_of_none(const AttendArgs &a, int nth,
 // tokens that the weights have.
 //
 // The running maximum and sum of the softmax are kept per wave and joined at the end, so the cache is read once.  Bound by memory where
-// sequences are long (2 of up to 131072 tokens, 8 heads of 128 in one segment, 8 queries each: 52.7 us, 4.8 TB/s with the join), otherwise
-// by latency: about 5 us of finding work and asking for the first tile, 2.5 to 3.6 us a tile, of which the split of the weights (conversions of
-// 32 numbers that take 73 cycles each) is the longest part, and 5 us of a second launch where pieces are joined (32 sequences of up to 8000
-// tokens, 4 queries per head, segments of 64: 44 us, 3.4 TB/s).  Splitting by value scale, not expanding the values, keeps the products exact in
+// sequences are long (2 of up to 131072 tokens, 8 heads of 128 in one segment, 8 queries each: 52.6 us, 4.85 TB/s with the join), otherwise
+// by latency: about 5 us of finding work and asking for the first tile, 2.5 to 3.6 us a tile, and 5 us of a second launch where pieces are
+// joined (32 sequences of up to 8000 tokens, 4 queries per head, segments of 64: 44 us, 3.4 TB/s).  By its counters such a tile is some 970 vector
+// instructions, 3900 cycles of the vector unit (the split of the weights, conversions of 32 numbers that take 73 cycles each, is 730 of
+// them), beside 1170 of the matrix pipe, which takes sixteen queries where four are; waves wait for a third of their time.  Splitting by value scale, not expanding the values, keeps the products exact in
 // the cache's numbers; four waves to a piece share nothing but the join, so no barrier stands in the loop.  DP: head_dim
 // rounded up to 64, 128 or 256; UNITS: 1, or DP / 64 where a vector has several scales (each 64 elements then have scores and weights of
 // their own).
 template <int DP, int UNITS, bool BF16>
 __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_kernel(const AttendArgs a) {
     constexpr int kPieces = BF16 ? 3 : 5, kQueryPieces = 5;         // of weights, and of queries (of bf16 queries the last two only where they matter)
-    // One or two rows of tiles read the cache: past the L2 (two sequences of 131072 tokens 58.8 -> 52.9 us).  Queries in 32 bits come in any number
-    // and read it again for every sixteen (4 x 2048 of them 1669 us, 1719 past the L2).
+    // One or two rows of tiles read a long sequence: past the L2 (two of 131072 tokens 58.8 -> 52.9 us).  More of them come in calls that are little work,
+    // which read it again and take the same time either way (2048 tokens by 4096 queries, one head of 128: 28.7 us).  Queries in 32 bits come in any
+    // number and read it again for every sixteen (4 x 2048 of them 1669 us, 1719 past the L2).
     constexpr bool kOnce = BF16;
     constexpr int kHalves = DP == 256 ? 2 : 1;              // 16-byte chunks of a row that a lane holds
     constexpr int kLoads = DP == 64 ? 4 : 8;                // loads of sixteen tokens by all lanes (thirty-two for rows of 32 bytes)
@@ -430,7 +432,8 @@ __global__ __launch_bounds__(256, few_waves(DP, UNITS, BF16)) void attend_few_ke
 
 // Joins the pieces of every row of tiles that was cut, a workgroup for each of its rows: what the pieces count for first, then a
 // share of them per group of DP / 4 threads.  Sums in a fixed order.  Bound by latency (about 5 us with its launch, of any number of pieces up
-// to some hundred); an atomic end in the first kernel would save the launch, at the price of results that depend on the order.
+// to some hundred).  The last piece of a row to arrive could join them all in this order and save the launch; that takes a counter per row that is
+// zero when a call begins and that no call on another stream shares, which scratch of the call is not.
 template <int DP, bool BF16>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendArgs a) {
     constexpr int kGroups = 1024 / DP;

@@ -8,12 +8,13 @@
 // Roundings: keys and values to fp16 (two of 2^-12: the scale and the product), queries times the scale of the scores to fp16, weights to fp16
 // (2^-12 each), all against 2^-9 of the result's type; sums, maxima and results in fp32.  fp16 has no range to spare, so keys and values
 // are held relative to powers of two that follow the largest scales of the tiles so far (where one outgrows them the workgroup begins again);
-// what does not fit beside the largest of its head is computed in fp32 (kUnfit).  Weights are 2^11 times what they are, which keeps those of 2^-25.
+// what does not fit beside the largest of its head is computed in fp32 (kUnfit).  Weights are 2^11 times what they are: those of 2^-25 of a query's
+// largest keep their bits, those below 2^-36 are dropped.
 //
-// 4 prompts of 1500 to 8192 tokens, 8 heads of 128 with 4 queries each: 1190 to 1255 us, 840 to 885 TFLOP/s, where a large product of the library
-// reaches 1155 in fp16.  Bound by power (the clock falls to 1.8 GHz) and by two waves per unit of four matrix pipes having to wait at a barrier a
-// tile: the pipes are busy 41 % of the cycles; the vector work of a tile is interleaved with its products, matrix instruction by
-// matrix instruction, and fills most of the rest.  Heads of 256 leave one wave per unit (registers): 320 TFLOP/s over a
+// 4 prompts of 1500 to 8192 tokens, 8 heads of 128 with 4 queries each: 1190 to 1260 us, 840 to 885 TFLOP/s, where a large product of the library
+// reaches 1155 in fp16.  By its counters the matrix pipes are busy 38 % of the cycles and the vector units 45 %, at 2.0 GHz; the two waves that a SIMD
+// holds wait for 31 % of their time, for one another at a barrier a tile too, though the vector work of a tile is interleaved with its
+// products, matrix instruction by matrix instruction.  Heads of 256 leave one wave per unit (registers): 320 TFLOP/s over a
 // window of 4096.  Multiplying the 4-bit codes as they are instead, queries in 6-bit pieces, took 1357 us: three instructions for one.
 #include "qt_attend.h"
 

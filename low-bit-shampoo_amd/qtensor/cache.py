@@ -141,7 +141,8 @@ class QTensorCache:
         must have already.  heads is a multiple of kv_heads: query head h reads head h // (heads // kv_heads).  A token sees its
         sequence up to itself; with a window only the last `window` tokens of that, itself included, and the first `sinks`
         of the sequence.  scale: 1 / sqrt(head_dim) unless given.  A token that sees nothing gets zeros.  out: optional result of the
-        shape and type of q."""
+        shape and type of q.  Many bf16 queries of a sequence are computed in fp16 (errors of 2^-12 in keys, values and weights); what fp16 does
+        not hold, as queries and keys of thousands or values 2^16 below the largest of their head, is computed in fp32 and far slower."""
         if _native is not None:
             done = _native.cache_attend(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, q, table, lengths,
                                         starts, scale, window, sinks, out)
