@@ -176,7 +176,12 @@ class QTensorCache:
 
     # ---- checks and descriptions
     def _ref(self):
+        # (what they were made as: the kernels go by the numbers below, whatever has taken the tensors' place)
         codes, scales = self.codes, self.scales
+        for name, t, dtype, shape in (("codes", codes, torch.uint8, (self.kv_heads, self.page_size, 16 * (-(-self.head_dim // 32)))),
+                                      ("scales", scales, torch.float32, (self.kv_heads, self.segments, self.page_size))):
+            if t.device != codes.device or t.dtype != dtype or tuple(t.shape) != (2, self.pages, *shape) or not t.is_contiguous():
+                raise ValueError(f"the cache's {name} are {t.dtype} {tuple(t.shape)} on {t.device}, not contiguous {dtype} {(2, self.pages, *shape)} on {codes.device}.")
         return _Cache((codes.data_ptr(), codes.data_ptr() + codes.stride(0)), (scales.data_ptr(), scales.data_ptr() + 4 * scales.stride(0)),
                       self.pages, self.page_size, self.kv_heads, self.head_dim, self.blocksize)
 

@@ -58,3 +58,23 @@ def test_the_oracle_attends_to_what_is_seen():
     out, size, _ = R.attend(torch.ones(2, 2, 2), [-1, 3], k, v, 1.0, 2, 1)
     assert not out[0].any() and torch.allclose(out[1, 0], (v[0, 0] + v[2, 0] + v[3, 0]) / 3)
     assert torch.allclose(size[1, 1], torch.tensor([(1.0 + 5.0 + 7.0) / 3], dtype=torch.float64))
+
+
+def test_tensors_that_are_not_the_caches_are_refused():
+    """Kernels go by the cache's numbers: a tensor of another size in the place of its own would be read past its end."""
+    from qtensor.cache import QTensorCache
+
+    def cache():
+        return QTensorCache(3, 2, 80, page_size=32, blocksize=64, device="cpu")
+    assert cache()._ref().pages == 3
+    for name in ("codes", "scales"):
+        for change in (lambda t: t[:, :2], lambda t: t[:, :2].contiguous(), lambda t: t.double(), lambda t: t[..., ::2], lambda t: t.flatten(),
+                       lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)):
+            c = cache()
+            setattr(c, name, change(getattr(c, name)))
+            with pytest.raises(ValueError):
+                c._ref()
+    c = cache()
+    c.pages = 4
+    with pytest.raises(ValueError):
+        c._ref()
