@@ -518,6 +518,29 @@ void qtensor_hip_cache_attend(const qtensor_cache *cache, const qtensor_cache_pl
                               const qtensor_cache_vectors *out, int heads, float scale, int window, int sinks, void *workspace,
                               long long workspace_bytes, qtensor_stream_t stream);
 
+/* ---- projections whose weights are held in 4 bits (no counterpart in the reference, which has no models) -------------------
+ * Weights [outputs, inputs] in segments of blocksize (64, 128 or 256) inputs of an output, numbers and scales as in the attention
+ * cache above.  codes: [ceil(outputs / 16)][ceil(inputs / 128)][1024] bytes in the order of the matrix instructions' operands
+ * (csrc/qt_linear.h); scales: [ceil(outputs / 16)][ceil(inputs / blocksize)][16]; both aligned to 16 bytes. */
+typedef struct {
+    unsigned char *codes;
+    float *scales;
+    int inputs, outputs, blocksize;
+} qtensor_linear;
+/* Encodes a weight matrix [outputs, inputs] of fp32 or bf16 with row_stride elements between its rows; decodes it. */
+void qtensor_hip_linear_quantize(const qtensor_linear *weights, const void *weight, int is_bf16, long long row_stride, qtensor_stream_t stream);
+void qtensor_hip_linear_dequantize(const qtensor_linear *weights, void *weight, int is_bf16, long long row_stride, qtensor_stream_t stream);
+/* out[t] = W x[t] + bias for tokens x [tokens, inputs] and results [tokens, outputs], both fp32 or both bf16 with x_stride and
+ * out_stride elements between tokens; bias [outputs] of fp32 or bf16, or NULL.  Products are exact and summed in fp32, a segment's
+ * sum is multiplied by its scale, the result is rounded once. */
+typedef struct {
+    const void *x, *bias;
+    void *out;
+    long long x_stride, out_stride, tokens;
+    int is_bf16, bias_is_bf16;
+} qtensor_linear_call;
+void qtensor_hip_linear_product(const qtensor_linear *weights, const qtensor_linear_call *call, qtensor_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

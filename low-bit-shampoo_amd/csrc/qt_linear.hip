@@ -1,0 +1,259 @@
+// Weights held in 4 bits: encoding, decoding, products with few tokens (layout: qt_linear.h).
+#include "qt_linear.h"
+
+namespace qt {
+namespace {
+
+constexpr int kCodeThreads = 256;
+
+struct LinearCopy {
+    uint8_t *codes;
+    float *scales;
+    void *weight;
+    long long row_stride;
+    int inputs, outputs, blocks, segments, blocksize;
+};
+
+// A wave takes 16 outputs x 256 inputs: two blocks, which hold whole segments of every size.  Bound by memory; weights are laid out once.
+template <bool BF16, bool WRITE>
+__global__ __launch_bounds__(kCodeThreads) void linear_copy_kernel(const LinearCopy a) {
+    const int lane = threadIdx.x & 63, quarter = lane >> 4;
+    const int pairs = (a.blocks + 1) >> 1;
+    const long long work = (long long)blockIdx.x * (kCodeThreads / 64) + (threadIdx.x >> 6);
+    const long long tile = work / pairs;
+    const int pair = (int)(work - tile * pairs);
+    const long long output = tile * kLinearOutputs + (lane & 15);
+    if (tile * kLinearOutputs >= a.outputs) return;
+    const bool there = output < a.outputs;
+    uint8_t *row = (uint8_t *)a.weight + output * a.row_stride * (BF16 ? 2 : 4);
+    uint8_t *codes = a.codes + ((tile * a.blocks + 2 * pair) << 10) + 16 * lane;
+    if constexpr (WRITE) {
+        Eight<BF16> raw[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) raw[j].load(row, 256 * pair + 32 * j + 8 * quarter, there ? a.inputs : 0);
+        float x[8][8];
+        uint32_t top[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            top[j] = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[j][e] = BF16 ? __uint_as_float(e & 1 ? raw[j].raw[e / 2] & 0xffff0000u : raw[j].raw[e / 2] << 16) : __uint_as_float(raw[j].raw[BF16 ? 0 : e]);
+                top[j] = max(top[j], __float_as_uint(x[j][e]) & 0x7fffffffu);
+            }
+        }
+        const int each = a.blocksize >> 5;              // steps of 32 inputs of a segment
+#pragma unroll
+        for (int half = 1; half < 8; half *= 2)
+            if (half < each) {
+                uint32_t other[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) other[j] = top[j ^ half];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top[j] = max(top[j], other[j]);
+            }
+        uint32_t word[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            top[j] = max(top[j], (uint32_t)__shfl_xor((int)top[j], 16, 64));
+            top[j] = max(top[j], (uint32_t)__shfl_xor((int)top[j], 32, 64));
+            float scale;
+            word[j] = encode_fp4<8>(x[j], top[j], scale);
+            const int segment = (256 * pair + 32 * j) / a.blocksize;
+            if (quarter == 0 && (32 * j) % a.blocksize == 0 && segment < a.segments) a.scales[(tile * a.segments + segment) * kLinearOutputs + (lane & 15)] = scale;
+        }
+        *(qt_u32x4 *)codes = (qt_u32x4){word[0], word[1], word[2], word[3]};
+        if (2 * pair + 1 < a.blocks) *(qt_u32x4 *)(codes + 1024) = (qt_u32x4){word[4], word[5], word[6], word[7]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (2 * pair + i >= a.blocks) break;
+            const qt_u32x4 words = *(const qt_u32x4 *)(codes + 1024 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int first = 256 * pair + 128 * i + 32 * j + 8 * quarter;
+                const float scale = a.scales[(tile * a.segments + min(first / a.blocksize, a.segments - 1)) * kLinearOutputs + (lane & 15)];
+                const bf16x8 numbers = fp4_to_bf16(words[j]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = (float)numbers[e] * scale;
+                    if (!there || first + e >= a.inputs) continue;
+                    if (BF16) ((uint16_t *)row)[first + e] = float_to_bf16_bits(y);
+                    else ((float *)row)[first + e] = y;
+                }
+            }
+        }
+    }
+}
+
+// Products of few tokens: a wave multiplies R tiles of 16 outputs with T of 16 tokens, and the WAVES waves of a workgroup take the blocks of 128
+// inputs in turn; their sums are joined through LDS, in the order of the waves.
+template <bool BF16, int T, int R, int WAVES, int GROUPS>
+__global__ __launch_bounds__(64 * WAVES) void linear_few_kernel(const LinearArgs a) {
+    constexpr int P = Eight<BF16>::kPieces;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
+    const int tiles = (a.outputs + kLinearOutputs - 1) / kLinearOutputs;
+    const int first_tile = blockIdx.x * R, first_token = blockIdx.y * 16 * T;
+    __shared__ fp4_f32x4 s_part[WAVES - 1][R * T][64];
+    const uint8_t *codes[R];
+    const float *scales[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const long long tile = min(first_tile + r, tiles - 1);
+        codes[r] = a.codes + ((tile * a.blocks) << 10) + 16 * lane;
+        scales[r] = a.scales + tile * a.segments * kLinearOutputs + (lane & 15);
+    }
+    const uint8_t *x[T];
+    int valid[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const int token = first_token + 16 * t + (lane & 15);
+        valid[t] = token < a.tokens ? a.inputs : 0;
+        x[t] = (const uint8_t *)a.x + (long long)min(token, a.tokens - 1) * a.x_stride * (BF16 ? 2 : 4);
+    }
+    fp4_f32x4 sum[R][T];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < T; ++t) sum[r][t] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int block = wave; block < a.blocks; block += WAVES) {
+        qt_u32x4 word[R];
+        float scale[R][GROUPS];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            word[r] = *(const qt_u32x4 *)(codes[r] + ((long long)block << 10));
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) scale[r][g] = scales[r][(long long)min((block * GROUPS + g) >> a.scales_shift, a.segments - 1) * kLinearOutputs];
+        }
+        Eight<BF16> raw[T][4];
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) raw[t][j].load(x[t], kLinearInputs * block + 32 * j + 8 * quarter, valid[t]);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            fp4_f32x4 part[R][T];
+#pragma unroll
+            for (int j = g * (4 / GROUPS); j < (g + 1) * (4 / GROUPS); ++j) {
+                bf16x8 numbers[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) numbers[r] = fp4_to_bf16(word[r][j]);
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    bf16x8 pieces[P];
+                    raw[t][j].pieces(pieces);
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        part[r][t] = multiply_pieces<P>(pieces, numbers[r], j == g * (4 / GROUPS) ? (fp4_f32x4){0.f, 0.f, 0.f, 0.f} : part[r][t]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int t = 0; t < T; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[r][t][i] = __builtin_fmaf(scale[r][g], part[r][t][i], sum[r][t][i]);
+        }
+    }
+    if (wave) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < T; ++t) s_part[wave - 1][r * T + t][lane] = sum[r][t];
+    }
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int output = (first_tile + r) * kLinearOutputs + (lane & 15);
+        const float bias = output < a.outputs ? linear_bias(a, output) : 0.0f;
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+#pragma unroll
+            for (int w = 0; w < WAVES - 1; ++w) sum[r][t] += s_part[w][r * T + t][lane];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int token = first_token + 16 * t + 4 * quarter + i;
+                if (output < a.outputs && token < a.tokens) linear_store<BF16>(a, token, output, sum[r][t][i] + bias);
+            }
+        }
+    }
+}
+
+template <bool BF16, int T, int R, int WAVES>
+void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
+    const dim3 grid((unsigned)(((a.outputs + 15) / 16 + R - 1) / R), (unsigned)((a.tokens + 16 * T - 1) / (16 * T)));
+    if (groups == 2) hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 2>), grid, dim3(64 * WAVES), 0, stream, a);
+    else hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 1>), grid, dim3(64 * WAVES), 0, stream, a);
+}
+
+template <bool BF16>
+void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
+    if (a.tokens <= 16) launch_few<BF16, 1, 1, 8>(a, groups, stream);
+    else launch_few<BF16, 2, 2, 8>(a, groups, stream);
+}
+
+bool linear_shape(const char *what, const qtensor_linear *w) {
+    if (!w || !w->codes || !w->scales) { set_error(kNullPointer, "%s: null pointer in the weights", what); return false; }
+    if (w->blocksize != 64 && w->blocksize != 128 && w->blocksize != 256) {
+        set_error(kBadBlocksize, "%s: blocksize %d is not one of 64,128,256", what, w->blocksize);
+        return false;
+    }
+    if (w->inputs < 1 || w->inputs > (1 << 24) || w->outputs < 1 || w->outputs > (1 << 24)) {
+        set_error(kBadArgument, "%s: needs 1 to 2^24 inputs and outputs (got %d, %d)", what, w->inputs, w->outputs);
+        return false;
+    }
+    if (!is_aligned(w->codes, 16) || !is_aligned(w->scales, 16)) { set_error(kBadArgument, "%s: unaligned weights", what); return false; }
+    return true;
+}
+
+void copy_linear(const char *what, bool write, const qtensor_linear *w, void *weight, int is_bf16, long long row_stride, hipStream_t stream) {
+    clear_error();
+    if (!linear_shape(what, w)) return;
+    if (!weight) { set_error(kNullPointer, "%s: null weight", what); return; }
+    if (!is_aligned(weight, is_bf16 ? 2 : 4) || row_stride < 0) { set_error(kBadArgument, "%s: a weight aligned to an element, with rows in ascending order", what); return; }
+    const int blocks = (w->inputs + kLinearInputs - 1) / kLinearInputs;
+    const LinearCopy a = {w->codes, w->scales, weight, row_stride, w->inputs, w->outputs, blocks, (w->inputs + w->blocksize - 1) / w->blocksize, w->blocksize};
+    const long long waves = (long long)((w->outputs + 15) / 16) * ((blocks + 1) / 2);
+    const long long groups = (waves + kCodeThreads / 64 - 1) / (kCodeThreads / 64);
+    if (groups > 0x7fffffffLL) { set_error(kBadArgument, "%s: too many weights", what); return; }
+    const dim3 grid((unsigned)groups);
+    if (write && is_bf16) hipLaunchKernelGGL((linear_copy_kernel<true, true>), grid, dim3(kCodeThreads), 0, stream, a);
+    else if (write) hipLaunchKernelGGL((linear_copy_kernel<false, true>), grid, dim3(kCodeThreads), 0, stream, a);
+    else if (is_bf16) hipLaunchKernelGGL((linear_copy_kernel<true, false>), grid, dim3(kCodeThreads), 0, stream, a);
+    else hipLaunchKernelGGL((linear_copy_kernel<false, false>), grid, dim3(kCodeThreads), 0, stream, a);
+    launch_ok(what);
+}
+
+}  // namespace
+}  // namespace qt
+
+extern "C" void qtensor_hip_linear_quantize(const qtensor_linear *weights, const void *weight, int is_bf16, long long row_stride, void *stream) {
+    qt::copy_linear("linear_quantize", true, weights, const_cast<void *>(weight), is_bf16, row_stride, (hipStream_t)stream);
+}
+
+extern "C" void qtensor_hip_linear_dequantize(const qtensor_linear *weights, void *weight, int is_bf16, long long row_stride, void *stream) {
+    qt::copy_linear("linear_dequantize", false, weights, weight, is_bf16, row_stride, (hipStream_t)stream);
+}
+
+extern "C" void qtensor_hip_linear_product(const qtensor_linear *weights, const qtensor_linear_call *call, void *stream) {
+    using namespace qt;
+    const char *what = "linear_product";
+    clear_error();
+    if (!linear_shape(what, weights)) return;
+    if (!call || (call->tokens > 0 && (!call->x || !call->out))) { set_error(kNullPointer, "%s: null pointer in the call", what); return; }
+    const int size = call->is_bf16 ? 2 : 4;
+    if (call->tokens < 0 || call->tokens > 0x7fffff00LL || call->x_stride < 0 || call->out_stride < weights->outputs || !is_aligned(call->x, size) || !is_aligned(call->out, size) ||
+        (call->bias && !is_aligned(call->bias, call->bias_is_bf16 ? 2 : 4))) {
+        set_error(kBadArgument, "%s: needs up to 2^31 - 256 tokens in ascending order, results that do not overlap, and tensors aligned to an element", what);
+        return;
+    }
+    if (call->tokens == 0) return;
+    const int blocks = (weights->inputs + kLinearInputs - 1) / kLinearInputs;
+    const LinearArgs a = {weights->codes, weights->scales, call->x, call->bias, call->out, call->x_stride, call->out_stride, (int)call->tokens, weights->inputs, weights->outputs,
+                          blocks, (weights->inputs + weights->blocksize - 1) / weights->blocksize, weights->blocksize == 256, call->bias_is_bf16 != 0};
+    const int groups = weights->blocksize == 64 ? 2 : 1;
+    if (call->is_bf16) launch_product<true>(a, groups, (hipStream_t)stream);
+    else launch_product<false>(a, groups, (hipStream_t)stream);
+    launch_ok(what);
+}
