@@ -541,6 +541,38 @@ typedef struct {
 } qtensor_linear_call;
 void qtensor_hip_linear_product(const qtensor_linear *weights, const qtensor_linear_call *call, qtensor_stream_t stream);
 
+/* ---- rotary positions (no counterpart in the reference) -----------------------------------------------------------------------
+ * Pair p of the first dims elements of a head, (x[2 p], x[2 p + 1]) if interleaved, else (x[p], x[p + dims / 2]), becomes
+ * (a c - b s, b c + a s): c and s the fp32 numbers nearest to magnitude * cos and sin of position * frequencies[p] (device, 64 bits),
+ * products and sum rounded to fp32, the result to its type.  The other elements stay.  back: s with the other sign (gradients). */
+typedef struct {
+    const double *frequencies;
+    double magnitude;
+    int dims, interleaved, back;
+} qtensor_rotary;
+/* Vectors [batch, tokens, heads, head_dim] (head_dim up to 1024): strides in elements, of fp32 or bf16, elements of a head side by
+ * side.  to shares no memory with from. */
+typedef struct {
+    const void *from;
+    void *to;
+    long long from_batch, from_token, from_head, to_batch, to_token, to_head;
+    int heads;
+} qtensor_rotary_part;
+/* positions: int, or long long where long_positions is set; of token t of sequence b at b * position_batch + t. */
+typedef struct {
+    qtensor_rotary_part part[2];
+    int parts, head_dim, is_bf16, long_positions;
+    long long batch, tokens, position_batch;
+    const void *positions;
+} qtensor_rotary_call;
+void qtensor_hip_rotary_turn(const qtensor_rotary *rotary, const qtensor_rotary_call *call, qtensor_stream_t stream);
+/* Queries [tokens, heads, head_dim] turned into `out`; keys turned, rounded to their type and encoded into the cache, values encoded as
+ * they are, as qtensor_hip_cache_write does.  positions [tokens] as above, or NULL: a token's place in its sequence.  Queries of
+ * tokens without a place (of no sequence, or of a negative position) become zeros. */
+void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_rotary *rotary,
+                                    const qtensor_cache_vectors *q, const qtensor_cache_vectors *out, int heads, const qtensor_cache_vectors *keys,
+                                    const qtensor_cache_vectors *values, const void *positions, int long_positions, qtensor_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

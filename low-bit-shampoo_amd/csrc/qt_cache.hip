@@ -1,6 +1,5 @@
 // Writing a 4-bit attention cache and reading it back (layout: qt_cache.h).
 #include "qt_cache.h"
-#include "qt_divide.h"
 
 namespace qt {
 
@@ -58,70 +57,6 @@ struct CacheCopy {
     FastDiv by_lanes;
 };
 
-// Sequence of `token` and its position there; -1 for a token that is of no sequence.
-__device__ __forceinline__ int token_position(const CachePlaces &at, int token, int &b) {
-    if (!at.starts) {
-        b = token;
-        return at.lengths[b] - 1;
-    }
-    b = sequence_from(at, token, b);
-    if (b >= at.batch || token < at.starts[b]) return -1;
-    return at.lengths[b] - (at.starts[b + 1] - token);
-}
-
-// A lane takes sixteen bytes of a vector: eight elements of bf16, four of fp32.
-template <bool BF16>
-constexpr int kLaneElements = BF16 ? 8 : 4;
-
-// As they lie in memory, zeros behind the end of a vector.
-template <bool BF16>
-__device__ __forceinline__ uint4 load_lane(const void *base, long long at, int valid) {
-    const uint8_t *p = (const uint8_t *)base + at * (BF16 ? 2 : 4);
-    if (valid >= kLaneElements<BF16> && is_aligned16(p)) return load_u32x4<true>(p);
-    uint32_t word[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (BF16) word[e] = (2 * e < valid ? ((const uint16_t *)p)[2 * e] : 0u) | ((2 * e + 1 < valid ? ((const uint16_t *)p)[2 * e + 1] : 0u) << 16);
-        else word[e] = e < valid ? ((const uint32_t *)p)[e] : 0u;
-    }
-    return make_uint4(word[0], word[1], word[2], word[3]);
-}
-template <bool BF16>
-__device__ __forceinline__ void unpack_lane(uint4 raw, float *x) {
-    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (BF16) x[2 * e] = __uint_as_float(word[e] << 16), x[2 * e + 1] = __uint_as_float(word[e] & 0xffff0000u);
-        else x[e] = __uint_as_float(word[e]);
-    }
-}
-template <bool BF16, bool STREAM>
-__device__ __forceinline__ void store_lane(void *base, long long at, int valid, const float *x) {
-    uint8_t *p = (uint8_t *)base + at * (BF16 ? 2 : 4);
-    if (valid >= kLaneElements<BF16> && is_aligned16(p)) {
-        qt_u32x4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = BF16 ? floats_to_bf16_pair(x[2 * e], x[2 * e + 1]) : __float_as_uint(x[e]);
-        if (STREAM) __builtin_nontemporal_store(y, (qt_u32x4 *)p);
-        else *(qt_u32x4 *)p = y;
-    } else {
-#pragma unroll
-        for (int e = 0; e < kLaneElements<BF16>; ++e) {
-            if (e >= valid) continue;
-            if (BF16) ((uint16_t *)p)[e] = float_to_bf16_bits(x[e]);
-            else ((float *)p)[e] = x[e];
-        }
-    }
-}
-// Its codes: four bytes, or two.
-template <bool BF16>
-__device__ __forceinline__ uint32_t load_codes(const uint8_t *p) { return BF16 ? *(const uint32_t *)p : *(const uint16_t *)p; }
-template <bool BF16>
-__device__ __forceinline__ void store_codes(uint8_t *p, uint32_t word) {
-    if (BF16) *(uint32_t *)p = word;
-    else *(uint16_t *)p = (uint16_t)word;
-}
-
 // A thread's place: a lane's elements of the vectors of one token, whose heads it goes through.  A workgroup takes some
 // sixteen tokens of a few heads: codes and scales of a head's consecutive tokens lie side by side, and where the token
 // lies is looked up once for all of them.
@@ -161,9 +96,7 @@ __device__ __forceinline__ void cache_look_up(const CacheCopy &a, CacheThread &t
 // between neighbours and its codes leave as one store per lane.
 //
 // A segment is 8, 16 or 32 lanes side by side in bf16, twice as many in fp32.  Largest magnitude by integer maximum of
-// the magnitudes' bits (NaN above infinity, so that a segment with a NaN gets a NaN for its scale and reads as NaN),
-// scale and quotients by correctly rounded division (qt_divide.h; quotients below 2^-40, which it may round otherwise, are code 0),
-// nearest number (ties to the even code, beyond 6 to 6) by the conversion instruction.
+// the magnitudes' bits, scale and numbers by encode_fp4 (qt_fp4.h).
 template <bool BF16, int HEADS>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheCopy a) {
     CacheThread t = cache_thread<BF16>(a);
@@ -185,34 +118,14 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(const CacheC
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             constexpr int kEach = kLaneElements<BF16>;
-            float x[kEach], y[kEach];
+            float x[kEach];
             unpack_lane<BF16>(raw[n][i], x);
             uint32_t top = 0;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-            top = group_max_u32<8>(top);
-            if (a.segment_lanes >= 16) top = max(top, dpp_u32<0x140>(top));
-            if (a.segment_lanes >= 32) top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-            if (a.segment_lanes >= 64) top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-            const float scale = __uint_as_float(top) / 6.0f;
-            const uint32_t bits = __float_as_uint(scale);
-            if (bits >= kFastDivLo && bits <= kFastDivHi) {
-                const float r = exact_reciprocal(scale);
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) y[e] = quotient(x[e], scale, r);
-            } else {
-                // (zeroes times a scale that is not finite are NaN)
-                const bool zero = bits == 0 || top >= 0x7f800000u;
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) y[e] = zero ? 0.0f : x[e] / scale;
-            }
-            uint32_t word = 0;
-            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[0], y[1], 1.0f, 0);
-            word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[2], y[3], 1.0f, 1);
-            if constexpr (BF16) {
-                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[4], y[5], 1.0f, 2);
-                word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[6], y[7], 1.0f, 3);
-            }
+            top = segment_max(top, a.segment_lanes);
+            float scale;
+            const uint32_t word = encode_fp4<kEach>(x, top, scale);
             if (there && t.first < 2 * a.shape.row_bytes) store_codes<BF16>(a.codes[i] + (line + t.inside) * a.shape.row_bytes + t.first / 2, word);
             if (there && (t.first & ((1 << a.shape.segment_shift) - 1)) == 0) a.scales[i][scale_at] = scale;
         }
@@ -295,10 +208,7 @@ void copy_cache(const char *what, bool write, const qtensor_cache *cache, const 
         a.scales[i] = cache->scales[i];
     }
     if (a.at.tokens == 0) return;
-    // a segment is no longer than the vector, rounded up to a power of two
-    int segment = cache->blocksize;
-    while (segment > 64 && segment / 2 >= cache->head_dim) segment /= 2;
-    a.segment_lanes = segment / (keys->is_bf16 ? 8 : 4);
+    a.segment_lanes = cache_segment_lanes(a.shape, keys->is_bf16);
     a.lanes = a.segment_lanes * a.shape.segments;
     a.block_tokens = kCacheThreads / a.lanes;
     a.by_lanes = make_fastdiv((uint32_t)a.lanes);

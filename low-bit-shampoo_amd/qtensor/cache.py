@@ -7,6 +7,7 @@ cache.  Everything runs on the GPU through libqtensor_hip.so, on torch's current
 
     cache = QTensorCache(pages, kv_heads, head_dim)            # one per layer
     cache.write(keys, values, table, lengths, starts)          # new tokens, after `lengths` has counted them
+    q = cache.write_turned(rotary, q, keys, values, table, lengths, starts)    # the same with rotary positions (qtensor.rotary)
     out = cache.attend(q, table, lengths, starts)              # every new token sees its sequence up to itself
 
 `table` int32 [batch, n]: the pages of every sequence in order; `lengths` int32 [batch]: its tokens, the new ones included;
@@ -25,6 +26,7 @@ import torch
 from torch import Tensor
 
 import qtensor.functional as F
+from qtensor.rotary import Rotary, _check_positions, _Rotary
 
 _BLOCKSIZES = (64, 128, 256)
 _MOST = 2 ** 31 - 1                                 # of anything that is counted: the library's numbers have 32 bits
@@ -48,6 +50,9 @@ if F.lib is not None:
     for _name in ("qtensor_hip_cache_write", "qtensor_hip_cache_read"):
         getattr(F.lib, _name).restype = None
         getattr(F.lib, _name).argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.POINTER(_Vectors), ct.POINTER(_Vectors), ct.c_void_p]
+    F.lib.qtensor_hip_cache_write_turned.restype = None
+    F.lib.qtensor_hip_cache_write_turned.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.POINTER(_Rotary), ct.POINTER(_Vectors), ct.POINTER(_Vectors),
+                                                     ct.c_int, ct.POINTER(_Vectors), ct.POINTER(_Vectors), ct.c_void_p, ct.c_int, ct.c_void_p]
     F.lib.qtensor_hip_cache_attend.restype = None
     F.lib.qtensor_hip_cache_attend.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.POINTER(_Vectors), ct.POINTER(_Vectors), ct.c_int,
                                                ct.c_float, ct.c_int, ct.c_int, ct.c_void_p, ct.c_longlong, ct.c_void_p]
@@ -113,6 +118,37 @@ class QTensorCache:
         self._check_vectors(values, "values", (tokens, self.kv_heads, self.head_dim), keys.dtype)
         places = self._places(table, lengths, starts, tokens)
         F._call(F.lib.qtensor_hip_cache_write, self.codes.device, self._ref(), places, _vectors(keys), _vectors(values))
+
+    def write_turned(self, rotary: Rotary, q: Tensor, keys: Tensor, values: Tensor, table: Tensor, lengths: Tensor, starts: Optional[Tensor] = None,
+                     positions: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
+        """Rotary positions on the way into the cache, in one launch: the queries q [tokens, heads, head_dim] turned; keys turned and encoded,
+        values encoded, as `write` does with what rotary.turn gives.  positions: int32 or int64 [tokens], or None: a token's
+        place in its sequence (which is another where tokens have been evicted).  Queries of tokens that are of no sequence or of a
+        negative place become zeros.  out: optional result of the shape and type of q that shares no memory with it."""
+        F._require_gpu(self.codes, "QTensorCache.write_turned")
+        F._dtype_slot(q.dtype, "q")
+        tokens, heads = (q.shape[0], q.shape[1]) if q.dim() == 3 else (-1, -1)
+        self._check_vectors(q, "q", (tokens, heads, self.head_dim), q.dtype)
+        if not 1 <= heads <= 32767:
+            raise ValueError(f"need 1 to 32767 query heads (got {heads}).")
+        self._check_vectors(keys, "keys", (tokens, self.kv_heads, self.head_dim), q.dtype)
+        self._check_vectors(values, "values", (tokens, self.kv_heads, self.head_dim), q.dtype)
+        if rotary.dims > self.head_dim or rotary.frequencies.device != self.codes.device:
+            raise ValueError(f"{rotary.dims} elements on {rotary.frequencies.device} cannot turn in heads of {self.head_dim} on {self.codes.device}.")
+        if positions is not None:
+            _check_positions(positions, self.codes.device, ((tokens,),))
+            if not positions.is_contiguous():
+                raise ValueError("positions must be contiguous.")
+        if out is None:
+            out = torch.empty(tokens, heads, self.head_dim, dtype=q.dtype, device=q.device)
+        else:
+            self._check_vectors(out, "out", (tokens, heads, self.head_dim), q.dtype)
+            if any(F._overlap(out, t) for t in (q, keys, values)):
+                raise ValueError("out shares memory with q, keys or values, which are read while it is written.")
+        places = self._places(table, lengths, starts, tokens)
+        F._call(F.lib.qtensor_hip_cache_write_turned, self.codes.device, self._ref(), places, rotary._ref(), _vectors(q), _vectors(out), heads, _vectors(keys),
+                _vectors(values), None if positions is None else positions.data_ptr(), positions is not None and positions.dtype == torch.int64)
+        return out
 
     def read(self, table: Tensor, lengths: Tensor, starts: Optional[Tensor] = None, tokens: Optional[int] = None,
              dtype: torch.dtype = torch.float32) -> Tuple[Tensor, Tensor]:

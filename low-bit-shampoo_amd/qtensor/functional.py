@@ -169,6 +169,16 @@ def _check_buffer(t: Tensor, name: str, numel: int, dtype: torch.dtype, device: 
         raise ValueError(f"{name} must be contiguous.")
 
 
+def _overlap(a: Tensor, b: Tensor) -> bool:
+    """Whether the memory between the first and the last element of two tensors meets."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _check_common(code: Tensor, order: int, blocksize: int, bits: int, device: torch.device) -> None:
     assert blocksize in _BLOCKSIZES
     assert code.shape == torch.Size([2 ** bits])

@@ -112,7 +112,7 @@ class QTensorLinear:
             if tuple(out.shape) != shape:
                 raise ValueError(f"out has shape {tuple(out.shape)}, expected {shape}.")
             F._check_buffer(out, "out", rows.shape[0] * self.outputs, x.dtype, self.codes.device)
-            if _overlap(out, rows):
+            if F._overlap(out, rows):
                 raise ValueError("out shares memory with x, which is read while out is written.")
         F._call(F.lib.qtensor_hip_linear_product, self.codes.device, self._ref(),
                 _Call(rows.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), rows.stride(0), self.outputs, rows.shape[0],
@@ -139,13 +139,3 @@ class QTensorLinear:
             raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}.")
         if t.shape[1] > 1 and t.stride(1) != 1:
             raise ValueError(f"the last dimension of {name} must be contiguous.")
-
-
-def _overlap(a: Tensor, b: Tensor) -> bool:
-    """Whether the memory between the first and the last element of two matrices meets."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
