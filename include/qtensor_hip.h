@@ -573,6 +573,25 @@ void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const qtensor_ca
                                     const qtensor_cache_vectors *q, const qtensor_cache_vectors *out, int heads, const qtensor_cache_vectors *keys,
                                     const qtensor_cache_vectors *values, const void *positions, int long_positions, qtensor_stream_t stream);
 
+/* ---- what of an attention cache is kept, by the attention it is given ---------------------------------------------------------
+ * totals[b * total_sequence + h * total_head + t] += the sum, over the call's tokens of sequence b and the query heads that read head
+ * h, of the weights softmax(scale q k) that they give token t: what qtensor_hip_cache_attend multiplies its value with.  Totals of tokens
+ * that are not seen stay as they are.  Totals are as long as the table: table_pages * page_size.  workspace: 16-byte aligned, as
+ * many bytes as qtensor_hip_cache_weigh_workspace says for these places' numbers (arrays are not looked at). */
+long long qtensor_hip_cache_weigh_workspace(const qtensor_cache *cache, const qtensor_cache_places *places, int heads);
+void qtensor_hip_cache_weigh(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *q, int heads, float scale,
+                             int window, int sinks, float *totals, long long total_sequence, long long total_head, void *workspace,
+                             long long workspace_bytes, qtensor_stream_t stream);
+/* Of every sequence and head `keep` of the tokens that are there (whose page is) stay: those of the first `sinks` and the last `recent`
+ * places, then those with the largest totals (NaN above all, ties to the earlier one).  Keys, values and totals of the nth token that stays
+ * move to the place of the nth that is there; new_lengths[b] (another array than lengths) is one behind the last of these places, 0
+ * if nothing is there.  What lies behind is left as it was.  Of the places, table and lengths count.  No two sequences may share
+ * a page.  sinks + recent <= keep.  workspace as above. */
+long long qtensor_hip_cache_evict_workspace(const qtensor_cache *cache, const qtensor_cache_places *places, long long keep);
+void qtensor_hip_cache_evict(const qtensor_cache *cache, const qtensor_cache_places *places, float *totals, long long total_sequence, long long total_head,
+                             long long keep, long long recent, long long sinks, int *new_lengths, void *workspace, long long workspace_bytes,
+                             qtensor_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,8 @@ cache.  Everything runs on the GPU through libqtensor_hip.so, on torch's current
     cache.write(keys, values, table, lengths, starts)          # new tokens, after `lengths` has counted them
     q = cache.write_turned(rotary, q, keys, values, table, lengths, starts)    # the same with rotary positions (qtensor.rotary)
     out = cache.attend(q, table, lengths, starts)              # every new token sees its sequence up to itself
+    cache.weigh(totals, q, table, lengths, starts)             # adds up the weights that tokens are given (totals = cache.totals(table))
+    shorter = cache.evict(totals, table, lengths, keep)        # those with the largest sums stay
 
 `table` int32 [batch, n]: the pages of every sequence in order; `lengths` int32 [batch]: its tokens, the new ones included;
 `starts` int32 [batch + 1]: where the new tokens of each sequence begin in the packed tensors (the first 0, the last their
@@ -58,6 +60,15 @@ if F.lib is not None:
                                                ct.c_float, ct.c_int, ct.c_int, ct.c_void_p, ct.c_longlong, ct.c_void_p]
     F.lib.qtensor_hip_cache_attend_workspace.restype = ct.c_longlong
     F.lib.qtensor_hip_cache_attend_workspace.argtypes = [ct.POINTER(_Cache), ct.c_int, ct.c_int, ct.c_int]
+
+    F.lib.qtensor_hip_cache_weigh_workspace.restype = F.lib.qtensor_hip_cache_evict_workspace.restype = ct.c_longlong
+    F.lib.qtensor_hip_cache_weigh_workspace.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.c_int]
+    F.lib.qtensor_hip_cache_evict_workspace.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.c_longlong]
+    F.lib.qtensor_hip_cache_weigh.restype = F.lib.qtensor_hip_cache_evict.restype = None
+    F.lib.qtensor_hip_cache_weigh.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.POINTER(_Vectors), ct.c_int, ct.c_float, ct.c_int, ct.c_int, ct.c_void_p,
+                                              ct.c_longlong, ct.c_longlong, ct.c_void_p, ct.c_longlong, ct.c_void_p]
+    F.lib.qtensor_hip_cache_evict.argtypes = [ct.POINTER(_Cache), ct.POINTER(_Places), ct.c_void_p] + [ct.c_longlong] * 5 + [ct.c_void_p, ct.c_void_p,
+                                              ct.c_longlong, ct.c_void_p]
 
     # the same calls with their host side in native code (csrc/direct_call.cpp): what it does not take goes the way below
     _native = F._direct
@@ -185,18 +196,7 @@ class QTensorCache:
             if done is not None:
                 return done
         F._require_gpu(self.codes, "QTensorCache.attend")
-        F._dtype_slot(q.dtype, "q")
-        tokens, heads = (q.shape[0], q.shape[1]) if q.dim() == 3 else (-1, -1)
-        self._check_vectors(q, "q", (tokens, heads, self.head_dim), q.dtype)
-        if heads < 1 or heads % self.kv_heads:
-            raise ValueError(f"{heads} query heads are not a multiple of the cache's {self.kv_heads}.")
-        if window is not None and window < 1:
-            raise ValueError(f"window {window} is not positive.")
-        if sinks < 0 or (sinks and window is None):
-            raise ValueError("sinks are the first tokens that stay visible beside a window.")
-        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
-        if not math.isfinite(scale):
-            raise ValueError(f"scale {scale} is not finite.")
+        tokens, heads, scale = self._check_queries(q, scale, window, sinks)
         if out is None:
             out = torch.empty(tokens, heads, self.head_dim, dtype=q.dtype, device=q.device)
         else:
@@ -210,7 +210,77 @@ class QTensorCache:
                 min(window or 0, _MOST), min(sinks, _MOST), scratch.data_ptr(), size)
         return out
 
+    # ---- what is kept, by the attention it is given
+    def totals(self, table: Tensor) -> Tensor:
+        """Zeros for `weigh` to add to: fp32 [batch, kv_heads, tokens that the table has room for]."""
+        return torch.zeros(table.shape[0], self.kv_heads, table.shape[1] * self.page_size, dtype=torch.float32, device=self.codes.device)
+
+    def weigh(self, totals: Tensor, q: Tensor, table: Tensor, lengths: Tensor, starts: Optional[Tensor] = None, scale: Optional[float] = None,
+              window: Optional[int] = None, sinks: int = 0) -> Tensor:
+        """Adds to totals (fp32 [batch, kv_heads, n], n at least what the table has room for) the weights softmax(scale q k) that `attend`, called with the
+        same arguments, multiplies values with: for every token of a sequence and head of the cache the sum over the call's queries and over the query
+        heads that read the head.  Sums are in fp32, in one order.  Returns totals."""
+        F._require_gpu(self.codes, "QTensorCache.weigh")
+        tokens, heads, scale = self._check_queries(q, scale, window, sinks)
+        places = self._places(table, lengths, starts, tokens)
+        self._check_totals(totals, places)
+        if tokens * (heads // self.kv_heads) > _MOST - 256 or places.batch > 65535:
+            raise ValueError(f"{tokens} tokens of {heads} heads in {places.batch} sequences are too many for one call.")
+        cache = self._ref()
+        with torch.cuda.device(q.device):
+            size = F.lib.qtensor_hip_cache_weigh_workspace(cache, places, heads)
+        scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+        F._call(F.lib.qtensor_hip_cache_weigh, q.device, cache, places, _vectors(q), heads, scale, min(window or 0, _MOST), min(sinks, _MOST), totals.data_ptr(),
+                totals.stride(0), totals.stride(1), scratch.data_ptr(), size)
+        return totals
+
+    def evict(self, totals: Tensor, table: Tensor, lengths: Tensor, keep: int, recent: int = 0, sinks: int = 0) -> Tensor:
+        """Of every sequence and head, `keep` tokens stay: the first `sinks` and the last `recent` of the sequence, then those with the largest totals (NaN
+        above all, ties to the earlier one); all of them where there are no more.  In their order they move to the front, keys, values and
+        totals, and what lies behind is left as it was.  Returns the new lengths, as a tensor of its own: layers with caches of their own share
+        `lengths`, so copy them there once all caches are done, set the totals behind them to zero before tokens are written there, and hand the
+        pages behind back.  A position that a token was turned by stays its own: give write_turned positions from now on.  Tokens without a
+        page are no candidates, and their places stay empty.  No two sequences of the call may share a page."""
+        F._require_gpu(self.codes, "QTensorCache.evict")
+        if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError(f"need a token to keep, and no more first and last ones than are kept (got {keep}, {sinks} and {recent}).")
+        places = self._places(table, lengths, None, lengths.numel())
+        self._check_totals(totals, places)
+        if places.batch > 65535:
+            raise ValueError(f"{places.batch} sequences are too many for one call.")
+        keep, recent, sinks = (min(n, 2 ** 62) for n in (keep, recent, sinks))
+        cache = self._ref()
+        size = F.lib.qtensor_hip_cache_evict_workspace(cache, places, keep)
+        scratch = torch.empty(size, dtype=torch.uint8, device=totals.device)
+        out = torch.empty(places.batch, dtype=torch.int32, device=totals.device)
+        F._call(F.lib.qtensor_hip_cache_evict, totals.device, cache, places, totals.data_ptr(), totals.stride(0), totals.stride(1), keep, recent, sinks,
+                out.data_ptr(), scratch.data_ptr(), size)
+        return out
+
     # ---- checks and descriptions
+    def _check_queries(self, q: Tensor, scale: Optional[float], window: Optional[int], sinks: int):
+        """(tokens, heads, scale) of queries and of what they see."""
+        F._dtype_slot(q.dtype, "q")
+        tokens, heads = (q.shape[0], q.shape[1]) if q.dim() == 3 else (-1, -1)
+        self._check_vectors(q, "q", (tokens, heads, self.head_dim), q.dtype)
+        if heads < 1 or heads % self.kv_heads:
+            raise ValueError(f"{heads} query heads are not a multiple of the cache's {self.kv_heads}.")
+        if window is not None and window < 1:
+            raise ValueError(f"window {window} is not positive.")
+        if sinks < 0 or (sinks and window is None):
+            raise ValueError("sinks are the first tokens that stay visible beside a window.")
+        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else float(scale)
+        if not math.isfinite(scale):
+            raise ValueError(f"scale {scale} is not finite.")
+        return tokens, heads, scale
+
+    def _check_totals(self, totals: Tensor, places: _Places) -> None:
+        if totals.device != self.codes.device or totals.dtype != torch.float32:
+            raise ValueError(f"totals are {totals.dtype} on {totals.device}, expected {torch.float32} on {self.codes.device}.")
+        room = places.table_pages * self.page_size
+        if totals.dim() != 3 or tuple(totals.shape[:2]) != (places.batch, self.kv_heads) or totals.shape[2] < room or not totals.is_contiguous():
+            raise ValueError(f"totals have shape {tuple(totals.shape)}, expected contiguous ({places.batch}, {self.kv_heads}, {room} or more).")
+
     def _ref(self):
         # (what they were made as: the kernels go by the numbers below, whatever has taken the tensors' place)
         codes, scales = self.codes, self.scales
