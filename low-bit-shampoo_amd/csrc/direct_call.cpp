@@ -1,5 +1,5 @@
 // qtensor/_direct: the host side of one quantize or dequantize call of qtensor/functional.py, or of one call of an attention cache
-// (qtensor/cache.py), in native code.
+// (qtensor/cache.py), of a projection (qtensor/linear.py) or of rotary positions (qtensor/rotary.py), in native code.
 //
 // A call on a small matrix is bound by its host side: kernels of 4 to 6 us, and 9 us of Python around each (checks, two or
 // three torch.empty, data_ptr, ctypes, the error slot).  This is the same sequence behind one call: what the tensors are is
@@ -20,10 +20,16 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <array>
 #include <climits>
 #include <cmath>
+#include <memory>
+#include <optional>
+#include <utility>
+#include <vector>
 
 #include "qtensor_hip.h"
 
@@ -225,6 +231,13 @@ using Copy = decltype(&qtensor_hip_cache_write);
 Copy cache_write_entry, cache_read_entry;
 decltype(&qtensor_hip_cache_attend) cache_attend_entry;
 decltype(&qtensor_hip_cache_attend_workspace) cache_workspace_entry;
+decltype(&qtensor_hip_cache_write_turned) write_turned_entry;
+decltype(&qtensor_hip_cache_weigh) weigh_entry;
+decltype(&qtensor_hip_cache_weigh_workspace) weigh_workspace_entry;
+decltype(&qtensor_hip_cache_evict) evict_entry;
+decltype(&qtensor_hip_cache_evict_workspace) evict_workspace_entry;
+decltype(&qtensor_hip_linear_product) linear_entry;
+decltype(&qtensor_hip_rotary_turn) turn_entry;
 
 struct CacheCall {
     qtensor_cache cache;
@@ -372,6 +385,309 @@ PyObject *cache_attend_checked(PyObject *const *args) {
     return THPVariable_Wrap(std::move(out));
 }
 
+struct Angles { qtensor_rotary rotary; const at::Tensor *frequencies; };
+
+// frequencies, magnitude, dims, interleaved: in heads of up to `most` elements
+bool angles_of(PyObject *const *args, int device, long long most, Angles &a) {
+    long long dims;
+    a.frequencies = plain(args[0], device);
+    if (a.frequencies == nullptr || !PyFloat_CheckExact(args[1]) || !whole(args[2], dims) || !PyBool_Check(args[3])) return false;
+    if (dims < 2 || dims % 2 != 0 || dims > most || a.frequencies->scalar_type() != at::kDouble || a.frequencies->numel() != dims / 2) return false;
+    a.rotary = {static_cast<const double *>(a.frequencies->data_ptr()), PyFloat_AS_DOUBLE(args[1]), (int)dims, args[3] == Py_True, 0};
+    return true;
+}
+
+// First and last byte of a tensor's elements.
+std::pair<const char *, const char *> span(const at::Tensor &t) {
+    long long last = 0;
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    const char *first = static_cast<const char *>(t.data_ptr());
+    return {first, first + (last + 1) * t.element_size()};
+}
+bool apart(const at::Tensor &a, const at::Tensor &b) {
+    if (a.numel() == 0 || b.numel() == 0) return true;
+    const auto x = span(a), y = span(b);
+    return x.second <= y.first || y.second <= x.first;
+}
+
+// cache_write_turned(codes, scales, page_size, kv_heads, head_dim, blocksize, frequencies, magnitude, dims, interleaved, q, keys, values, table,
+// lengths, starts, positions, out) -> out or None
+PyObject *cache_write_turned_checked(PyObject *const *args) {
+    CacheCall c;
+    Angles angles;
+    qtensor_cache_vectors q, keys, values, result;
+    if (write_turned_entry == nullptr || !cache_of(args, c) || !angles_of(args + 6, c.device, c.cache.head_dim, angles)) Py_RETURN_NONE;
+    const at::Tensor *t = vectors_of(args[10], c, nullptr, -1, -1, q);
+    if (t == nullptr || t->size(1) < 1 || t->size(1) > 32767) Py_RETURN_NONE;
+    const at::Tensor *k = vectors_of(args[11], c, t, t->size(0), c.cache.kv_heads, keys), *v = vectors_of(args[12], c, t, t->size(0), c.cache.kv_heads, values);
+    if (k == nullptr || v == nullptr || !places_of(args + 13, c, t->size(0))) Py_RETURN_NONE;
+    const void *positions = nullptr;
+    bool long_positions = false;
+    if (args[16] != Py_None) {
+        const at::Tensor *p = plain(args[16], c.device);
+        if (p == nullptr || p->dim() != 1 || p->numel() != t->size(0) || (p->scalar_type() != at::kInt && p->scalar_type() != at::kLong)) Py_RETURN_NONE;
+        positions = p->data_ptr(), long_positions = p->scalar_type() == at::kLong;
+    }
+    at::Tensor out;
+    if (args[17] == Py_None) {
+        out = at::empty({t->size(0), t->size(1), t->size(2)}, at::TensorOptions().device(t->device()).dtype(t->scalar_type()));
+        if (!in_plain_memory(out, c.device)) Py_RETURN_NONE;
+        result = {out.data_ptr(), q.is_bf16, out.stride(0), out.stride(1)};
+    } else {
+        const at::Tensor *given = vectors_of(args[17], c, t, t->size(0), t->size(1), result);
+        if (given == nullptr || !apart(*given, *t) || !apart(*given, *k) || !apart(*given, *v)) Py_RETURN_NONE;
+    }
+    const int heads = (int)t->size(1);
+    void *stream = stream_of(c);
+    if (!launched([&] { write_turned_entry(&c.cache, &c.places, &angles.rotary, &q, &result, heads, &keys, &values, positions, long_positions, stream); })) return nullptr;
+    if (args[17] != Py_None) {
+        Py_INCREF(args[17]);
+        return args[17];
+    }
+    return THPVariable_Wrap(std::move(out));
+}
+
+// Totals of the call's sequences, heads and places.
+const at::Tensor *totals_of(PyObject *obj, const CacheCall &c) {
+    const at::Tensor *t = plain(obj, c.device);
+    return t != nullptr && t->scalar_type() == at::kFloat && t->dim() == 3 && t->size(0) == c.places.batch && t->size(1) == c.cache.kv_heads &&
+                   t->size(2) >= (long long)c.places.table_pages * c.cache.page_size && c.places.batch <= 65535
+               ? t
+               : nullptr;
+}
+
+// cache_weigh(codes, scales, page_size, kv_heads, head_dim, blocksize, totals, q, table, lengths, starts, scale, window, sinks) -> totals or None
+PyObject *cache_weigh_checked(PyObject *const *args) {
+    CacheCall c;
+    qtensor_cache_vectors q;
+    long long window = 0, sinks;
+    if (weigh_entry == nullptr || !cache_of(args, c)) Py_RETURN_NONE;
+    const at::Tensor *t = vectors_of(args[7], c, nullptr, -1, -1, q);
+    if (t == nullptr || t->size(1) < 1 || t->size(1) > 32767 || t->size(1) % c.cache.kv_heads != 0 || !places_of(args + 8, c, t->size(0))) Py_RETURN_NONE;
+    const at::Tensor *totals = totals_of(args[6], c);
+    const int heads = (int)t->size(1);
+    if (totals == nullptr || t->size(0) * (heads / c.cache.kv_heads) > INT_MAX - 256) Py_RETURN_NONE;
+    double scale = 1.0 / std::sqrt((double)c.cache.head_dim);
+    if (args[11] != Py_None) {
+        if (!PyFloat_CheckExact(args[11])) Py_RETURN_NONE;
+        scale = PyFloat_AS_DOUBLE(args[11]);
+    }
+    if (args[12] != Py_None && (!whole(args[12], window) || window < 1)) Py_RETURN_NONE;
+    if (!whole(args[13], sinks) || sinks < 0 || sinks > INT_MAX || window > INT_MAX || (sinks != 0 && window == 0) || !std::isfinite((float)scale)) Py_RETURN_NONE;
+    const long long size = weigh_workspace_entry(&c.cache, &c.places, heads);
+    if (size <= 0) Py_RETURN_NONE;
+    at::Tensor scratch = at::empty({size}, at::TensorOptions().device(t->device()).dtype(at::kByte));
+    if (!in_plain_memory(scratch, c.device)) Py_RETURN_NONE;
+    void *stream = stream_of(c), *workspace = scratch.data_ptr();
+    float *sums = static_cast<float *>(totals->data_ptr());
+    const long long of_sequence = totals->stride(0), of_head = totals->stride(1);
+    if (!launched([&] { weigh_entry(&c.cache, &c.places, &q, heads, (float)scale, (int)window, (int)sinks, sums, of_sequence, of_head, workspace, size, stream); }))
+        return nullptr;
+    Py_INCREF(args[6]);
+    return args[6];
+}
+
+// cache_evict(codes, scales, page_size, kv_heads, head_dim, blocksize, totals, table, lengths, keep, recent, sinks) -> new lengths or None
+PyObject *cache_evict_checked(PyObject *const *args) {
+    CacheCall c;
+    long long keep, recent, sinks;
+    if (evict_entry == nullptr || !cache_of(args, c) || !THPVariable_CheckExact(args[8])) Py_RETURN_NONE;
+    PyObject *where[3] = {args[7], args[8], Py_None};
+    if (!places_of(where, c, THPVariable_Unpack(args[8]).numel())) Py_RETURN_NONE;
+    const at::Tensor *totals = totals_of(args[6], c);
+    if (totals == nullptr || !whole(args[9], keep) || !whole(args[10], recent) || !whole(args[11], sinks)) Py_RETURN_NONE;
+    if (keep < 1 || recent < 0 || sinks < 0 || recent > keep || sinks > keep - recent) Py_RETURN_NONE;
+    const long long size = evict_workspace_entry(&c.cache, &c.places, keep);
+    if (size <= 0) Py_RETURN_NONE;
+    const at::TensorOptions like = at::TensorOptions().device(totals->device());
+    at::Tensor scratch = at::empty({size}, like.dtype(at::kByte)), out = at::empty({c.places.batch}, like.dtype(at::kInt));
+    if (!in_plain_memory(scratch, c.device) || !in_plain_memory(out, c.device)) Py_RETURN_NONE;
+    void *stream = stream_of(c), *workspace = scratch.data_ptr();
+    float *sums = static_cast<float *>(totals->data_ptr());
+    int *lengths = static_cast<int *>(out.data_ptr());
+    const long long of_sequence = totals->stride(0), of_head = totals->stride(1);
+    if (!launched([&] { evict_entry(&c.cache, &c.places, sums, of_sequence, of_head, keep, recent, sinks, lengths, workspace, size, stream); })) return nullptr;
+    return THPVariable_Wrap(std::move(out));
+}
+
+// ------------------------------------------------------------------------------------------------ projections
+// linear_product(codes, scales, inputs, outputs, blocksize, x, bias, out) -> out or None
+PyObject *linear_product_checked(PyObject *const *args) {
+    long long inputs, outputs, blocksize;
+    if (linear_entry == nullptr || !THPVariable_CheckExact(args[0]) || !THPVariable_Unpack(args[0]).is_cuda() || watched()) Py_RETURN_NONE;
+    const int device = c10::hip::current_device();
+    const at::Tensor *codes = plain(args[0], device), *scales = plain(args[1], device);
+    if (codes == nullptr || scales == nullptr || !whole(args[2], inputs) || !whole(args[3], outputs) || !whole(args[4], blocksize)) Py_RETURN_NONE;
+    if (inputs < 1 || inputs > 1 << 24 || outputs < 1 || outputs > 1 << 24 || (blocksize != 64 && blocksize != 128 && blocksize != 256)) Py_RETURN_NONE;
+    const long long tiles = (outputs + 15) / 16;
+    if (codes->scalar_type() != at::kByte || scales->scalar_type() != at::kFloat || codes->numel() != tiles * ((inputs + 127) / 128) * 1024 ||
+        scales->numel() != tiles * ((inputs + blocksize - 1) / blocksize) * 16)
+        Py_RETURN_NONE;
+    if (!THPVariable_CheckExact(args[5])) Py_RETURN_NONE;
+    const at::Tensor &x = THPVariable_Unpack(args[5]);
+    if (!in_memory(x, device) || slot_of(x.scalar_type()) < 0 || x.dim() < 1 || x.size(-1) != inputs || (x.requires_grad() && c10::GradMode::is_enabled())) Py_RETURN_NONE;
+    if (x.dim() == 2 ? inputs > 1 && x.stride(1) != 1 : !x.is_contiguous()) Py_RETURN_NONE;
+    const long long tokens = x.numel() / inputs;
+    const at::Tensor *bias = nullptr;
+    if (args[6] != Py_None) {
+        bias = plain(args[6], device);
+        if (bias == nullptr || bias->numel() != outputs || (bias->scalar_type() != at::kFloat && bias->scalar_type() != x.scalar_type()) ||
+            (bias->requires_grad() && c10::GradMode::is_enabled()))
+            Py_RETURN_NONE;
+    }
+    at::Tensor out;
+    if (args[7] == Py_None) {
+        c10::SmallVector<int64_t, 6> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = outputs;
+        out = at::empty(shape, at::TensorOptions().device(x.device()).dtype(x.scalar_type()));
+        if (!in_plain_memory(out, device)) Py_RETURN_NONE;
+    } else {
+        const at::Tensor *given = plain(args[7], device);
+        if (given == nullptr || given->scalar_type() != x.scalar_type() || given->dim() != x.dim() || given->size(-1) != outputs || !apart(*given, x)) Py_RETURN_NONE;
+        for (int64_t d = 0; d + 1 < x.dim(); ++d)
+            if (given->size(d) != x.size(d)) Py_RETURN_NONE;
+        out = *given;
+    }
+    const qtensor_linear weights = {static_cast<unsigned char *>(codes->data_ptr()), static_cast<float *>(scales->data_ptr()), (int)inputs, (int)outputs, (int)blocksize};
+    const qtensor_linear_call call = {x.data_ptr(), bias != nullptr ? bias->data_ptr() : nullptr, out.data_ptr(), x.dim() == 2 ? x.stride(0) : inputs, outputs, tokens,
+                                      slot_of(x.scalar_type()), bias != nullptr && bias->scalar_type() == at::kBFloat16};
+    void *stream = c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(device)).stream();
+    if (!launched([&] { linear_entry(&weights, &call, stream); })) return nullptr;
+    if (args[7] != Py_None) {
+        Py_INCREF(args[7]);
+        return args[7];
+    }
+    return THPVariable_Wrap(std::move(out));
+}
+
+// ------------------------------------------------------------------------------------------------ rotary positions
+// Queries and keys (which may be undefined) that turn_fits has passed, turned or turned back.
+bool turn_fits(const at::Tensor &t, const at::Tensor &first, int device, long long dims) {
+    return in_memory(t, device) && t.scalar_type() == first.scalar_type() && slot_of(t.scalar_type()) >= 0 && (t.dim() == 3 || t.dim() == 4) && t.dim() == first.dim() &&
+           t.size(-1) == first.size(-1) && t.size(-3) == first.size(-3) && t.size(0) == first.size(0) && t.size(-1) >= dims && t.size(-1) <= 1024 && t.size(-2) >= 1 &&
+           t.size(-2) <= 32767 && t.stride(-1) == 1;
+}
+bool positions_fit(const at::Tensor &p, const at::Tensor &first, int device) {
+    if (!in_memory(p, device) || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) || p.dim() < 1 || p.dim() > first.dim() - 2) return false;
+    return p.size(-1) == first.size(-3) && (p.dim() == 1 || p.size(0) == first.size(0)) && (p.size(-1) < 2 || p.stride(-1) == 1);
+}
+std::array<at::Tensor, 2> turned(const qtensor_rotary &rotary, const at::Tensor &q, const at::Tensor &k, const at::Tensor &positions) {
+    std::array<at::Tensor, 2> out;
+    qtensor_rotary_call call = {};
+    for (const at::Tensor *t : {&q, &k}) {
+        if (!t->defined()) continue;
+        at::Tensor &y = out[t == &k];
+        y = at::empty(t->sizes(), at::TensorOptions().device(t->device()).dtype(t->scalar_type()));
+        TORCH_CHECK(in_plain_memory(y, (int)t->get_device()), "a result that is not in memory");
+        const bool batch = t->dim() == 4;
+        call.part[call.parts++] = {t->data_ptr(), y.data_ptr(), batch ? t->stride(0) : 0, t->stride(-3), t->stride(-2), batch ? y.stride(0) : 0, y.stride(-3), y.stride(-2),
+                                   (int)t->size(-2)};
+    }
+    call.head_dim = (int)q.size(-1), call.is_bf16 = slot_of(q.scalar_type()), call.long_positions = positions.scalar_type() == at::kLong;
+    call.batch = q.dim() == 4 ? q.size(0) : 1, call.tokens = q.size(-3), call.position_batch = positions.dim() == 2 ? positions.stride(0) : 0;
+    call.positions = positions.data_ptr();
+    turn_entry(&rotary, &call, c10::hip::getCurrentHIPStream(static_cast<c10::DeviceIndex>(q.get_device())).stream());
+    TORCH_CHECK(last_error() == 0, "libqtensor_hip: ", last_error_string());
+    return out;
+}
+
+// The gradient of turning is turning back.  It is given what fits the kernel; gradients come as they are.
+struct Turn : torch::autograd::Function<Turn> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext *ctx, const at::Tensor &q, const std::optional<at::Tensor> &k, const at::Tensor &positions,
+                                                  const at::Tensor &frequencies, double magnitude, int64_t dims, bool interleaved, bool back) {
+        ctx->save_for_backward({positions, frequencies});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["magnitude"] = magnitude, ctx->saved_data["dims"] = dims, ctx->saved_data["interleaved"] = interleaved, ctx->saved_data["back"] = back;
+        const qtensor_rotary rotary = {static_cast<const double *>(frequencies.data_ptr()), magnitude, (int)dims, interleaved, back};
+        std::array<at::Tensor, 2> out = turned(rotary, q, k.value_or(at::Tensor()), positions);
+        return out[1].defined() ? torch::autograd::variable_list{out[0], out[1]} : torch::autograd::variable_list{out[0]};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        torch::autograd::variable_list out(8);
+        std::vector<at::Tensor> given;
+        std::vector<int> whose;
+        for (int i = 0; i < (int)grads.size(); ++i) {
+            if (!grads[i].defined() || !ctx->needs_input_grad(i)) continue;
+            given.push_back(grads[i].stride(-1) == 1 ? grads[i] : grads[i].contiguous());
+            whose.push_back(i);
+        }
+        if (given.empty()) return out;
+        const auto saved = ctx->get_saved_variables();
+        const c10::OptionalDeviceGuard guard(given[0].device());
+        const auto back = Turn::apply(given[0], given.size() > 1 ? std::optional<at::Tensor>(given[1]) : std::nullopt, saved[0], saved[1], ctx->saved_data["magnitude"].toDouble(),
+                                      ctx->saved_data["dims"].toInt(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["back"].toBool());
+        for (size_t n = 0; n < whose.size(); ++n) out[whose[n]] = back[n];
+        return out;
+    }
+};
+
+// rotary_turn(frequencies, magnitude, dims, interleaved, q, k, positions) -> (q, k) or None
+PyObject *rotary_turn_checked(PyObject *const *args) {
+    Angles angles;
+    if (turn_entry == nullptr || !THPVariable_CheckExact(args[0]) || !THPVariable_Unpack(args[0]).is_cuda() || watched()) Py_RETURN_NONE;
+    const int device = c10::hip::current_device();
+    if (!angles_of(args, device, 1024, angles) || !THPVariable_CheckExact(args[4]) || !THPVariable_CheckExact(args[6])) Py_RETURN_NONE;
+    const at::Tensor &q = THPVariable_Unpack(args[4]), &positions = THPVariable_Unpack(args[6]);
+    if (!turn_fits(q, q, device, angles.rotary.dims) || !positions_fit(positions, q, device)) Py_RETURN_NONE;
+    at::Tensor k;
+    if (args[5] != Py_None) {
+        if (!THPVariable_CheckExact(args[5])) Py_RETURN_NONE;
+        k = THPVariable_Unpack(args[5]);
+        if (!turn_fits(k, q, device, angles.rotary.dims)) Py_RETURN_NONE;
+    }
+    std::array<at::Tensor, 2> out;
+    struct Unlocked {                       // (a full queue blocks; exceptions pass with the lock taken again)
+        PyThreadState *state = PyEval_SaveThread();
+        ~Unlocked() { PyEval_RestoreThread(state); }
+    };
+    auto unlocked = std::make_unique<Unlocked>();
+    if (c10::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
+        const auto both = Turn::apply(q, k.defined() ? std::optional<at::Tensor>(k) : std::nullopt, positions, *angles.frequencies, angles.rotary.magnitude, (int64_t)angles.rotary.dims, angles.rotary.interleaved != 0, false);
+        out = {both[0], both.size() > 1 ? both[1] : at::Tensor()};
+    } else {
+        out = turned(angles.rotary, q, k, positions);
+    }
+    unlocked.reset();
+    PyObject *result = PyTuple_New(2);
+    if (result == nullptr) return nullptr;
+    PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(std::move(out[0])));
+    if (out[1].defined()) {
+        PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(std::move(out[1])));
+    } else {
+        Py_INCREF(Py_None);
+        PyTuple_SET_ITEM(result, 1, Py_None);
+    }
+    return result;
+}
+
+// Takes `count` addresses from a sequence; false with a Python error set.
+bool addresses_of(PyObject *list, const char *what, Py_ssize_t count, void **address) {
+    PyObject *items = PySequence_Fast(list, "a sequence of addresses is wanted");
+    if (items == nullptr) return false;
+    bool good = PySequence_Fast_GET_SIZE(items) == count;
+    for (Py_ssize_t i = 0; good && i < count; ++i) {
+        address[i] = PyLong_AsVoidPtr(PySequence_Fast_GET_ITEM(items, i));
+        good = address[i] != nullptr;
+    }
+    Py_DECREF(items);
+    if (!good && !PyErr_Occurred()) PyErr_Format(PyExc_ValueError, "%s takes %zd addresses", what, count);
+    return good;
+}
+
+// bind_model(addresses): the linear product, rotary turn, the cache's write_turned, weigh, weigh's workspace, evict, evict's workspace
+PyObject *bind_model(PyObject *, PyObject *list) {
+    void *address[7];
+    if (!addresses_of(list, "bind_model", 7, address)) return nullptr;
+    linear_entry = reinterpret_cast<decltype(linear_entry)>(address[0]);
+    turn_entry = reinterpret_cast<decltype(turn_entry)>(address[1]);
+    write_turned_entry = reinterpret_cast<decltype(write_turned_entry)>(address[2]);
+    weigh_entry = reinterpret_cast<decltype(weigh_entry)>(address[3]);
+    weigh_workspace_entry = reinterpret_cast<decltype(weigh_workspace_entry)>(address[4]);
+    evict_entry = reinterpret_cast<decltype(evict_entry)>(address[5]);
+    evict_workspace_entry = reinterpret_cast<decltype(evict_workspace_entry)>(address[6]);
+    Py_RETURN_NONE;
+}
+
 // bind_cache(addresses): write, read, attend, attend's workspace
 PyObject *bind_cache(PyObject *, PyObject *list) {
     PyObject *items = PySequence_Fast(list, "bind_cache takes a sequence of addresses");
@@ -405,8 +721,19 @@ PyMethodDef methods[] = {
      "cache_read(codes, scales, page_size, kv_heads, head_dim, blocksize, table, lengths, starts, tokens, dtype): (keys, values), None if not taken"},
     {"cache_attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<cache_attend_checked, 14>)), METH_FASTCALL,
      "cache_attend(codes, scales, page_size, kv_heads, head_dim, blocksize, q, table, lengths, starts, scale, window, sinks, out): out, None if not taken"},
+    {"cache_write_turned", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<cache_write_turned_checked, 18>)), METH_FASTCALL,
+     "cache_write_turned(codes, scales, page_size, kv_heads, head_dim, blocksize, frequencies, magnitude, dims, interleaved, q, keys, values, table, lengths, starts, positions, out): out, None if not taken"},
+    {"cache_weigh", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<cache_weigh_checked, 14>)), METH_FASTCALL,
+     "cache_weigh(codes, scales, page_size, kv_heads, head_dim, blocksize, totals, q, table, lengths, starts, scale, window, sinks): totals, None if not taken"},
+    {"cache_evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<cache_evict_checked, 12>)), METH_FASTCALL,
+     "cache_evict(codes, scales, page_size, kv_heads, head_dim, blocksize, totals, table, lengths, keep, recent, sinks): new lengths, None if not taken"},
+    {"bind_model", bind_model, METH_O, "addresses of the library's entry points for projections, rotary positions and eviction"},
+    {"linear_product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<linear_product_checked, 8>)), METH_FASTCALL,
+     "linear_product(codes, scales, inputs, outputs, blocksize, x, bias, out): out, None if not taken"},
+    {"rotary_turn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(guarded<rotary_turn_checked, 7>)), METH_FASTCALL,
+     "rotary_turn(frequencies, magnitude, dims, interleaved, q, k, positions): (q, k), None if not taken"},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", "one quantize, dequantize or attention cache call in native code", -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_direct", "one call of the quantizers, an attention cache, a projection or rotary positions in native code", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

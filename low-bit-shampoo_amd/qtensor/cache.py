@@ -136,6 +136,11 @@ class QTensorCache:
         values encoded, as `write` does with what rotary.turn gives.  positions: int32 or int64 [tokens], or None: a token's
         place in its sequence (which is another where tokens have been evicted).  Queries of tokens that are of no sequence or of a
         negative place become zeros.  out: optional result of the shape and type of q that shares no memory with it."""
+        if _native is not None:
+            done = _native.cache_write_turned(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, rotary.frequencies,
+                                              rotary.magnitude, rotary.dims, rotary.interleaved, q, keys, values, table, lengths, starts, positions, out)
+            if done is not None:
+                return done
         F._require_gpu(self.codes, "QTensorCache.write_turned")
         F._dtype_slot(q.dtype, "q")
         tokens, heads = (q.shape[0], q.shape[1]) if q.dim() == 3 else (-1, -1)
@@ -220,6 +225,11 @@ class QTensorCache:
         """Adds to totals (fp32 [batch, kv_heads, n], n at least what the table has room for) the weights softmax(scale q k) that `attend`, called with the
         same arguments, multiplies values with: for every token of a sequence and head of the cache the sum over the call's queries and over the query
         heads that read the head.  Sums are in fp32, in one order.  Returns totals."""
+        if _native is not None:
+            done = _native.cache_weigh(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, totals, q, table, lengths,
+                                       starts, scale, window, sinks)
+            if done is not None:
+                return done
         F._require_gpu(self.codes, "QTensorCache.weigh")
         tokens, heads, scale = self._check_queries(q, scale, window, sinks)
         places = self._places(table, lengths, starts, tokens)
@@ -241,6 +251,11 @@ class QTensorCache:
         `lengths`, so copy them there once all caches are done, set the totals behind them to zero before tokens are written there, and hand the
         pages behind back.  A position that a token was turned by stays its own: give write_turned positions from now on.  Tokens without a
         page are no candidates, and their places stay empty.  No two sequences of the call may share a page."""
+        if _native is not None:
+            done = _native.cache_evict(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, totals, table, lengths,
+                                       keep, recent, sinks)
+            if done is not None:
+                return done
         F._require_gpu(self.codes, "QTensorCache.evict")
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError(f"need a token to keep, and no more first and last ones than are kept (got {keep}, {sinks} and {recent}).")

@@ -84,6 +84,9 @@ if lib is not None:
         _direct.bind([ct.cast(fn, ct.c_void_p).value for fn in
                       [_STREAM_FN[(kind, bits, slot, diag)] for kind in ("quantize", "dequantize") for bits in (4, 8)
                        for slot in (0, 1) for diag in (False, True)] + [lib.qtensor_hip_last_error, lib.qtensor_hip_last_error_string]])
+        _direct.bind_model([ct.cast(getattr(lib, "qtensor_hip_" + name), ct.c_void_p).value
+                            for name in ("linear_product", "rotary_turn", "cache_write_turned", "cache_weigh", "cache_weigh_workspace", "cache_evict",
+                                         "cache_evict_workspace")])
 else:
     _direct = None
     lib_quan = {}

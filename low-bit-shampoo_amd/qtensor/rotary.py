@@ -92,6 +92,10 @@ class Rotary:
         """(q, k) turned: [.., tokens, heads, head_dim] with at most one dimension in front (fp32 or bf16, the last dimension contiguous),
         heads of both may differ in number; k may be None.  positions: int32 or int64 [tokens] or [batch, tokens], any values.  The
         gradients of q and k are theirs turned back."""
+        if F._direct is not None:
+            done = F._direct.rotary_turn(self.frequencies, self.magnitude, self.dims, self.interleaved, q, k, positions)
+            if done is not None:
+                return done
         return _Turn.apply(self, False, q, k, positions)
 
     def _turned(self, back, tensors, positions):
