@@ -190,7 +190,8 @@ void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
 template <bool BF16>
 void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
     if (a.tokens <= 16) launch_few<BF16, 1, 1, 8>(a, groups, stream);
-    else launch_few<BF16, 2, 2, 8>(a, groups, stream);
+    else if (a.tokens <= 128) launch_few<BF16, 2, 2, 8>(a, groups, stream);
+    else launch_linear_many(a, BF16, groups, stream);
 }
 
 bool linear_shape(const char *what, const qtensor_linear *w) {

@@ -1,0 +1,187 @@
+// Products of weights held in 4 bits with many tokens (layout: qt_linear.h).
+#include "qt_linear.h"
+
+#define QT_LDS __attribute__((address_space(3)))
+#define QT_GLOBAL __attribute__((address_space(1)))
+
+namespace qt {
+namespace {
+
+constexpr int kManyWaves = 4, kManyThreads = 64 * kManyWaves;
+constexpr int kManyTiles = 4;                       // of sixteen outputs of a wave
+constexpr int kManyOutputs = kManyWaves * kManyTiles * kLinearOutputs;
+constexpr int kXcds = 8;
+
+struct ManyGrid { int rows, columns, group; };      // tiles of tokens and of outputs; rows that are gone through together
+
+// A workgroup's tile: neighbours on an XCD (workgroups go round the XCDs in turn) take tiles that share tokens and outputs.
+__device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &column) {
+    const int all = g.rows * g.columns, each = (all + kXcds - 1) / kXcds;
+    const int index = (int)(blockIdx.x % kXcds) * each + (int)(blockIdx.x / kXcds);
+    if ((int)(blockIdx.x / kXcds) >= each || index >= all) return false;
+    const int group = index / (g.group * g.columns), rest = index - group * g.group * g.columns;
+    const int rows = min(g.group, g.rows - group * g.group);
+    column = rest / rows, row = group * g.group + rest - column * rows;
+    return true;
+}
+
+// A workgroup takes 16 MT tokens x 256 outputs, each wave all of the tokens and 64 outputs.  Tokens lie in LDS as the matrix instructions take
+// them (sixteen tokens x 32 inputs are 1 KB, 16 bytes a lane), two blocks of 128 inputs in turn; numbers of the next block are on their way in registers.
+template <bool BF16, int MT>
+__global__ __launch_bounds__(kManyThreads, 2) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift, const bool aligned) {
+    constexpr int P = Eight<BF16>::kPieces, GROUPS = 2, J = 4 / GROUPS, kBuffers = BF16 ? 2 : 1;
+    constexpr int kPlane = MT * 4 * 64;             // sixteen bytes each
+    __shared__ qt_u32x4 s_x[kBuffers * P * kPlane];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+    int row, column;
+    if (!many_tile(grid, row, column)) return;
+    const int first_token = row * 16 * MT, first_tile = column * (kManyOutputs / 16) + wave * kManyTiles;
+    const int tiles = (a.outputs + 15) >> 4;
+    const uint32_t code_at = 16 * lane, scale_at = lane & 15;
+    qt_u32x4 word[kManyTiles];
+    float scale[kManyTiles][GROUPS];
+    const auto load_weights = [&](int block) {
+#pragma unroll
+        for (int n = 0; n < kManyTiles; ++n) {
+            const long long tile = min(first_tile + n, tiles - 1);
+            word[n] = *(const qt_u32x4 *)(a.codes + ((tile * a.blocks + block) << 10) + code_at);
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g)
+                scale[n][g] = (a.scales + (tile * a.segments + min((block * GROUPS + g) >> shift, a.segments - 1)) * kLinearOutputs)[scale_at];
+        }
+    };
+    // a wave's part of a block of tokens: MT of the 4 MT pieces of 1 KB
+    Eight<BF16> raw[BF16 ? 1 : MT];
+    const uint8_t *from[MT / 4];
+    int valid[MT / 4];
+#pragma unroll
+    for (int i = 0; i < MT / 4; ++i) {
+        const int token = first_token + 16 * (wave * (MT / 4) + i) + (lane & 15);
+        valid[i] = token < a.tokens ? a.inputs : 0;
+        from[i] = (const uint8_t *)a.x + (long long)min(token, a.tokens - 1) * a.x_stride * (BF16 ? 2 : 4) + 8 * quarter * (BF16 ? 2 : 4);
+    }
+    const auto load_tokens = [&](int block, int buffer) {
+        const int first = block * kLinearInputs;
+        if constexpr (BF16) {
+            if (aligned && first + kLinearInputs <= a.inputs) {
+                // (tokens behind the last are the last one again: their results are not stored)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    __builtin_amdgcn_global_load_lds((const QT_GLOBAL void *)(from[i >> 2] + 2 * (first + 32 * (i & 3))),
+                                                     (QT_LDS void *)(s_x + buffer * kPlane + (wave * MT + i) * 64), 16, 0, 0);
+            } else {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    Eight<BF16> x;
+                    x.load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - 8 * quarter);
+                    s_x[buffer * kPlane + (wave * MT + i) * 64 + lane] = (qt_u32x4){x.raw[0], x.raw[1], x.raw[2], x.raw[3]};
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) raw[i].load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - 8 * quarter);
+        }
+    };
+    const auto put_tokens = [&]() {
+        if constexpr (!BF16) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                bf16x8 pieces[P];
+                raw[i].pieces(pieces);
+#pragma unroll
+                for (int n = 0; n < P; ++n) s_x[n * kPlane + (wave * MT + i) * 64 + lane] = __builtin_bit_cast(qt_u32x4, pieces[n]);
+                __builtin_amdgcn_sched_barrier(0);          // (one at a time: registers)
+            }
+        }
+    };
+    fp4_f32x4 sum[MT][kManyTiles];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < kManyTiles; ++n) sum[m][n] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
+    load_tokens(0, 0);
+    load_weights(0);
+    put_tokens();
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int block = 0; block < a.blocks; ++block) {
+        const int buffer = BF16 ? block & 1 : 0;
+        qt_u32x4 now[kManyTiles];
+        float by[kManyTiles][GROUPS];
+#pragma unroll
+        for (int n = 0; n < kManyTiles; ++n) {
+            now[n] = word[n];
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) by[n][g] = scale[n][g];
+        }
+        const bool more = block + 1 < a.blocks;
+        if (more) {
+            load_tokens(block + 1, BF16 ? buffer ^ 1 : 0);
+            load_weights(block + 1);
+        }
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            bf16x8 numbers[kManyTiles][J];
+#pragma unroll
+            for (int n = 0; n < kManyTiles; ++n)
+#pragma unroll
+                for (int j = 0; j < J; ++j) numbers[n][j] = fp4_to_bf16(now[n][g * J + j]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                fp4_f32x4 part[kManyTiles];
+#pragma unroll
+                for (int n = 0; n < kManyTiles; ++n) part[n] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    bf16x8 x[P];
+#pragma unroll
+                    for (int p = 0; p < P; ++p) x[p] = __builtin_bit_cast(bf16x8, s_x[(buffer * P + p) * kPlane + (m * 4 + g * J + j) * 64 + lane]);
+#pragma unroll
+                    for (int n = 0; n < kManyTiles; ++n) part[n] = multiply_pieces<P>(x, numbers[n][j], part[n]);
+                }
+#pragma unroll
+                for (int n = 0; n < kManyTiles; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[m][n][i] = __builtin_fmaf(by[n][g], part[n][i], sum[m][n][i]);
+            }
+        }
+        if constexpr (!BF16) {
+            __syncthreads();
+            if (more) put_tokens();
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < kManyTiles; ++n) {
+        const int output = (first_tile + n) * kLinearOutputs + (lane & 15);
+        if (output >= a.outputs) continue;
+        const float bias = linear_bias(a, output);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int token = first_token + 16 * m + 4 * quarter + i;
+                if (token < a.tokens) linear_store<BF16>(a, token, output, sum[m][n][i] + bias);
+            }
+    }
+}
+
+template <bool BF16, int MT>
+void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
+    const ManyGrid grid = {(a.tokens + 16 * MT - 1) / (16 * MT), (a.outputs + kManyOutputs - 1) / kManyOutputs, 8};
+    const long long all = (long long)grid.rows * grid.columns, blocks = (all + kXcds - 1) / kXcds * kXcds;
+    if (blocks > 0x7ffffff0LL) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
+    const int shift = scales_of_block == 2 ? 0 : 1 + a.scales_shift;
+    const bool aligned = is_aligned(a.x, 16) && a.x_stride % 8 == 0;
+    hipLaunchKernelGGL((linear_many_kernel<BF16, MT>), dim3((unsigned)blocks), dim3(kManyThreads), 0, stream, a, grid, shift, aligned);
+}
+
+}  // namespace
+
+void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
+    if (bf16) launch_many<true, 8>(a, scales_of_block, stream);
+    else launch_many<false, 4>(a, scales_of_block, stream);
+}
+
+}  // namespace qt
