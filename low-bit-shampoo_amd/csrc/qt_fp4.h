@@ -67,18 +67,24 @@ struct Eight {
 #pragma unroll
         for (uint32_t &r : raw) r = 0;
     }
-    // elements at .. at + 7 of a row, those from `valid` on as zeros
+    // elements at .. at + 7 of a row
+    __device__ __forceinline__ void load(const void *row, int at) {
+        if constexpr (BF16) {
+            const qt_u32x4 v = ((const Unaligned16 *)((const uint16_t *)row + at))->v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[e] = v[e];
+        } else {
+            const qt_u32x4 v = ((const Unaligned16of4 *)((const float *)row + at))->v, w = ((const Unaligned16of4 *)((const float *)row + at + 4))->v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[e] = v[e], raw[4 + e] = w[e];
+        }
+    }
+    // those from `valid` on as zeros
     __device__ __forceinline__ void load(const void *row, int at, int valid) {
         if (at + 8 <= valid) {
-            if constexpr (BF16) {
-                const qt_u32x4 v = ((const Unaligned16 *)((const uint16_t *)row + at))->v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) raw[e] = v[e];
-            } else {
-                const qt_u32x4 v = ((const Unaligned16of4 *)((const float *)row + at))->v, w = ((const Unaligned16of4 *)((const float *)row + at + 4))->v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) raw[e] = v[e], raw[4 + e] = w[e];
-            }
+            load(row, at);
+        } else if (at >= valid) {
+            zero();
         } else {
 #pragma unroll
             for (int e = 0; e < (BF16 ? 4 : 8); ++e) {
@@ -96,23 +102,29 @@ struct Eight {
         if constexpr (BF16) {
             out[0] = __builtin_bit_cast(bf16x8, (qt_u32x4){raw[0], raw[1], raw[2], raw[3]});
         } else {
+            uint32_t part[3][8];
+            float last = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float rest = __uint_as_float(raw[e]) - __uint_as_float(raw[e] & 0xffff0000u);
+                part[0][e] = raw[e], part[1][e] = __float_as_uint(rest);
+                const float tail = rest - __uint_as_float(part[1][e] & 0xffff0000u);
+                part[2][e] = __float_as_uint(tail);
+                last = e ? last + tail : tail;
+            }
+            if (__builtin_expect(__builtin_isunordered(last, last), 0)) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if ((raw[e] & 0x7f800000u) != 0x7f800000u) continue;
+                    if (raw[e] & 0x7fffffu) part[0][e] |= 0x400000u;            // (NaN whose bits are all in the part cut off)
+                    part[1][e] = part[2][e] = 0;
+                }
+            }
             qt_u32x4 p[3];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t part[2][3];
+            for (int n = 0; n < 3; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t u = raw[2 * e + i];
-                    const bool finite = (u & 0x7f800000u) != 0x7f800000u;
-                    if (!finite && (u & 0x7fffffu)) u |= 0x400000u;             // (NaN whose bits are all in the part cut off)
-                    const float rest = finite ? __uint_as_float(u) - __uint_as_float(u & 0xffff0000u) : 0.0f;
-                    part[i][0] = u;
-                    part[i][1] = __float_as_uint(rest);
-                    part[i][2] = __float_as_uint(rest - __uint_as_float(part[i][1] & 0xffff0000u));
-                }
-#pragma unroll
-                for (int n = 0; n < 3; ++n) p[n][e] = __builtin_amdgcn_perm(part[1][n], part[0][n], 0x07060302u);     // (upper halves of both)
-            }
+                for (int e = 0; e < 4; ++e) p[n][e] = __builtin_amdgcn_perm(part[n][2 * e + 1], part[n][2 * e], 0x07060302u);     // (upper halves of both)
 #pragma unroll
             for (int n = 0; n < 3; ++n) out[n] = __builtin_bit_cast(bf16x8, p[n]);
         }

@@ -28,7 +28,8 @@ struct LinearArgs {
     bool bias_bf16;
 };
 
-// The product for many tokens (qt_linear_many.hip).
+// The product for many tokens (qt_linear_many.hip), and of how many workgroups it is at least.
+long long linear_many_workgroups(const LinearArgs &a);
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream);
 
 #if defined(__HIPCC__)

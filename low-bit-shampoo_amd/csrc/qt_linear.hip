@@ -88,29 +88,19 @@ __global__ __launch_bounds__(kCodeThreads) void linear_copy_kernel(const LinearC
 
 // Products of few tokens: a wave multiplies R tiles of 16 outputs with T of 16 tokens, and the WAVES waves of a workgroup take the blocks of 128
 // inputs in turn; their sums are joined through LDS, in the order of the waves.
-template <bool BF16, int T, int R, int WAVES, int GROUPS>
+template <bool BF16, int T, int R, int WAVES, int GROUPS, bool STREAM>
 __global__ __launch_bounds__(64 * WAVES) void linear_few_kernel(const LinearArgs a) {
-    constexpr int P = Eight<BF16>::kPieces;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
+    constexpr int P = Eight<BF16>::kPieces, J = 4 / GROUPS;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
     const int tiles = (a.outputs + kLinearOutputs - 1) / kLinearOutputs;
     const int first_tile = blockIdx.x * R, first_token = blockIdx.y * 16 * T;
     __shared__ fp4_f32x4 s_part[WAVES - 1][R * T][64];
-    const uint8_t *codes[R];
-    const float *scales[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const long long tile = min(first_tile + r, tiles - 1);
-        codes[r] = a.codes + ((tile * a.blocks) << 10) + 16 * lane;
-        scales[r] = a.scales + tile * a.segments * kLinearOutputs + (lane & 15);
-    }
+    const uint32_t code_at = 16 * lane, scale_at = lane & 15;
+    // (tokens and tiles behind the last are the last one again: what comes of them is not stored)
     const uint8_t *x[T];
-    int valid[T];
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-        const int token = first_token + 16 * t + (lane & 15);
-        valid[t] = token < a.tokens ? a.inputs : 0;
-        x[t] = (const uint8_t *)a.x + (long long)min(token, a.tokens - 1) * a.x_stride * (BF16 ? 2 : 4);
-    }
+    for (int t = 0; t < T; ++t)
+        x[t] = (const uint8_t *)a.x + ((long long)min(first_token + 16 * t + (lane & 15), a.tokens - 1) * a.x_stride + 8 * quarter) * (BF16 ? 2 : 4);
     fp4_f32x4 sum[R][T];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -121,38 +111,49 @@ __global__ __launch_bounds__(64 * WAVES) void linear_few_kernel(const LinearArgs
         float scale[R][GROUPS];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            word[r] = *(const qt_u32x4 *)(codes[r] + ((long long)block << 10));
+            const long long tile = min(first_tile + r, tiles - 1);
+            word[r] = __builtin_bit_cast(qt_u32x4, load_u32x4<STREAM>(a.codes + ((tile * a.blocks + block) << 10) + code_at));
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) scale[r][g] = scales[r][(long long)min((block * GROUPS + g) >> a.scales_shift, a.segments - 1) * kLinearOutputs];
+            for (int g = 0; g < GROUPS; ++g)
+                scale[r][g] = (a.scales + (tile * a.segments + min((block * GROUPS + g) >> a.scales_shift, a.segments - 1)) * kLinearOutputs)[scale_at];
         }
         Eight<BF16> raw[T][4];
+        const int at = block * kLinearInputs;
+        if (at + kLinearInputs <= a.inputs) {
 #pragma unroll
-        for (int t = 0; t < T; ++t)
+            for (int t = 0; t < T; ++t)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) raw[t][j].load(x[t], kLinearInputs * block + 32 * j + 8 * quarter, valid[t]);
+                for (int j = 0; j < 4; ++j) raw[t][j].load(x[t], at + 32 * j);
+        } else {
+#pragma unroll
+            for (int t = 0; t < T; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) raw[t][j].load(x[t], at + 32 * j, a.inputs - 8 * quarter);
+        }
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-            fp4_f32x4 part[R][T];
-#pragma unroll
-            for (int j = g * (4 / GROUPS); j < (g + 1) * (4 / GROUPS); ++j) {
-                bf16x8 numbers[R];
-#pragma unroll
-                for (int r = 0; r < R; ++r) numbers[r] = fp4_to_bf16(word[r][j]);
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    bf16x8 pieces[P];
-                    raw[t][j].pieces(pieces);
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-                        part[r][t] = multiply_pieces<P>(pieces, numbers[r], j == g * (4 / GROUPS) ? (fp4_f32x4){0.f, 0.f, 0.f, 0.f} : part[r][t]);
-                }
-            }
+            bf16x8 numbers[R][J];
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int t = 0; t < T; ++t)
+                for (int j = 0; j < J; ++j) numbers[r][j] = fp4_to_bf16(word[r][g * J + j]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum[r][t][i] = __builtin_fmaf(scale[r][g], part[r][t][i], sum[r][t][i]);
+            for (int t = 0; t < T; ++t) {
+                fp4_f32x4 part[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) part[r] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    bf16x8 pieces[P];
+                    raw[t][g * J + j].pieces(pieces);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) part[r] = multiply_pieces<P>(pieces, numbers[r][j], part[r]);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[r][t][i] = __builtin_fmaf(scale[r][g], part[r][i], sum[r][t][i]);
+            }
         }
     }
     if (wave) {
@@ -183,15 +184,28 @@ __global__ __launch_bounds__(64 * WAVES) void linear_few_kernel(const LinearArgs
 template <bool BF16, int T, int R, int WAVES>
 void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
     const dim3 grid((unsigned)(((a.outputs + 15) / 16 + R - 1) / R), (unsigned)((a.tokens + 16 * T - 1) / (16 * T)));
-    if (groups == 2) hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 2>), grid, dim3(64 * WAVES), 0, stream, a);
-    else hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 1>), grid, dim3(64 * WAVES), 0, stream, a);
+    if (groups == 2) hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 2, T == 1>), grid, dim3(64 * WAVES), 0, stream, a);
+    else hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 1, T == 1>), grid, dim3(64 * WAVES), 0, stream, a);
 }
 
+// Many tokens as soon as the kernel for them has a workgroup for every unit: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 24 us here
+// and 38 there, 512 and 4096 (256) 41 and 39, 256 and 11008 (344) 58 and 42.
+// Else the smallest tile of a workgroup whose workgroups have a unit each: every one reads all of its tokens (from L2) and joins its waves, so
+// more of them than that cost more than they spread.  By tiles of outputs x tokens: 16 tokens, 4096 outputs 1 x 1 6.7 us, 2 x 1 7.9, 4 x 1 10.1; 14336
+// outputs 18.3, 12.6, 10.5; 64 tokens, 4096 outputs 4 x 1 10.5, 4 x 2 15.4.  Four waves to a workgroup where there are several for each unit (32 tokens, 28672
+// outputs 25.1 us against 26.0 of eight).
 template <bool BF16>
 void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
-    if (a.tokens <= 16) launch_few<BF16, 1, 1, 8>(a, groups, stream);
-    else if (a.tokens <= 128) launch_few<BF16, 2, 2, 8>(a, groups, stream);
-    else launch_linear_many(a, BF16, groups, stream);
+    const long long tiles = (a.outputs + 15) / 16, rows = (a.tokens + 15) / 16, units = compute_units();
+    if (linear_many_workgroups(a) >= units) return launch_linear_many(a, BF16, groups, stream);
+    if (tiles * rows <= units) return launch_few<BF16, 1, 1, 8>(a, groups, stream);
+    if ((tiles + 1) / 2 * rows <= units) return launch_few<BF16, 1, 2, 8>(a, groups, stream);
+    if ((tiles + 3) / 4 * rows <= units) return launch_few<BF16, 1, 4, 8>(a, groups, stream);
+    if constexpr (BF16) {
+        if (rows > 1 && (tiles + 3) / 4 * ((rows + 1) / 2) <= units) return launch_few<BF16, 2, 4, 8>(a, groups, stream);
+        if (rows > 1) return launch_few<BF16, 2, 4, 4>(a, groups, stream);
+    }
+    launch_few<BF16, 1, 4, 4>(a, groups, stream);
 }
 
 bool linear_shape(const char *what, const qtensor_linear *w) {

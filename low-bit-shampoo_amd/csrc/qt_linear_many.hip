@@ -8,8 +8,6 @@ namespace qt {
 namespace {
 
 constexpr int kManyWaves = 4, kManyThreads = 64 * kManyWaves;
-constexpr int kManyTiles = 4;                       // of sixteen outputs of a wave
-constexpr int kManyOutputs = kManyWaves * kManyTiles * kLinearOutputs;
 constexpr int kXcds = 8;
 
 struct ManyGrid { int rows, columns, group; };      // tiles of tokens and of outputs; rows that are gone through together
@@ -25,24 +23,30 @@ __device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &colu
     return true;
 }
 
-// A workgroup takes 16 MT tokens x 256 outputs, each wave all of the tokens and 64 outputs.  Tokens lie in LDS as the matrix instructions take
-// them (sixteen tokens x 32 inputs are 1 KB, 16 bytes a lane), two blocks of 128 inputs in turn; numbers of the next block are on their way in registers.
-template <bool BF16, int MT>
-__global__ __launch_bounds__(kManyThreads, 2) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift, const bool aligned) {
+// A workgroup takes 16 MT tokens x 64 N outputs, each wave all of the tokens and 16 N outputs.  Tokens lie in LDS as the matrix instructions take
+// them (sixteen tokens x 32 inputs are 1 KB, 16 bytes a lane), in bf16 two blocks of 128 inputs in turn, straight from memory where rows are aligned;
+// numbers of the next block are on their way in registers.  They are exact in bf16, and scales multiply the sums of 64 inputs: four vector
+// operations beside every two matrix ones, and as many to expand the numbers, are what a wave does beside them.
+//
+// Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 535 us, 1010 TFLOP/s, where the
+// library's product of bf16 matrices takes 519 us; 1024 tokens through 4096 x 4096 43 us, 800 TFLOP/s; 2048 tokens through 11008 x 4096 in fp32 (three
+// matrix operations for each) 514 us, 359 TFLOP/s.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers).
+template <bool BF16, int MT, int N>
+__global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift, const bool aligned) {
     constexpr int P = Eight<BF16>::kPieces, GROUPS = 2, J = 4 / GROUPS, kBuffers = BF16 ? 2 : 1;
     constexpr int kPlane = MT * 4 * 64;             // sixteen bytes each
     __shared__ qt_u32x4 s_x[kBuffers * P * kPlane];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
     int row, column;
     if (!many_tile(grid, row, column)) return;
-    const int first_token = row * 16 * MT, first_tile = column * (kManyOutputs / 16) + wave * kManyTiles;
+    const int first_token = row * 16 * MT, first_tile = column * (kManyWaves * N) + wave * N;
     const int tiles = (a.outputs + 15) >> 4;
     const uint32_t code_at = 16 * lane, scale_at = lane & 15;
-    qt_u32x4 word[kManyTiles];
-    float scale[kManyTiles][GROUPS];
+    qt_u32x4 word[N];
+    float scale[N][GROUPS];
     const auto load_weights = [&](int block) {
 #pragma unroll
-        for (int n = 0; n < kManyTiles; ++n) {
+        for (int n = 0; n < N; ++n) {
             const long long tile = min(first_tile + n, tiles - 1);
             word[n] = *(const qt_u32x4 *)(a.codes + ((tile * a.blocks + block) << 10) + code_at);
 #pragma unroll
@@ -94,11 +98,11 @@ __global__ __launch_bounds__(kManyThreads, 2) void linear_many_kernel(const Line
             }
         }
     };
-    fp4_f32x4 sum[MT][kManyTiles];
+    fp4_f32x4 sum[MT][N];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int n = 0; n < kManyTiles; ++n) sum[m][n] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < N; ++n) sum[m][n] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
     load_tokens(0, 0);
     load_weights(0);
     put_tokens();
@@ -106,10 +110,10 @@ __global__ __launch_bounds__(kManyThreads, 2) void linear_many_kernel(const Line
     __syncthreads();
     for (int block = 0; block < a.blocks; ++block) {
         const int buffer = BF16 ? block & 1 : 0;
-        qt_u32x4 now[kManyTiles];
-        float by[kManyTiles][GROUPS];
+        qt_u32x4 now[N];
+        float by[N][GROUPS];
 #pragma unroll
-        for (int n = 0; n < kManyTiles; ++n) {
+        for (int n = 0; n < N; ++n) {
             now[n] = word[n];
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) by[n][g] = scale[n][g];
@@ -121,26 +125,26 @@ __global__ __launch_bounds__(kManyThreads, 2) void linear_many_kernel(const Line
         }
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-            bf16x8 numbers[kManyTiles][J];
+            bf16x8 numbers[N][J];
 #pragma unroll
-            for (int n = 0; n < kManyTiles; ++n)
+            for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int j = 0; j < J; ++j) numbers[n][j] = fp4_to_bf16(now[n][g * J + j]);
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                fp4_f32x4 part[kManyTiles];
+                fp4_f32x4 part[N];
 #pragma unroll
-                for (int n = 0; n < kManyTiles; ++n) part[n] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
+                for (int n = 0; n < N; ++n) part[n] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     bf16x8 x[P];
 #pragma unroll
                     for (int p = 0; p < P; ++p) x[p] = __builtin_bit_cast(bf16x8, s_x[(buffer * P + p) * kPlane + (m * 4 + g * J + j) * 64 + lane]);
 #pragma unroll
-                    for (int n = 0; n < kManyTiles; ++n) part[n] = multiply_pieces<P>(x, numbers[n][j], part[n]);
+                    for (int n = 0; n < N; ++n) part[n] = multiply_pieces<P>(x, numbers[n][j], part[n]);
                 }
 #pragma unroll
-                for (int n = 0; n < kManyTiles; ++n)
+                for (int n = 0; n < N; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum[m][n][i] = __builtin_fmaf(by[n][g], part[n][i], sum[m][n][i]);
             }
@@ -153,7 +157,7 @@ __global__ __launch_bounds__(kManyThreads, 2) void linear_many_kernel(const Line
         __syncthreads();
     }
 #pragma unroll
-    for (int n = 0; n < kManyTiles; ++n) {
+    for (int n = 0; n < N; ++n) {
         const int output = (first_tile + n) * kLinearOutputs + (lane & 15);
         if (output >= a.outputs) continue;
         const float bias = linear_bias(a, output);
@@ -167,21 +171,32 @@ __global__ __launch_bounds__(kManyThreads, 2) void linear_many_kernel(const Line
     }
 }
 
-template <bool BF16, int MT>
+template <bool BF16, int MT, int N>
 void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
-    const ManyGrid grid = {(a.tokens + 16 * MT - 1) / (16 * MT), (a.outputs + kManyOutputs - 1) / kManyOutputs, 8};
+    const ManyGrid grid = {(a.tokens + 16 * MT - 1) / (16 * MT), (a.outputs + 64 * N - 1) / (64 * N), 8};
     const long long all = (long long)grid.rows * grid.columns, blocks = (all + kXcds - 1) / kXcds * kXcds;
     if (blocks > 0x7ffffff0LL) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
     const int shift = scales_of_block == 2 ? 0 : 1 + a.scales_shift;
     const bool aligned = is_aligned(a.x, 16) && a.x_stride % 8 == 0;
-    hipLaunchKernelGGL((linear_many_kernel<BF16, MT>), dim3((unsigned)blocks), dim3(kManyThreads), 0, stream, a, grid, shift, aligned);
+    hipLaunchKernelGGL((linear_many_kernel<BF16, MT, N>), dim3((unsigned)blocks), dim3(kManyThreads), 0, stream, a, grid, shift, aligned);
 }
 
 }  // namespace
 
+long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.tokens + 63) / 64) * ((a.outputs + 127) / 128); }
+
+// Large tiles use what they read more often, but leave units idle until there are four workgroups for each: 4096 inputs in bf16, 128 x 256 against
+// 64 x 128, 1024 tokens and 4096 outputs 101 and 43 us, 2048 and 11008 218 and 219, 6000 and 11008 545 and 634; in fp32 64 x 192 against 64 x 128,
+// 256 and 4096 99 and 80, 2048 and 11008 514 and 567.
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
-    if (bf16) launch_many<true, 8>(a, scales_of_block, stream);
-    else launch_many<false, 4>(a, scales_of_block, stream);
+    const long long large = bf16 ? (long long)((a.tokens + 127) / 128) * ((a.outputs + 255) / 256) : (long long)((a.tokens + 63) / 64) * ((a.outputs + 191) / 192);
+    if (large >= 4LL * compute_units()) {
+        if (bf16) launch_many<true, 8, 4>(a, scales_of_block, stream);
+        else launch_many<false, 4, 3>(a, scales_of_block, stream);
+    } else {
+        if (bf16) launch_many<true, 4, 2>(a, scales_of_block, stream);
+        else launch_many<false, 4, 2>(a, scales_of_block, stream);
+    }
 }
 
 }  // namespace qt

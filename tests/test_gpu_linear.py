@@ -77,6 +77,26 @@ def test_larger_products(Linear, tokens, inputs, outputs, dtype):
     check(Linear(inputs, outputs).quantize(w.cuda()).product(x.cuda()), x, w, 64)
 
 
+@pytest.mark.parametrize("tokens,inputs,outputs", [(1030, 130, 2100), (1100, 64, 2050), (4200, 70, 8200), (70, 385, 33000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_tokens_and_outputs(Linear, tokens, inputs, outputs, dtype):
+    """Enough of both for the kernels of many tokens, with edges in every direction; tokens that are not finite, rows that are not aligned."""
+    w, x = matrix(outputs, inputs, dtype, 4), matrix(tokens, inputs, dtype, 5)
+    held, bias = Linear(inputs, outputs, blocksize=128).quantize(w.cuda()), torch.randn(outputs, generator=torch.Generator().manual_seed(6))
+    got = held.product(x.cuda(), bias.cuda())
+    check(got, x, w, 128, bias)
+    wide = torch.full((tokens, inputs + 3), math.nan, dtype=dtype, device="cuda")
+    wide[:, 1:inputs + 1] = x.cuda()
+    assert torch.equal(held.product(wide[:, 1:inputs + 1], bias.cuda()), got)
+    wide = torch.full((tokens, inputs + 8 - inputs % 8), math.nan, dtype=dtype, device="cuda")
+    wide[:, :inputs] = x.cuda()
+    wide[tokens // 2, 3] = math.inf
+    other = held.product(wide[:, :inputs], bias.cuda())
+    assert not bool(torch.isfinite(other[tokens // 2]).any())
+    other[tokens // 2] = got[tokens // 2]
+    assert torch.equal(other, got)
+
+
 @pytest.mark.parametrize("tokens", [1, 20, 300])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strides_shapes_and_given_results(Linear, tokens, dtype):
