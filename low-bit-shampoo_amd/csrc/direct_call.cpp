@@ -466,7 +466,7 @@ PyObject *cache_weigh_checked(PyObject *const *args) {
     if (t == nullptr || t->size(1) < 1 || t->size(1) > 32767 || t->size(1) % c.cache.kv_heads != 0 || !places_of(args + 8, c, t->size(0))) Py_RETURN_NONE;
     const at::Tensor *totals = totals_of(args[6], c);
     const int heads = (int)t->size(1);
-    if (totals == nullptr || t->size(0) * (heads / c.cache.kv_heads) > INT_MAX - 256) Py_RETURN_NONE;
+    if (totals == nullptr || t->size(0) * (heads / c.cache.kv_heads) >= 1ll << 29) Py_RETURN_NONE;
     double scale = 1.0 / std::sqrt((double)c.cache.head_dim);
     if (args[11] != Py_None) {
         if (!PyFloat_CheckExact(args[11])) Py_RETURN_NONE;

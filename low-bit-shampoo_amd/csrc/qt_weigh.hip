@@ -8,16 +8,21 @@
 // Scores come from the matrix cores with all bits: keys' numbers are exact in bf16, fp32 queries go through in three pieces (qt_fp4.h).
 #include "qt_cache.h"
 
+#define QT_CONSTANT __attribute__((address_space(4)))
+
 namespace qt {
 namespace {
 
 constexpr int kWeighThreads = 256, kWeighWaves = 4;
+constexpr int kParts = 16;             // of a row's tokens, at most
+constexpr int kLeastTiles = 16;        // of a part
 
 struct WeighArgs {
     CacheShape shape;
     CachePlaces at;
     const uint8_t *codes;
     const float *scales;
+    long long code_page, scale_page;    // bytes and scales of a page
     const void *q;
     long long q_token, q_head;
     int group;
@@ -25,19 +30,34 @@ struct WeighArgs {
     int window, sinks;                  // window 0: no window
     float *totals;
     long long total_sequence, total_head;
-    float2 *partial;                    // [token][head][splits]: (m, l) of a row
-    int splits;
+    float2 *partial;                    // [head][row][parts]: (m, l) of each part of a row's tokens, rows of all sequences in order
+    float2 *statistics;                 // [head][row]: (m, 1 / l); (0, 0) where nothing is seen
+    int parts;                          // at most
+    long long wanted;                   // workgroups that the rows' work is cut for
+    FastDiv by_group, by_tiles;         // and by tiles of rows of a token
 };
 
 // Rows (i, g) of a sequence and what they see.
 struct WeighSequence {
     int start, count, first_position, end;
+
+    __device__ __forceinline__ int position(const WeighArgs &a, int row) const { return first_position + (int)fastdiv((uint32_t)row, a.by_group); }
 };
+// Where a row's statistics lie.
+__device__ __forceinline__ long long row_entry(const WeighArgs &a, const WeighSequence &v, int head, int row) {
+    return ((long long)head * a.at.tokens + v.start) * a.group + row;
+}
+template <bool UNIFORM>
+__device__ __forceinline__ int load_int(const int *p) {
+    return UNIFORM ? *(const QT_CONSTANT int *)p : *p;
+}
+// UNIFORM: b is the same for all lanes
+template <bool UNIFORM>
 __device__ __forceinline__ WeighSequence weigh_sequence(const WeighArgs &a, int b) {
     WeighSequence v;
-    const int length = a.at.lengths[b];
-    v.start = a.at.starts ? a.at.starts[b] : b;
-    v.count = a.at.starts ? a.at.starts[b + 1] - v.start : 1;
+    const int length = load_int<UNIFORM>(a.at.lengths + b);
+    v.start = a.at.starts ? load_int<UNIFORM>(a.at.starts + b) : b;
+    v.count = a.at.starts ? load_int<UNIFORM>(a.at.starts + b + 1) - v.start : 1;
     if (v.start < 0 || v.count < 0 || (long long)v.start + v.count > a.at.tokens) v.count = 0;      // (not a list of starts: nothing)
     v.first_position = length - v.count;
     const long long covered = (long long)a.at.table_pages << a.shape.page_shift;
@@ -54,73 +74,154 @@ template <bool BF16, int STEPS>
 struct WeighRows {
     bf16x8 x[STEPS][Eight<BF16>::kPieces];
 
-    __device__ __forceinline__ void load(const WeighArgs &a, const WeighSequence &v, int head, int first_row, int steps) {
-        const int lane = threadIdx.x & 63, row = first_row + (lane & 15), rows = v.count * a.group;
-        const int i = row / a.group;
-        const uint8_t *p = (const uint8_t *)a.q + ((long long)(v.start + (row < rows ? i : 0)) * a.q_token + (long long)(head * a.group + (row < rows ? row - i * a.group : 0)) * a.q_head) * (BF16 ? 2 : 4);
-        Eight<BF16> raw[STEPS];
+    Eight<BF16> raw[STEPS];
+
+    __device__ __forceinline__ void fetch(const WeighArgs &a, const WeighSequence &v, int head, int first_row) {
+        const int lane = threadIdx.x & 63, row = min(first_row + (lane & 15), v.count * a.group - 1), i = (int)fastdiv((uint32_t)row, a.by_group);
+        const int steps = a.shape.row_bytes >> 4;
+        const uint8_t *p = (const uint8_t *)a.q + ((v.start + i) * a.q_token + (head * a.group + row - i * a.group) * a.q_head + 8 * (lane >> 4)) * (BF16 ? 2 : 4);
+        if (a.shape.head_dim == 32 * STEPS) {
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) {
-            raw[j].zero();
-            if (j < steps) raw[j].load(p, 32 * j + 8 * (lane >> 4), row < rows ? a.shape.head_dim : 0);
+            for (int j = 0; j < STEPS; ++j) raw[j].load(p, 32 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) {
+                raw[j].zero();
+                if (j < steps) raw[j].load(p, 32 * j, a.shape.head_dim - 8 * (lane >> 4));
+            }
         }
+    }
+    // (rows behind the last are the last one again: what comes of them is not used)
+    __device__ __forceinline__ void arrange() {
 #pragma unroll
         for (int j = 0; j < STEPS; ++j) raw[j].pieces(x[j]);
     }
 };
 
-// Sixteen tokens' keys: numbers as they lie, and the scales of up to four segments.
-template <int STEPS>
-struct WeighKeys {
-    uint32_t word[STEPS];
-    float scale[STEPS / 2];
-    bool there;
+// Four words of the lanes l, l + 16, l + 32, l + 48: word j of the qth of them and word q of the jth change places.
+__device__ __forceinline__ void transpose_quarters(uint32_t *w) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const auto two = __builtin_amdgcn_permlane32_swap(w[i], w[i + 2], false, false);
+        w[i] = two[0], w[i + 2] = two[1];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        const auto two = __builtin_amdgcn_permlane16_swap(w[i], w[i + 1], false, false);
+        w[i] = two[0], w[i + 1] = two[1];
+    }
+}
+// Word q of lane l to all of l % 16 + 16 i, where it is that of lane l % 16 + 16 q.
+__device__ __forceinline__ void spread_quarters(uint32_t w, uint32_t *each) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    const auto low = __builtin_amdgcn_permlane16_swap(halves[0], halves[0], false, false), high = __builtin_amdgcn_permlane16_swap(halves[1], halves[1], false, false);
+    each[0] = low[0], each[1] = low[1], each[2] = high[0], each[3] = high[1];
+}
 
-    // `tile`: of sixteen tokens of sequence b, in front of `end`
-    __device__ __forceinline__ void load(const WeighArgs &a, int b, int head, int tile, int end, int steps) {
-        const int lane = threadIdx.x & 63;
-        const int first = tile << 4, nth = first >> a.shape.page_shift;
-        int page = -1;
-        if (first < end) page = a.at.table[b * a.at.table_stride + nth];
-        there = (unsigned)page < (unsigned)a.shape.pages;
-        const long long line = ((long long)(there ? page : 0) * a.shape.kv_heads + head) << a.shape.page_shift;
-        const long long inside = (there ? first & ((1 << a.shape.page_shift) - 1) : 0) + (lane & 15);
-        const uint8_t *p = a.codes + (line + inside) * a.shape.row_bytes + 4 * (lane >> 4);
+// Keys of N tiles of sixteen tokens: numbers as matrix operands want them, eight of each step of 32 elements a lane, and scales.  Lanes load sixteen
+// bytes, a quarter of the wave a step of all tokens, and exchange words; scales likewise, a quarter 64 elements (which are in one segment of any size).
+template <int STEPS, int N>
+struct WeighKeys {
+    static constexpr int kSegments = STEPS / 2, kFetches = N * STEPS / 4, kScales = N * kSegments / 4;
+    qt_u32x4 raw[kFetches];
+    float raw_scale[kScales];
+    bool there[N];
+    uint32_t word[N][STEPS];
+    float scale[N][kSegments];
+
+    // asks for tile `first` and those behind it, of sequence b in front of `end`; `first` a multiple of N and the same for all lanes
+    __device__ __forceinline__ void fetch(const WeighArgs &a, int b, int head, int first, int end) {
+        const int lane = threadIdx.x & 63, quarter = lane >> 4, token = lane & 15, steps = a.shape.row_bytes >> 4;
+        // (steps and segments that the heads do not have are the first and the last one again: queries are zero there)
+        const auto page_of = [&](int tile) {
+            const int at = tile << 4;
+            return at < end ? load_int<true>(a.at.table + b * a.at.table_stride + (at >> a.shape.page_shift)) : -1;
+        };
+        const auto codes_of = [&](int page, int tile) {
+            return a.codes + (long long)page * a.code_page + (((long long)head << a.shape.page_shift) + ((tile << 4) & ((1 << a.shape.page_shift) - 1))) * a.shape.row_bytes;
+        };
+        const auto scales_of = [&](int page, int tile) {
+            return a.scales + (long long)page * a.scale_page + ((long long)(head * a.shape.segments) << a.shape.page_shift) + ((tile << 4) & ((1 << a.shape.page_shift) - 1));
+        };
+        const auto step_of = [&](int f) {                   // what a lane loads of a tile: a step, and for short heads one of two tiles
+            const int step = STEPS == 2 ? quarter & 1 : quarter + 4 * (f % (STEPS / 4));
+            return (token + (STEPS == 2 ? 16 * (quarter >> 1) : 0)) * a.shape.row_bytes + (step < steps ? 16 * step : 0);
+        };
+        const auto segment_of = [&](int f) { return min(((4 * f + quarter) % kSegments) >> (a.shape.segment_shift - 6), a.shape.segments - 1) << a.shape.page_shift; };
+        if (16 * N <= 1 << a.shape.page_shift) {
+            const int page = page_of(first);
+            const bool is = (unsigned)page < (unsigned)a.shape.pages;
+            const uint8_t *codes = codes_of(is ? page : 0, first);
+            const float *scales = scales_of(is ? page : 0, first);
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) word[j] = j < steps ? *(const uint32_t *)(p + 16 * j) : 0u;
-        const float *s = a.scales + line * a.shape.segments + inside;
+            for (int n = 0; n < N; ++n) there[n] = is;
 #pragma unroll
-        for (int g = 0; g < STEPS / 2; ++g) scale[g] = g < a.shape.segments ? s[(long long)g << a.shape.page_shift] : 0.0f;
+            for (int f = 0; f < kFetches; ++f) {
+                const int n = STEPS == 2 ? 2 * f : f / (STEPS / 4);
+                raw[f] = *(const qt_u32x4 *)(codes + (uint32_t)(step_of(f) + 16 * n * a.shape.row_bytes));
+            }
+#pragma unroll
+            for (int f = 0; f < kScales; ++f) raw_scale[f] = scales[(uint32_t)(segment_of(f) + 16 * ((4 * f + quarter) / kSegments) + token)];
+        } else {
+            const uint8_t *codes[N];
+            const float *scales[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const int page = page_of(first + n);
+                there[n] = (unsigned)page < (unsigned)a.shape.pages;
+                codes[n] = codes_of(there[n] ? page : 0, first + n), scales[n] = scales_of(there[n] ? page : 0, first + n);
+            }
+#pragma unroll
+            for (int f = 0; f < kFetches; ++f) {
+                if constexpr (STEPS == 2) raw[f] = *(const qt_u32x4 *)((quarter < 2 ? codes[2 * f] : codes[2 * f + 1] - 16 * a.shape.row_bytes) + step_of(f));
+                else raw[f] = *(const qt_u32x4 *)(codes[f / (STEPS / 4)] + step_of(f));
+            }
+#pragma unroll
+            for (int f = 0; f < kScales; ++f) {
+                const float *p = scales[(4 * f) / kSegments];
+#pragma unroll
+                for (int q = 1; q < 4; ++q) p = quarter == q ? scales[(4 * f + q) / kSegments] : p;
+                raw_scale[f] = p[segment_of(f) + token];
+            }
+        }
+    }
+    __device__ __forceinline__ void arrange(float factor) {
+#pragma unroll
+        for (int f = 0; f < kFetches; ++f) {
+            uint32_t w[4] = {raw[f][0], raw[f][1], raw[f][2], raw[f][3]};
+            transpose_quarters(w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) word[(4 * f + i) / STEPS][(4 * f + i) % STEPS] = w[i];
+        }
+#pragma unroll
+        for (int f = 0; f < kScales; ++f) {
+            uint32_t each[4];
+            spread_quarters(__float_as_uint(raw_scale[f] * factor), each);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) scale[(4 * f + q) / kSegments][(4 * f + q) % kSegments] = __uint_as_float(each[q]);
+        }
     }
 };
 
-// Scores of sixteen rows (4 (lane / 16) + i) and a token (lane % 16), times log2 e: `numbers` are its keys' numbers.
+// Scores of sixteen rows (4 (lane / 16) + i) and a token (lane % 16), times log2 e: `numbers` are its keys' numbers, `scale` has the factor already.
 template <bool BF16, int STEPS>
 __device__ __forceinline__ fp4_f32x4 weigh_scores(const WeighArgs &a, const WeighRows<BF16, STEPS> &rows, const bf16x8 *numbers, const float *scale) {
     constexpr int P = Eight<BF16>::kPieces;
-    fp4_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    const int each = 1 << (a.shape.segment_shift - 5);          // steps of a segment
-    fp4_f32x4 part = {0.f, 0.f, 0.f, 0.f};
+    fp4_f32x4 sum;
 #pragma unroll
-    for (int j = 0; j < STEPS; ++j) {
-        part = multiply_pieces<P>(rows.x[j], numbers[j], part);
-        if (((j + 1) & (each - 1)) == 0 || j == STEPS - 1) {
-            float by = scale[0];
+    for (int g = 0; g < STEPS / 2; ++g) {
+        const fp4_f32x4 part = multiply_pieces<P>(rows.x[2 * g + 1], numbers[2 * g + 1], multiply_pieces<P>(rows.x[2 * g], numbers[2 * g], (fp4_f32x4){0.f, 0.f, 0.f, 0.f}));
 #pragma unroll
-            for (int g = 1; g < STEPS / 2; ++g) by = (j >> (a.shape.segment_shift - 5)) == g ? scale[g] : by;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(by, part[i], sum[i]);
-            part = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
-        }
+        for (int i = 0; i < 4; ++i) sum[i] = g ? __builtin_fmaf(scale[g], part[i], sum[i]) : scale[g] * part[i];
     }
-    return sum * a.factor;
+    return sum;
 }
 
-// Finds the tile of sixteen rows that is the `index`th of the call: its sequence and the row that it begins with.
+// Finds the tile of ROWS rows that is the `index`th of the call: its sequence and the row that it begins with.
+template <int ROWS>
 __device__ __forceinline__ bool find_rows(const WeighArgs &a, int index, int &b, int &first_row) {
     if (!a.at.starts) {
-        const int each = (a.group + 15) >> 4;
-        b = index / each, first_row = (index - b * each) << 4;
+        b = (int)fastdiv((uint32_t)index, a.by_tiles), first_row = (index - b * ((a.group + ROWS - 1) / ROWS)) * ROWS;
         return b < a.at.batch;
     }
     const int lane = threadIdx.x & 63;
@@ -128,8 +229,8 @@ __device__ __forceinline__ bool find_rows(const WeighArgs &a, int index, int &b,
     for (int first = 0; first < a.at.batch; first += 64) {
         int tiles = 0;
         if (first + lane < a.at.batch) {
-            const WeighSequence v = weigh_sequence(a, first + lane);
-            tiles = (int)(((long long)v.count * a.group + 15) >> 4);
+            const WeighSequence v = weigh_sequence<false>(a, first + lane);
+            tiles = (v.count * a.group + ROWS - 1) / ROWS;
         }
         int upto = tiles;
 #pragma unroll
@@ -141,12 +242,36 @@ __device__ __forceinline__ bool find_rows(const WeighArgs &a, int index, int &b,
         if (at) {
             const int found = __builtin_ctzll(at);
             b = first + found;
-            first_row = (index - before - __shfl(upto - tiles, found, 64)) << 4;
+            first_row = (index - before - __shfl(upto - tiles, found, 64)) * ROWS;
             return true;
         }
         before += __shfl(upto, 63, 64);
     }
     return false;
+}
+
+// Over the sixteen lanes of a row of the wave, and over its four rows, for all lanes.
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) { return __uint_as_float(dpp_u32<CTRL>(__float_as_uint(x))); }
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, dpp_f32<0xB1>(x)), x = fmaxf(x, dpp_f32<0x4E>(x)), x = fmaxf(x, dpp_f32<0x141>(x));
+    return fmaxf(x, dpp_f32<0x140>(x));
+}
+__device__ __forceinline__ float row_sum(float x) {
+    x += dpp_f32<0xB1>(x), x += dpp_f32<0x4E>(x), x += dpp_f32<0x141>(x);
+    return x + dpp_f32<0x140>(x);
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const uint32_t both = __float_as_uint(__uint_as_float(halves[0]) + __uint_as_float(halves[1]));
+    const auto rest = __builtin_amdgcn_permlane16_swap(both, both, false, false);
+    return __uint_as_float(rest[0]) + __uint_as_float(rest[1]);
+}
+__device__ __forceinline__ float quarters_max(float x) {
+    const auto halves = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    const uint32_t both = __float_as_uint(fmaxf(__uint_as_float(halves[0]), __uint_as_float(halves[1])));
+    const auto rest = __builtin_amdgcn_permlane16_swap(both, both, false, false);
+    return fmaxf(__uint_as_float(rest[0]), __uint_as_float(rest[1]));
 }
 
 // Joins (m, l) of two parts of a row.
@@ -155,187 +280,364 @@ __device__ __forceinline__ float2 join_parts(float2 x, float2 y) {
     return make_float2(m, x.y * __builtin_amdgcn_exp2f(x.x - by) + y.y * __builtin_amdgcn_exp2f(y.x - by));
 }
 
-template <bool BF16, int STEPS>
-__global__ __launch_bounds__(kWeighThreads) void weigh_rows_kernel(const WeighArgs a) {
-    constexpr int kAtOnce = 4;
-    __shared__ float2 s_part[kWeighWaves][16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
-    const int head = blockIdx.y, steps = a.shape.row_bytes >> 4;
-    int b, first_row;
-    if (!find_rows(a, blockIdx.x, b, first_row)) return;
-    const WeighSequence v = weigh_sequence(a, b);
-    const int rows = v.count * a.group;
-    if (first_row >= rows) return;
-    WeighRows<BF16, STEPS> q;
-    q.load(a, v, head, first_row, steps);
-    // tiles of tokens that any of them sees
-    const int nearest = v.first_position + first_row / a.group, furthest = v.first_position + min(rows - 1, first_row + 15) / a.group;
-    const int high = min(furthest + 1, v.end);
-    const int low = a.window ? min(max(high, 0), max(0, max(nearest, 0) - (a.window - 1))) : 0;
-    const int first_tile = low >> 4, sink_tiles = min((int)(((long long)min(a.sinks, low) + 15) >> 4), first_tile);
-    const int tiles = high <= 0 ? 0 : sink_tiles + ((high + 15) >> 4) - first_tile;
-    const int each = (tiles + a.splits - 1) / a.splits;
-    const int from = min(tiles, (int)blockIdx.z * each), to = min(tiles, from + each);
-    int position[4];
+// (m, 1 / l) of the row `first_row` + lane % 16, from its parts; (0, 0) where nothing is seen, (infinity, 0) behind the last row.
+__device__ __forceinline__ float2 row_statistics(const WeighArgs &a, const WeighSequence &v, int head, int first_row) {
+    const int lane = threadIdx.x & 63, quarter = lane >> 4, row = first_row + (lane & 15);
+    static_assert(kParts == 16, "four parts a lane");
+    float2 each[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = first_row + 4 * quarter + i;
-        position[i] = row < rows ? v.first_position + row / a.group : -1;
+    for (int n = 0; n < 4; ++n) each[n] = make_float2(-INFINITY, 0.0f);
+    if (row < v.count * a.group) {
+        const float2 *p = a.partial + row_entry(a, v, head, row) * a.parts;
+#pragma unroll
+        for (int n = 0; n < kParts / 4; ++n)
+            if (4 * n + quarter < a.parts) each[n] = p[4 * n + quarter];
     }
-    float m[4], l[4];
+    float m = fmaxf(fmaxf(each[0].x, each[1].x), fmaxf(each[2].x, each[3].x));
+    m = quarters_max(m);
+    m = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = -INFINITY, l[i] = 0.0f;
-    for (int index = from + wave * kAtOnce; index < to; index += kWeighWaves * kAtOnce) {
-        WeighKeys<STEPS> keys[kAtOnce];
-        int tile[kAtOnce];
+    for (int n = 0; n < kParts / 4; ++n) l += each[n].y * __builtin_amdgcn_exp2f(each[n].x - m);
+    l = quarters_sum(l);
+    return row < v.count * a.group ? make_float2(m, l == 0.0f ? 0.0f : 1.0f / l) : make_float2(INFINITY, 0.0f);
+}
+
+// Sums over the rows of N tiles' tokens (lane % 16): of the tile that a lane is to write.
+template <int N>
+__device__ __forceinline__ float sum_of_rows(float *sum, int &tile, bool &writes) {
+    const int quarter = (threadIdx.x & 63) >> 4;
+    uint32_t w[4];
+    if constexpr (N == 4) {
 #pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-            const int at = min(index + n, to - 1);
-            tile[n] = at < sink_tiles ? at : first_tile + at - sink_tiles;
-            keys[n].load(a, b, head, tile[n], v.end, steps);
-        }
-        fp4_f32x4 s[kAtOnce];
-#pragma unroll
-        for (int n = 0; n < kAtOnce; ++n) {
-            bf16x8 numbers[STEPS];
-#pragma unroll
-            for (int j = 0; j < STEPS; ++j) numbers[j] = fp4_to_bf16(keys[n].word[j]);
-            s[n] = weigh_scores<BF16, STEPS>(a, q, numbers, keys[n].scale);
-            const int token = (tile[n] << 4) + (lane & 15);
-            const bool there = keys[n].there && index + n < to && token < v.end;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] = there && row_sees(a, position[i], token) ? s[n][i] : -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float top = m[i];
-#pragma unroll
-            for (int n = 0; n < kAtOnce; ++n) top = fmaxf(top, s[n][i]);
-            const float by = top == -INFINITY ? 0.0f : top;
-            l[i] *= __builtin_amdgcn_exp2f(m[i] - by);
-#pragma unroll
-            for (int n = 0; n < kAtOnce; ++n) l[i] += __builtin_amdgcn_exp2f(s[n][i] - by);
-            m[i] = top;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float2 part = make_float2(m[i], l[i]);
-#pragma unroll
-        for (int off = 1; off < 16; off *= 2) part = join_parts(part, make_float2(__shfl_xor(part.x, off, 64), __shfl_xor(part.y, off, 64)));
-        if ((lane & 15) == 0) s_part[wave][4 * quarter + i] = part;
-    }
-    __syncthreads();
-    const int row = first_row + (int)threadIdx.x;
-    if (threadIdx.x < 16 && row < rows) {
-        float2 part = s_part[0][threadIdx.x];
-#pragma unroll
-        for (int w = 1; w < kWeighWaves; ++w) part = join_parts(part, s_part[w][threadIdx.x]);
-        const int i = row / a.group;
-        a.partial[((long long)(v.start + i) * (a.shape.kv_heads * a.group) + head * a.group + (row - i * a.group)) * a.splits + blockIdx.z] = part;
+        for (int n = 0; n < 4; ++n) w[n] = __float_as_uint(sum[n]);
+        transpose_quarters(w);
+        tile = quarter, writes = true;
+        return (__uint_as_float(w[0]) + __uint_as_float(w[1])) + (__uint_as_float(w[2]) + __uint_as_float(w[3]));
+    } else {
+        const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[0]), __float_as_uint(sum[1]), false, false);
+        const uint32_t half = __float_as_uint(__uint_as_float(two[0]) + __uint_as_float(two[1]));
+        const auto both = __builtin_amdgcn_permlane16_swap(half, half, false, false);
+        tile = quarter >> 1, writes = (quarter & 1) == 0;
+        return __uint_as_float(both[0]) + __uint_as_float(both[1]);
     }
 }
 
-template <bool BF16, int STEPS>
-__global__ __launch_bounds__(kWeighThreads) void weigh_tokens_kernel(const WeighArgs a) {
-    constexpr int N = STEPS == 8 ? 2 : 4;           // tiles of sixteen tokens of a wave
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quarter = lane >> 4;
-    const int head = blockIdx.y, b = blockIdx.z, steps = a.shape.row_bytes >> 4;
-    const WeighSequence v = weigh_sequence(a, b);
+// Tiles of sixteen tokens that rows at `nearest` to `furthest` see of a sequence with `end` tokens: `sink_tiles` from the first, then `first_tile` and
+// those behind it, both whole fours.
+struct WeighView { int first_tile, sink_tiles, tiles; };
+__device__ __forceinline__ WeighView weigh_view(const WeighArgs &a, int nearest, int furthest, int end) {
+    const int high = min(furthest + 1, end);
+    const int low = a.window ? min(max(high, 0), max(0, max(nearest, 0) - (a.window - 1))) : 0;
+    WeighView w;
+    w.first_tile = (low >> 4) & ~3, w.sink_tiles = min((int)(((long long)min(a.sinks, low) + 63) >> 6) * 4, w.first_tile);
+    w.tiles = high <= 0 ? 0 : w.sink_tiles + ((high + 15) >> 4) - w.first_tile;
+    return w;
+}
+
+// Tiles of a part of ROWS rows' tokens: as many as all rows' work makes for every workgroup that is wanted, but no more than kParts parts of these.
+template <int ROWS>
+__device__ __forceinline__ int part_tiles(const WeighArgs &a, int tiles) {
+    const int lane = threadIdx.x & 63;
+    float all = 0.0f;
+    for (int first = 0; first < a.at.batch; first += 64) {
+        if (first + lane < a.at.batch) {
+            const WeighSequence v = weigh_sequence<false>(a, first + lane);
+            all += (float)((v.count * a.group + ROWS - 1) / ROWS) * (float)weigh_view(a, v.first_position, v.first_position + v.count - 1, v.end).tiles;
+        }
+    }
+    all = quarters_sum(row_sum(all));
+    const int even = (int)fminf(ceilf(all * (float)a.shape.kv_heads / (float)a.wanted), 1.0e9f);
+    return (max(max(even, kLeastTiles), (tiles + a.parts - 1) / a.parts) + 3) & ~3;
+}
+
+// 16 T rows and a part of the tokens that they see: m and l of each, or (WEIGHTS, where a sequence has no more rows than these) the
+// weights themselves, added to the totals.
+template <bool BF16, int STEPS, int T, bool WEIGHTS>
+__global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 : 3) void weigh_rows_kernel(const WeighArgs a) {
+    static_assert(T == 1 || !WEIGHTS, "weights of sixteen rows");
+    constexpr int N = STEPS == 8 ? 2 : 4, kRows = 16 * T;
+    __shared__ float2 s_part[kWeighWaves][kRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+    const int head = blockIdx.y;
+    int b, first_row;
+    // (workgroups go round the XCDs, and on each round its engines, in turn: parts and heads of a long sequence are spread over all of them)
+    const unsigned turned = (blockIdx.x + 9 * blockIdx.y + 11 * blockIdx.z) % gridDim.x;
+    if (!find_rows<kRows>(a, (int)turned, b, first_row)) return;
+    b = __builtin_amdgcn_readfirstlane(b), first_row = __builtin_amdgcn_readfirstlane(first_row);
+    const WeighSequence v = weigh_sequence<true>(a, b);
     const int rows = v.count * a.group;
-    const int first = ((int)blockIdx.x * kWeighWaves + wave) * 16 * N;
+    if (first_row >= rows) return;
+    const int nearest = v.position(a, first_row), furthest = v.position(a, min(rows, first_row + kRows) - 1);
+    const WeighView view = weigh_view(a, nearest, furthest, v.end);
+    const int each = __builtin_amdgcn_readfirstlane(part_tiles<kRows>(a, view.tiles));
+    const int from = (int)min((long long)view.tiles, (long long)blockIdx.z * each), to = min(view.tiles, from + each);
+    const auto put = [&](float2 part) {
+        const long long entry = row_entry(a, v, head, first_row + (int)threadIdx.x);
+        if (a.parts == 1 && a.statistics)
+            a.statistics[entry] = make_float2(part.x == -INFINITY ? 0.0f : part.x, part.y == 0.0f ? 0.0f : 1.0f / part.y);
+        else
+            a.partial[entry * a.parts + blockIdx.z] = part;
+    };
+    if (from >= to) {
+        if (!WEIGHTS && threadIdx.x < kRows && first_row + (int)threadIdx.x < rows) put(make_float2(-INFINITY, 0.0f));
+        return;
+    }
+    const auto tile_at = [&](int index) { return index < view.sink_tiles ? index : view.first_tile + index - view.sink_tiles; };
+    WeighKeys<STEPS, N> keys;
+    int tile = 0;
+    const int first = from + wave * N;
+    if (first < to) {
+        tile = tile_at(first);
+        keys.fetch(a, b, head, tile, v.end);
+    }
+    WeighRows<BF16, STEPS> q[T];
+#pragma unroll
+    for (int r = 0; r < T; ++r) q[r].fetch(a, v, head, first_row + 16 * r);
+#pragma unroll
+    for (int r = 0; r < T; ++r) q[r].arrange();
+    float m[T][4], l[T][4];             // WEIGHTS: 1 / l
+    if constexpr (WEIGHTS) {
+        const float2 part = row_statistics(a, v, head, first_row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m[0][i] = __shfl(part.x, 4 * quarter + i, 64), l[0][i] = __shfl(part.y, 4 * quarter + i, 64);
+    } else {
+#pragma unroll
+        for (int r = 0; r < T; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[r][i] = -INFINITY, l[r][i] = 0.0f;
+    }
+    for (int index = first; index < to; index += kWeighWaves * N) {
+        keys.arrange(a.factor);
+        const int token = tile << 4;
+        bool there[N], all = token + 16 * N - 1 <= nearest && token + 16 * N <= v.end && (!a.window || furthest - token < a.window || token + 16 * N <= a.sinks);
+#pragma unroll
+        for (int n = 0; n < N; ++n) there[n] = keys.there[n], all = all && there[n];
+        if (index + kWeighWaves * N < to) {
+            tile = tile_at(index + kWeighWaves * N);
+            keys.fetch(a, b, head, tile, v.end);
+        }
+        fp4_f32x4 s[T][N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            bf16x8 numbers[STEPS];
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) numbers[j] = fp4_to_bf16(keys.word[n][j]);
+#pragma unroll
+            for (int r = 0; r < T; ++r) s[r][n] = weigh_scores<BF16, STEPS>(a, q[r], numbers, keys.scale[n]);
+        }
+        if (!all) {
+#pragma unroll
+            for (int r = 0; r < T; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = first_row + 16 * r + 4 * quarter + i, position = row < rows ? v.position(a, row) : -1;
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        const int t = token + 16 * n + (lane & 15);
+                        s[r][n][i] = there[n] && t < v.end && row_sees(a, position, t) ? s[r][n][i] : -INFINITY;
+                    }
+                }
+        }
+        if constexpr (WEIGHTS) {
+            float sum[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                sum[n] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[n] += __builtin_amdgcn_exp2f(s[0][n][i] - m[0][i]) * l[0][i];
+            }
+            int mine;
+            bool writes;
+            const float weight = sum_of_rows<N>(sum, mine, writes);
+            const int t = token + 16 * mine + (lane & 15);
+            bool is = there[0];
+#pragma unroll
+            for (int n = 1; n < N; ++n) is = mine == n ? there[n] : is;
+            if (writes && is && t < v.end && row_sees(a, furthest, t)) a.totals[b * a.total_sequence + head * a.total_head + t] += weight;
+        } else {
+#pragma unroll
+            for (int r = 0; r < T; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float top = m[r][i];
+#pragma unroll
+                    for (int n = 0; n < N; ++n) top = fmaxf(top, s[r][n][i]);
+                    const float by = top == -INFINITY ? 0.0f : top;
+                    l[r][i] *= __builtin_amdgcn_exp2f(m[r][i] - by);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) l[r][i] += __builtin_amdgcn_exp2f(s[r][n][i] - by);
+                    m[r][i] = top;
+                }
+        }
+    }
+    if constexpr (!WEIGHTS) {
+#pragma unroll
+        for (int r = 0; r < T; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float top = row_max(m[r][i]), by = top == -INFINITY ? 0.0f : top;
+                const float all = row_sum(l[r][i] * __builtin_amdgcn_exp2f(m[r][i] - by));
+                if ((lane & 15) == 0) s_part[wave][16 * r + 4 * quarter + i] = make_float2(top, all);
+            }
+        __syncthreads();
+        if (threadIdx.x < kRows && first_row + (int)threadIdx.x < rows) {
+            float2 part = s_part[0][threadIdx.x];
+#pragma unroll
+            for (int w = 1; w < kWeighWaves; ++w) part = join_parts(part, s_part[w][threadIdx.x]);
+            put(part);
+        }
+    }
+}
+
+// (m, 1 / l) of every row from its parts: of all rows that a sequence may have (what is behind the last sequence is not used).
+__global__ __launch_bounds__(kWeighThreads) void weigh_join_kernel(const WeighArgs a, long long entries) {
+    const long long entry = (long long)blockIdx.x * kWeighThreads + threadIdx.x;
+    if (entry >= entries) return;
+    float2 part = a.partial[entry * a.parts];
+    for (int n = 1; n < a.parts; ++n) part = join_parts(part, a.partial[entry * a.parts + n]);
+    a.statistics[entry] = make_float2(part.x == -INFINITY ? 0.0f : part.x, part.y == 0.0f ? 0.0f : 1.0f / part.y);
+}
+
+// Tokens and the rows that see them, sixteen at a time: a wave keeps 16 N tokens' keys and goes through all rows, or (SHARED) the waves of
+// a workgroup have the same tokens and take rows in turn.
+template <bool BF16, int STEPS, bool SHARED>
+__global__ __launch_bounds__(kWeighThreads, BF16 && STEPS < 8 ? 3 : 2) void weigh_tokens_kernel(const WeighArgs a) {
+    constexpr int N = STEPS == 8 ? 2 : 4;           // tiles of sixteen tokens of a wave
+    __shared__ float s_sum[SHARED ? kWeighWaves : 1][16 * N];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+    const int head = blockIdx.y, b = blockIdx.z;
+    const WeighSequence v = weigh_sequence<true>(a, b);
+    const int rows = v.count * a.group;
+    const int first = (SHARED ? (int)blockIdx.x : (int)blockIdx.x * kWeighWaves + wave) * 16 * N;
     if (first >= v.end) return;
     // rows that see any of the tokens: those at or behind the first, and with a window not too far behind the last
     const long long from = max(0LL, ((long long)first - v.first_position) * a.group);
     long long to = rows;
     if (a.window && first >= a.sinks) to = min(to, ((long long)first + 16 * N - 1 + a.window - v.first_position) * a.group);
     if (from >= to) return;
-    bf16x8 numbers[N][STEPS];
-    float scale[N][STEPS / 2];
-    bool there[N];
-    {
-        WeighKeys<STEPS> keys[N];
+    constexpr int kStep = SHARED ? 16 * kWeighWaves : 16;
+    int first_row = ((int)from & ~15) + (SHARED ? 16 * wave : 0);
+    WeighKeys<STEPS, N> keys;
+    keys.fetch(a, b, head, first >> 4, v.end);
+    WeighRows<BF16, STEPS> q;
+    float2 next[4];
+    const auto fetch_rows = [&](int at) {
+        q.fetch(a, v, head, at);
 #pragma unroll
-        for (int n = 0; n < N; ++n) keys[n].load(a, b, head, (first >> 4) + n, v.end, steps);
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-#pragma unroll
-            for (int j = 0; j < STEPS; ++j) numbers[n][j] = fp4_to_bf16(keys[n].word[j]);
-#pragma unroll
-            for (int g = 0; g < STEPS / 2; ++g) scale[n][g] = keys[n].scale[g];
-            there[n] = keys[n].there && first + 16 * n + (lane & 15) < v.end;
+        for (int i = 0; i < 4; ++i) {
+            const int row = at + 4 * quarter + i;
+            next[i] = row < rows ? a.statistics[row_entry(a, v, head, row)] : make_float2(INFINITY, 0.0f);
         }
+    };
+    if (first_row < (int)to) fetch_rows(first_row);
+    keys.arrange(a.factor);
+    bf16x8 numbers[BF16 ? N : 1][STEPS];            // (fp32 queries take the registers: expanded again for every sixteen rows)
+    bool all_there = first + 16 * N <= v.end;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if constexpr (BF16) {
+#pragma unroll
+            for (int j = 0; j < STEPS; ++j) numbers[n][j] = fp4_to_bf16(keys.word[n][j]);
+        }
+        all_there = all_there && keys.there[n];
+        keys.there[n] = keys.there[n] && first + 16 * n + (lane & 15) < v.end;
     }
     float sum[N];
 #pragma unroll
     for (int n = 0; n < N; ++n) sum[n] = 0.0f;
-    for (int first_row = (int)from & ~15; first_row < (int)to; first_row += 16) {
-        WeighRows<BF16, STEPS> q;
-        q.load(a, v, head, first_row, steps);
-        // (m, 1 / l) of row lane % 16, parts of it in turn
-        float2 part = make_float2(-INFINITY, 0.0f);
-        {
-            const int row = first_row + (lane & 15), i = row / a.group;
-            if (row < rows) {
-                const float2 *p = a.partial + ((long long)(v.start + i) * (a.shape.kv_heads * a.group) + head * a.group + (row - i * a.group)) * a.splits;
-                for (int n = quarter; n < a.splits; n += 4) part = join_parts(part, p[n]);
-            }
-            part = join_parts(part, make_float2(__shfl_xor(part.x, 16, 64), __shfl_xor(part.y, 16, 64)));
-            part = join_parts(part, make_float2(__shfl_xor(part.x, 32, 64), __shfl_xor(part.y, 32, 64)));
-            part.x = part.x == -INFINITY ? 0.0f : part.x;
-            part.y = part.y == 0.0f ? 0.0f : 1.0f / part.y;
-        }
+    for (; first_row < (int)to; first_row += kStep) {
+        q.arrange();
         float m[4], by[4];
-        int position[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = first_row + 4 * quarter + i;
-            m[i] = __shfl(part.x, 4 * quarter + i, 64), by[i] = __shfl(part.y, 4 * quarter + i, 64);
-            position[i] = row < rows ? v.first_position + row / a.group : -1;
-        }
+        for (int i = 0; i < 4; ++i) m[i] = next[i].x, by[i] = next[i].y;
+        if (first_row + kStep < (int)to) fetch_rows(first_row + kStep);
+        const bool all = all_there && first + 16 * N - 1 <= v.position(a, first_row) &&
+                         (!a.window || v.position(a, min(rows, first_row + 16) - 1) - first < a.window || first + 16 * N <= a.sinks);
+        fp4_f32x4 s[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const fp4_f32x4 s = weigh_scores<BF16, STEPS>(a, q, numbers[n], scale[n]);
-            const int token = first + 16 * n + (lane & 15);
+            if constexpr (!BF16) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[n] += there[n] && row_sees(a, position[i], token) ? __builtin_amdgcn_exp2f(s[i] - m[i]) * by[i] : 0.0f;
+                for (int j = 0; j < STEPS; ++j) {
+                    uint32_t word = keys.word[n][j];
+                    asm volatile("" : "+v"(word));          // (not in front of the loop)
+                    numbers[0][j] = fp4_to_bf16(word);
+                }
+            }
+            s[n] = weigh_scores<BF16, STEPS>(a, q, numbers[BF16 ? n : 0], keys.scale[n]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] -= m[i];
+        }
+        if (all) {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[n] += __builtin_amdgcn_exp2f(s[n][i]) * by[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = first_row + 4 * quarter + i, position = row < rows ? v.position(a, row) : -1;
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    sum[n] += keys.there[n] && row_sees(a, position, first + 16 * n + (lane & 15)) ? __builtin_amdgcn_exp2f(s[n][i]) * by[i] : 0.0f;
+            }
         }
     }
+    int mine;
+    bool writes;
+    const float weight = sum_of_rows<N>(sum, mine, writes);
+    bool is = keys.there[0];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-        sum[n] += __shfl_xor(sum[n], 16, 64);
-        sum[n] += __shfl_xor(sum[n], 32, 64);
-        const int token = first + 16 * n + (lane & 15);
-        if (quarter == 0 && there[n]) a.totals[b * a.total_sequence + head * a.total_head + token] += sum[n];
+    for (int n = 1; n < N; ++n) is = mine == n ? keys.there[n] : is;
+    float *total = a.totals + b * a.total_sequence + head * a.total_head + first;
+    const int t = 16 * mine + (lane & 15);
+    if constexpr (SHARED) {
+        if (writes) s_sum[wave][t] = weight;
+        __syncthreads();
+        if (wave == 0 && writes && is) total[t] += (s_sum[0][t] + s_sum[1][t]) + (s_sum[2][t] + s_sum[3][t]);
+    } else {
+        if (writes && is) total[t] += weight;
     }
 }
 
+template <bool BF16, int STEPS, int T>
+void launch_rows(const WeighArgs &a, unsigned row_tiles, hipStream_t stream) {
+    hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, T, false>), dim3(row_tiles, a.shape.kv_heads, a.parts), dim3(kWeighThreads), 0, stream, a);
+}
 template <bool BF16, int STEPS>
-void launch_weigh(const WeighArgs &a, unsigned row_tiles, hipStream_t stream) {
-    constexpr int kTokens = kWeighWaves * 16 * (STEPS == 8 ? 2 : 4);
-    const long long covered = (long long)a.at.table_pages << a.shape.page_shift;
-    const unsigned blocks = (unsigned)((covered + kTokens - 1) / kTokens);
-    hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS>), dim3(row_tiles, a.shape.kv_heads, a.splits), dim3(kWeighThreads), 0, stream, a);
-    hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS>), dim3(blocks, a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
+void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
+    constexpr int N = STEPS == 8 ? 2 : 4, T = BF16 ? 2 : 1;
+    const int rows = few ? 16 : 16 * T;
+    // tiles of rows at most, and parts of their tokens: no more than make two workgroups for each that is wanted, nor than there are tokens to
+    // see (the table's, or a window of each row's and the first ones)
+    const long long row_tiles = a.at.starts ? (long long)a.at.tokens * a.group / rows + a.at.batch : (long long)a.at.batch * ((a.group + rows - 1) / rows);
+    const long long covered = (long long)a.at.table_pages << a.shape.page_shift, seen = a.window ? (long long)a.window + a.sinks + 80 : covered;
+    const long long least = ((covered < seen ? covered : seen) + 16 * kLeastTiles - 1) / (16 * kLeastTiles), spread = 2 * a.wanted / (row_tiles * a.shape.kv_heads) + 1;
+    a.parts = (int)(least < spread ? least : spread);
+    a.parts = a.parts < kParts ? a.parts : kParts;
+    a.by_tiles = make_fastdiv((uint32_t)((a.group + rows - 1) / rows));
+    if (few) {
+        a.statistics = nullptr;
+        launch_rows<BF16, STEPS, 1>(a, (unsigned)row_tiles, stream);
+        hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, 1, true>), dim3((unsigned)row_tiles, a.shape.kv_heads, a.parts), dim3(kWeighThreads), 0, stream, a);
+        return;
+    }
+    launch_rows<BF16, STEPS, T>(a, (unsigned)row_tiles, stream);
+    const long long entries = (long long)a.at.tokens * a.group * a.shape.kv_heads;
+    if (a.parts > 1) hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)((entries + kWeighThreads - 1) / kWeighThreads)), dim3(kWeighThreads), 0, stream, a, entries);
+    const long long blocks = (covered + 16 * N - 1) / (16 * N), apart = (blocks + kWeighWaves - 1) / kWeighWaves;
+    if (apart * a.shape.kv_heads * a.at.batch >= a.wanted)
+        hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, false>), dim3((unsigned)apart, a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
+    else
+        hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, true>), dim3((unsigned)blocks, a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
 }
 
 template <bool BF16>
-void launch_weigh_type(const WeighArgs &a, unsigned row_tiles, hipStream_t stream) {
-    if (a.shape.head_dim <= 64) launch_weigh<BF16, 2>(a, row_tiles, stream);
-    else if (a.shape.head_dim <= 128) launch_weigh<BF16, 4>(a, row_tiles, stream);
-    else launch_weigh<BF16, 8>(a, row_tiles, stream);
-}
-
-// Tiles of sixteen rows at most, and parts that the tokens of each are cut into: enough workgroups for every unit, pieces of no fewer than 256 tokens.
-long long weigh_row_tiles(int group, int batch, int tokens, bool starts) {
-    return starts ? (long long)tokens * group / 16 + batch : (long long)batch * ((group + 15) / 16);
-}
-int weigh_splits(const qtensor_cache *cache, const qtensor_cache_places *at, int group) {
-    const long long work = weigh_row_tiles(group, at->batch, at->tokens, at->starts != nullptr) * cache->kv_heads;
-    const long long wanted = (8LL * compute_units() + work - 1) / (work < 1 ? 1 : work);
-    const long long most = ((long long)at->table_pages * cache->page_size + 255) / 256;
-    const long long n = wanted < most ? wanted : most;
-    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+void launch_weigh_type(const WeighArgs &a, bool few, hipStream_t stream) {
+    if (a.shape.head_dim <= 64) launch_weigh<BF16, 2>(a, few, stream);
+    else if (a.shape.head_dim <= 128) launch_weigh<BF16, 4>(a, few, stream);
+    else launch_weigh<BF16, 8>(a, few, stream);
 }
 
 }  // namespace
@@ -348,7 +650,7 @@ extern "C" long long qtensor_hip_cache_weigh_workspace(const qtensor_cache *cach
     CachePlaces at;
     if (!cache_shape("cache_weigh", cache, shape) || !cache_places("cache_weigh", places, at)) return 0;
     if (heads < 1 || heads % shape.kv_heads) { set_error(kBadArgument, "cache_weigh: %d query heads are not a multiple of the cache's %d", heads, shape.kv_heads); return 0; }
-    const long long size = (long long)at.tokens * heads * weigh_splits(cache, places, heads / shape.kv_heads) * (long long)sizeof(float2);
+    const long long size = (long long)at.tokens * heads * (kParts + 1) * (long long)sizeof(float2);
     return size < 16 ? 16 : size;
 }
 
@@ -371,19 +673,22 @@ extern "C" void qtensor_hip_cache_weigh(const qtensor_cache *cache, const qtenso
     if (workspace_bytes < size) { set_error(kBadArgument, "%s: needs %lld bytes of workspace, got %lld", what, size, workspace_bytes); return; }
     if (a.at.tokens == 0) return;
     a.codes = cache->codes[0], a.scales = cache->scales[0];
+    a.scale_page = (long long)a.shape.kv_heads << a.shape.page_shift, a.code_page = a.scale_page * a.shape.row_bytes, a.scale_page *= a.shape.segments;
     a.q = q->base, a.q_token = q->token_stride, a.q_head = q->head_stride;
     a.group = heads / a.shape.kv_heads;
     a.factor = scale * 1.4426950408889634f;
     a.window = window, a.sinks = sinks;
     a.totals = totals, a.total_sequence = total_sequence, a.total_head = total_head;
     a.partial = (float2 *)workspace;
-    a.splits = weigh_splits(cache, places, a.group);
-    const long long row_tiles = weigh_row_tiles(a.group, a.at.batch, a.at.tokens, a.at.starts != nullptr);
-    if ((long long)a.at.tokens * a.group > 0x7fffff00LL || a.at.batch > 65535 || a.shape.kv_heads > 65535) {
+    a.statistics = a.partial + (long long)a.at.tokens * heads * kParts;
+    a.wanted = 6LL * compute_units();
+    a.by_group = make_fastdiv((uint32_t)a.group);
+    if ((long long)a.at.tokens * a.group >= 1 << 29 || a.group >= 1 << 15 || a.at.batch > 65535 || a.shape.kv_heads > 65535) {
         set_error(kBadArgument, "%s: too many tokens, heads or sequences (%d, %d, %d)", what, a.at.tokens, heads, a.at.batch);
         return;
     }
-    if (bf16) launch_weigh_type<true>(a, (unsigned)row_tiles, (hipStream_t)stream);
-    else launch_weigh_type<false>(a, (unsigned)row_tiles, (hipStream_t)stream);
+    const bool few = !a.at.starts && a.group <= 16;         // a tile of rows for every sequence
+    if (bf16) launch_weigh_type<true>(a, few, (hipStream_t)stream);
+    else launch_weigh_type<false>(a, few, (hipStream_t)stream);
     launch_ok(what);
 }

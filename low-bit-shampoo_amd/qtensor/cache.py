@@ -234,7 +234,7 @@ class QTensorCache:
         tokens, heads, scale = self._check_queries(q, scale, window, sinks)
         places = self._places(table, lengths, starts, tokens)
         self._check_totals(totals, places)
-        if tokens * (heads // self.kv_heads) > _MOST - 256 or places.batch > 65535:
+        if tokens * (heads // self.kv_heads) >= 2 ** 29 or places.batch > 65535:
             raise ValueError(f"{tokens} tokens of {heads} heads in {places.batch} sequences are too many for one call.")
         cache = self._ref()
         with torch.cuda.device(q.device):
