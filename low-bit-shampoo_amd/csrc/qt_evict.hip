@@ -2,17 +2,16 @@
 //
 // A token is there if its page is.  `keep` of them stay (all, where there are no more): the first `sinks` and the last `recent` places
 // of the sequence, then those with the largest totals, ties to the earlier one.  The nth token that stays moves to the place of the nth
-// token that is there, which is never behind it.  As heads keep different tokens and every place may be read for one that is written
-// before it, all that moves goes through scratch memory: gathered, then put down.
+// token that is there, which is never behind it.
 //
-// Three launches: the choice (a workgroup a sequence and head), which lists where tokens come from and go to; gathering; putting down.
+// Two launches: the choice (a workgroup a sequence and head), which lists where tokens come from and go to; the moves.
 #include "qt_cache.h"
 
 namespace qt {
 namespace {
 
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 512;
 
 struct EvictArgs {
     CacheShape shape;
@@ -27,8 +26,6 @@ struct EvictArgs {
     int *new_lengths;
     // scratch, an entry a token that stays, of [batch][kv_heads][keep]
     int *from, *to, *count;             // places; how many stay of a sequence
-    uint8_t *held_codes[2];
-    float *held_scales[2], *held_totals;
 };
 
 __device__ __forceinline__ int evict_end(const EvictArgs &a, int b) {
@@ -45,57 +42,120 @@ __device__ __forceinline__ uint32_t total_key(float x) {
     return __builtin_isunordered(x, x) ? 0xffffffffu : float_to_key(x + 0.0f);
 }
 
-// Sum over the threads in front of this one, and over all; `s_waves`: scratch.
-__device__ __forceinline__ int flags_before(bool flag, int *s_waves, int &all) {
+// A workgroup looks at kChunk tokens at a time, up to kEach side by side a thread, whose keys stay in LDS where they are all of the sequence.
+constexpr int kEach = 16, kChunk = kEach * kChooseThreads;
+
+// Sums over the threads in front of this one, and over all, of two counts below 2^16 (in the halves of x); `s_waves`: scratch.
+__device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t *s_waves, uint32_t &all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const unsigned long long at = __ballot(flag);
-    __syncthreads();
-    if (lane == 0) s_waves[wave] = __popcll(at);
-    __syncthreads();
-    int before = __popcll(at & ((1ull << lane) - 1));
-    all = 0;
+    uint32_t upto = x;
 #pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+        const uint32_t other = (uint32_t)__shfl_up((int)upto, off, 64);
+        if (lane >= off) upto += other;
+    }
+    __syncthreads();
+    if (lane == 63) s_waves[wave] = upto;
+    __syncthreads();
+    uint32_t before = upto - x;
+    all = 0;
+#pragma unroll 1
     for (int w = 0; w < kChooseWaves; ++w) {
-        const int n = s_waves[w];
+        const uint32_t n = s_waves[w];
         before += w < wave ? n : 0;
         all += n;
     }
     return before;
 }
 
+// Bound by the latency of its steps, and of fetching its instructions, which run once: loops stay loops (16384 keys in registers, all unrolled: 27 us for the
+// fewest tokens, 37 for 24 x 8 of 12000; CHOICE).  The least key of those that stay is found eight bits at a time, from counts in LDS; lanes
+// that have the digit of the first one among them are counted together, as totals of one size are most of them.
 __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const EvictArgs a) {
-    __shared__ int s_count[256], s_waves[kChooseWaves], s_there, s_kept_anyhow, s_digit, s_above;
-    const int head = blockIdx.x, b = blockIdx.y;
+    __shared__ uint32_t s_key[kEach][kChooseThreads], s_waves[kChooseWaves];
+    __shared__ int s_count[256], s_digit, s_above;
+    const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63;
     const int length = max(a.lengths[b], 0), end = evict_end(a, b);
     const float *totals = a.totals + b * a.total_sequence + head * a.total_head;
-    const auto anyhow = [&](int place) { return place < a.sinks || place >= length - a.recent; };
-    if (threadIdx.x == 0) s_there = 0, s_kept_anyhow = 0;
-    __syncthreads();
-    int there = 0, protect = 0;
-    for (int place = threadIdx.x; place < end; place += kChooseThreads) {
-        const bool is = evict_line(a, b, place) >= 0;
-        there += is, protect += is && anyhow(place);
+    const int chunks = max(1, (end + kChunk - 1) / kChunk);
+    // tokens of a thread in every chunk: all kEach but where there is only one
+    const int each = chunks > 1 ? kEach : ((end + kChooseThreads - 1) / kChooseThreads + 3) & ~3;
+    // bits of a thread's tokens: those that are there, those that stay whatever their totals are
+    uint32_t there = 0, anyhow = 0;
+    const auto load = [&](int chunk) {
+        const int first = chunk * kChunk + (int)threadIdx.x * each, last = max(end - 1, 0) & ~3;
+        there = anyhow = 0;
+#pragma unroll 1
+        for (int i = 0; i < each; i += 4) {
+            // (four places are of one page, and totals are as long as the pages: what is not looked at is read from the last places instead)
+            const int place = min(first + i, last);
+            const int page = a.table[b * a.table_stride + (place >> a.shape.page_shift)];
+            const qt_u32x4 total = ((const Unaligned16of4 *)(totals + place))->v;
+            const bool is = (unsigned)page < (unsigned)a.shape.pages;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int here = first + i + e;
+                if (is && here < end) {
+                    there |= 1u << (i + e);
+                    if (here < a.sinks || here >= length - a.recent) anyhow |= 1u << (i + e);
+                }
+                s_key[i + e][threadIdx.x] = total_key(__uint_as_float(total[e]));
+            }
+        }
+    };
+    int all_there = 0, all_protect = 0;
+#pragma unroll 1
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        load(chunk);
+        uint32_t all;
+        sum_before((uint32_t)__popc(there) | (uint32_t)__popc(anyhow) << 16, s_waves, all);
+        all_there += all & 0xffff, all_protect += all >> 16;
     }
-    atomicAdd(&s_there, there), atomicAdd(&s_kept_anyhow, protect);
-    __syncthreads();
-    const int stay = min(s_there, a.keep);
-    int wanted = stay - s_kept_anyhow;          // by their totals
-    // the least key of those that stay, eight bits at a time, and how many of the tokens with that key do
+    const int stay = min(all_there, a.keep);
+    int wanted = stay - all_protect;            // by their totals
+    // the least key of those that stay, and how many of the tokens with that key do
     uint32_t least = 0;
+#pragma unroll 1
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
         if (threadIdx.x < 256) s_count[threadIdx.x] = 0;
         __syncthreads();
-        for (int place = threadIdx.x; place < end; place += kChooseThreads) {
-            if (anyhow(place) || evict_line(a, b, place) < 0) continue;
-            const uint32_t key = total_key(totals[place]);
-            if (shift == 24 || (key >> (shift + 8)) == (least >> (shift + 8))) atomicAdd(&s_count[(key >> shift) & 255], 1);
+#pragma unroll 1
+        for (int chunk = 0; chunk < chunks; ++chunk) {
+            if (chunks > 1) load(chunk);
+#pragma unroll 1
+            for (int i = 0; i < each; ++i) {
+                const uint32_t key = s_key[i][threadIdx.x];
+                const bool counts = ((there & ~anyhow) >> i & 1) && (shift == 24 || (key >> (shift + 8)) == (least >> (shift + 8)));
+                const int digit = (key >> shift) & 255;
+                const unsigned long long some = __ballot(counts);
+                if (!some) continue;
+                const int common = __builtin_amdgcn_readlane(digit, __builtin_ctzll(some));
+                const unsigned long long same = __ballot(counts && digit == common);
+                if (lane == 0) atomicAdd(&s_count[common], __popcll(same));
+                if (counts && digit != common) atomicAdd(&s_count[digit], 1);
+            }
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int above = 0, digit = 255;
-            for (; digit > 0 && above + s_count[digit] < wanted; --digit) above += s_count[digit];
-            s_digit = digit, s_above = above;
+        if (threadIdx.x < 64) {
+            // counts of the digits from this lane's four on
+            int mine[4], above = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine[i] = s_count[4 * lane + i], above += mine[i];
+#pragma unroll
+            for (int off = 1; off < 64; off *= 2) {
+                const int other = __shfl_down(above, off, 64);
+                if (lane + off < 64) above += other;
+            }
+            // the digit at which the wanted are reached from above (the largest if nothing is wanted)
+            const unsigned long long reach = __ballot(above >= wanted);
+            if (lane == 63 - __builtin_clzll(reach)) {
+                int digit = 0, before = above - mine[0];
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (before >= wanted) digit = i + 1, before -= mine[i + 1];
+                s_digit = 4 * lane + digit, s_above = before;
+            }
         }
         __syncthreads();
         least |= (uint32_t)s_digit << shift;
@@ -103,22 +163,29 @@ __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const Evic
     }
     int *from = a.from + ((long long)b * a.shape.kv_heads + head) * a.keep, *to = a.to + ((long long)b * a.shape.kv_heads + head) * a.keep;
     int there_before = 0, stay_before = 0, ties_before = 0;
-    for (int first = 0; first < end; first += kChooseThreads) {
-        const int place = first + (int)threadIdx.x;
-        const bool is = place < end && evict_line(a, b, place) >= 0;
-        const bool by_total = is && !anyhow(place);
-        const uint32_t key = by_total ? total_key(totals[place]) : 0u;
-        int all;
-        const bool tie = by_total && key == least;
-        const int ties = ties_before + flags_before(tie, s_waves, all);
-        ties_before += all;
-        const bool stays = is && (!by_total || key > least || (tie && ties < wanted));
-        const int nth = stay_before + flags_before(stays, s_waves, all);
-        stay_before += all;
-        if (stays && nth < stay) from[nth] = place;
-        const int slot = there_before + flags_before(is, s_waves, all);
-        there_before += all;
-        if (is && slot < stay) {
+#pragma unroll 1
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        if (chunks > 1) load(chunk);
+        uint32_t tie = 0, stays = anyhow, all;
+#pragma unroll 1
+        for (int i = 0; i < each; ++i) {
+            const uint32_t key = s_key[i][threadIdx.x], is = (there & ~anyhow) >> i & 1;
+            tie |= (is & (uint32_t)(key == least)) << i, stays |= (is & (uint32_t)(key > least)) << i;
+        }
+        int ties = ties_before + (int)sum_before((uint32_t)__popc(tie), s_waves, all);
+        ties_before += (int)all;
+#pragma unroll 1
+        for (; tie && ties < wanted; ++ties, tie &= tie - 1) stays |= tie & -tie;
+        const uint32_t before = sum_before((uint32_t)__popc(stays) | (uint32_t)__popc(there) << 16, s_waves, all);
+        int nth = stay_before + (int)(before & 0xffff), slot = there_before + (int)(before >> 16);
+        stay_before += (int)(all & 0xffff), there_before += (int)(all >> 16);
+        const int first = chunk * kChunk + (int)threadIdx.x * each;
+#pragma unroll 1
+        for (; stays && nth < stay; stays &= stays - 1, ++nth) from[nth] = first + __builtin_ctz(stays);
+        uint32_t places = there;
+#pragma unroll 1
+        for (; places && slot < stay; places &= places - 1, ++slot) {
+            const int place = first + __builtin_ctz(places);
             to[slot] = place;
             if (slot == stay - 1 && head == 0) a.new_lengths[b] = place + 1;
         }
@@ -129,47 +196,75 @@ __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const Evic
     }
 }
 
-// A thread moves sixteen bytes of keys and of values, or (the first one of a token behind those) its scales and total.
-template <bool GATHER>
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const EvictArgs a) {
-    const int head = blockIdx.y, b = blockIdx.z;
-    const int parts = a.shape.row_bytes / 16 + 1;
-    const long long index = (long long)blockIdx.x * kMoveThreads + threadIdx.x;
-    const int nth = (int)(index / parts), part = (int)(index - (long long)nth * parts);
-    if (nth >= a.count[b]) return;
-    const long long sequence = (long long)b * a.shape.kv_heads + head, entry = sequence * a.keep + nth;
-    const int from = a.from[entry], to = a.to[entry];
-    if (from == to) return;
-    const int place = GATHER ? from : to;
-    const long long line = evict_line(a, b, place) + ((long long)head << a.shape.page_shift), inside = place & ((1 << a.shape.page_shift) - 1);
-    if (part < parts - 1) {
+// The tokens that stay of a sequence and head by one workgroup in their order, kItems pieces a thread at a time: of keys' or values' codes sixteen
+// bytes of a token each, of their scales (or, with the keys', totals) one number.
+//
+// In place: a token goes to a place that is not behind its own, so what is written is behind no token that has been read, and only the tokens
+// that are read at the same time may lie there: they are all in registers before any is written.
+constexpr int kItems = 4;
+template <typename Piece, typename Address>
+__device__ __forceinline__ void move_pieces(int count, int parts, const int *from, const int *to, const Address &address) {
+    const int each = kMoveThreads / parts, nth = (int)threadIdx.x / parts, part = (int)threadIdx.x - nth * parts;
+    const int step = kItems * each;
+    Piece *source[kItems], *target[kItems], held[kItems];
+    // (null: nothing to do)
+    const auto find = [&](int first) {
+        int place[kItems], there[kItems];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            qt_u32x4 *there = (qt_u32x4 *)(a.codes[i] + (line + inside) * a.shape.row_bytes + 16 * part), *held = (qt_u32x4 *)(a.held_codes[i] + entry * a.shape.row_bytes + 16 * part);
-            if (GATHER) *held = *there;
-            else *there = *held;
+        for (int k = 0; k < kItems; ++k) {
+            const int at = min(first + k * each + nth, count - 1);
+            place[k] = from[at], there[k] = to[at];
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            for (int g = 0; g < a.shape.segments; ++g) {
-                float *there = a.scales[i] + line * a.shape.segments + ((long long)g << a.shape.page_shift) + inside, *held = a.held_scales[i] + entry * a.shape.segments + g;
-                if (GATHER) *held = *there;
-                else *there = *held;
-            }
-        float *there = a.totals + b * a.total_sequence + head * a.total_head + place, *held = a.held_totals + entry;
-        if (GATHER) *held = *there;
-        else *there = *held;
+        for (int k = 0; k < kItems; ++k) {
+            const bool moves = nth < each && first + k * each + nth < count && place[k] != there[k];
+            source[k] = address(place[k], part), target[k] = moves ? address(there[k], part) : nullptr;
+        }
+    };
+    find(0);
+    for (int first = 0; first < count; first += step) {
+        Piece *now[kItems];
+#pragma unroll
+        for (int k = 0; k < kItems; ++k) {
+            now[k] = target[k];
+            if (now[k]) held[k] = *source[k];
+        }
+        if (first + step < count) find(first + step);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // (read, not only asked for)
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kItems; ++k)
+            if (now[k]) *now[k] = held[k];
+    }
+}
+
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const EvictArgs a) {
+    const int what = blockIdx.x, values = what & 1, head = blockIdx.y, b = blockIdx.z;
+    const long long sequence = (long long)b * a.shape.kv_heads + head;
+    const int *from = a.from + sequence * a.keep, *to = a.to + sequence * a.keep;
+    const int count = a.count[b];
+    if (count == 0) return;
+    const auto inside = [&](int place) { return place & ((1 << a.shape.page_shift) - 1); };
+    const auto line = [&](int place) { return evict_line(a, b, place) + ((long long)head << a.shape.page_shift); };
+    if (what < 2) {
+        uint8_t *codes = a.codes[values];
+        move_pieces<qt_u32x4>(count, a.shape.row_bytes / 16, from, to,
+                              [&](int place, int part) { return (qt_u32x4 *)(codes + (line(place) + inside(place)) * a.shape.row_bytes) + part; });
+    } else {
+        // (a token's segments, and behind the keys' its total)
+        float *scales = a.scales[values], *totals = a.totals + b * a.total_sequence + head * a.total_head;
+        move_pieces<float>(count, a.shape.segments + 1 - values, from, to, [&](int place, int part) {
+            return part == a.shape.segments ? totals + place : scales + line(place) * a.shape.segments + ((long long)part << a.shape.page_shift) + inside(place);
+        });
     }
 }
 
 long long rounded(long long bytes) { return (bytes + 255) & ~255LL; }
 
-struct EvictSizes { long long lists, count, codes, scales, totals, all; };
+struct EvictSizes { long long lists, count, all; };
 EvictSizes evict_sizes(const CacheShape &shape, int batch, long long keep) {
-    const long long entries = (long long)batch * shape.kv_heads * keep;
-    EvictSizes s = {rounded(4 * entries), rounded(4LL * batch), rounded(entries * shape.row_bytes), rounded(4 * entries * shape.segments), rounded(4 * entries), 0};
-    s.all = 2 * s.lists + s.count + 2 * s.codes + 2 * s.scales + s.totals;
+    EvictSizes s = {rounded(4LL * batch * shape.kv_heads * keep), rounded(4LL * batch), 0};
+    s.all = 2 * s.lists + s.count;
     return s;
 }
 
@@ -216,22 +311,13 @@ extern "C" void qtensor_hip_cache_evict(const qtensor_cache *cache, const qtenso
     if (workspace_bytes < size.all) { set_error(kBadArgument, "%s: needs %lld bytes of workspace, got %lld", what, size.all, workspace_bytes); return; }
     a.table = at.table, a.lengths = at.lengths, a.table_stride = at.table_stride, a.table_pages = at.table_pages, a.batch = at.batch;
     uint8_t *p = (uint8_t *)workspace;
-    const auto take = [&](long long bytes) { uint8_t *here = p; p += bytes; return here; };
-    a.from = (int *)take(size.lists), a.to = (int *)take(size.lists), a.count = (int *)take(size.count);
-    for (int i = 0; i < 2; ++i) {
-        a.codes[i] = cache->codes[i], a.scales[i] = cache->scales[i];
-        a.held_codes[i] = take(size.codes), a.held_scales[i] = (float *)take(size.scales);
-    }
-    a.held_totals = (float *)take(size.totals);
+    a.from = (int *)p, a.to = (int *)(p + size.lists), a.count = (int *)(p + 2 * size.lists);
+    for (int i = 0; i < 2; ++i) a.codes[i] = cache->codes[i], a.scales[i] = cache->scales[i];
     a.totals = totals, a.total_sequence = total_sequence, a.total_head = total_head;
     const long long most = 0x7fffffff;
     a.keep = (int)kept, a.recent = (int)(recent < most ? recent : most), a.sinks = (int)(sinks < most ? sinks : most);
     a.new_lengths = new_lengths;
-    const long long blocks = (kept * (a.shape.row_bytes / 16 + 1) + kMoveThreads - 1) / kMoveThreads;
-    if (blocks > 0x7fffffffLL) { set_error(kBadArgument, "%s: too many tokens to keep (%lld)", what, kept); return; }
-    const dim3 grid((unsigned)blocks, (unsigned)a.shape.kv_heads, (unsigned)a.batch);
     hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)a.shape.kv_heads, (unsigned)a.batch), dim3(kChooseThreads), 0, (hipStream_t)stream, a);
-    hipLaunchKernelGGL((evict_move_kernel<true>), grid, dim3(kMoveThreads), 0, (hipStream_t)stream, a);
-    hipLaunchKernelGGL((evict_move_kernel<false>), grid, dim3(kMoveThreads), 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL(evict_move_kernel, dim3(4, (unsigned)a.shape.kv_heads, (unsigned)a.batch), dim3(kMoveThreads), 0, (hipStream_t)stream, a);
     launch_ok(what);
 }
