@@ -153,7 +153,8 @@ struct TurnCall {
     int heads_each;                     // heads that a thread goes through
 };
 
-// 8 sequences of 2048 tokens, 40 heads of 128 in bf16
+// 8 sequences of 2048 tokens, 40 heads of 128 in bf16: 72 us, 4.7 TB/s (a copy of the library's 4.9); a thread goes through four of
+// them (69 us, one 133, eight 67; 2048 tokens 10.6, 18.2 and 11.4).
 template <bool BF16>
 __global__ __launch_bounds__(kTurnThreads) void turn_kernel(const TurnCall a) {
     __shared__ float2 s_turn[kTurnPairs];
@@ -187,65 +188,83 @@ __global__ __launch_bounds__(kTurnThreads) void turn_kernel(const TurnCall a) {
     }
 }
 
-// On the way into the cache: workgroups in y of the queries, then of the cache's heads.
+// On the way into the cache: workgroups of the cache's heads, then of the queries, each with tokens and heads of its own number.
 struct TurnWrite {
-    TurnArgs turn;
+    TurnArgs keys, queries;
+    int key_blocks, query_blocks;       // workgroups that the tokens are cut for, of each
+    long long key_groups;               // all of the cache's heads
+    int keys_each, queries_each;        // heads that a thread goes through
     CacheShape shape;
     CachePlaces at;
     const void *q, *vectors[2];
     void *out;
     long long q_token, q_head, out_token, out_head, token_stride[2], head_stride[2];
-    int heads, query_groups;            // workgroups in y of the queries
+    int heads;
     const void *positions;              // or their places in the sequences
     int long_positions;
     uint8_t *codes[2];
     float *scales[2];
     int segment_lanes;
-    int heads_each;
 };
 
-template <bool BF16>
-__global__ __launch_bounds__(kTurnThreads) void turn_write_kernel(const TurnWrite a) {
-    constexpr int kEach = kLaneElements<BF16>;
+// Bound by memory, with the places' look-up, cosines and sines in front of the first loads: the more heads a workgroup goes through, the less of
+// that, and tokens side by side in a head of the cache are written together.  9 prompts of up to 3500 tokens, 32 query heads, 8 of 128 in the cache, bf16:
+// 103 us, of which the queries alone are 62 and keys and values 38; turned, then written by two calls 87.
+template <bool BF16, bool LARGE>
+__global__ __launch_bounds__(kTurnThreads, 4) void turn_write_kernel(const TurnWrite a) {
+    constexpr int kEach = kLaneElements<BF16>, kAtOnce = LARGE ? 4 : 1, kHeads = LARGE ? 2 : 1;
     __shared__ float2 s_turn[kTurnPairs];
     __shared__ int s_sequence[kTurnThreads], s_place[kTurnThreads];
-    const int first = (int)blockIdx.x * a.turn.block_tokens;
+    const bool is_keys = (long long)blockIdx.x < a.key_groups;
+    const TurnArgs &turn = is_keys ? a.keys : a.queries;
+    const int index = (int)(blockIdx.x - (is_keys ? 0 : a.key_groups)), blocks = is_keys ? a.key_blocks : a.query_blocks;
+    const int group = index / blocks, first = (index - group * blocks) * turn.block_tokens;
     int b = 0;
     if (a.at.starts) b = sequence_of_block(a.at, first);
-    if ((int)threadIdx.x < a.turn.block_tokens) {
+    if ((int)threadIdx.x < turn.block_tokens) {
         const int token = first + (int)threadIdx.x;
         int place = -1;
         if (token < a.at.tokens) place = token_position(a.at, token, b);
         s_sequence[threadIdx.x] = b, s_place[threadIdx.x] = place;
     }
     __syncthreads();
-    work_out_turns(a.turn, s_turn, [&](int nth, double &at) {
+    work_out_turns(turn, s_turn, [&](int nth, double &at) {
         const int place = s_place[nth];
         if (place < 0) return false;
         at = !a.positions ? (double)place : a.long_positions ? (double)((const long long *)a.positions)[first + nth] : (double)((const int *)a.positions)[first + nth];
         return true;
     });
     __syncthreads();
-    const TurnThread t = turn_thread<BF16>(a.turn);
-    const bool mine = t.row < a.turn.rows && first + t.nth < a.at.tokens;
-    const int token = mine ? first + t.nth : 0, valid = mine ? max(0, a.turn.head_dim - t.first) : 0;
+    const TurnThread t = turn_thread<BF16>(turn);
+    const bool mine = t.row < turn.rows && first + t.nth < a.at.tokens;
+    const int token = mine ? first + t.nth : 0, valid = mine ? max(0, turn.head_dim - t.first) : 0;
     const int place = mine ? s_place[t.nth] : -1;
     LaneTurn<BF16> lane;
-    lane.set(a.turn, s_turn + (mine ? t.nth : 0) * a.turn.pairs, t.first);
-    if ((int)blockIdx.y < a.query_groups) {
+    lane.set(turn, s_turn + (mine ? t.nth : 0) * turn.pairs, t.first);
+    if (!is_keys) {
         const uint8_t *from = (const uint8_t *)a.q + token * a.q_token * (BF16 ? 2 : 4);
         uint8_t *to = (uint8_t *)a.out + token * a.out_token * (BF16 ? 2 : 4);
         if (valid <= 0) return;
-        const int group = (int)blockIdx.y, last = min(a.heads, (group + 1) * a.turn.rows * a.heads_each);
-        for (int h = group * a.turn.rows * a.heads_each + t.row; h < last; h += a.turn.rows) {
-            const uint8_t *row = from + h * a.q_head * (BF16 ? 2 : 4);
-            uint4 y = make_uint4(0, 0, 0, 0);
-            if (place >= 0) {
-                float turned[kEach];
-                lane.apply(a.turn, load_any<BF16>(row, t.first, valid), lane.load_partner(row), row, turned);
-                y = pack_lane<BF16>(turned);
+        const int last = min(a.heads, (group + 1) * turn.rows * a.queries_each);
+        for (int h = group * turn.rows * a.queries_each + t.row; h < last; h += kAtOnce * turn.rows) {
+            uint4 own[kAtOnce], other[kAtOnce];
+            const uint8_t *row[kAtOnce];
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n) {
+                row[n] = from + min(h + n * turn.rows, last - 1) * a.q_head * (BF16 ? 2 : 4);
+                own[n] = load_any<BF16>(row[n], t.first, valid), other[n] = lane.load_partner(row[n]);
             }
-            store_any<BF16>(to + h * a.out_head * (BF16 ? 2 : 4), t.first, valid, y);
+#pragma unroll
+            for (int n = 0; n < kAtOnce; ++n) {
+                if (h + n * turn.rows >= last) break;
+                uint4 y = make_uint4(0, 0, 0, 0);
+                if (place >= 0) {
+                    float turned[kEach];
+                    lane.apply(turn, own[n], other[n], row[n], turned);
+                    y = pack_lane<BF16>(turned);
+                }
+                store_any<BF16>(to + (h + n * turn.rows) * a.out_head * (BF16 ? 2 : 4), t.first, valid, y);
+            }
         }
         return;
     }
@@ -260,35 +279,47 @@ __global__ __launch_bounds__(kTurnThreads) void turn_write_kernel(const TurnWrit
         }
     }
     const int segment = t.first >> a.shape.segment_shift;
-    const int group = (int)blockIdx.y - a.query_groups;
-    for (int n = 0; n < a.heads_each; ++n) {
-        const int h = (group * a.heads_each + n) * a.turn.rows + t.row;
-        const bool there = line >= 0 && h < a.shape.kv_heads && valid > 0;
-        const long long head_line = line + ((long long)h << a.shape.page_shift);
+    for (int n = 0; n < a.keys_each; n += kHeads) {
+        uint4 own[kHeads][2], other[kHeads];
+        const uint8_t *row[kHeads];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const uint8_t *row = (const uint8_t *)a.vectors[i] + (token * a.token_stride[i] + (there ? h : 0) * a.head_stride[i]) * (BF16 ? 2 : 4);
-            const int own_valid = there ? valid : 0;
-            float x[kEach];
-            const uint4 own = load_any<BF16>(row, t.first, own_valid);
-            if (i == 0 && own_valid > 0) {
-                float turned[kEach];
-                lane.apply(a.turn, own, lane.load_partner(row), row, turned);
-                unpack_lane<BF16>(pack_lane<BF16>(turned), x);
+        for (int e = 0; e < kHeads; ++e) {
+            const int h = min((group * a.keys_each + n + e) * turn.rows + t.row, a.shape.kv_heads - 1);
 #pragma unroll
-                for (int e = 0; e < kEach; ++e) x[e] = e < own_valid ? x[e] : 0.0f;
-            } else {
-                unpack_lane<BF16>(own, x);
+            for (int i = 0; i < 2; ++i) {
+                const uint8_t *p = (const uint8_t *)a.vectors[i] + (token * a.token_stride[i] + h * a.head_stride[i]) * (BF16 ? 2 : 4);
+                own[e][i] = load_any<BF16>(p, t.first, valid);
+                if (i == 0) row[e] = p, other[e] = valid > 0 ? lane.load_partner(p) : make_uint4(0, 0, 0, 0);
             }
-            uint32_t top = 0;
+        }
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-            top = segment_max(top, a.segment_lanes);
-            float scale;
-            const uint32_t word = encode_fp4<kEach>(x, top, scale);
-            if (there && t.first < 2 * a.shape.row_bytes) store_codes<BF16>(a.codes[i] + (head_line + inside) * a.shape.row_bytes + t.first / 2, word);
-            if (there && (t.first & ((1 << a.shape.segment_shift) - 1)) == 0)
-                a.scales[i][head_line * a.shape.segments + ((long long)segment << a.shape.page_shift) + inside] = scale;
+        for (int e = 0; e < kHeads; ++e) {
+            if (n + e >= a.keys_each) break;
+            const int h = (group * a.keys_each + n + e) * turn.rows + t.row;
+            const bool there = line >= 0 && h < a.shape.kv_heads && valid > 0;
+            const long long head_line = line + ((long long)h << a.shape.page_shift);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x[kEach];
+                if (i == 0 && valid > 0) {
+                    float turned[kEach];
+                    lane.apply(turn, own[e][0], other[e], row[e], turned);
+                    unpack_lane<BF16>(pack_lane<BF16>(turned), x);
+#pragma unroll
+                    for (int k = 0; k < kEach; ++k) x[k] = k < valid ? x[k] : 0.0f;
+                } else {
+                    unpack_lane<BF16>(own[e][i], x);
+                }
+                uint32_t top = 0;
+#pragma unroll
+                for (int k = 0; k < kEach; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+                top = segment_max(top, a.segment_lanes);
+                float scale;
+                const uint32_t word = encode_fp4<kEach>(x, top, scale);
+                if (there && t.first < 2 * a.shape.row_bytes) store_codes<BF16>(a.codes[i] + (head_line + inside) * a.shape.row_bytes + t.first / 2, word);
+                if (there && (t.first & ((1 << a.shape.segment_shift) - 1)) == 0)
+                    a.scales[i][head_line * a.shape.segments + ((long long)segment << a.shape.page_shift) + inside] = scale;
+            }
         }
     }
 }
@@ -368,8 +399,15 @@ extern "C" void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const
     if (positions && !is_aligned(positions, long_positions ? 8 : 4)) { set_error(kBadArgument, "%s: unaligned positions", what); return; }
     a.segment_lanes = cache_segment_lanes(a.shape, bf16);
     const int lanes = a.segment_lanes * a.shape.segments;
-    const int block_tokens = kTurnThreads / lanes < 4 ? kTurnThreads / lanes : 4;
-    if (!turn_args(what, rotary, a.shape.head_dim, bf16, lanes, block_tokens, a.turn)) return;
+    // Few tokens: as many workgroups as there are.  Many, from about a thousand: 1050 tokens of 32 heads of 128 in bf16 13.8 us against 19.1, 529 11.8
+    // against 11.6, 18378 103 against 275.
+    const long long elements = (long long)a.at.tokens * heads * a.shape.head_dim;
+    const bool large = elements >= 1LL << 22;
+    const int most = kTurnThreads / lanes, keys_tokens = large ? 16 : 4, few = most < 4 ? most : 4;
+    if (!turn_args(what, rotary, a.shape.head_dim, bf16, lanes, most < keys_tokens ? most : keys_tokens, a.keys) ||
+        !turn_args(what, rotary, a.shape.head_dim, bf16, lanes, few, a.queries))
+        return;
+    a.keys_each = large ? 4 : 1, a.queries_each = large ? 8 : 1;
     if (a.at.tokens == 0) return;
     a.q = q->base, a.out = out->base, a.q_token = q->token_stride, a.q_head = q->head_stride, a.out_token = out->token_stride, a.out_head = out->head_stride;
     const qtensor_cache_vectors *both[2] = {keys, values};
@@ -378,12 +416,15 @@ extern "C" void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const
         a.codes[i] = cache->codes[i], a.scales[i] = cache->scales[i];
     }
     a.heads = heads, a.positions = positions, a.long_positions = long_positions != 0;
-    a.heads_each = 1;
-    const int at_once = a.turn.rows * a.heads_each;
-    a.query_groups = (heads + at_once - 1) / at_once;
-    const dim3 grid((unsigned)((a.at.tokens + block_tokens - 1) / block_tokens), (unsigned)(a.query_groups + (a.shape.kv_heads + at_once - 1) / at_once));
-    if (grid.y > 65535u) { set_error(kBadArgument, "%s: too many heads", what); return; }
-    if (bf16) hipLaunchKernelGGL(turn_write_kernel<true>, grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(turn_write_kernel<false>, grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
+    const auto cut = [](long long n, long long by) { return (n + by - 1) / by; };
+    a.key_blocks = (int)cut(a.at.tokens, a.keys.block_tokens), a.query_blocks = (int)cut(a.at.tokens, a.queries.block_tokens);
+    a.key_groups = a.key_blocks * cut(a.shape.kv_heads, a.keys.rows * a.keys_each);
+    const long long workgroups = a.key_groups + a.query_blocks * cut(heads, a.queries.rows * a.queries_each);
+    if (workgroups > 0x7fffffffLL) { set_error(kBadArgument, "%s: too many tokens and heads (%d, %d)", what, a.at.tokens, heads); return; }
+    const dim3 grid((unsigned)workgroups);
+    if (bf16 && large) hipLaunchKernelGGL((turn_write_kernel<true, true>), grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
+    else if (bf16) hipLaunchKernelGGL((turn_write_kernel<true, false>), grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
+    else if (large) hipLaunchKernelGGL((turn_write_kernel<false, true>), grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((turn_write_kernel<false, false>), grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
     launch_ok(what);
 }
