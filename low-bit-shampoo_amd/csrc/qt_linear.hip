@@ -94,7 +94,7 @@ __global__ __launch_bounds__(64 * WAVES) void linear_few_kernel(const LinearArgs
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
     const int tiles = (a.outputs + kLinearOutputs - 1) / kLinearOutputs;
     const int first_tile = blockIdx.x * R, first_token = blockIdx.y * 16 * T;
-    __shared__ fp4_f32x4 s_part[WAVES - 1][R * T][64];
+    __shared__ fp4_f32x4 s_part[WAVES][R * T][64];
     const uint32_t code_at = 16 * lane, scale_at = lane & 15;
     // (tokens and tiles behind the last are the last one again: what comes of them is not stored)
     const uint8_t *x[T];
@@ -156,28 +156,25 @@ __global__ __launch_bounds__(64 * WAVES) void linear_few_kernel(const LinearArgs
             }
         }
     }
-    if (wave) {
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int t = 0; t < T; ++t) s_part[wave - 1][r * T + t][lane] = sum[r][t];
-    }
+        for (int t = 0; t < T; ++t) s_part[wave][r * T + t][lane] = sum[r][t];
     __syncthreads();
-    if (wave) return;
+    // every wave joins tiles of its own
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int output = (first_tile + r) * kLinearOutputs + (lane & 15);
-        const float bias = output < a.outputs ? linear_bias(a, output) : 0.0f;
+    for (int n = 0; n < (R * T + WAVES - 1) / WAVES; ++n) {
+        const int tile = n * WAVES + wave;
+        if (tile >= R * T) break;
+        fp4_f32x4 y = s_part[0][tile][lane];
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
+        for (int w = 1; w < WAVES; ++w) y += s_part[w][tile][lane];
+        const int output = (first_tile + tile / T) * kLinearOutputs + (lane & 15), token = first_token + 16 * (tile % T) + 4 * quarter;
+        if (output >= a.outputs) continue;
+        const float bias = linear_bias(a, output);
 #pragma unroll
-            for (int w = 0; w < WAVES - 1; ++w) sum[r][t] += s_part[w][r * T + t][lane];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int token = first_token + 16 * t + 4 * quarter + i;
-                if (output < a.outputs && token < a.tokens) linear_store<BF16>(a, token, output, sum[r][t][i] + bias);
-            }
-        }
+        for (int i = 0; i < 4; ++i)
+            if (token + i < a.tokens) linear_store<BF16>(a, token + i, output, y[i] + bias);
     }
 }
 
