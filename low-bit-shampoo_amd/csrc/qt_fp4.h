@@ -97,6 +97,13 @@ struct Eight {
             }
         }
     }
+    // what lane 4 (l % 16) + l / 16 has loaded: a wave's loads of sixteen rows touch each row's line once if four lanes side by side have a row, the
+    // matrix instructions want lanes l, l + 16, l + 32, l + 48 to have it
+    __device__ __forceinline__ void exchange() {
+        const int lane = threadIdx.x & 63, from = 4 * (4 * (lane & 15) + (lane >> 4));
+#pragma unroll
+        for (uint32_t &r : raw) r = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)r);
+    }
     // piece 0 holds the first bits
     __device__ __forceinline__ void pieces(bf16x8 *out) const {
         if constexpr (BF16) {

@@ -56,13 +56,15 @@ __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linea
     };
     // a wave's part of a block of tokens: MT of the 4 MT pieces of 1 KB
     Eight<BF16> raw[BF16 ? 1 : MT];
+    // (four lanes side by side load 64 bytes of a token, in an order that keeps the lanes which read them off each other's banks)
+    const int eighth = 8 * ((lane & 3) ^ quarter), mine = 4 * (lane & 15) + (quarter ^ ((lane >> 2) & 3));
     const uint8_t *from[MT / 4];
     int valid[MT / 4];
 #pragma unroll
     for (int i = 0; i < MT / 4; ++i) {
-        const int token = first_token + 16 * (wave * (MT / 4) + i) + (lane & 15);
+        const int token = first_token + 16 * (wave * (MT / 4) + i) + (lane >> 2);
         valid[i] = token < a.tokens ? a.inputs : 0;
-        from[i] = (const uint8_t *)a.x + (long long)min(token, a.tokens - 1) * a.x_stride * (BF16 ? 2 : 4) + 8 * quarter * (BF16 ? 2 : 4);
+        from[i] = (const uint8_t *)a.x + (long long)min(token, a.tokens - 1) * a.x_stride * (BF16 ? 2 : 4) + eighth * (BF16 ? 2 : 4);
     }
     const auto load_tokens = [&](int block, int buffer) {
         const int first = block * kLinearInputs;
@@ -77,13 +79,13 @@ __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linea
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
                     Eight<BF16> x;
-                    x.load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - 8 * quarter);
+                    x.load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - eighth);
                     s_x[buffer * kPlane + (wave * MT + i) * 64 + lane] = (qt_u32x4){x.raw[0], x.raw[1], x.raw[2], x.raw[3]};
                 }
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) raw[i].load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - 8 * quarter);
+            for (int i = 0; i < MT; ++i) raw[i].load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - eighth);
         }
     };
     const auto put_tokens = [&]() {
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linea
                 for (int j = 0; j < J; ++j) {
                     bf16x8 x[P];
 #pragma unroll
-                    for (int p = 0; p < P; ++p) x[p] = __builtin_bit_cast(bf16x8, s_x[(buffer * P + p) * kPlane + (m * 4 + g * J + j) * 64 + lane]);
+                    for (int p = 0; p < P; ++p) x[p] = __builtin_bit_cast(bf16x8, s_x[(buffer * P + p) * kPlane + (m * 4 + g * J + j) * 64 + mine]);
 #pragma unroll
                     for (int n = 0; n < N; ++n) part[n] = multiply_pieces<P>(x, numbers[n][j], part[n]);
                 }
