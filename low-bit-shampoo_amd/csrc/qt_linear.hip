@@ -194,12 +194,13 @@ void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
     else hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 1, T == 1>), grid, dim3(64 * WAVES), 0, stream, a);
 }
 
-// Many tokens as soon as the kernel for them has a workgroup for every unit: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 24 us here
-// and 38 there, 512 and 4096 (256) 41 and 39, 256 and 11008 (344) 58 and 42.
+// Many tokens as soon as the kernel for them has a workgroup for every unit: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 15.3 us here
+// and 30.5 there, 256 and 11008 (344) 46 and 39.
 // Else the smallest tile of a workgroup whose workgroups have a unit each: every one reads all of its tokens (from L2) and joins its waves, so
-// more of them than that cost more than they spread.  By tiles of outputs x tokens: 16 tokens, 4096 outputs 1 x 1 6.7 us, 2 x 1 7.9, 4 x 1 10.1; 14336
-// outputs 18.3, 12.6, 10.5; 64 tokens, 4096 outputs 4 x 1 10.5, 4 x 2 15.4.  Four waves to a workgroup where there are several for each unit (32 tokens, 28672
-// outputs 25.1 us against 26.0 of eight).
+// more of them than that cost more than they spread.  By tiles of outputs x tokens, before loads of tokens and joins were as they are: 16 tokens, 4096
+// outputs 1 x 1 6.7 us, 2 x 1 7.9, 4 x 1 10.1; 14336 outputs 18.3, 12.6, 10.5; 64 tokens, 4096 outputs 4 x 1 10.5, 4 x 2 15.4; as they are, 64 tokens, 11008
+// outputs 4 x 4 14.5, 4 x 2 16.6.  Four waves to a workgroup where there are several for each unit (32 tokens, 28672 outputs 25.1 us against 26.0 of
+// eight).
 template <bool BF16>
 void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
     const long long tiles = (a.outputs + 15) / 16, rows = (a.tokens + 15) / 16, units = compute_units();
@@ -209,6 +210,7 @@ void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
     if ((tiles + 3) / 4 * rows <= units) return launch_few<BF16, 1, 4, 8>(a, groups, stream);
     if constexpr (BF16) {
         if (rows > 1 && (tiles + 3) / 4 * ((rows + 1) / 2) <= units) return launch_few<BF16, 2, 4, 8>(a, groups, stream);
+        if (rows > 2 && (tiles + 3) / 4 * ((rows + 3) / 4) <= units) return launch_few<BF16, 4, 4, 8>(a, groups, stream);
         if (rows > 1) return launch_few<BF16, 2, 4, 4>(a, groups, stream);
     }
     launch_few<BF16, 1, 4, 4>(a, groups, stream);

@@ -95,6 +95,40 @@ def test_weights_over_long_sequences(Cache, dtype):
         assert torch.equal(totals, once + once)                     # (the same sum again, every time)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_with_room_for_many_more_tokens(Cache, dim, dtype):
+    """A table that has room for so many tokens that scores are worked out twice, or that every wave has tokens of its own."""
+    lengths = [300]
+    cache, table, counts, keys, _ = filled(Cache, lengths, 1, dim, dtype, 4096)
+    table = torch.cat([table, torch.full((1, 2099), -1, dtype=torch.int32, device="cuda")], 1)
+    q = vectors((1, 16, dim), dtype, 9)
+    totals = torch.rand(1, 1, table.shape[1] * 4096, generator=torch.Generator().manual_seed(3))
+    for window, sinks in ((None, 0), (100, 7)):
+        got = cache.weigh(totals.cuda(), q.cuda(), table, counts, window=window, sinks=sinks)
+        check_weights(cache, got, totals, q, lengths, [1], keys, 64, window=window, sinks=sinks)
+    lengths, news = [200, 33, 0, 64, 1, 100, 90, 300], [40, 5, 0, 64, 1, 100, 2, 3]
+    cache, table, counts, keys, _ = filled(Cache, lengths, 8, dim, dtype, 16, wide=500)
+    q = vectors((sum(news), 16, dim), dtype, 9)
+    starts = torch.tensor([sum(news[:b]) for b in range(9)], dtype=torch.int32).cuda()
+    for window, sinks in ((None, 0), (30, 20)):
+        totals = cache.weigh(cache.totals(table), q.cuda(), table, counts, starts, window=window, sinks=sinks)
+        check_weights(cache, totals, torch.zeros(totals.shape), q, lengths, news, keys, 64, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(17, 1), (40, 2), (130, 1), (16, 16), (15, 5)])
+def test_weights_of_groups_of_all_sizes(Cache, heads, kv_heads):
+    lengths = [1, 70, 300]
+    cache, table, counts, keys, _ = filled(Cache, lengths, kv_heads, 64, torch.bfloat16)
+    q = vectors((3, heads, 64), torch.bfloat16, 9)
+    totals = cache.weigh(cache.totals(table), q.cuda(), table, counts)
+    check_weights(cache, totals, torch.zeros(totals.shape), q, lengths, [1] * 3, keys, 64)
+    news = [1, 5, 40]
+    q = vectors((46, heads, 64), torch.bfloat16, 9)
+    totals = cache.weigh(cache.totals(table), q.cuda(), table, counts, torch.tensor([0, 1, 6, 46], dtype=torch.int32).cuda())
+    check_weights(cache, totals, torch.zeros(totals.shape), q, lengths, news, keys, 64)
+
+
 def test_weights_are_those_of_attention(Cache):
     """Values that are 1 for one token at a time: attention gives its weight."""
     cache, table, counts, keys, _ = filled(Cache, [37], 1, 64, torch.float32)

@@ -77,6 +77,16 @@ def test_larger_products(Linear, tokens, inputs, outputs, dtype):
     check(Linear(inputs, outputs).quantize(w.cuda()).product(x.cuda()), x, w, 64)
 
 
+@pytest.mark.parametrize("tokens,inputs,outputs", [(3, 70, 17000), (20, 129, 17000), (40, 70, 17001), (30, 200, 9000), (60, 70, 8300), (64, 257, 8321),
+                                                   (15, 300, 9000), (9, 140, 5000), (250, 131, 4090)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tiles_of_all_sizes(Linear, tokens, inputs, outputs, dtype):
+    w, x = matrix(outputs, inputs, dtype, 14), matrix(tokens, inputs, dtype, 15)
+    for blocksize in (64, 128, 256):
+        held, bias = Linear(inputs, outputs, blocksize=blocksize).quantize(w.cuda()), torch.randn(outputs, generator=torch.Generator().manual_seed(16))
+        check(held.product(x.cuda(), bias.cuda()), x, w, blocksize, bias)
+
+
 @pytest.mark.parametrize("tokens,inputs,outputs", [(1030, 130, 2100), (1100, 64, 2050), (4200, 70, 8200), (70, 385, 33000)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_many_tokens_and_outputs(Linear, tokens, inputs, outputs, dtype):

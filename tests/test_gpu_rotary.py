@@ -195,6 +195,31 @@ def test_turned_into_the_cache_is_turned_then_written(Rotary, dim, dims, blocksi
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dim,dims,heads,kv_heads", [(128, 128, 56, 7), (80, 64, 90, 9), (256, 256, 30, 5), (33, 32, 220, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_tokens_turned_into_the_cache(Rotary, dim, dims, heads, kv_heads, dtype):
+    """As many as take the kernel's other tiles; rows behind the last sequence, a sequence that is shorter than its part."""
+    from qtensor.cache import QTensorCache
+    lengths, news = [403, 0, 17, 150, 4], [400, 0, 9, 150, 40]
+    rows = sum(news) + 7
+    width = -(-max(lengths) // 16)
+    table = torch.randperm(5 * width, generator=torch.Generator().manual_seed(1)).view(5, width).to(torch.int32).cuda()
+    table[3, 2] = 5 * width
+    counts = torch.tensor(lengths, dtype=torch.int32).cuda()
+    starts = torch.tensor([sum(news[:b]) for b in range(6)], dtype=torch.int32).cuda()
+    places = torch.tensor([n - a + i for n, a in zip(lengths, news) for i in range(a)] + [-1] * 7)
+    q, k, v = (vectors((rows, h, dim), dtype, 10 + i).cuda() for i, h in enumerate((heads, kv_heads, kv_heads)))
+    assert q.numel() >= 2 ** 22 or dim < 128
+    for interleaved in (False, True):
+        rotary = Rotary(dims, interleaved=interleaved)
+        caches = [QTensorCache(5 * width, kv_heads, dim, page_size=16) for _ in range(2)]
+        got = caches[0].write_turned(rotary, q, k, v, table, counts, starts)
+        want, turned = rotary.turn(q, k, places.cuda())
+        caches[1].write(turned, v, table, counts, starts)
+        want[(places < 0).cuda()] = 0
+        assert torch.equal(got, want) and torch.equal(caches[0].codes, caches[1].codes) and torch.equal(caches[0].scales, caches[1].scales)
+
+
 def test_a_token_of_each_sequence(Rotary):
     from qtensor.cache import QTensorCache
     rotary = Rotary(128)
