@@ -1,13 +1,14 @@
 """A small language model from training to answering: low-bit Shampoo trains it, then it generates with its attention cache held
-in 4 bits (qtensor.cache).
+in 4 bits (qtensor.cache), and if wanted its projections too (qtensor.linear).
 
-    python examples/generate.py [--steps 150] [--new 48]
+    python examples/generate.py [--steps 150] [--new 48] [--held]
 
 The text is synthetic: a random passage of PERIOD tokens, repeated; a model that has learnt it looks back one period.  Training runs in
 fp32 over whole sequences.  Serving takes prompts of different lengths in one call (every layer writes its keys and values, then
 attends), then one token of each sequence at a time, a step that is captured in a graph and replayed: what changes from step to step
 (tokens, lengths) lives on the GPU."""
 import argparse
+import copy
 import math
 import sys
 import time
@@ -19,6 +20,7 @@ from torch import nn
 sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "low-bit-shampoo_amd"))
 from optimizers.shampoo1 import ShampooAdamW  # noqa: E402
 from qtensor.cache import QTensorCache  # noqa: E402
+from qtensor.linear import QTensorLinear  # noqa: E402
 
 VOCABULARY, PERIOD, LONGEST = 32, 12, 128
 
@@ -85,10 +87,33 @@ def train(model, steps, batch=64, length=LONGEST, seed=0):
     return float(losses[0]), float(losses[-1])
 
 
-class Server:
-    """Generates for a batch of sequences: a cache per layer, pages handed out in front."""
+class Held(nn.Module):
+    """A projection as it is served: weights in 4 bits, no gradient."""
 
-    def __init__(self, model, batch, dtype=torch.bfloat16, page_size=16):
+    def __init__(self, linear):
+        super().__init__()
+        self.weights = QTensorLinear(linear.in_features, linear.out_features, device=linear.weight.device).quantize(linear.weight)
+        self.bias = linear.bias
+
+    def forward(self, x):
+        return self.weights.product(x, self.bias)
+
+
+def with_held_projections(model):
+    """A copy of the model whose projections are held in 4 bits."""
+    model = copy.deepcopy(model)
+    for module in list(model.modules()):
+        for name, child in module.named_children():
+            if isinstance(child, nn.Linear):
+                setattr(module, name, Held(child))
+    return model
+
+
+class Server:
+    """Generates for a batch of sequences: a cache per layer, pages handed out in front.  held: projections in 4 bits too."""
+
+    def __init__(self, model, batch, dtype=torch.bfloat16, page_size=16, held=False):
+        model = with_held_projections(model) if held else model
         first = model.layers[0]
         width = -(-LONGEST // page_size)
         self.model, self.dtype = model, dtype
@@ -149,6 +174,7 @@ def main():
     parser = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     parser.add_argument("--steps", type=int, default=150)
     parser.add_argument("--new", type=int, default=48)
+    parser.add_argument("--held", action="store_true", help="projections in 4 bits too")
     arguments = parser.parse_args()
     torch.manual_seed(0)
     model = Model().cuda()
@@ -157,7 +183,7 @@ def main():
     x = text(8, LONGEST, torch.Generator(device="cuda").manual_seed(1))
     counts = [24 + 5 * b for b in range(8)]
     new = min(arguments.new, LONGEST - max(counts))
-    server = Server(model, 8)
+    server = Server(model, 8, held=arguments.held)
     begin = time.perf_counter()
     got = server.generate([x[b, :n].cpu() for b, n in enumerate(counts)], new)
     torch.cuda.synchronize()

@@ -12,6 +12,7 @@ namespace {
 
 constexpr int kChooseThreads = 1024, kChooseWaves = kChooseThreads / 64;
 constexpr int kMoveThreads = 512;
+constexpr long long kMostTokens = 0x7fff0000;       // of a sequence: whole chunks (below), so that places do not pass 32 bits
 
 struct EvictArgs {
     CacheShape shape;
@@ -30,7 +31,7 @@ struct EvictArgs {
 
 __device__ __forceinline__ int evict_end(const EvictArgs &a, int b) {
     const long long covered = (long long)a.table_pages << a.shape.page_shift;
-    return (int)min((long long)max(a.lengths[b], 0), min(covered, 0x7fffff00LL));
+    return (int)min((long long)max(a.lengths[b], 0), min(covered, kMostTokens));
 }
 // First row of head 0 of the page of a place; negative: there is none.
 __device__ __forceinline__ long long evict_line(const EvictArgs &a, int b, int place) {
@@ -69,7 +70,7 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t *s_waves, ui
 }
 
 // Bound by the latency of its steps, and of fetching its instructions, which run once: loops stay loops (16384 keys in registers, all unrolled: 27 us for the
-// fewest tokens, 37 for 24 x 8 of 12000; CHOICE).  The least key of those that stay is found eight bits at a time, from counts in LDS; lanes
+// fewest tokens, 37 for 24 x 8 of 12000; so 13.5 and 23).  The least key of those that stay is found eight bits at a time, from counts in LDS; lanes
 // that have the digit of the first one among them are counted together, as totals of one size are most of them.
 __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const EvictArgs a) {
     __shared__ uint32_t s_key[kEach][kChooseThreads], s_waves[kChooseWaves];
@@ -275,7 +276,7 @@ bool evict_shape(const char *what, const qtensor_cache *cache, const qtensor_cac
     return true;
 }
 long long evict_keep(const CacheShape &shape, const CachePlaces &at, long long keep) {
-    const long long covered = (long long)at.table_pages << shape.page_shift, most = covered < 0x7fffff00LL ? covered : 0x7fffff00LL;
+    const long long covered = (long long)at.table_pages << shape.page_shift, most = covered < kMostTokens ? covered : kMostTokens;
     return keep < most ? keep : most;
 }
 

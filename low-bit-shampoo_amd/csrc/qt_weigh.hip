@@ -16,6 +16,7 @@ namespace {
 constexpr int kWeighThreads = 256, kWeighWaves = 4;
 constexpr int kParts = 16;             // of a row's tokens, at most
 constexpr int kLeastTiles = 16;        // of a part
+constexpr long long kMostTokens = 0x7fffff00;       // of a sequence
 
 struct WeighArgs {
     CacheShape shape;
@@ -63,7 +64,7 @@ __device__ __forceinline__ WeighSequence weigh_sequence(const WeighArgs &a, int 
     if (v.start < 0 || v.count < 0 || (long long)v.start + v.count > a.at.tokens) v.count = 0;      // (not a list of starts: nothing)
     v.first_position = length - v.count;
     const long long covered = (long long)a.at.table_pages << a.shape.page_shift;
-    v.end = (int)min((long long)max(length, 0), min(covered, 0x7fffff00LL));
+    v.end = (int)min((long long)max(length, 0), min(covered, kMostTokens));
     return v;
 }
 
@@ -663,7 +664,7 @@ void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
     // tiles of rows at most, and parts of their tokens: no more than make two workgroups for each that is wanted, nor than there are tokens to
     // see (the table's, or a window of each row's and the first ones)
     const long long row_tiles = a.at.starts ? (long long)a.at.tokens * a.group / rows + a.at.batch : (long long)a.at.batch * ((a.group + rows - 1) / rows);
-    const long long covered = (long long)a.at.table_pages << a.shape.page_shift, seen = a.window ? (long long)a.window + a.sinks + 80 : covered;
+    const long long room = (long long)a.at.table_pages << a.shape.page_shift, covered = room < kMostTokens ? room : kMostTokens, seen = a.window ? (long long)a.window + a.sinks + 80 : covered;
     const long long least = ((covered < seen ? covered : seen) + 16 * kLeastTiles - 1) / (16 * kLeastTiles), spread = 2 * a.wanted / (row_tiles * a.shape.kv_heads) + 1;
     a.parts = (int)(least < spread ? least : spread);
     a.parts = a.parts < kParts ? a.parts : kParts;
