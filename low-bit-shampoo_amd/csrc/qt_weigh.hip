@@ -14,7 +14,8 @@ namespace qt {
 namespace {
 
 constexpr int kWeighThreads = 256, kWeighWaves = 4;
-constexpr int kParts = 16;             // of a row's tokens, at most
+constexpr int kParts = 16;             // of a row's tokens, at most, where there is one tile of rows to a sequence
+constexpr int kMostParts = 64;         // and else
 constexpr int kLeastTiles = 16;        // of a part
 constexpr long long kMostTokens = 0x7fffff00;       // of a sequence
 
@@ -338,7 +339,7 @@ __device__ __forceinline__ WeighView weigh_view(const WeighArgs &a, int nearest,
     return w;
 }
 
-// Tiles of a part of ROWS rows' tokens: as many as all rows' work makes for every workgroup that is wanted, but no more than kParts parts of these.
+// Tiles of a part of ROWS rows' tokens: as many as all rows' work makes for every workgroup that is wanted, but no more than a.parts parts of these.
 template <int ROWS>
 __device__ __forceinline__ int part_tiles(const WeighArgs &a, int tiles) {
     const int lane = threadIdx.x & 63;
@@ -541,13 +542,14 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_scores_kernel(const Weigh
         if (token + e < end && row_sees(a, v.first_position, token + e)) total[e] += sum[e];
 }
 
-// (m, 1 / l) of every row from its parts: of all rows that a sequence may have (what is behind the last sequence is not used).
+// (m, 1 / l) of every row from its parts, sixteen lanes a row: of all rows that a sequence may have (what is behind the last sequence is not used).
 __global__ __launch_bounds__(kWeighThreads) void weigh_join_kernel(const WeighArgs a, long long entries) {
-    const long long entry = (long long)blockIdx.x * kWeighThreads + threadIdx.x;
-    if (entry >= entries) return;
-    float2 part = a.partial[entry * a.parts];
-    for (int n = 1; n < a.parts; ++n) part = join_parts(part, a.partial[entry * a.parts + n]);
-    a.statistics[entry] = make_float2(part.x == -INFINITY ? 0.0f : part.x, part.y == 0.0f ? 0.0f : 1.0f / part.y);
+    const long long entry = ((long long)blockIdx.x * kWeighThreads + threadIdx.x) >> 4;
+    float2 part = make_float2(-INFINITY, 0.0f);
+    for (int n = threadIdx.x & 15; n < a.parts && entry < entries; n += 16) part = join_parts(part, a.partial[entry * a.parts + n]);
+    const float top = row_max(part.x), m = top == -INFINITY ? 0.0f : top;
+    const float l = row_sum(part.y * __builtin_amdgcn_exp2f(part.x - m));
+    if (entry < entries && (threadIdx.x & 15) == 0) a.statistics[entry] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
 }
 
 // Tokens and the rows that see them, sixteen at a time: a wave keeps 16 N tokens' keys and goes through all rows, or (SHARED) the waves of
@@ -653,6 +655,16 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS < 8 ? 3 : 2) void weig
     }
 }
 
+// Tiles of rows at most, and parts of the tokens that they see: no more than make two rounds of workgroups, nor than there are tokens to see.
+long long weigh_row_tiles(const CachePlaces &at, int group, int rows) {
+    return at.starts ? (long long)at.tokens * group / rows + at.batch : (long long)at.batch * ((group + rows - 1) / rows);
+}
+int weigh_parts(long long workgroups, long long seen, bool few) {
+    const long long least = (seen + 16 * kLeastTiles - 1) / (16 * kLeastTiles), spread = 6LL * compute_units() / (workgroups < 1 ? 1 : workgroups) + 1, most = few ? kParts : kMostParts;
+    const long long parts = least < spread ? least : spread;
+    return (int)(parts < 1 ? 1 : parts < most ? parts : most);
+}
+
 template <bool BF16, int STEPS, int T>
 void launch_rows(const WeighArgs &a, unsigned row_tiles, hipStream_t stream) {
     hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, T, false>), dim3(row_tiles, a.shape.kv_heads, a.parts), dim3(kWeighThreads), 0, stream, a);
@@ -661,13 +673,11 @@ template <bool BF16, int STEPS>
 void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
     constexpr int N = STEPS == 8 ? 2 : 4, T = BF16 ? 2 : 1;
     const int rows = few ? 16 : 16 * T;
-    // tiles of rows at most, and parts of their tokens: no more than make two workgroups for each that is wanted, nor than there are tokens to
-    // see (the table's, or a window of each row's and the first ones)
-    const long long row_tiles = a.at.starts ? (long long)a.at.tokens * a.group / rows + a.at.batch : (long long)a.at.batch * ((a.group + rows - 1) / rows);
+    const long long row_tiles = weigh_row_tiles(a.at, a.group, rows);
     const long long room = (long long)a.at.table_pages << a.shape.page_shift, covered = room < kMostTokens ? room : kMostTokens, seen = a.window ? (long long)a.window + a.sinks + 80 : covered;
-    const long long least = ((covered < seen ? covered : seen) + 16 * kLeastTiles - 1) / (16 * kLeastTiles), spread = 2 * a.wanted / (row_tiles * a.shape.kv_heads) + 1;
-    a.parts = (int)(least < spread ? least : spread);
-    a.parts = a.parts < kParts ? a.parts : kParts;
+    // workgroups that the units hold
+    a.wanted = (few ? 6LL : BF16 ? 3LL : 4LL) * compute_units();
+    a.parts = weigh_parts(row_tiles * a.shape.kv_heads, covered < seen ? covered : seen, few);
     a.by_tiles = make_fastdiv((uint32_t)((a.group + rows - 1) / rows));
     if (few) {
         a.statistics = nullptr;
@@ -681,9 +691,9 @@ void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
     }
     launch_rows<BF16, STEPS, T>(a, (unsigned)row_tiles, stream);
     const long long entries = (long long)a.at.tokens * a.group * a.shape.kv_heads;
-    if (a.parts > 1) hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)((entries + kWeighThreads - 1) / kWeighThreads)), dim3(kWeighThreads), 0, stream, a, entries);
+    if (a.parts > 1) hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)((16 * entries + kWeighThreads - 1) / kWeighThreads)), dim3(kWeighThreads), 0, stream, a, entries);
     const long long blocks = (covered + 16 * N - 1) / (16 * N), apart = (blocks + kWeighWaves - 1) / kWeighWaves;
-    if (apart * a.shape.kv_heads * a.at.batch >= a.wanted)
+    if (apart * a.shape.kv_heads * a.at.batch >= 6LL * compute_units())
         hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, false>), dim3((unsigned)apart, a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
     else
         hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, true>), dim3((unsigned)blocks, a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
@@ -699,11 +709,13 @@ void launch_weigh_type(const WeighArgs &a, bool few, hipStream_t stream) {
 // Scores of a token of each sequence are kept, if they take up to 512 MB, instead of being worked out twice: 32 sequences of 100 to 8000 tokens 47 us
 // without and 38 with them.
 constexpr long long kMostScores = 1LL << 29;
-struct WeighSizes { long long partial, scores, stride, all; bool few; };
+struct WeighSizes { long long partial, scores, stride, all; int parts; bool few; };
 WeighSizes weigh_sizes(const CacheShape &shape, const CachePlaces &at, int heads) {
     WeighSizes s;
     s.few = !at.starts && heads / shape.kv_heads <= 16;         // a tile of rows for every sequence
-    s.partial = ((long long)at.tokens * heads * (kParts + 1) * (long long)sizeof(float2) + 255) & ~255LL;
+    // (the tiles of bf16 queries, of which there are fewest, and without a window)
+    s.parts = s.few ? kParts : weigh_parts(weigh_row_tiles(at, heads / shape.kv_heads, 32) * shape.kv_heads, (long long)at.table_pages << shape.page_shift, false);
+    s.partial = ((long long)at.tokens * heads * (s.parts + 1) * (long long)sizeof(float2) + 255) & ~255LL;
     s.stride = (((long long)at.table_pages << shape.page_shift) + 63) & ~63LL;
     s.scores = s.few && s.stride <= kMostScores / 4 / heads / at.batch ? s.stride * heads * at.batch * 4 : 0;
     s.all = s.partial + s.scores;
@@ -750,9 +762,8 @@ extern "C" void qtensor_hip_cache_weigh(const qtensor_cache *cache, const qtenso
     a.window = window, a.sinks = sinks;
     a.totals = totals, a.total_sequence = total_sequence, a.total_head = total_head;
     a.partial = (float2 *)workspace;
-    a.statistics = a.partial + (long long)a.at.tokens * heads * kParts;
+    a.statistics = a.partial + (long long)a.at.tokens * heads * size.parts;
     a.scores = size.scores ? (float *)((uint8_t *)workspace + size.partial) : nullptr, a.score_stride = size.stride;
-    a.wanted = 6LL * compute_units();
     a.by_group = make_fastdiv((uint32_t)a.group);
     if ((long long)a.at.tokens * a.group >= 1 << 29 || a.group >= 1 << 15 || a.at.batch > 65535 || a.shape.kv_heads > 65535) {
         set_error(kBadArgument, "%s: too many tokens, heads or sequences (%d, %d, %d)", what, a.at.tokens, heads, a.at.batch);
