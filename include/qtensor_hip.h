@@ -531,7 +531,7 @@ typedef struct {
 void qtensor_hip_linear_quantize(const qtensor_linear *weights, const void *weight, int is_bf16, long long row_stride, qtensor_stream_t stream);
 void qtensor_hip_linear_dequantize(const qtensor_linear *weights, void *weight, int is_bf16, long long row_stride, qtensor_stream_t stream);
 /* out[t] = W x[t] + bias for tokens x [tokens, inputs] and results [tokens, outputs], both fp32 or both bf16 with x_stride and
- * out_stride elements between tokens; bias [outputs] of fp32 or bf16, or NULL.  Products are exact and summed in fp32, a segment's
+ * out_stride elements between tokens; bias [outputs] of fp32 or bf16, or NULL; out shares no memory with them.  Products are exact and summed in fp32, a segment's
  * sum is multiplied by its scale, the result is rounded once. */
 typedef struct {
     const void *x, *bias;
@@ -577,7 +577,8 @@ void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const qtensor_ca
  * totals[b * total_sequence + h * total_head + t] += the sum, over the call's tokens of sequence b and the query heads that read head
  * h, of the weights softmax(scale q k) that they give token t: what qtensor_hip_cache_attend multiplies its value with.  Totals of tokens
  * that are not seen stay as they are.  Totals are as long as the table: table_pages * page_size.  workspace: 16-byte aligned, as
- * many bytes as qtensor_hip_cache_weigh_workspace says for these places' numbers (arrays are not looked at). */
+ * many bytes as qtensor_hip_cache_weigh_workspace says for these places' numbers (arrays are not looked at).  tokens * heads / kv_heads
+ * below 2^27. */
 long long qtensor_hip_cache_weigh_workspace(const qtensor_cache *cache, const qtensor_cache_places *places, int heads);
 void qtensor_hip_cache_weigh(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_cache_vectors *q, int heads, float scale,
                              int window, int sinks, float *totals, long long total_sequence, long long total_head, void *workspace,
@@ -585,8 +586,8 @@ void qtensor_hip_cache_weigh(const qtensor_cache *cache, const qtensor_cache_pla
 /* Of every sequence and head `keep` of the tokens that are there (whose page is) stay: those of the first `sinks` and the last `recent`
  * places, then those with the largest totals (NaN above all, ties to the earlier one).  Keys, values and totals of the nth token that stays
  * move to the place of the nth that is there; new_lengths[b] (another array than lengths) is one behind the last of these places, 0
- * if nothing is there.  What lies behind is left as it was.  Of the places, table and lengths count.  No two sequences may share
- * a page.  sinks + recent <= keep.  workspace as above. */
+ * if nothing is there.  What lies behind is left as it was.  Of the places, table and lengths count.  No page may be
+ * twice in the call.  sinks + recent <= keep.  workspace as above. */
 long long qtensor_hip_cache_evict_workspace(const qtensor_cache *cache, const qtensor_cache_places *places, long long keep);
 void qtensor_hip_cache_evict(const qtensor_cache *cache, const qtensor_cache_places *places, float *totals, long long total_sequence, long long total_head,
                              long long keep, long long recent, long long sinks, int *new_lengths, void *workspace, long long workspace_bytes,

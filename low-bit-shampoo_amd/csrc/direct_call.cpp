@@ -23,6 +23,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <array>
 #include <climits>
 #include <cmath>
@@ -404,6 +405,12 @@ std::pair<const char *, const char *> span(const at::Tensor &t) {
     const char *first = static_cast<const char *>(t.data_ptr());
     return {first, first + (last + 1) * t.element_size()};
 }
+// Whether the elements of a tensor [tokens, heads, head_dim] lie apart from each other.
+bool apart_within(const at::Tensor &t) {
+    const int64_t near = std::min(t.stride(0), t.stride(1)), far = std::max(t.stride(0), t.stride(1)), of_near = t.stride(0) < t.stride(1) ? t.size(0) : t.size(1);
+    if (t.size(0) < 2 || t.size(1) < 2) return t.numel() == 0 || std::max(t.size(0), t.size(1)) < 2 || (t.size(0) < 2 ? t.stride(1) : t.stride(0)) >= t.size(2);
+    return near >= t.size(2) && far >= near * (of_near - 1) + t.size(2);
+}
 bool apart(const at::Tensor &a, const at::Tensor &b) {
     if (a.numel() == 0 || b.numel() == 0) return true;
     const auto x = span(a), y = span(b);
@@ -435,7 +442,7 @@ PyObject *cache_write_turned_checked(PyObject *const *args) {
         result = {out.data_ptr(), q.is_bf16, out.stride(0), out.stride(1)};
     } else {
         const at::Tensor *given = vectors_of(args[17], c, t, t->size(0), t->size(1), result);
-        if (given == nullptr || !apart(*given, *t) || !apart(*given, *k) || !apart(*given, *v)) Py_RETURN_NONE;
+        if (given == nullptr || !apart_within(*given) || !apart(*given, *t) || !apart(*given, *k) || !apart(*given, *v)) Py_RETURN_NONE;
     }
     const int heads = (int)t->size(1);
     void *stream = stream_of(c);
@@ -466,7 +473,7 @@ PyObject *cache_weigh_checked(PyObject *const *args) {
     if (t == nullptr || t->size(1) < 1 || t->size(1) > 32767 || t->size(1) % c.cache.kv_heads != 0 || !places_of(args + 8, c, t->size(0))) Py_RETURN_NONE;
     const at::Tensor *totals = totals_of(args[6], c);
     const int heads = (int)t->size(1);
-    if (totals == nullptr || t->size(0) * (heads / c.cache.kv_heads) >= 1ll << 29) Py_RETURN_NONE;
+    if (totals == nullptr || t->size(0) * (heads / c.cache.kv_heads) >= 1ll << 27 || !apart(*totals, *t)) Py_RETURN_NONE;
     double scale = 1.0 / std::sqrt((double)c.cache.head_dim);
     if (args[11] != Py_None) {
         if (!PyFloat_CheckExact(args[11])) Py_RETURN_NONE;
@@ -543,7 +550,9 @@ PyObject *linear_product_checked(PyObject *const *args) {
         if (!in_plain_memory(out, device)) Py_RETURN_NONE;
     } else {
         const at::Tensor *given = plain(args[7], device);
-        if (given == nullptr || given->scalar_type() != x.scalar_type() || given->dim() != x.dim() || given->size(-1) != outputs || !apart(*given, x)) Py_RETURN_NONE;
+        if (given == nullptr || given->scalar_type() != x.scalar_type() || given->dim() != x.dim() || given->size(-1) != outputs || !apart(*given, x) ||
+            (bias != nullptr && !apart(*given, *bias)))
+            Py_RETURN_NONE;
         for (int64_t d = 0; d + 1 < x.dim(); ++d)
             if (given->size(d) != x.size(d)) Py_RETURN_NONE;
         out = *given;

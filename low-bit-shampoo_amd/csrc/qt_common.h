@@ -14,6 +14,7 @@ int error_code();          // this host thread's slot (0: the last call went thr
 bool launch_ok(const char *what);
 // Compute units of the current device (cached per device ordinal).
 int compute_units();
+constexpr long long kMostThreads = 1LL << 32;     // of a launch in x: less than these
 
 enum ErrorCode : int {
     kOk = 0,

@@ -239,7 +239,7 @@ void copy_linear(const char *what, bool write, const qtensor_linear *w, void *we
     const LinearCopy a = {w->codes, w->scales, weight, row_stride, w->inputs, w->outputs, blocks, (w->inputs + w->blocksize - 1) / w->blocksize, w->blocksize};
     const long long waves = (long long)((w->outputs + 15) / 16) * ((blocks + 1) / 2);
     const long long groups = (waves + kCodeThreads / 64 - 1) / (kCodeThreads / 64);
-    if (groups > 0x7fffffffLL) { set_error(kBadArgument, "%s: too many weights", what); return; }
+    if (groups >= kMostThreads / kCodeThreads) { set_error(kBadArgument, "%s: too many weights", what); return; }
     const dim3 grid((unsigned)groups);
     if (write && is_bf16) hipLaunchKernelGGL((linear_copy_kernel<true, true>), grid, dim3(kCodeThreads), 0, stream, a);
     else if (write) hipLaunchKernelGGL((linear_copy_kernel<false, true>), grid, dim3(kCodeThreads), 0, stream, a);

@@ -177,7 +177,7 @@ template <bool BF16, int MT, int N>
 void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
     const ManyGrid grid = {(a.tokens + 16 * MT - 1) / (16 * MT), (a.outputs + 64 * N - 1) / (64 * N), 8};
     const long long all = (long long)grid.rows * grid.columns, blocks = (all + kXcds - 1) / kXcds * kXcds;
-    if (blocks > 0x7ffffff0LL) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
+    if (blocks >= kMostThreads / kManyThreads) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
     const int shift = scales_of_block == 2 ? 0 : 1 + a.scales_shift;
     const bool aligned = is_aligned(a.x, 16) && a.x_stride % 8 == 0;
     hipLaunchKernelGGL((linear_many_kernel<BF16, MT, N>), dim3((unsigned)blocks), dim3(kManyThreads), 0, stream, a, grid, shift, aligned);

@@ -151,6 +151,7 @@ struct TurnCall {
     int long_positions;
     long long tokens, vectors;          // of a sequence, of all
     int heads_each;                     // heads that a thread goes through
+    long long first_block;              // of the launch
 };
 
 // 8 sequences of 2048 tokens, 40 heads of 128 in bf16: 72 us, 4.7 TB/s (a copy of the library's 4.9); a thread goes through four of
@@ -158,7 +159,7 @@ struct TurnCall {
 template <bool BF16>
 __global__ __launch_bounds__(kTurnThreads) void turn_kernel(const TurnCall a) {
     __shared__ float2 s_turn[kTurnPairs];
-    const long long first = (long long)blockIdx.x * a.turn.block_tokens;
+    const long long first = (a.first_block + blockIdx.x) * a.turn.block_tokens;
     work_out_turns(a.turn, s_turn, [&](int nth, double &at) {
         const long long n = first + nth;
         if (n >= a.vectors) return false;
@@ -375,11 +376,13 @@ extern "C" void qtensor_hip_rotary_turn(const qtensor_rotary *rotary, const qten
     a.positions = call->positions, a.position_batch = call->position_batch, a.long_positions = call->long_positions != 0;
     a.tokens = call->tokens, a.vectors = vectors;
     const long long blocks = (vectors + block_tokens - 1) / block_tokens;
-    if (blocks > 0x7fffffffLL) { set_error(kBadArgument, "%s: too many tokens (%lld)", what, vectors); return; }
-    const dim3 grid((unsigned)blocks, (unsigned)groups);
-    if (bf16) hipLaunchKernelGGL(turn_kernel<true>, grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL(turn_kernel<false>, grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
-    launch_ok(what);
+    const long long most = kMostThreads / kTurnThreads - 1;
+    for (; a.first_block < blocks; a.first_block += most) {
+        const dim3 grid((unsigned)(blocks - a.first_block < most ? blocks - a.first_block : most), (unsigned)groups);
+        if (bf16) hipLaunchKernelGGL(turn_kernel<true>, grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL(turn_kernel<false>, grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
+        if (!launch_ok(what)) return;
+    }
 }
 
 extern "C" void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const qtensor_cache_places *places, const qtensor_rotary *rotary,
@@ -420,7 +423,7 @@ extern "C" void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const
     a.key_blocks = (int)cut(a.at.tokens, a.keys.block_tokens), a.query_blocks = (int)cut(a.at.tokens, a.queries.block_tokens);
     a.key_groups = a.key_blocks * cut(a.shape.kv_heads, a.keys.rows * a.keys_each);
     const long long workgroups = a.key_groups + a.query_blocks * cut(heads, a.queries.rows * a.queries_each);
-    if (workgroups > 0x7fffffffLL) { set_error(kBadArgument, "%s: too many tokens and heads (%d, %d)", what, a.at.tokens, heads); return; }
+    if (workgroups >= kMostThreads / kTurnThreads) { set_error(kBadArgument, "%s: too many tokens and heads (%d, %d)", what, a.at.tokens, heads); return; }
     const dim3 grid((unsigned)workgroups);
     if (bf16 && large) hipLaunchKernelGGL((turn_write_kernel<true, true>), grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);
     else if (bf16) hipLaunchKernelGGL((turn_write_kernel<true, false>), grid, dim3(kTurnThreads), 0, (hipStream_t)stream, a);

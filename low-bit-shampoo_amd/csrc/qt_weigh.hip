@@ -765,7 +765,7 @@ extern "C" void qtensor_hip_cache_weigh(const qtensor_cache *cache, const qtenso
     a.statistics = a.partial + (long long)a.at.tokens * heads * size.parts;
     a.scores = size.scores ? (float *)((uint8_t *)workspace + size.partial) : nullptr, a.score_stride = size.stride;
     a.by_group = make_fastdiv((uint32_t)a.group);
-    if ((long long)a.at.tokens * a.group >= 1 << 29 || a.group >= 1 << 15 || a.at.batch > 65535 || a.shape.kv_heads > 65535) {
+    if ((long long)a.at.tokens * a.group >= 1 << 27 || a.group >= 1 << 15 || a.at.batch > 65535 || a.shape.kv_heads > 65535) {
         set_error(kBadArgument, "%s: too many tokens, heads or sequences (%d, %d, %d)", what, a.at.tokens, heads, a.at.batch);
         return;
     }

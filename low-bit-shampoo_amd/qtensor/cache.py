@@ -135,7 +135,7 @@ class QTensorCache:
         """Rotary positions on the way into the cache, in one launch: the queries q [tokens, heads, head_dim] turned; keys turned and encoded,
         values encoded, as `write` does with what rotary.turn gives.  positions: int32 or int64 [tokens], or None: a token's
         place in its sequence (which is another where tokens have been evicted).  Queries of tokens that are of no sequence or of a
-        negative place become zeros.  out: optional result of the shape and type of q that shares no memory with it."""
+        negative place become zeros.  out: optional result of the shape and type of q that shares no memory with q, keys or values."""
         if _native is not None:
             done = _native.cache_write_turned(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, rotary.frequencies,
                                               rotary.magnitude, rotary.dims, rotary.interleaved, q, keys, values, table, lengths, starts, positions, out)
@@ -161,6 +161,10 @@ class QTensorCache:
             self._check_vectors(out, "out", (tokens, heads, self.head_dim), q.dtype)
             if any(F._overlap(out, t) for t in (q, keys, values)):
                 raise ValueError("out shares memory with q, keys or values, which are read while it is written.")
+            by_stride = sorted((s, n) for s, n in zip(out.stride()[:2], out.shape[:2]) if n > 1)
+            for (stride, _), least in zip(by_stride, [self.head_dim] + [s * (n - 1) + self.head_dim for s, n in by_stride]):
+                if stride < least and out.numel():
+                    raise ValueError("out has elements that share memory with each other.")
         places = self._places(table, lengths, starts, tokens)
         F._call(F.lib.qtensor_hip_cache_write_turned, self.codes.device, self._ref(), places, rotary._ref(), _vectors(q), _vectors(out), heads, _vectors(keys),
                 _vectors(values), None if positions is None else positions.data_ptr(), positions is not None and positions.dtype == torch.int64)
@@ -234,8 +238,10 @@ class QTensorCache:
         tokens, heads, scale = self._check_queries(q, scale, window, sinks)
         places = self._places(table, lengths, starts, tokens)
         self._check_totals(totals, places)
-        if tokens * (heads // self.kv_heads) >= 2 ** 29 or places.batch > 65535:
+        if tokens * (heads // self.kv_heads) >= 2 ** 27 or places.batch > 65535:
             raise ValueError(f"{tokens} tokens of {heads} heads in {places.batch} sequences are too many for one call.")
+        if F._overlap(totals, q):
+            raise ValueError("totals share memory with q, which is read while they are written.")
         cache = self._ref()
         with torch.cuda.device(q.device):
             size = F.lib.qtensor_hip_cache_weigh_workspace(cache, places, heads)
@@ -250,7 +256,7 @@ class QTensorCache:
         totals, and what lies behind is left as it was.  Returns the new lengths, as a tensor of its own: layers with caches of their own share
         `lengths`, so copy them there once all caches are done, set the totals behind them to zero before tokens are written there, and hand the
         pages behind back.  A position that a token was turned by stays its own: give write_turned positions from now on.  Tokens without a
-        page are no candidates, and their places stay empty.  No two sequences of the call may share a page."""
+        page are no candidates, and their places stay empty.  No page may be twice in the call, in one sequence or in two."""
         if _native is not None:
             done = _native.cache_evict(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, totals, table, lengths,
                                        keep, recent, sinks)

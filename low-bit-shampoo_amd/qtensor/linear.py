@@ -91,7 +91,7 @@ class QTensorLinear:
 
     def product(self, x: Tensor, bias: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
         """W x + bias for every token: x [.., inputs] (fp32 or bf16) -> [.., outputs] of its type; bias [outputs] of fp32 or x's type.  Products are
-        exact and summed in fp32, the result is rounded once.  out: optional result, contiguous, that shares no memory with x.  Any number of
+        exact and summed in fp32, the result is rounded once.  out: optional result, contiguous, that shares no memory with x or bias.  Any number of
         tokens; sums in front of the scales, so up to 768 of x's largest magnitude, have to stay below 2^128."""
         if F._direct is not None:
             done = F._direct.linear_product(self.codes, self.scales, self.inputs, self.outputs, self.blocksize, x, bias, out)
@@ -116,8 +116,8 @@ class QTensorLinear:
             if tuple(out.shape) != shape:
                 raise ValueError(f"out has shape {tuple(out.shape)}, expected {shape}.")
             F._check_buffer(out, "out", rows.shape[0] * self.outputs, x.dtype, self.codes.device)
-            if F._overlap(out, rows):
-                raise ValueError("out shares memory with x, which is read while out is written.")
+            if F._overlap(out, rows) or (bias is not None and F._overlap(out, bias)):
+                raise ValueError("out shares memory with x or bias, which are read while it is written.")
         F._call(F.lib.qtensor_hip_linear_product, self.codes.device, self._ref(),
                 _Call(rows.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), rows.stride(0), self.outputs, rows.shape[0],
                       x.dtype == torch.bfloat16, bias is not None and bias.dtype == torch.bfloat16))
