@@ -388,6 +388,9 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
         return;
     }
     const auto tile_at = [&](int index) { return index < view.sink_tiles ? index : view.first_tile + index - view.sink_tiles; };
+    WeighRows<BF16, STEPS> q[T];
+#pragma unroll
+    for (int r = 0; r < T; ++r) q[r].fetch(a, v, head, first_row + 16 * r);
     WeighKeys<STEPS, N> keys;
     int tile = 0;
     const int first = from + wave * N;
@@ -395,9 +398,6 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
         tile = tile_at(first);
         keys.fetch(a, b, head, tile, v.end);
     }
-    WeighRows<BF16, STEPS> q[T];
-#pragma unroll
-    for (int r = 0; r < T; ++r) q[r].fetch(a, v, head, first_row + 16 * r);
 #pragma unroll
     for (int r = 0; r < T; ++r) q[r].arrange();
     float m[T][4], l[T][4];             // WEIGHTS: 1 / l
@@ -519,27 +519,40 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_scores_kernel(const Weigh
     const WeighView view = weigh_view(a, v.first_position, v.first_position, v.end);
     const int end = min(v.first_position + 1, v.end);
     if (first >= end) return;
+    // (what is read hangs on the length alone)
+    constexpr int kAhead = 4;
+    const int token = first + 4 * (int)threadIdx.x;
+    const bool mine = token < end && (token < 16 * view.sink_tiles || token >= 16 * view.first_tile);
+    float *total = a.totals + b * a.total_sequence + head * a.total_head + token;
+    const float *from = a.scores + ((long long)b * a.shape.kv_heads + head) * a.group * a.score_stride + token;
+    int page = -1;
+    float4 ahead[kAhead];
+    qt_u32x4 before;
+    if (mine) {
+        page = a.at.table[b * a.at.table_stride + (token >> a.shape.page_shift)];
+#pragma unroll
+        for (int g = 0; g < kAhead; ++g) ahead[g] = load_f32x4<true>(from + min(g, a.group - 1) * a.score_stride);
+        before = ((const Unaligned16of4 *)total)->v;
+    }
     if (threadIdx.x < 64) {
         const float2 row = row_statistics(a, v, head, 0);
         if (threadIdx.x < 16) s_row[threadIdx.x] = row;
     }
     __syncthreads();
-    const int token = first + 4 * (int)threadIdx.x;
-    if (token >= end || (token >= 16 * view.sink_tiles && token < 16 * view.first_tile)) return;
-    const int page = a.at.table[b * a.at.table_stride + (token >> a.shape.page_shift)];
     if ((unsigned)page >= (unsigned)a.shape.pages) return;
-    float *total = a.totals + b * a.total_sequence + head * a.total_head + token;
-    const float *from = a.scores + ((long long)b * a.shape.kv_heads + head) * a.group * a.score_stride + token;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g = 0; g < a.group; ++g) {
-        const float4 s = load_f32x4<true>(from + g * a.score_stride);
+    const auto add = [&](const float4 &s, int g) {
         const float2 row = s_row[g];
         sum[0] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.x - row.x), row.y, sum[0]), sum[1] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.y - row.x), row.y, sum[1]);
         sum[2] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.z - row.x), row.y, sum[2]), sum[3] = __builtin_fmaf(__builtin_amdgcn_exp2f(s.w - row.x), row.y, sum[3]);
-    }
+    };
+#pragma unroll
+    for (int g = 0; g < kAhead; ++g)
+        if (g < a.group) add(ahead[g], g);
+    for (int g = kAhead; g < a.group; ++g) add(load_f32x4<true>(from + g * a.score_stride), g);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        if (token + e < end && row_sees(a, v.first_position, token + e)) total[e] += sum[e];
+        if (token + e < end && row_sees(a, v.first_position, token + e)) total[e] = __uint_as_float(before[e]) + sum[e];
 }
 
 // (m, 1 / l) of every row from its parts, sixteen lanes a row: of all rows that a sequence may have (what is behind the last sequence is not used).
