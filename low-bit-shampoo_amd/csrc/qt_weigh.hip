@@ -221,39 +221,6 @@ __device__ __forceinline__ fp4_f32x4 weigh_scores(const WeighRows<BF16, STEPS> &
     return sum;
 }
 
-// Finds the tile of ROWS rows that is the `index`th of the call: its sequence and the row that it begins with.
-template <int ROWS>
-__device__ __forceinline__ bool find_rows(const WeighArgs &a, int index, int &b, int &first_row) {
-    if (!a.at.starts) {
-        b = (int)fastdiv((uint32_t)index, a.by_tiles), first_row = (index - b * ((a.group + ROWS - 1) / ROWS)) * ROWS;
-        return b < a.at.batch;
-    }
-    const int lane = threadIdx.x & 63;
-    int before = 0;
-    for (int first = 0; first < a.at.batch; first += 64) {
-        int tiles = 0;
-        if (first + lane < a.at.batch) {
-            const WeighSequence v = weigh_sequence<false>(a, first + lane);
-            tiles = (v.count * a.group + ROWS - 1) / ROWS;
-        }
-        int upto = tiles;
-#pragma unroll
-        for (int off = 1; off < 64; off *= 2) {
-            const int other = __shfl_up(upto, off, 64);
-            if (lane >= off) upto += other;
-        }
-        const unsigned long long at = __ballot(index < before + upto);
-        if (at) {
-            const int found = __builtin_ctzll(at);
-            b = first + found;
-            first_row = (index - before - __shfl(upto - tiles, found, 64)) * ROWS;
-            return true;
-        }
-        before += __shfl(upto, 63, 64);
-    }
-    return false;
-}
-
 // Over the sixteen lanes of a row of the wave, and over its four rows, for all lanes.
 template <int CTRL>
 __device__ __forceinline__ float dpp_f32(float x) { return __uint_as_float(dpp_u32<CTRL>(__float_as_uint(x))); }
@@ -339,20 +306,61 @@ __device__ __forceinline__ WeighView weigh_view(const WeighArgs &a, int nearest,
     return w;
 }
 
-// Tiles of a part of ROWS rows' tokens: as many as all rows' work makes for every workgroup that is wanted, but no more than a.parts parts of these.
+// The `index`th piece of work of the call: ROWS rows of a sequence, and which of how many parts of the tokens that they see, of `each` tiles.  Every part of
+// all rows has as many tiles as make a.wanted of them, at least kLeastTiles and no more than a.parts for a row; a sequence's rows have equally many.
+struct WeighWork { int b, first_row, part, parts, each; };
 template <int ROWS>
-__device__ __forceinline__ int part_tiles(const WeighArgs &a, int tiles) {
+__device__ __forceinline__ bool find_work(const WeighArgs &a, int index, WeighWork &w) {
     const int lane = threadIdx.x & 63;
-    float all = 0.0f;
-    for (int first = 0; first < a.at.batch; first += 64) {
-        if (first + lane < a.at.batch) {
-            const WeighSequence v = weigh_sequence<false>(a, first + lane);
-            all += (float)((v.count * a.group + ROWS - 1) / ROWS) * (float)weigh_view(a, v.first_position, v.first_position + v.count - 1, v.end).tiles;
-        }
+    if (!a.at.starts && a.parts == 1) {
+        const int b = (int)fastdiv((uint32_t)index, a.by_tiles);
+        w = {b, (index - b * ((a.group + ROWS - 1) / ROWS)) * ROWS, 0, 1, 0x7fffffff};
+        return b < a.at.batch;
     }
-    all = quarters_sum(row_sum(all));
-    const int even = (int)fminf(ceilf(all * (float)a.shape.kv_heads / (float)a.wanted), 1.0e9f);
-    return (max(max(even, kLeastTiles), (tiles + a.parts - 1) / a.parts) + 3) & ~3;
+    int rows = 0, tiles = 0;                            // tiles of rows of this lane's sequence, of tokens that any of them may see
+    const auto look = [&](int b) {
+        rows = tiles = 0;
+        if (b >= a.at.batch) return;
+        const WeighSequence v = weigh_sequence<false>(a, b);
+        rows = (v.count * a.group + ROWS - 1) / ROWS;
+        tiles = weigh_view(a, v.first_position, v.first_position + v.count - 1, v.end).tiles;
+        // (with a window fewer than the whole call's: sinks in whole fours, the window and as many places more as rows, from a whole four on)
+        if (a.window) tiles = (int)min((long long)tiles, (((long long)a.sinks + 63) >> 6) * 4 + (((long long)a.window + ROWS + 63) >> 4) + 2);
+    };
+    int least = kLeastTiles;
+    if (a.parts > 1) {
+        float all = 0.0f;
+        for (int first = 0; first < a.at.batch; first += 64) {
+            look(first + lane);
+            all += (float)rows * (float)tiles;
+        }
+        all = quarters_sum(row_sum(all));
+        least = max(least, (int)fminf(ceilf(all * (float)a.shape.kv_heads / (float)a.wanted), 1.0e9f));
+    }
+    int before = 0;
+    for (int first = 0; first < a.at.batch; first += 64) {
+        if (a.parts == 1 || a.at.batch > 64) look(first + lane);
+        const int each = (max(least, (int)((uint32_t)(tiles + a.parts - 1) / (uint32_t)a.parts)) + 3) & ~3;
+        const int parts = a.parts == 1 ? 1 : max(1, (int)((uint32_t)(tiles + each - 1) / (uint32_t)each));
+        int upto = rows * parts;
+#pragma unroll
+        for (int off = 1; off < 64; off *= 2) {
+            const int other = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += other;
+        }
+        const unsigned long long at = __ballot(index < before + upto);
+        if (at) {
+            const int found = __builtin_ctzll(at);
+            w.b = first + found;
+            w.parts = __builtin_amdgcn_readlane(parts, found), w.each = a.parts == 1 ? 0x7fffffff : __builtin_amdgcn_readlane(each, found);
+            const int nth = index - before - __builtin_amdgcn_readlane(upto - rows * parts, found);
+            const int tile = (int)((uint32_t)nth / (uint32_t)w.parts);
+            w.first_row = tile * ROWS, w.part = nth - tile * w.parts;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
 }
 
 // 16 T rows and a part of the tokens that they see: m and l of each, or (WEIGHTS, where a sequence has no more rows than these) the
@@ -363,25 +371,30 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
     constexpr int N = STEPS == 8 ? 2 : 4, kRows = 16 * T;
     __shared__ float2 s_part[kWeighWaves][kRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
-    const int head = blockIdx.y;
-    int b, first_row;
-    // (workgroups go round the XCDs, and on each round its engines, in turn: parts and heads of a long sequence are spread over all of them)
-    const unsigned turned = (blockIdx.x + 9 * blockIdx.y + 11 * blockIdx.z) % gridDim.x;
-    if (!find_rows<kRows>(a, (int)turned, b, first_row)) return;
-    b = __builtin_amdgcn_readfirstlane(b), first_row = __builtin_amdgcn_readfirstlane(first_row);
+    // (heads first: workgroups without work, of which the host knows no better, are the last ones)
+    const int head = blockIdx.x;
+    WeighWork work;
+    if (!find_work<kRows>(a, (int)(blockIdx.y + gridDim.y * blockIdx.z), work)) return;
+    const int b = __builtin_amdgcn_readfirstlane(work.b), first_row = __builtin_amdgcn_readfirstlane(work.first_row);
     const WeighSequence v = weigh_sequence<true>(a, b);
     const int rows = v.count * a.group;
     if (first_row >= rows) return;
     const int nearest = v.position(a, first_row), furthest = v.position(a, min(rows, first_row + kRows) - 1);
     const WeighView view = weigh_view(a, nearest, furthest, v.end);
-    const int each = __builtin_amdgcn_readfirstlane(part_tiles<kRows>(a, view.tiles));
-    const int from = (int)min((long long)view.tiles, (long long)blockIdx.z * each), to = min(view.tiles, from + each);
+    const int each = __builtin_amdgcn_readfirstlane(work.each), nth = __builtin_amdgcn_readfirstlane(work.part);
+    const int from = (int)min((long long)view.tiles, (long long)nth * each), to = (int)min((long long)view.tiles, (long long)from + each);
+    if (!WEIGHTS && nth == work.parts - 1) {
+        // (parts of other sequences' rows)
+        const int row = first_row + (int)threadIdx.x % kRows;
+        for (int n = work.parts + (int)threadIdx.x / kRows; n < a.parts && row < rows; n += kWeighThreads / kRows)
+            a.partial[row_entry(a, v, head, row) * a.parts + n] = make_float2(-INFINITY, 0.0f);
+    }
     const auto put = [&](float2 part) {
         const long long entry = row_entry(a, v, head, first_row + (int)threadIdx.x);
         if (a.parts == 1 && a.statistics)
             a.statistics[entry] = make_float2(part.x == -INFINITY ? 0.0f : part.x, part.y == 0.0f ? 0.0f : 1.0f / part.y);
         else
-            a.partial[entry * a.parts + blockIdx.z] = part;
+            a.partial[entry * a.parts + nth] = part;
     };
     if (from >= to) {
         if (!WEIGHTS && threadIdx.x < kRows && first_row + (int)threadIdx.x < rows) put(make_float2(-INFINITY, 0.0f));
@@ -679,8 +692,8 @@ int weigh_parts(long long workgroups, long long seen, bool few) {
 }
 
 template <bool BF16, int STEPS, int T>
-void launch_rows(const WeighArgs &a, unsigned row_tiles, hipStream_t stream) {
-    hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, T, false>), dim3(row_tiles, a.shape.kv_heads, a.parts), dim3(kWeighThreads), 0, stream, a);
+void launch_rows(const WeighArgs &a, const dim3 &work, hipStream_t stream) {
+    hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, T, false>), work, dim3(kWeighThreads), 0, stream, a);
 }
 template <bool BF16, int STEPS>
 void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
@@ -688,21 +701,27 @@ void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
     const int rows = few ? 16 : 16 * T;
     const long long row_tiles = weigh_row_tiles(a.at, a.group, rows);
     const long long room = (long long)a.at.table_pages << a.shape.page_shift, covered = room < kMostTokens ? room : kMostTokens, seen = a.window ? (long long)a.window + a.sinks + 80 : covered;
-    // workgroups that the units hold
-    a.wanted = (few ? 6LL : BF16 ? 3LL : 4LL) * compute_units();
+    // Parts of rows as make one round of the workgroups that the units hold, or, where tiles of rows are so many that this would leave few, three quarters of it:
+    // 16 sequences of up to 7600 tokens and 8 heads 21.4 us of 896, 24.1 of 1536; 64 of up to 7975 74.1 us of 512, 63.7 of 768; parts that go to workgroups in order of
+    // their own, for lack of one of these, began in a second round at 20 us where the first took 25.
+    const long long held = (BF16 ? (few ? 4 : 3) - (STEPS == 8) : STEPS == 8 ? 2 : 3) * compute_units(), tiles = row_tiles * a.shape.kv_heads;
+    a.wanted = held - tiles > 3 * held / 4 ? held - tiles : 3 * held / 4;
     a.parts = weigh_parts(row_tiles * a.shape.kv_heads, covered < seen ? covered : seen, few);
     a.by_tiles = make_fastdiv((uint32_t)((a.group + rows - 1) / rows));
+    // (parts of equal size, and one more for each tile of rows that they do not divide)
+    const long long pieces = a.parts == 1 ? row_tiles : min(row_tiles * a.parts, row_tiles + a.wanted / a.shape.kv_heads + 1), most = 32768;
+    const dim3 work(a.shape.kv_heads, (unsigned)min(pieces, most), (unsigned)((pieces + most - 1) / most));
     if (few) {
         a.statistics = nullptr;
-        launch_rows<BF16, STEPS, 1>(a, (unsigned)row_tiles, stream);
+        launch_rows<BF16, STEPS, 1>(a, work, stream);
         if (a.scores) {
             const dim3 grid((unsigned)((covered + 4 * kWeighThreads - 1) / (4 * kWeighThreads)), a.shape.kv_heads, a.at.batch);
             hipLaunchKernelGGL(weigh_scores_kernel, grid, dim3(kWeighThreads), 0, stream, a);
         } else
-            hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, 1, true>), dim3((unsigned)row_tiles, a.shape.kv_heads, a.parts), dim3(kWeighThreads), 0, stream, a);
+            hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, 1, true>), work, dim3(kWeighThreads), 0, stream, a);
         return;
     }
-    launch_rows<BF16, STEPS, T>(a, (unsigned)row_tiles, stream);
+    launch_rows<BF16, STEPS, T>(a, work, stream);
     const long long entries = (long long)a.at.tokens * a.group * a.shape.kv_heads;
     if (a.parts > 1) hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)((16 * entries + kWeighThreads - 1) / kWeighThreads)), dim3(kWeighThreads), 0, stream, a, entries);
     const long long blocks = (covered + 16 * N - 1) / (16 * N), apart = (blocks + kWeighWaves - 1) / kWeighWaves;
