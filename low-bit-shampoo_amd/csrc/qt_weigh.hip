@@ -14,8 +14,7 @@ namespace qt {
 namespace {
 
 constexpr int kWeighThreads = 256, kWeighWaves = 4;
-constexpr int kParts = 16;             // of a row's tokens, at most, where there is one tile of rows to a sequence
-constexpr int kMostParts = 64;         // and else
+constexpr int kMostParts = 64;         // of a row's tokens
 constexpr int kLeastTiles = 16;        // of a part
 constexpr long long kMostTokens = 0x7fffff00;       // of a sequence
 
@@ -254,23 +253,25 @@ __device__ __forceinline__ float2 join_parts(float2 x, float2 y) {
 // (m, 1 / l) of the row `first_row` + lane % 16, from its parts; (0, 0) where nothing is seen, (infinity, 0) behind the last row.
 __device__ __forceinline__ float2 row_statistics(const WeighArgs &a, const WeighSequence &v, int head, int first_row) {
     const int lane = threadIdx.x & 63, quarter = lane >> 4, row = first_row + (lane & 15);
-    static_assert(kParts == 16, "four parts a lane");
-    float2 each[4];
+    float m = -INFINITY, l = 0.0f;
+    const float2 *p = a.partial + row_entry(a, v, head, min(row, v.count * a.group - 1)) * a.parts;
+    for (int first = 0; first < a.parts; first += 16) {
+        float2 each[4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) each[n] = make_float2(-INFINITY, 0.0f);
-    if (row < v.count * a.group) {
-        const float2 *p = a.partial + row_entry(a, v, head, row) * a.parts;
+        for (int n = 0; n < 4; ++n) {
+            const int at = first + 4 * n + quarter;
+            each[n] = at < a.parts ? p[at] : make_float2(-INFINITY, 0.0f);
+        }
+        const float top = fmaxf(fmaxf(fmaxf(each[0].x, each[1].x), fmaxf(each[2].x, each[3].x)), m), by = top == -INFINITY ? 0.0f : top;
+        l *= __builtin_amdgcn_exp2f(m - by);
 #pragma unroll
-        for (int n = 0; n < kParts / 4; ++n)
-            if (4 * n + quarter < a.parts) each[n] = p[4 * n + quarter];
+        for (int n = 0; n < 4; ++n) l += each[n].y * __builtin_amdgcn_exp2f(each[n].x - by);
+        m = top;
     }
-    float m = fmaxf(fmaxf(each[0].x, each[1].x), fmaxf(each[2].x, each[3].x));
+    const float mine = m;
     m = quarters_max(m);
     m = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-#pragma unroll
-    for (int n = 0; n < kParts / 4; ++n) l += each[n].y * __builtin_amdgcn_exp2f(each[n].x - m);
-    l = quarters_sum(l);
+    l = quarters_sum(l * __builtin_amdgcn_exp2f(mine - m));
     return row < v.count * a.group ? make_float2(m, l == 0.0f ? 0.0f : 1.0f / l) : make_float2(INFINITY, 0.0f);
 }
 
@@ -681,14 +682,14 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS < 8 ? 3 : 2) void weig
     }
 }
 
-// Tiles of rows at most, and parts of the tokens that they see: no more than make two rounds of workgroups, nor than there are tokens to see.
+// Tiles of rows at most, and parts of the tokens that they see: no more than leave several to a workgroup of a round, nor than there are tokens to see.
 long long weigh_row_tiles(const CachePlaces &at, int group, int rows) {
     return at.starts ? (long long)at.tokens * group / rows + at.batch : (long long)at.batch * ((group + rows - 1) / rows);
 }
-int weigh_parts(long long workgroups, long long seen, bool few) {
-    const long long least = (seen + 16 * kLeastTiles - 1) / (16 * kLeastTiles), spread = 6LL * compute_units() / (workgroups < 1 ? 1 : workgroups) + 1, most = few ? kParts : kMostParts;
+int weigh_parts(long long workgroups, long long seen) {
+    const long long least = (seen + 16 * kLeastTiles - 1) / (16 * kLeastTiles), spread = 6LL * compute_units() / (workgroups < 1 ? 1 : workgroups) + 1;
     const long long parts = least < spread ? least : spread;
-    return (int)(parts < 1 ? 1 : parts < most ? parts : most);
+    return (int)(parts < 1 ? 1 : parts < kMostParts ? parts : kMostParts);
 }
 
 template <bool BF16, int STEPS, int T>
@@ -706,7 +707,7 @@ void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
     // their own, for lack of one of these, began in a second round at 20 us where the first took 25.
     const long long held = (BF16 ? (few ? 4 : 3) - (STEPS == 8) : STEPS == 8 ? 2 : 3) * compute_units(), tiles = row_tiles * a.shape.kv_heads;
     a.wanted = held - tiles > 3 * held / 4 ? held - tiles : 3 * held / 4;
-    a.parts = weigh_parts(row_tiles * a.shape.kv_heads, covered < seen ? covered : seen, few);
+    a.parts = weigh_parts(row_tiles * a.shape.kv_heads, covered < seen ? covered : seen);
     a.by_tiles = make_fastdiv((uint32_t)((a.group + rows - 1) / rows));
     // (parts of equal size, and one more for each tile of rows that they do not divide)
     const long long pieces = a.parts == 1 ? row_tiles : min(row_tiles * a.parts, row_tiles + a.wanted / a.shape.kv_heads + 1), most = 32768;
@@ -746,7 +747,7 @@ WeighSizes weigh_sizes(const CacheShape &shape, const CachePlaces &at, int heads
     WeighSizes s;
     s.few = !at.starts && heads / shape.kv_heads <= 16;         // a tile of rows for every sequence
     // (the tiles of bf16 queries, of which there are fewest, and without a window)
-    s.parts = s.few ? kParts : weigh_parts(weigh_row_tiles(at, heads / shape.kv_heads, 32) * shape.kv_heads, (long long)at.table_pages << shape.page_shift, false);
+    s.parts = weigh_parts(weigh_row_tiles(at, heads / shape.kv_heads, 32) * shape.kv_heads, (long long)at.table_pages << shape.page_shift);
     s.partial = ((long long)at.tokens * heads * (s.parts + 1) * (long long)sizeof(float2) + 255) & ~255LL;
     s.stride = (((long long)at.table_pages << shape.page_shift) + 63) & ~63LL;
     s.scores = s.few && s.stride <= kMostScores / 4 / heads / at.batch ? s.stride * heads * at.batch * 4 : 0;
