@@ -275,22 +275,19 @@ __device__ __forceinline__ float2 row_statistics(const WeighArgs &a, const Weigh
     return row < v.count * a.group ? make_float2(m, l == 0.0f ? 0.0f : 1.0f / l) : make_float2(INFINITY, 0.0f);
 }
 
-// Sums over the rows of N tiles' tokens (lane % 16): of the tile that a lane is to write.
+// Sums over the rows of N tiles' tokens (lane % 16): of the tile lane / 16, or with two of lane / 32.
 template <int N>
-__device__ __forceinline__ float sum_of_rows(float *sum, int &tile, bool &writes) {
-    const int quarter = (threadIdx.x & 63) >> 4;
-    uint32_t w[4];
+__device__ __forceinline__ float sum_of_rows(const float *sum) {
     if constexpr (N == 4) {
+        uint32_t w[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) w[n] = __float_as_uint(sum[n]);
         transpose_quarters(w);
-        tile = quarter, writes = true;
         return (__uint_as_float(w[0]) + __uint_as_float(w[1])) + (__uint_as_float(w[2]) + __uint_as_float(w[3]));
     } else {
         const auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[0]), __float_as_uint(sum[1]), false, false);
         const uint32_t half = __float_as_uint(__uint_as_float(two[0]) + __uint_as_float(two[1]));
         const auto both = __builtin_amdgcn_permlane16_swap(half, half, false, false);
-        tile = quarter >> 1, writes = (quarter & 1) == 0;
         return __uint_as_float(both[0]) + __uint_as_float(both[1]);
     }
 }
@@ -482,14 +479,12 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[0][n][i] - m[0][i]), l[0][i], sum[n]);
             }
-            int mine;
-            bool writes;
-            const float weight = sum_of_rows<N>(sum, mine, writes);
-            const int t = token + 16 * mine + (lane & 15);
-            bool is = there[0];
+            const float weight = sum_of_rows<N>(sum);
+            const int mine = N == 4 ? quarter : quarter >> 1, t = token + 16 * mine + (lane & 15);
+            bool is = N == 4 || (quarter & 1) == 0;
 #pragma unroll
-            for (int n = 1; n < N; ++n) is = mine == n ? there[n] : is;
-            if (writes && is && t < v.end && row_sees(a, furthest, t)) a.totals[b * a.total_sequence + head * a.total_head + t] += weight;
+            for (int n = 0; n < N; ++n) is = is && (mine != n || there[n]);
+            if (is && t < v.end && row_sees(a, furthest, t)) a.totals[b * a.total_sequence + head * a.total_head + t] += weight;
         } else {
 #pragma unroll
             for (int r = 0; r < T; ++r)
@@ -579,106 +574,208 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_join_kernel(const WeighAr
     if (entry < entries && (threadIdx.x & 15) == 0) a.statistics[entry] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
 }
 
+// Groups of 16 N tokens of all sequences that rows see, one sequence after the other, cut into parts of equal cost: a group's is its ROWS rows at a time, and
+// two more for its keys.  (Groups in turn: the waves with most of the longest work took half as long again as all on average.)
+struct WeighGroup { int b, first; WeighSequence v; };
+template <int N, int ROWS>
+struct WeighGroups {
+    typedef unsigned long long Cost;
+    int block;                          // of 64 sequences, one a lane:
+    int groups, sinks, skip, cost;      // groups, those of sinks, what is left out behind these, cost of each
+    Cost before;                        // of all groups in front of the sequence's
+    Cost base;                          // of the sequences behind the block
+    Cost at, end;                       // the next group's, and where this part ends
+    int b, nth;
+
+    __device__ __forceinline__ void look(const WeighArgs &a, int first) {
+        const int lane = threadIdx.x & 63;
+        block = first, groups = sinks = skip = cost = 0;
+        if (first + lane < a.at.batch) {
+            const WeighSequence v = weigh_sequence<false>(a, first + lane);
+            if (v.count > 0) {
+                const WeighView w = weigh_view(a, v.first_position, v.first_position + v.count - 1, v.end);
+                groups = (w.tiles + N - 1) / N, sinks = w.sink_tiles / N, skip = w.first_tile / N - sinks;
+                long long rows = (long long)v.count * a.group;
+                if (a.window) rows = min(rows, ((long long)a.window + 16 * N) * a.group);
+                cost = (int)((rows + ROWS - 1) / ROWS) + 2;
+            }
+        }
+        const Cost mine = (Cost)groups * (Cost)cost;
+        Cost upto = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off *= 2) {
+            const Cost other = __shfl_up(upto, off, 64);
+            if (lane >= off) upto += other;
+        }
+        before = base + upto - mine;
+        base += of_lane(upto, 63);
+    }
+    static __device__ __forceinline__ Cost of_lane(Cost x, int lane) {
+        return (Cost)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+    }
+    // part `part` of `parts`
+    __device__ __forceinline__ void cut(const WeighArgs &a, int part, int parts) {
+        base = 0;
+        for (int first = 0; first < a.at.batch; first += 64) look(a, first);
+        const Cost each = base / (uint32_t)parts, rest = base - each * (uint32_t)parts;
+        at = each * (uint32_t)part + min((Cost)part, rest), end = at + each + ((Cost)part < rest ? 1 : 0);
+        if (a.at.batch > 64) base = 0, look(a, 0);
+        b = -1, nth = 0;
+        if (at >= end) return;
+        // the first group that begins at or behind `at`
+        while (true) {
+            const unsigned long long in = __ballot(at < before + (Cost)groups * (Cost)cost);
+            if (in) {
+                const int lane = __builtin_ctzll(in);
+                const Cost first = of_lane(before, lane);
+                const uint32_t price = (uint32_t)__builtin_amdgcn_readlane(cost, lane);
+                b = block + lane, nth = at > first ? (int)((at - first + price - 1) / price) : 0;
+                at = first + (Cost)nth * price;
+                return;
+            }
+            look(a, block + 64);            // (at is in front of all groups' end)
+        }
+    }
+    __device__ __forceinline__ bool next(const WeighArgs &a, WeighGroup &g) {
+        if (b < 0 || at >= end) return false;
+        while (nth >= __builtin_amdgcn_readlane(groups, b - block)) {
+            nth = 0, ++b;
+            if (b >= a.at.batch) return false;
+            if (b - block >= 64) look(a, block + 64);
+        }
+        const int lane = b - block;
+        g.b = b, g.v = weigh_sequence<true>(a, b);
+        g.first = (nth + (nth < __builtin_amdgcn_readlane(sinks, lane) ? 0 : __builtin_amdgcn_readlane(skip, lane))) * 16 * N;
+        ++nth, at += (uint32_t)__builtin_amdgcn_readlane(cost, lane);
+        return true;
+    }
+};
+
 // Tokens and the rows that see them, sixteen at a time: a wave keeps 16 N tokens' keys and goes through all rows, or (SHARED) the waves of
-// a workgroup have the same tokens and take rows in turn.
+// a workgroup have the same tokens and take rows in turn.  Then the next tokens, whose keys and first rows are on their way by then.
 template <bool BF16, int STEPS, bool SHARED>
-__global__ __launch_bounds__(kWeighThreads, BF16 && STEPS < 8 ? 3 : 2) void weigh_tokens_kernel(const WeighArgs a) {
+__global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void weigh_tokens_kernel(const WeighArgs a) {
     constexpr int N = STEPS == 8 ? 2 : 4;           // tiles of sixteen tokens of a wave
-    __shared__ float s_sum[SHARED ? kWeighWaves : 1][16 * N];
+    __shared__ float s_sum[2][SHARED ? kWeighWaves : 1][16 * N];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
-    const int head = blockIdx.y, b = blockIdx.z;
-    const WeighSequence v = weigh_sequence<true>(a, b);
-    const int rows = v.count * a.group;
-    const int first = (SHARED ? (int)blockIdx.x : (int)blockIdx.x * kWeighWaves + wave) * 16 * N;
-    if (first >= v.end) return;
-    // rows that see any of the tokens: those at or behind the first, and with a window not too far behind the last
-    const long long from = max(0LL, ((long long)first - v.first_position) * a.group);
-    long long to = rows;
-    if (a.window && first >= a.sinks) to = min(to, ((long long)first + 16 * N - 1 + a.window - v.first_position) * a.group);
-    if (from >= to) return;
+    const int head = blockIdx.x;
     constexpr int kStep = SHARED ? 16 * kWeighWaves : 16;
-    int first_row = ((int)from & ~15) + (SHARED ? 16 * wave : 0);
+    constexpr bool kAhead = BF16 || STEPS < 8;         // (or registers are too few)
+    int buffer = 0;
+    WeighGroups<N, kStep> groups;
+    if (SHARED) groups.cut(a, (int)blockIdx.y, (int)gridDim.y);
+    else groups.cut(a, (int)blockIdx.y * kWeighWaves + wave, (int)gridDim.y * kWeighWaves);
+    WeighGroup g;
+    if (!groups.next(a, g)) return;
     WeighKeys<STEPS, N> keys;
-    keys.fetch(a, b, head, first >> 4, v.end);
     WeighRows<BF16, STEPS> q;
     float2 next[4];
-    const float2 *statistics = a.statistics + row_entry(a, v, head, 0);
-    const auto fetch_rows = [&](int at) {
+    const auto fetch_rows = [&](const WeighSequence &v, int at) {
         q.fetch(a, v, head, at);
+        const float2 *statistics = a.statistics + row_entry(a, v, head, 0);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int row = at + 4 * quarter + i;
-            next[i] = row < rows ? statistics[(uint32_t)row] : make_float2(INFINITY, 0.0f);
+            next[i] = row < v.count * a.group ? statistics[(uint32_t)row] : make_float2(INFINITY, 0.0f);
         }
     };
-    if (first_row < (int)to) fetch_rows(first_row);
-    keys.arrange(a.factor);
-    bf16x8 numbers[BF16 ? N : 1][STEPS];            // (fp32 queries take the registers: expanded again for every sixteen rows)
-    bool all_there = first + 16 * N <= v.end;
-#pragma unroll
-    for (int n = 0; n < N; ++n) {
-        if constexpr (BF16) {
-#pragma unroll
-            for (int j = 0; j < STEPS; ++j) numbers[n][j] = fp4_to_bf16(keys.word[n][j]);
-        }
-        all_there = all_there && keys.there[n];
-        keys.there[n] = keys.there[n] && first + 16 * n + (lane & 15) < v.end;
-    }
-    float sum[N];
-#pragma unroll
-    for (int n = 0; n < N; ++n) sum[n] = 0.0f;
-    for (; first_row < (int)to; first_row += kStep) {
-        q.arrange();
-        float m[4], by[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m[i] = next[i].x, by[i] = next[i].y;
-        if (first_row + kStep < (int)to) fetch_rows(first_row + kStep);
-        const bool all = all_there && first + 16 * N - 1 <= v.position(a, first_row) &&
-                         (!a.window || v.position(a, min(rows, first_row + 16) - 1) - first < a.window || first + 16 * N <= a.sinks);
-        fp4_f32x4 s[N];
+    // rows that see any of the tokens: those at or behind the first, and with a window not too far behind the last
+    int first_row, to;
+    const auto range = [&](const WeighGroup &g) {
+        const long long from = max(0LL, ((long long)g.first - g.v.first_position) * a.group);
+        long long end = (long long)g.v.count * a.group;
+        if (a.window && g.first >= a.sinks) end = min(end, ((long long)g.first + 16 * N - 1 + a.window - g.v.first_position) * a.group);
+        first_row = from < end ? ((int)from & ~15) + (SHARED ? 16 * wave : 0) : 0, to = from < end ? (int)end : 0;
+    };
+    keys.fetch(a, g.b, head, g.first >> 4, g.v.end);
+    range(g);
+    if (first_row < to) fetch_rows(g.v, first_row);
+    while (true) {
+        const int rows = g.v.count * a.group, first = g.first;
+        keys.arrange(a.factor);
+        bf16x8 numbers[BF16 ? N : 1][STEPS];            // (fp32 queries take the registers: expanded again for every sixteen rows)
+        bool all_there = first + 16 * N <= g.v.end, there[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            if constexpr (!BF16) {
+            if constexpr (BF16) {
 #pragma unroll
-                for (int j = 0; j < STEPS; ++j) {
-                    uint32_t word = keys.word[n][j];
-                    asm volatile("" : "+v"(word));          // (not in front of the loop)
-                    numbers[0][j] = fp4_to_bf16(word);
-                }
+                for (int j = 0; j < STEPS; ++j) numbers[n][j] = fp4_to_bf16(keys.word[n][j]);
             }
-            s[n] = weigh_scores<BF16, STEPS>(q, numbers[BF16 ? n : 0], keys.scale[n]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[n][i] -= m[i];        // (m is one of these, bit for bit: a token seen alone has weight 1)
+            all_there = all_there && keys.there[n], there[n] = keys.there[n];
         }
-        if (all) {
+        const int mine = N == 4 ? quarter : quarter >> 1, t = 16 * mine + (lane & 15);
+        bool writes = first + t < g.v.end && (N == 4 || (quarter & 1) == 0);
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n) writes = writes && (mine != n || there[n]);
+        float *total = a.totals + g.b * a.total_sequence + head * a.total_head + first + t;
+        const float held = writes && (!SHARED || wave == 0) ? *total : 0.0f;
+        WeighGroup after;
+        const bool more = groups.next(a, after);
+        if (kAhead && more) keys.fetch(a, after.b, head, after.first >> 4, after.v.end);
+        float sum[N];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[n][i]), by[i], sum[n]);
-        } else {
+        for (int n = 0; n < N; ++n) sum[n] = 0.0f;
+        const int end = to;
+        int row_at = first_row;
+        if (more) range(after);
+        writes = writes && end > 0;
+        if (kAhead && row_at >= end && more && first_row < to) fetch_rows(after.v, first_row);
+        for (; row_at < end; row_at += kStep) {
+            q.arrange();
+            float m[4], by[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = first_row + 4 * quarter + i, position = row < rows ? v.position(a, row) : -1;
+            for (int i = 0; i < 4; ++i) m[i] = next[i].x, by[i] = next[i].y;
+            if (row_at + kStep < end) fetch_rows(g.v, row_at + kStep);
+            else if (kAhead && more && first_row < to) fetch_rows(after.v, first_row);
+            const bool all = all_there && first + 16 * N - 1 <= g.v.position(a, row_at) &&
+                             (!a.window || g.v.position(a, min(rows, row_at + 16) - 1) - first < a.window || first + 16 * N <= a.sinks);
+            fp4_f32x4 s[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                if constexpr (!BF16) {
+#pragma unroll
+                    for (int j = 0; j < STEPS; ++j) {
+                        uint32_t word = keys.word[n][j];
+                        asm volatile("" : "+v"(word));          // (not in front of the loop)
+                        numbers[0][j] = fp4_to_bf16(word);
+                    }
+                }
+                s[n] = weigh_scores<BF16, STEPS>(q, numbers[BF16 ? n : 0], keys.scale[n]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] -= m[i];        // (m is one of these, bit for bit: a token seen alone has weight 1)
+            }
+            if (all) {
 #pragma unroll
                 for (int n = 0; n < N; ++n)
-                    sum[n] += keys.there[n] && row_sees(a, position, first + 16 * n + (lane & 15)) ? __builtin_amdgcn_exp2f(s[n][i]) * by[i] : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[n][i]), by[i], sum[n]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = row_at + 4 * quarter + i, position = row < rows ? g.v.position(a, row) : -1;
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        const int at = first + 16 * n + (lane & 15);
+                        sum[n] += there[n] && at < g.v.end && row_sees(a, position, at) ? __builtin_amdgcn_exp2f(s[n][i]) * by[i] : 0.0f;
+                    }
+                }
             }
         }
-    }
-    int mine;
-    bool writes;
-    const float weight = sum_of_rows<N>(sum, mine, writes);
-    bool is = keys.there[0];
-#pragma unroll
-    for (int n = 1; n < N; ++n) is = mine == n ? keys.there[n] : is;
-    float *total = a.totals + b * a.total_sequence + head * a.total_head + first;
-    const int t = 16 * mine + (lane & 15);
-    if constexpr (SHARED) {
-        if (writes) s_sum[wave][t] = weight;
-        __syncthreads();
-        if (wave == 0 && writes && is) total[t] += (s_sum[0][t] + s_sum[1][t]) + (s_sum[2][t] + s_sum[3][t]);
-    } else {
-        if (writes && is) total[t] += weight;
+        const float weight = sum_of_rows<N>(sum);
+        if constexpr (SHARED) {
+            s_sum[buffer][wave][t] = weight;
+            __syncthreads();
+            if (wave == 0 && writes) *total = held + ((s_sum[buffer][0][t] + s_sum[buffer][1][t]) + (s_sum[buffer][2][t] + s_sum[buffer][3][t]));
+            buffer ^= 1;
+        } else {
+            if (writes) *total = held + weight;
+        }
+        if (!more) break;
+        g = after;
+        if (!kAhead) {
+            keys.fetch(a, g.b, head, g.first >> 4, g.v.end);
+            if (first_row < to) fetch_rows(g.v, first_row);
+        }
     }
 }
 
@@ -725,11 +822,12 @@ void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
     launch_rows<BF16, STEPS, T>(a, work, stream);
     const long long entries = (long long)a.at.tokens * a.group * a.shape.kv_heads;
     if (a.parts > 1) hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)((16 * entries + kWeighThreads - 1) / kWeighThreads)), dim3(kWeighThreads), 0, stream, a, entries);
-    const long long blocks = (covered + 16 * N - 1) / (16 * N), apart = (blocks + kWeighWaves - 1) / kWeighWaves;
-    if (apart * a.shape.kv_heads * a.at.batch >= 6LL * compute_units())
-        hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, false>), dim3((unsigned)apart, a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
-    else
-        hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, true>), dim3((unsigned)blocks, a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
+    // a round of workgroups, or fewer where there are not as many tokens; of waves with tokens of their own if every one has some then
+    const long long round = (BF16 && STEPS == 2 ? 3 : 2) * compute_units(), blocks = (covered + 16 * N - 1) / (16 * N) * a.at.batch;
+    const long long heads = a.shape.kv_heads, each = round / heads < 1 ? 1 : round / heads;
+    const dim3 grid((unsigned)heads, (unsigned)min(min(blocks, each), 65535LL));
+    if (blocks >= kWeighWaves * each) hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, false>), grid, dim3(kWeighThreads), 0, stream, a);
+    else hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, true>), grid, dim3(kWeighThreads), 0, stream, a);
 }
 
 template <bool BF16>
