@@ -72,17 +72,19 @@ __device__ __forceinline__ bool row_sees(const WeighArgs &a, int position, int t
     return token <= position && (!a.window || position - token < a.window || token < a.sinks);
 }
 
-// Sixteen rows as a matrix operand: STEPS of 32 elements.
-template <bool BF16, int STEPS>
+// Sixteen rows as a matrix operand: STEPS of 32 elements.  SIDE: loaded by four lanes side by side a row, which touches a row's line once instead of four
+// times, and exchanged.
+template <bool BF16, int STEPS, bool SIDE>
 struct WeighRows {
     bf16x8 x[STEPS][Eight<BF16>::kPieces];
 
     Eight<BF16> raw[STEPS];
 
     __device__ __forceinline__ void fetch(const WeighArgs &a, const WeighSequence &v, int head, int first_row) {
-        const int lane = threadIdx.x & 63, row = min(first_row + (lane & 15), v.count * a.group - 1), i = (int)fastdiv((uint32_t)row, a.by_group);
+        const int lane = threadIdx.x & 63, quarter = SIDE ? lane & 3 : lane >> 4;
+        const int row = min(first_row + (SIDE ? lane >> 2 : lane & 15), v.count * a.group - 1), i = (int)fastdiv((uint32_t)row, a.by_group);
         const int steps = a.shape.row_bytes >> 4;
-        const uint8_t *p = (const uint8_t *)a.q + ((v.start + i) * a.q_token + (head * a.group + row - i * a.group) * a.q_head + 8 * (lane >> 4)) * (BF16 ? 2 : 4);
+        const uint8_t *p = (const uint8_t *)a.q + ((v.start + i) * a.q_token + (head * a.group + row - i * a.group) * a.q_head + 8 * quarter) * (BF16 ? 2 : 4);
         if (a.shape.head_dim == 32 * STEPS) {
 #pragma unroll
             for (int j = 0; j < STEPS; ++j) raw[j].load(p, 32 * j);
@@ -90,14 +92,17 @@ struct WeighRows {
 #pragma unroll
             for (int j = 0; j < STEPS; ++j) {
                 raw[j].zero();
-                if (j < steps) raw[j].load(p, 32 * j, a.shape.head_dim - 8 * (lane >> 4));
+                if (j < steps) raw[j].load(p, 32 * j, a.shape.head_dim - 8 * quarter);
             }
         }
     }
     // (rows behind the last are the last one again: what comes of them is not used)
     __device__ __forceinline__ void arrange() {
 #pragma unroll
-        for (int j = 0; j < STEPS; ++j) raw[j].pieces(x[j]);
+        for (int j = 0; j < STEPS; ++j) {
+            if (SIDE) raw[j].exchange();
+            raw[j].pieces(x[j]);
+        }
     }
 };
 
@@ -207,8 +212,8 @@ struct WeighKeys {
 };
 
 // Scores of sixteen rows (4 (lane / 16) + i) and a token (lane % 16), times log2 e: `numbers` are its keys' numbers, `scale` has the factor already.
-template <bool BF16, int STEPS>
-__device__ __forceinline__ fp4_f32x4 weigh_scores(const WeighRows<BF16, STEPS> &rows, const bf16x8 *numbers, const float *scale) {
+template <bool BF16, int STEPS, bool SIDE>
+__device__ __forceinline__ fp4_f32x4 weigh_scores(const WeighRows<BF16, STEPS, SIDE> &rows, const bf16x8 *numbers, const float *scale) {
     constexpr int P = Eight<BF16>::kPieces;
     fp4_f32x4 sum;
 #pragma unroll
@@ -217,6 +222,17 @@ __device__ __forceinline__ fp4_f32x4 weigh_scores(const WeighRows<BF16, STEPS> &
 #pragma unroll
         for (int i = 0; i < 4; ++i) sum[i] = g ? __builtin_fmaf(scale[g], part[i], sum[i]) : scale[g] * part[i];
     }
+    return sum;
+}
+
+// The same from the segments' products of N tiles, for the nth.
+template <int STEPS, int N>
+__device__ __forceinline__ fp4_f32x4 scale_scores(const fp4_f32x4 (&part)[STEPS / 2][N], int n, const float *scale) {
+    fp4_f32x4 sum;
+#pragma unroll
+    for (int g = 0; g < STEPS / 2; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] = g ? __builtin_fmaf(scale[g], part[g][n][i], sum[i]) : scale[g] * part[g][n][i];
     return sum;
 }
 
@@ -399,7 +415,7 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
         return;
     }
     const auto tile_at = [&](int index) { return index < view.sink_tiles ? index : view.first_tile + index - view.sink_tiles; };
-    WeighRows<BF16, STEPS> q[T];
+    WeighRows<BF16, STEPS, false> q[T];
 #pragma unroll
     for (int r = 0; r < T; ++r) q[r].fetch(a, v, head, first_row + 16 * r);
     WeighKeys<STEPS, N> keys;
@@ -439,7 +455,7 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
 #pragma unroll
             for (int j = 0; j < STEPS; ++j) numbers[j] = fp4_to_bf16(keys.word[n][j]);
 #pragma unroll
-            for (int r = 0; r < T; ++r) s[r][n] = weigh_scores<BF16, STEPS>(q[r], numbers, keys.scale[n]);
+            for (int r = 0; r < T; ++r) s[r][n] = weigh_scores(q[r], numbers, keys.scale[n]);
         }
         if (!all) {
 #pragma unroll
@@ -668,16 +684,13 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
     WeighGroup g;
     if (!groups.next(a, g)) return;
     WeighKeys<STEPS, N> keys;
-    WeighRows<BF16, STEPS> q;
-    float2 next[4];
+    WeighRows<BF16, STEPS, BF16> q;            // (fp32: 17 rows over 32000 tokens 77 us, side by side 79)
+    qt_u32x4 next[2];
     const auto fetch_rows = [&](const WeighSequence &v, int at) {
         q.fetch(a, v, head, at);
-        const float2 *statistics = a.statistics + row_entry(a, v, head, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = at + 4 * quarter + i;
-            next[i] = row < v.count * a.group ? statistics[(uint32_t)row] : make_float2(INFINITY, 0.0f);
-        }
+        // (behind the last row: what lies there, or room that is kept free)
+        const Unaligned16of4 *p = (const Unaligned16of4 *)(a.statistics + row_entry(a, v, head, at + 4 * quarter));
+        next[0] = p[0].v, next[1] = p[1].v;
     };
     // rows that see any of the tokens: those at or behind the first, and with a window not too far behind the last
     int first_row, to;
@@ -724,26 +737,42 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
             q.arrange();
             float m[4], by[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) m[i] = next[i].x, by[i] = next[i].y;
+            for (int i = 0; i < 4; ++i) m[i] = __uint_as_float(next[i / 2][2 * (i % 2)]), by[i] = __uint_as_float(next[i / 2][2 * (i % 2) + 1]);
+            if (row_at + 16 > rows) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (row_at + 4 * quarter + i >= rows) m[i] = INFINITY, by[i] = 0.0f;
+            }
             if (row_at + kStep < end) fetch_rows(g.v, row_at + kStep);
             else if (kAhead && more && first_row < to) fetch_rows(after.v, first_row);
             const bool all = all_there && first + 16 * N - 1 <= g.v.position(a, row_at) &&
                              (!a.window || g.v.position(a, min(rows, row_at + 16) - 1) - first < a.window || first + 16 * N <= a.sinks);
             fp4_f32x4 s[N];
+            if constexpr (BF16) {
+                // (all tiles' products first)
+                fp4_f32x4 part[STEPS / 2][N];
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                if constexpr (!BF16) {
+                for (int j = 0; j < STEPS; ++j)
+#pragma unroll
+                    for (int n = 0; n < N; ++n) part[j / 2][n] = multiply_pieces<1>(q.x[j], numbers[n][j], j & 1 ? part[j / 2][n] : (fp4_f32x4){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int n = 0; n < N; ++n) s[n] = scale_scores<STEPS>(part, n, keys.scale[n]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < N; ++n) {
 #pragma unroll
                     for (int j = 0; j < STEPS; ++j) {
                         uint32_t word = keys.word[n][j];
                         asm volatile("" : "+v"(word));          // (not in front of the loop)
                         numbers[0][j] = fp4_to_bf16(word);
                     }
+                    s[n] = weigh_scores(q, numbers[0], keys.scale[n]);
                 }
-                s[n] = weigh_scores<BF16, STEPS>(q, numbers[BF16 ? n : 0], keys.scale[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) s[n][i] -= m[i];        // (m is one of these, bit for bit: a token seen alone has weight 1)
-            }
             if (all) {
 #pragma unroll
                 for (int n = 0; n < N; ++n)
@@ -846,7 +875,7 @@ WeighSizes weigh_sizes(const CacheShape &shape, const CachePlaces &at, int heads
     s.few = !at.starts && heads / shape.kv_heads <= 16;         // a tile of rows for every sequence
     // (the tiles of bf16 queries, of which there are fewest, and without a window)
     s.parts = weigh_parts(weigh_row_tiles(at, heads / shape.kv_heads, 32) * shape.kv_heads, (long long)at.table_pages << shape.page_shift);
-    s.partial = ((long long)at.tokens * heads * (s.parts + 1) * (long long)sizeof(float2) + 255) & ~255LL;
+    s.partial = (((long long)at.tokens * heads * (s.parts + 1) + 16) * (long long)sizeof(float2) + 255) & ~255LL;      // (and room behind the statistics)
     s.stride = (((long long)at.table_pages << shape.page_shift) + 63) & ~63LL;
     s.scores = s.few && s.stride <= kMostScores / 4 / heads / at.batch ? s.stride * heads * at.batch * 4 : 0;
     s.all = s.partial + s.scores;
