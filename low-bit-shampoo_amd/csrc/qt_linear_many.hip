@@ -28,9 +28,9 @@ __device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &colu
 // numbers of the next block are on their way in registers.  They are exact in bf16, and scales multiply the sums of 64 inputs: four vector
 // operations beside every two matrix ones, and as many to expand the numbers, are what a wave does beside them.
 //
-// Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 535 us, 1010 TFLOP/s, where the
+// Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 506 us, 1070 TFLOP/s, where the
 // library's product of bf16 matrices takes 519 us; 1024 tokens through 4096 x 4096 43 us, 800 TFLOP/s; 2048 tokens through 11008 x 4096 in fp32 (three
-// matrix operations for each) 514 us, 359 TFLOP/s.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers).
+// matrix operations for each) 508 us, 364 TFLOP/s.  Four lanes side by side load a token's line: 547 us where sixteen tokens' lines were touched by each.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers).
 template <bool BF16, int MT, int N>
 __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift, const bool aligned) {
     constexpr int P = Eight<BF16>::kPieces, GROUPS = 2, J = 4 / GROUPS, kBuffers = BF16 ? 2 : 1;
@@ -188,7 +188,7 @@ void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
 long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.tokens + 63) / 64) * ((a.outputs + 127) / 128); }
 
 // Large tiles use what they read more often, but leave units idle until there are four workgroups for each: 4096 inputs in bf16, 128 x 256 against
-// 64 x 128, 1024 tokens and 4096 outputs 101 and 43 us, 2048 and 11008 218 and 219, 6000 and 11008 545 and 634; in fp32 64 x 192 against 64 x 128,
+// 64 x 128, as loads of tokens were then, 1024 tokens and 4096 outputs 101 and 43 us, 2048 and 11008 218 and 219, 6000 and 11008 545 and 634; in fp32 64 x 192 against 64 x 128,
 // 256 and 4096 99 and 80, 2048 and 11008 514 and 567.
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
     const long long large = bf16 ? (long long)((a.tokens + 127) / 128) * ((a.outputs + 255) / 256) : (long long)((a.tokens + 63) / 64) * ((a.outputs + 191) / 192);

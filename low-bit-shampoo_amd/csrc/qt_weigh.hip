@@ -3,7 +3,7 @@
 // For every new token i and query head g of a cache's head h, w(i, g, t) = 2^(s(t) - m) / l over the tokens t that i sees, s = scale log2(e) q k, m the
 // largest and l the sum of 2^(s - m); totals[b][h][t] += sum over i and g of w.  As t is summed over first and i afterwards, the scores are
 // worked out twice: once a row (i, g) at a time for m and l, once a token at a time for the sums, instead of being kept (a score is 4
-// bytes, as much as a key's 8 elements).  Every sum has one order: results do not change from call to call.
+// bytes, as much as a key's 8 elements); but where each sequence has one token they are, if there is room.  Every sum has one order: results do not change from call to call.
 //
 // Scores come from the matrix cores with all bits: keys' numbers are exact in bf16, fp32 queries go through in three pieces (qt_fp4.h).
 #include "qt_cache.h"
@@ -378,7 +378,13 @@ __device__ __forceinline__ bool find_work(const WeighArgs &a, int index, WeighWo
 }
 
 // 16 T rows and a part of the tokens that they see: m and l of each, or (WEIGHTS, where a sequence has no more rows than these) the
-// weights themselves, added to the totals.
+// weights themselves, added to the totals.  A wave goes through the tokens of its part 16 N at a time, the next ones' keys on their way.
+//
+// A step of 32 sequences of 100 to 8000 tokens, 8 heads of 128, groups of 4, bf16: 26 us for 85 MB of keys and scores written, 3.3 TB/s; 4 us are the
+// launch and the work found, 2.5 to 5 the first keys (length, page, keys: three loads that wait for each other), and a part has so few tokens that this is a third of its
+// time.  The last 1 to 27 tokens of four prompts of up to 32768, two tiles of rows at a time: 29 us, bound by the vector instructions (exponentials, scales, numbers
+// expanded; 45 % of all cycles) and the loads before them.  Tried: scores of a step transposed, so that no lane works on rows that are not there (31 us against 28: more
+// registers), all tiles' products in front (31 against 29).
 template <bool BF16, int STEPS, int T, bool WEIGHTS>
 __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 : 3) void weigh_rows_kernel(const WeighArgs a) {
     static_assert(T == 1 || !WEIGHTS, "weights of sixteen rows");
@@ -536,7 +542,8 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
     }
 }
 
-// Weights of the only token of a sequence from its scores: four tokens a thread.  Bound by reading them.
+// Weights of the only token of a sequence from its scores: four tokens a thread.  Bound by latency, length to scores: 9.3 us for the step above, whose 25 MB
+// are 5 us at a copy's rate; 10.5 with the statistics in front of the loads.
 __global__ __launch_bounds__(kWeighThreads) void weigh_scores_kernel(const WeighArgs a) {
     __shared__ float2 s_row[16];
     const int head = blockIdx.y, b = blockIdx.z, first = (int)blockIdx.x * 4 * kWeighThreads;
@@ -581,6 +588,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_scores_kernel(const Weigh
 }
 
 // (m, 1 / l) of every row from its parts, sixteen lanes a row: of all rows that a sequence may have (what is behind the last sequence is not used).
+// A launch and two loads: 4.7 us for 1440 rows in 21 parts.
 __global__ __launch_bounds__(kWeighThreads) void weigh_join_kernel(const WeighArgs a, long long entries) {
     const long long entry = ((long long)blockIdx.x * kWeighThreads + threadIdx.x) >> 4;
     float2 part = make_float2(-INFINITY, 0.0f);
@@ -668,7 +676,12 @@ struct WeighGroups {
 };
 
 // Tokens and the rows that see them, sixteen at a time: a wave keeps 16 N tokens' keys and goes through all rows, or (SHARED) the waves of
-// a workgroup have the same tokens and take rows in turn.  Then the next tokens, whose keys and first rows are on their way by then.
+// a workgroup have the same tokens and take rows in turn.  Then the next tokens, whose keys and first rows are on their way by then: one round of waves has
+// all tokens, a round for each four tokens' tiles took 179 us where this takes 118 (the last 100 tokens of six prompts of up to 9000, 8 heads of 128, groups of 4, bf16).
+//
+// Bound by the vector instructions, an exponential, a multiplication, two fused ones and a difference for each score and lane (4 us of 33 for the four prompts above are
+// matrix instructions), and with two waves a SIMD by what they wait for: rows' 16 bytes a lane touch sixteen lines an instruction where four lanes side by side load a
+// row, else 64 (36 us, 129 for the six prompts), and products of all tiles go first (35, 122).  Tried: 32 tokens a wave and four waves a SIMD, 57 us.
 template <bool BF16, int STEPS, bool SHARED>
 __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void weigh_tokens_kernel(const WeighArgs a) {
     constexpr int N = STEPS == 8 ? 2 : 4;           // tiles of sixteen tokens of a wave

@@ -1,7 +1,11 @@
 """Projections, rotary positions and eviction in calls at the edge of what is allowed: the most tokens, graphs that share memory, captured gradients, results in places that
 are read."""
+import math
+
 import pytest
 import torch
+
+from oracle import evict_ref as E
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +141,26 @@ def test_many_prompts_weighed_in_parts():
     total = all_of_them.double().sum(-1).cpu()
     for b in range(3):
         assert float((total[b] - news[b] * 4).abs().max()) <= 2.0 ** -15 * news[b] * 4
+
+
+@pytest.mark.parametrize("batch,heads,kv_heads,dim,window,sinks,single", [(150, 4, 2, 64, None, 0, False), (150, 8, 2, 128, 40, 5, False), (200, 20, 1, 64, None, 0, True),
+                                                                          (130, 4, 4, 96, None, 0, True), (65, 3, 1, 256, 30, 0, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_batches_of_more_sequences_than_a_wave_has_lanes(batch, heads, kv_heads, dim, window, sinks, single, dtype):
+    """Work is found by lanes that have a sequence each, sixty-four at a time: batches of several times that, with empty ones among them."""
+    lengths = [(37 * b) % 130 + (b % 7 == 0) * 300 if b % 11 else 0 for b in range(batch)]
+    news = [1] * batch if single else [min(n, (5 * b) % 23) for b, n in enumerate(lengths)]
+    cache, table, counts = made(lengths, kv_heads, dim, seed=30)
+    q = random((sum(news), heads, dim), 33, dtype)
+    starts = None if single else torch.tensor([sum(news[:b]) for b in range(batch + 1)], dtype=torch.int32, device="cuda")
+    totals = cache.weigh(cache.totals(table), q, table, counts, starts, window=window, sinks=sinks)
+    keys, _ = cache.read(table, counts, torch.tensor([sum(lengths[:b]) for b in range(batch + 1)], dtype=torch.int32, device="cuda"), tokens=sum(lengths))
+    at = first = 0
+    for b, (n, new) in enumerate(zip(lengths, news)):
+        if n:
+            want, spread = E.weigh(q[at:at + new].cpu(), range(n - new, n), keys[first:first + n].double().cpu(), 1 / math.sqrt(dim), window, sinks)
+            off = (totals[b, :, :n].double().cpu() - want).abs()
+            limit = E.bound(dim, new * heads // kv_heads, want, spread) + 2.0 ** -23 * want
+            assert bool((off <= limit).all()), f"sequence {b}: off by {float((off / limit).max()):.3g} of the bound"
+        assert not totals[b, :, n:].any()
+        at, first = at + new, first + n
