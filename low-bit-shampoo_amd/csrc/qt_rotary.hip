@@ -210,7 +210,9 @@ struct TurnWrite {
 
 // Bound by memory, with the places' look-up, cosines and sines in front of the first loads: the more heads a workgroup goes through, the less of
 // that, and tokens side by side in a head of the cache are written together.  9 prompts of up to 3500 tokens, 32 query heads, 8 of 128 in the cache, bf16:
-// 103 us, of which the queries alone are 62 and keys and values 38; turned, then written by two calls 87.
+// 102 us for 397 MB, 3.9 TB/s, of which some 20 are cosines and sines of the keys' and of the queries' workgroups in 64 bits; turned, then written by two calls 114
+// (1 token of 32 sequences 5.8 and 9.2).  Tried: the first heads' loads in front of the places (registers: 125 us), keys' and queries' workgroups in turn (106),
+// more waves (105 to 194: registers), 16 tokens of the keys (105).
 template <bool BF16, bool LARGE>
 __global__ __launch_bounds__(kTurnThreads, 4) void turn_write_kernel(const TurnWrite a) {
     constexpr int kEach = kLaneElements<BF16>, kAtOnce = LARGE ? 4 : 1, kHeads = LARGE ? 2 : 1;
@@ -403,10 +405,10 @@ extern "C" void qtensor_hip_cache_write_turned(const qtensor_cache *cache, const
     a.segment_lanes = cache_segment_lanes(a.shape, bf16);
     const int lanes = a.segment_lanes * a.shape.segments;
     // Few tokens: as many workgroups as there are.  Many, from about a thousand: 1050 tokens of 32 heads of 128 in bf16 13.8 us against 19.1, 529 11.8
-    // against 11.6, 18378 103 against 275.
+    // against 11.6, 18378 102 against 275.
     const long long elements = (long long)a.at.tokens * heads * a.shape.head_dim;
     const bool large = elements >= 1LL << 22;
-    const int most = kTurnThreads / lanes, keys_tokens = large ? 16 : 4, few = most < 4 ? most : 4;
+    const int most = kTurnThreads / lanes, keys_tokens = large ? 8 : 4, few = most < 4 ? most : 4;
     if (!turn_args(what, rotary, a.shape.head_dim, bf16, lanes, most < keys_tokens ? most : keys_tokens, a.keys) ||
         !turn_args(what, rotary, a.shape.head_dim, bf16, lanes, few, a.queries))
         return;
