@@ -115,15 +115,18 @@ struct LaneTurn {
     }
 };
 
-// Cosines and sines of all pairs of the workgroup's tokens; position(n, there): of its nth token, if there is one.
-template <typename Position>
+// Cosines and sines of all pairs of the workgroup's tokens; position(n, there): of its nth token, if there is one.  AHEAD: frequencies are asked for in front of
+// positions (8 x 2048 tokens turned and turned back 136.5 us, else 143.5; where places have to be found first it costs registers, prompts turned and written 129 us, else 117).
+template <bool AHEAD, typename Position>
 __device__ __forceinline__ void work_out_turns(const TurnArgs &a, float2 *turn, Position position) {
     for (int i = threadIdx.x; i < a.block_tokens * a.pairs; i += kTurnThreads) {
         const int nth = (int)fastdiv((uint32_t)i, a.by_pairs);
-        double at;
+        double at, speed;
+        if (AHEAD) speed = a.frequencies[i - nth * a.pairs];
         if (!position(nth, at)) continue;
+        if (!AHEAD) speed = a.frequencies[i - nth * a.pairs];
         double s, c;
-        sincos(at * a.frequencies[i - nth * a.pairs], &s, &c);
+        sincos(at * speed, &s, &c);
         turn[i] = make_float2((float)(a.magnitude * c), (float)(a.sine * s));
     }
 }
@@ -154,13 +157,13 @@ struct TurnCall {
     long long first_block;              // of the launch
 };
 
-// 8 sequences of 2048 tokens, 40 heads of 128 in bf16: 72 us, 4.7 TB/s (a copy of the library's 4.9); a thread goes through four of
-// them (69 us, one 133, eight 67; 2048 tokens 10.6, 18.2 and 11.4).
+// 8 sequences of 2048 tokens, 40 heads of 128 in bf16: 68 us, 4.9 TB/s, a copy's rate; a thread goes through four of
+// them (69 us, one 133, eight 67; 2048 tokens 10.6, 18.2 and 11.4, as positions were read then).
 template <bool BF16>
 __global__ __launch_bounds__(kTurnThreads) void turn_kernel(const TurnCall a) {
     __shared__ float2 s_turn[kTurnPairs];
     const long long first = (a.first_block + blockIdx.x) * a.turn.block_tokens;
-    work_out_turns(a.turn, s_turn, [&](int nth, double &at) {
+    work_out_turns<true>(a.turn, s_turn, [&](int nth, double &at) {
         const long long n = first + nth;
         if (n >= a.vectors) return false;
         const long long b = n / a.tokens, i = b * a.position_batch + (n - b * a.tokens);
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(kTurnThreads, 4) void turn_write_kernel(const TurnW
         s_sequence[threadIdx.x] = b, s_place[threadIdx.x] = place;
     }
     __syncthreads();
-    work_out_turns(turn, s_turn, [&](int nth, double &at) {
+    work_out_turns<false>(turn, s_turn, [&](int nth, double &at) {
         const int place = s_place[nth];
         if (place < 0) return false;
         at = !a.positions ? (double)place : a.long_positions ? (double)((const long long *)a.positions)[first + nth] : (double)((const int *)a.positions)[first + nth];
