@@ -164,3 +164,26 @@ def test_batches_of_more_sequences_than_a_wave_has_lanes(batch, heads, kv_heads,
             assert bool((off <= limit).all()), f"sequence {b}: off by {float((off / limit).max()):.3g} of the bound"
         assert not totals[b, :, n:].any()
         at, first = at + new, first + n
+
+
+def test_more_tiles_of_rows_than_a_dimension_of_a_grid():
+    """A prompt whose rows are more than 2^15 tiles, with a window: weights of a query add up to 1, and the last tokens' are those of a call with the last queries."""
+    from qtensor.cache import QTensorCache
+    tokens, heads, window = 270000, 4, 32
+    cache = QTensorCache(-(-tokens // 4096), 1, 64, page_size=4096)
+    table = torch.arange(cache.pages, dtype=torch.int32, device="cuda").view(1, -1)
+    counts = torch.tensor([tokens], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(40)
+    q, k = (torch.randn(tokens, n, 64, generator=g, device="cuda").bfloat16() for n in (heads, 1))
+    starts = torch.tensor([0, tokens], dtype=torch.int32, device="cuda")
+    cache.write(k, k, table, counts, starts)
+    totals = cache.weigh(cache.totals(table), q, table, counts, starts, window=window)
+    last = cache.weigh(cache.totals(table), q[-1000:], table, counts, torch.tensor([0, 1000], dtype=torch.int32, device="cuda"), window=window)
+    # (as above: a weight is good to 2^-16, and a token has 32 x 4 of them; all of them in 64 bits)
+    some = slice(tokens - 900, tokens)
+    assert float((totals[0, 0, some] - last[0, 0, some]).abs().max()) <= 2.0 ** -16 * window * heads
+    per = totals[0, 0, :tokens].double()
+    assert abs(float(per.sum()) - tokens * heads) <= 2.0 ** -16 * tokens * heads
+    # any stretch of tokens has what its queries give it, less or more what a window reaches over both ends
+    for first in (0, 100000, 200000):
+        assert abs(float(per[first:first + 5000].sum()) - 5000 * heads) <= window * heads * 2
