@@ -200,8 +200,8 @@ void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
     else hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 1, T == 1>), grid, dim3(64 * WAVES), 0, stream, a);
 }
 
-// Many tokens as soon as the kernel for them has a workgroup for every unit: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 15.3 us here
-// and 30.5 there, 256 and 11008 (344) 46 and 39.
+// Many tokens as soon as the kernel for them has a workgroup for seven of eight units: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 15.1 us here
+// and 25.8 there, 384 and 4096 (192) 22.0 and 26.1, 128 and 14336 (224) 29.4 and 26.9, in fp32 70.6 and 57.4.
 // Else the smallest tile of a workgroup whose workgroups have a unit each: every one reads all of its tokens (from L2) and joins its waves, so
 // more of them than that cost more than they spread.  By tiles of outputs x tokens, before loads of tokens and joins were as they are: 16 tokens, 4096
 // outputs 1 x 1 6.7 us, 2 x 1 7.9, 4 x 1 10.1; 14336 outputs 18.3, 12.6, 10.5; 64 tokens, 4096 outputs 4 x 1 10.5, 4 x 2 15.4; as they are, 64 tokens, 11008
@@ -210,7 +210,7 @@ void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
 template <bool BF16>
 void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
     const long long tiles = (a.outputs + 15) / 16, rows = (a.tokens + 15) / 16, units = compute_units();
-    if (linear_many_workgroups(a) >= units) return launch_linear_many(a, BF16, groups, stream);
+    if (8 * linear_many_workgroups(a) >= 7 * units) return launch_linear_many(a, BF16, groups, stream);
     if (tiles * rows <= units) return launch_few<BF16, 1, 1, 8>(a, groups, stream);
     if ((tiles + 1) / 2 * rows <= units) return launch_few<BF16, 1, 2, 8>(a, groups, stream);
     if ((tiles + 3) / 4 * rows <= units) return launch_few<BF16, 1, 4, 8>(a, groups, stream);

@@ -30,13 +30,19 @@ __device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &colu
 //
 // Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 506 us, 1070 TFLOP/s, where the
 // library's product of bf16 matrices takes 519 us; 1024 tokens through 4096 x 4096 43 us, 800 TFLOP/s; 2048 tokens through 11008 x 4096 in fp32 (three
-// matrix operations for each) 508 us, 364 TFLOP/s.  Four lanes side by side load a token's line: 547 us where sixteen tokens' lines were touched by each.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers).
-template <bool BF16, int MT, int N>
-__global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift, const bool aligned) {
+// matrix operations for each) 508 us, 364 TFLOP/s.  Four lanes side by side load a token's line: 547 us where sixteen tokens' lines were touched by each.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers), the
+// matrix instructions at a higher priority, in groups with the vector ones, or one tile ahead of them (512 to 529 us beside 513: the pipes are busy all the time, at a clock that falls to
+// 2.0 GHz).
+//
+// SPLIT: two times four waves, which take the blocks of 128 inputs in turn and join their sums through LDS.
+template <bool BF16, int MT, int N, int SPLIT>
+__global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4 ? 3 : 2) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift, const bool aligned) {
     constexpr int P = Eight<BF16>::kPieces, GROUPS = 2, J = 4 / GROUPS, kBuffers = BF16 ? 2 : 1;
     constexpr int kPlane = MT * 4 * 64;             // sixteen bytes each
-    __shared__ qt_u32x4 s_x[kBuffers * P * kPlane];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+    __shared__ qt_u32x4 s_all[SPLIT][kBuffers * P * kPlane];
+    const int lane = threadIdx.x & 63, turn = __builtin_amdgcn_readfirstlane(threadIdx.x / kManyThreads), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % kManyWaves;
+    const int quarter = lane >> 4;
+    qt_u32x4 *const s_x = s_all[turn];
     int row, column;
     if (!many_tile(grid, row, column)) return;
     const int first_token = row * 16 * MT, first_tile = column * (kManyWaves * N) + wave * N;
@@ -105,13 +111,15 @@ __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linea
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < N; ++n) sum[m][n] = (fp4_f32x4){0.f, 0.f, 0.f, 0.f};
-    load_tokens(0, 0);
-    load_weights(0);
-    put_tokens();
+    if (turn < a.blocks) {
+        load_tokens(turn, 0);
+        load_weights(turn);
+        put_tokens();
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    for (int block = 0; block < a.blocks; ++block) {
-        const int buffer = BF16 ? block & 1 : 0;
+    for (int first = 0; first < a.blocks; first += SPLIT) {
+        const int block = first + turn, buffer = BF16 ? (first / SPLIT) & 1 : 0;
         qt_u32x4 now[N];
         float by[N][GROUPS];
 #pragma unroll
@@ -120,13 +128,16 @@ __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linea
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) by[n][g] = scale[n][g];
         }
-        const bool more = block + 1 < a.blocks;
+        const bool more = block + SPLIT < a.blocks;
         if (more) {
-            load_tokens(block + 1, BF16 ? buffer ^ 1 : 0);
-            load_weights(block + 1);
+            load_tokens(block + SPLIT, BF16 ? buffer ^ 1 : 0);
+            load_weights(block + SPLIT);
         }
+        // (of an odd number of blocks the last is one of the first waves')
+        const bool mine_too = SPLIT == 1 || block < a.blocks;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
+            if (!mine_too) break;
             bf16x8 numbers[N][J];
 #pragma unroll
             for (int n = 0; n < N; ++n)
@@ -158,6 +169,22 @@ __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linea
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
+    if constexpr (SPLIT > 1) {
+        static_assert(SPLIT == 2 && MT * N <= kBuffers * P * kPlane / kManyThreads, "room for the sums of one half");
+        fp4_f32x4 *const s_sum = (fp4_f32x4 *)s_all[1];
+        if (turn == 1) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < N; ++n) s_sum[((wave * MT + m) * N + n) * 64 + lane] = sum[m][n];
+        }
+        __syncthreads();
+        if (turn == 1) return;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < N; ++n) sum[m][n] += s_sum[((wave * MT + m) * N + n) * 64 + lane];
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
         const int output = (first_tile + n) * kLinearOutputs + (lane & 15);
@@ -173,14 +200,14 @@ __global__ __launch_bounds__(kManyThreads, (BF16 && MT == 4 ? 3 : 2)) void linea
     }
 }
 
-template <bool BF16, int MT, int N>
+template <bool BF16, int MT, int N, int SPLIT>
 void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
     const ManyGrid grid = {(a.tokens + 16 * MT - 1) / (16 * MT), (a.outputs + 64 * N - 1) / (64 * N), 8};
     const long long all = (long long)grid.rows * grid.columns, blocks = (all + kXcds - 1) / kXcds * kXcds;
-    if (blocks >= kMostThreads / kManyThreads) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
+    if (blocks >= kMostThreads / (SPLIT * kManyThreads)) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
     const int shift = scales_of_block == 2 ? 0 : 1 + a.scales_shift;
     const bool aligned = is_aligned(a.x, 16) && a.x_stride % 8 == 0;
-    hipLaunchKernelGGL((linear_many_kernel<BF16, MT, N>), dim3((unsigned)blocks), dim3(kManyThreads), 0, stream, a, grid, shift, aligned);
+    hipLaunchKernelGGL((linear_many_kernel<BF16, MT, N, SPLIT>), dim3((unsigned)blocks), dim3(SPLIT * kManyThreads), 0, stream, a, grid, shift, aligned);
 }
 
 }  // namespace
@@ -190,14 +217,19 @@ long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.to
 // Large tiles use what they read more often, but leave units idle until there are four workgroups for each: 4096 inputs in bf16, 128 x 256 against
 // 64 x 128, as loads of tokens were then, 1024 tokens and 4096 outputs 101 and 43 us, 2048 and 11008 218 and 219, 6000 and 11008 545 and 634; in fp32 64 x 192 against 64 x 128,
 // 256 and 4096 99 and 80, 2048 and 11008 514 and 567.
+// With no more than one workgroup a unit, eight waves of it cover each other's loads: 512 tokens and 4096 outputs (256 workgroups) 26.9 us, of four waves 30.4, in fp32 58.7
+// and 74.5; 256 and 14336 (448) in fp32 112 and 97.6, as a unit's LDS holds one of them.
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
     const long long large = bf16 ? (long long)((a.tokens + 127) / 128) * ((a.outputs + 255) / 256) : (long long)((a.tokens + 63) / 64) * ((a.outputs + 191) / 192);
     if (large >= 4LL * compute_units()) {
-        if (bf16) launch_many<true, 8, 4>(a, scales_of_block, stream);
-        else launch_many<false, 4, 3>(a, scales_of_block, stream);
+        if (bf16) launch_many<true, 8, 4, 1>(a, scales_of_block, stream);
+        else launch_many<false, 4, 3, 1>(a, scales_of_block, stream);
+    } else if (linear_many_workgroups(a) > compute_units()) {
+        if (bf16) launch_many<true, 4, 2, 1>(a, scales_of_block, stream);
+        else launch_many<false, 4, 2, 1>(a, scales_of_block, stream);
     } else {
-        if (bf16) launch_many<true, 4, 2>(a, scales_of_block, stream);
-        else launch_many<false, 4, 2>(a, scales_of_block, stream);
+        if (bf16) launch_many<true, 4, 2, 2>(a, scales_of_block, stream);
+        else launch_many<false, 4, 2, 2>(a, scales_of_block, stream);
     }
 }
 

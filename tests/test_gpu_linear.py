@@ -219,3 +219,18 @@ def test_a_checkpoint(Linear, tmp_path):
     assert torch.equal(other.dequantize(), held.dequantize())
     with pytest.raises(ValueError):
         Linear(200, 30).load_state_dict(held.state_dict())
+
+
+@pytest.mark.parametrize("inputs", [50, 128, 130, 384, 520, 1000])
+@pytest.mark.parametrize("tokens,outputs", [(900, 2048), (1000, 1950), (130, 10001)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_inputs_shared_by_the_halves_of_a_workgroup(Linear, tokens, outputs, inputs, dtype):
+    """As many tiles as units or a little less: one block of inputs, which leaves a half without any, odd and even numbers of them."""
+    w, x = matrix(outputs, inputs, dtype, 24), matrix(tokens, inputs, dtype, 25)
+    held, bias = Linear(inputs, outputs).quantize(w.cuda()), torch.randn(outputs, generator=torch.Generator().manual_seed(26))
+    got = held.product(x.cuda(), bias.cuda())
+    check(got, x, w, 64, bias)
+    assert torch.equal(held.product(x.cuda(), bias.cuda()), got)
+    wide = torch.full((tokens, inputs + 3), math.nan, dtype=dtype, device="cuda")
+    wide[:, 1:inputs + 1] = x.cuda()
+    assert torch.equal(held.product(wide[:, 1:inputs + 1], bias.cuda()), got)
