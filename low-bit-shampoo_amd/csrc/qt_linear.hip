@@ -202,15 +202,17 @@ void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
 
 // Many tokens as soon as the kernel for them has a workgroup for seven of eight units: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 15.1 us here
 // and 25.8 there, 384 and 4096 (192) 22.0 and 26.1, 128 and 14336 (224) 29.4 and 26.9, in fp32 70.6 and 57.4.
+// Its tile is of 64 tokens: 32 tokens, 128000 outputs 74 us here and 80 there, 33 126 and 80, in fp32 48 217 and 203, 32 147 and 188, one 67 and 213.
 // Else the smallest tile of a workgroup whose workgroups have a unit each: every one reads all of its tokens (from L2) and joins its waves, so
 // more of them than that cost more than they spread.  By tiles of outputs x tokens, before loads of tokens and joins were as they are: 16 tokens, 4096
 // outputs 1 x 1 6.7 us, 2 x 1 7.9, 4 x 1 10.1; 14336 outputs 18.3, 12.6, 10.5; 64 tokens, 4096 outputs 4 x 1 10.5, 4 x 2 15.4; as they are, 64 tokens, 11008
 // outputs 4 x 4 14.5, 4 x 2 16.6.  Four waves to a workgroup where there are several for each unit (32 tokens, 28672 outputs 25.1 us against 26.0 of
-// eight).
+// eight).  In fp32 eight tiles of outputs share a token's pieces, which take as long to cut as twelve matrix instructions: 128 tokens, 4096 outputs 17.3 us, four tiles 20.9, with two
+// of 16 tokens 18.8; one token, 28672 outputs 18.6 us, four tiles and waves 19.8.
 template <bool BF16>
 void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
     const long long tiles = (a.outputs + 15) / 16, rows = (a.tokens + 15) / 16, units = compute_units();
-    if (8 * linear_many_workgroups(a) >= 7 * units) return launch_linear_many(a, BF16, groups, stream);
+    if (a.tokens > (BF16 ? 32 : 48) && 8 * linear_many_workgroups(a) >= 7 * units) return launch_linear_many(a, BF16, groups, stream);
     if (tiles * rows <= units) return launch_few<BF16, 1, 1, 8>(a, groups, stream);
     if ((tiles + 1) / 2 * rows <= units) return launch_few<BF16, 1, 2, 8>(a, groups, stream);
     if ((tiles + 3) / 4 * rows <= units) return launch_few<BF16, 1, 4, 8>(a, groups, stream);
@@ -218,8 +220,10 @@ void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
         if (rows > 1 && (tiles + 3) / 4 * ((rows + 1) / 2) <= units) return launch_few<BF16, 2, 4, 8>(a, groups, stream);
         if (rows > 2 && (tiles + 3) / 4 * ((rows + 3) / 4) <= units) return launch_few<BF16, 4, 4, 8>(a, groups, stream);
         if (rows > 1) return launch_few<BF16, 2, 4, 4>(a, groups, stream);
+        return launch_few<BF16, 1, 4, 4>(a, groups, stream);
+    } else {
+        return launch_few<BF16, 1, 8, 8>(a, groups, stream);
     }
-    launch_few<BF16, 1, 4, 4>(a, groups, stream);
 }
 
 bool linear_shape(const char *what, const qtensor_linear *w) {

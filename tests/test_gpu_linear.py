@@ -234,3 +234,12 @@ def test_inputs_shared_by_the_halves_of_a_workgroup(Linear, tokens, outputs, inp
     wide = torch.full((tokens, inputs + 3), math.nan, dtype=dtype, device="cuda")
     wide[:, 1:inputs + 1] = x.cuda()
     assert torch.equal(held.product(wide[:, 1:inputs + 1], bias.cuda()), got)
+
+
+@pytest.mark.parametrize("tokens", [1, 7, 16, 32, 33, 48, 49])
+@pytest.mark.parametrize("inputs,outputs", [(130, 40001), (257, 30000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_few_tokens_and_as_many_outputs_as_a_vocabulary(Linear, tokens, inputs, outputs, dtype):
+    w, x = matrix(outputs, inputs, dtype, 34), matrix(tokens, inputs, dtype, 35)
+    for blocksize in (64, 256):
+        check(Linear(inputs, outputs, blocksize=blocksize).quantize(w.cuda()).product(x.cuda()), x, w, blocksize)
