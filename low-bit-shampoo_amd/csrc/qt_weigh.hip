@@ -38,6 +38,9 @@ struct WeighArgs {
     int parts;                          // at most
     long long wanted;                   // workgroups that the rows' work is cut for
     FastDiv by_group, by_tiles;         // and by tiles of rows of a token
+    float *sums;                        // [row part][sequence][head][sums_stride]: of the rows of a token cut into row_parts, if these are more than one
+    long long sums_stride;
+    int row_parts;
 };
 
 // Rows (i, g) of a sequence and what they see.
@@ -712,6 +715,10 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
         long long end = (long long)g.v.count * a.group;
         if (a.window && g.first >= a.sinks) end = min(end, ((long long)g.first + 16 * N - 1 + a.window - g.v.first_position) * a.group);
         first_row = from < end ? ((int)from & ~15) + (SHARED ? 16 * wave : 0) : 0, to = from < end ? (int)end : 0;
+        if (SHARED && a.row_parts > 1 && to) {
+            const int begin = (int)from & ~15, each = ((to - begin + kStep - 1) / kStep + a.row_parts - 1) / a.row_parts * kStep;
+            first_row = (int)min((long long)to, begin + (long long)blockIdx.z * each) + 16 * wave, to = (int)min((long long)to, begin + (long long)(blockIdx.z + 1) * each);
+        }
     };
     keys.fetch(a, g.b, head, g.first >> 4, g.v.end);
     range(g);
@@ -734,7 +741,8 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
 #pragma unroll
         for (int n = 0; n < N; ++n) writes = writes && (mine != n || there[n]);
         float *total = a.totals + g.b * a.total_sequence + head * a.total_head + first + t;
-        const float held = writes && (!SHARED || wave == 0) ? *total : 0.0f;
+        const bool parted = SHARED && a.row_parts > 1;
+        const float held = writes && !parted && (!SHARED || wave == 0) ? *total : 0.0f;
         WeighGroup after;
         const bool more = groups.next(a, after);
         if (kAhead && more) keys.fetch(a, after.b, head, after.first >> 4, after.v.end);
@@ -798,7 +806,9 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
 #pragma unroll
                     for (int n = 0; n < N; ++n) {
                         const int at = first + 16 * n + (lane & 15);
-                        sum[n] += there[n] && at < g.v.end && row_sees(a, position, at) ? __builtin_amdgcn_exp2f(s[n][i]) * by[i] : 0.0f;
+                        float weight = __builtin_amdgcn_exp2f(s[n][i]) * by[i];
+                        asm volatile("" : "+v"(weight));        // (and then looked at: a branch for each takes longer)
+                        sum[n] += there[n] && at < g.v.end && row_sees(a, position, at) ? weight : 0.0f;
                     }
                 }
             }
@@ -807,7 +817,11 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
         if constexpr (SHARED) {
             s_sum[buffer][wave][t] = weight;
             __syncthreads();
-            if (wave == 0 && writes) *total = held + ((s_sum[buffer][0][t] + s_sum[buffer][1][t]) + (s_sum[buffer][2][t] + s_sum[buffer][3][t]));
+            if (wave == 0) {
+                const float all = (s_sum[buffer][0][t] + s_sum[buffer][1][t]) + (s_sum[buffer][2][t] + s_sum[buffer][3][t]);
+                if (parted) a.sums[(((long long)blockIdx.z * a.at.batch + g.b) * a.shape.kv_heads + head) * a.sums_stride + first + t] = all;
+                else if (writes) *total = held + all;
+            }
             buffer ^= 1;
         } else {
             if (writes) *total = held + weight;
@@ -819,6 +833,28 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
             if (first_row < to) fetch_rows(g.v, first_row);
         }
     }
+}
+
+// Adds the sums of all row parts to the totals, in order: of the tokens whose groups the kernel above goes through.
+__global__ __launch_bounds__(kWeighThreads) void weigh_add_kernel(const WeighArgs a) {
+    const int head = blockIdx.y, b = blockIdx.z, token = ((int)blockIdx.x * kWeighThreads + (int)threadIdx.x) * 4;
+    const WeighSequence v = weigh_sequence<true>(a, b);
+    if (v.count <= 0 || token >= v.end) return;
+    const WeighView view = weigh_view(a, v.first_position, v.first_position + v.count - 1, v.end);
+    if (view.tiles == 0 || (token >= 16 * view.sink_tiles && token < 16 * view.first_tile)) return;
+    if ((unsigned)a.at.table[b * a.at.table_stride + (token >> a.shape.page_shift)] >= (unsigned)a.shape.pages) return;
+    float *total = a.totals + b * a.total_sequence + head * a.total_head + token;
+    const float *from = a.sums + ((long long)b * a.shape.kv_heads + head) * a.sums_stride + token;
+    const long long part = (long long)a.at.batch * a.shape.kv_heads * a.sums_stride;
+    float4 all = load_f32x4<true>(from);
+    for (int n = 1; n < a.row_parts; ++n) {
+        const float4 more = load_f32x4<true>(from + n * part);
+        all.x += more.x, all.y += more.y, all.z += more.z, all.w += more.w;
+    }
+    const float sum[4] = {all.x, all.y, all.z, all.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (token + e < v.end) total[e] += sum[e];
 }
 
 // Tiles of rows at most, and parts of the tokens that they see: no more than leave several to a workgroup of a round, nor than there are tokens to see.
@@ -868,7 +904,10 @@ void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
     const long long round = (BF16 && STEPS == 2 ? 3 : 2) * compute_units(), blocks = (covered + 16 * N - 1) / (16 * N) * a.at.batch;
     const long long heads = a.shape.kv_heads, each = round / heads < 1 ? 1 : round / heads;
     const dim3 grid((unsigned)heads, (unsigned)min(min(blocks, each), 65535LL));
-    if (blocks >= kWeighWaves * each) hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, false>), grid, dim3(kWeighThreads), 0, stream, a);
+    if (a.row_parts > 1) {
+        hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, true>), dim3(grid.x, grid.y, (unsigned)a.row_parts), dim3(kWeighThreads), 0, stream, a);
+        hipLaunchKernelGGL(weigh_add_kernel, dim3((unsigned)((covered + 4 * kWeighThreads - 1) / (4 * kWeighThreads)), a.shape.kv_heads, a.at.batch), dim3(kWeighThreads), 0, stream, a);
+    } else if (blocks >= kWeighWaves * each) hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, false>), grid, dim3(kWeighThreads), 0, stream, a);
     else hipLaunchKernelGGL((weigh_tokens_kernel<BF16, STEPS, true>), grid, dim3(kWeighThreads), 0, stream, a);
 }
 
@@ -882,7 +921,15 @@ void launch_weigh_type(const WeighArgs &a, bool few, hipStream_t stream) {
 // Scores of a token of each sequence are kept, if they take up to 512 MB, instead of being worked out twice: 32 sequences of 100 to 8000 tokens 47 us
 // without and 38 with them.
 constexpr long long kMostScores = 1LL << 29;
-struct WeighSizes { long long partial, scores, stride, all; int parts; bool few; };
+struct WeighSizes { long long partial, scores, stride, all; int parts, row_parts; bool few; };
+// Parts of the rows that see a token, where the tokens alone do not make two workgroups for each unit, of at least 256 rows on average.  A prompt of 1487 tokens, 3
+// heads, groups of 8, a window of 349, bf16: 76 us, whole 237; three of 371, 2 heads, groups of 4 36 and 42.
+int weigh_row_parts(const CacheShape &shape, const CachePlaces &at, int group, long long room) {
+    const int tokens = shape.head_dim > 128 ? 32 : 64;
+    const long long groups = (room + tokens - 1) / tokens * at.batch * shape.kv_heads, rows = (long long)at.tokens * group / at.batch;
+    const long long parts = min(2LL * compute_units() / groups, rows / 256);
+    return (int)(parts < 2 ? 1 : parts < 16 ? parts : 16);
+}
 WeighSizes weigh_sizes(const CacheShape &shape, const CachePlaces &at, int heads) {
     WeighSizes s;
     s.few = !at.starts && heads / shape.kv_heads <= 16;         // a tile of rows for every sequence
@@ -891,6 +938,8 @@ WeighSizes weigh_sizes(const CacheShape &shape, const CachePlaces &at, int heads
     s.partial = (((long long)at.tokens * heads * (s.parts + 1) + 16) * (long long)sizeof(float2) + 255) & ~255LL;      // (and room behind the statistics)
     s.stride = (((long long)at.table_pages << shape.page_shift) + 63) & ~63LL;
     s.scores = s.few && s.stride <= kMostScores / 4 / heads / at.batch ? s.stride * heads * at.batch * 4 : 0;
+    s.row_parts = s.few ? 1 : weigh_row_parts(shape, at, heads / shape.kv_heads, (long long)at.table_pages << shape.page_shift);
+    if (s.row_parts > 1) s.scores = (long long)s.row_parts * at.batch * shape.kv_heads * s.stride * 4;          // (of parts of rows in their place)
     s.all = s.partial + s.scores;
     s.all = s.all < 16 ? 16 : s.all;
     return s;
@@ -936,7 +985,9 @@ extern "C" void qtensor_hip_cache_weigh(const qtensor_cache *cache, const qtenso
     a.totals = totals, a.total_sequence = total_sequence, a.total_head = total_head;
     a.partial = (float2 *)workspace;
     a.statistics = a.partial + (long long)a.at.tokens * heads * size.parts;
-    a.scores = size.scores ? (float *)((uint8_t *)workspace + size.partial) : nullptr, a.score_stride = size.stride;
+    float *behind = size.scores ? (float *)((uint8_t *)workspace + size.partial) : nullptr;
+    a.scores = size.few ? behind : nullptr, a.score_stride = size.stride;
+    a.sums = behind, a.sums_stride = size.stride, a.row_parts = size.row_parts;
     a.by_group = make_fastdiv((uint32_t)a.group);
     if ((long long)a.at.tokens * a.group >= 1 << 27 || a.group >= 1 << 15 || a.at.batch > 65535 || a.shape.kv_heads > 65535) {
         set_error(kBadArgument, "%s: too many tokens, heads or sequences (%d, %d, %d)", what, a.at.tokens, heads, a.at.batch);

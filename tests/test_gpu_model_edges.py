@@ -187,3 +187,30 @@ def test_more_tiles_of_rows_than_a_dimension_of_a_grid():
     # any stretch of tokens has what its queries give it, less or more what a window reaches over both ends
     for first in (0, 100000, 200000):
         assert abs(float(per[first:first + 5000].sum()) - 5000 * heads) <= window * heads * 2
+
+
+@pytest.mark.parametrize("lengths,news,heads,kv_heads,dim,window,sinks", [([700, 33, 0, 1100], [700, 33, 0, 1100], 8, 2, 64, None, 0), ([1300], [1300], 8, 1, 128, 200, 7),
+                                                                          ([900, 500], [640, 500], 4, 2, 256, None, 0), ([2000, 1, 64], [700, 1, 64], 16, 1, 80, 64, 0)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_prompts_cut_into_parts(lengths, news, heads, kv_heads, dim, window, sinks, dtype):
+    """Few tokens that many rows see: the rows are cut too, and their sums added in order; a page that is not there, totals that were not zero."""
+    cache, table, counts = made(lengths, kv_heads, dim, seed=50)
+    keys, _ = cache.read(table, counts, torch.tensor([sum(lengths[:b]) for b in range(len(lengths) + 1)], dtype=torch.int32, device="cuda"), tokens=sum(lengths))
+    table[0, 2] = -1
+    q = random((sum(news), heads, dim), 53, dtype)
+    starts = torch.tensor([sum(news[:b]) for b in range(len(news) + 1)], dtype=torch.int32, device="cuda")
+    before = torch.rand(cache.totals(table).shape, generator=torch.Generator().manual_seed(54)).cuda()
+    totals = cache.weigh(before.clone(), q, table, counts, starts, window=window, sinks=sinks)
+    assert torch.equal(cache.weigh(before.clone(), q, table, counts, starts, window=window, sinks=sinks), totals)
+    at = first = 0
+    for b, (n, new) in enumerate(zip(lengths, news)):
+        there = torch.ones(n, dtype=torch.bool)
+        if b == 0:
+            there[32:48] = False
+        want, spread = E.weigh(q[at:at + new].cpu(), range(n - new, n), keys[first:first + n].double().cpu(), 1 / math.sqrt(dim), window, sinks, there)
+        start = before[b, :, :n].double().cpu()
+        off = (totals[b, :, :n].double().cpu() - start - want).abs()
+        limit = E.bound(dim, new * heads // kv_heads, want, spread) + 2.0 ** -23 * (start + want)
+        assert bool((off <= limit).all()), f"sequence {b}: off by {float((off / limit).max()):.3g} of the bound"
+        assert torch.equal(totals[b, :, n:], before[b, :, n:])
+        at, first = at + new, first + n
