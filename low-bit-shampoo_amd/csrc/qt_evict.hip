@@ -27,6 +27,7 @@ struct EvictArgs {
     int *new_lengths;
     // scratch, an entry a token that stays, of [batch][kv_heads][keep]
     int *from, *to, *count;             // places; how many stay of a sequence
+    uint8_t *apart[4];                  // room for what moves: codes of keys and of values, scales (with the keys' totals)
 };
 
 __device__ __forceinline__ int evict_end(const EvictArgs &a, int b) {
@@ -43,7 +44,8 @@ __device__ __forceinline__ uint32_t total_key(float x) {
     return __builtin_isunordered(x, x) ? 0xffffffffu : float_to_key(x + 0.0f);
 }
 
-// A workgroup looks at kChunk tokens at a time, up to kEach side by side a thread, whose keys stay in LDS where they are all of the sequence.
+// A workgroup looks at kChunk tokens at a time, up to kEach side by side a thread, whose keys stay in LDS where they are all of the sequence.  (32 a thread: 131 us
+// for 9 sequences of 58000 tokens, 16 124.)
 constexpr int kEach = 16, kChunk = kEach * kChooseThreads;
 constexpr int kCopies = 4;             // of the counts: waves that take one in turn wait for each other less
 
@@ -291,12 +293,55 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(const EvictArg
     }
 }
 
+// The same for few sequences and heads, through room of their own, by all units: out of the cache, then back.  8 sequences and heads, 26000 tokens of
+// 128 chosen, moved and read back 155 us, in place 245; 2048 36 and 39; 32 of 2048 46 and 43, 8 of 1100 35 and 33.
+constexpr int kCopyThreads = 256, kCopyItems = 4;
+template <bool BACK, typename Piece, typename Address>
+__device__ __forceinline__ void copy_pieces(int count, int parts, const int *from, const int *to, Piece *apart, const Address &address) {
+    const int *place = BACK ? to : from;
+#pragma unroll
+    for (int k = 0; k < kCopyItems; ++k) {
+        const long long i = ((long long)blockIdx.x * kCopyItems + k) * kCopyThreads + threadIdx.x;
+        const int nth = (int)(i / parts), part = (int)(i - (long long)nth * parts);
+        if (nth >= count) break;
+        if (from[nth] == to[nth]) continue;
+        Piece *there = address(place[nth], part);
+        if (BACK) *there = apart[i];
+        else apart[i] = *there;
+    }
+}
+template <bool BACK>
+__global__ __launch_bounds__(kCopyThreads) void evict_copy_kernel(const EvictArgs a) {
+    const int what = blockIdx.y & 3, values = what & 1, head = blockIdx.y >> 2, b = blockIdx.z;
+    const long long sequence = (long long)b * a.shape.kv_heads + head;
+    const int *from = a.from + sequence * a.keep, *to = a.to + sequence * a.keep;
+    const int count = a.count[b];
+    const auto inside = [&](int place) { return place & ((1 << a.shape.page_shift) - 1); };
+    const auto line = [&](int place) { return evict_line(a, b, place) + ((long long)head << a.shape.page_shift); };
+    if (what < 2) {
+        uint8_t *codes = a.codes[values];
+        const int parts = a.shape.row_bytes / 16;
+        copy_pieces<BACK>(count, parts, from, to, (qt_u32x4 *)a.apart[values] + sequence * a.keep * parts,
+                          [&](int place, int part) { return (qt_u32x4 *)(codes + (line(place) + inside(place)) * a.shape.row_bytes) + part; });
+    } else {
+        float *scales = a.scales[values], *totals = a.totals + b * a.total_sequence + head * a.total_head;
+        const int parts = a.shape.segments + 1 - values;
+        copy_pieces<BACK>(count, parts, from, to, (float *)a.apart[2 + values] + sequence * a.keep * parts, [&](int place, int part) {
+            return part == a.shape.segments ? totals + place : scales + line(place) * a.shape.segments + ((long long)part << a.shape.page_shift) + inside(place);
+        });
+    }
+}
+
 long long rounded(long long bytes) { return (bytes + 255) & ~255LL; }
 
-struct EvictSizes { long long lists, count, all; };
+struct EvictSizes { long long lists, count, codes, scales[2], all; };
 EvictSizes evict_sizes(const CacheShape &shape, int batch, long long keep) {
-    EvictSizes s = {rounded(4LL * batch * shape.kv_heads * keep), rounded(4LL * batch), 0};
-    s.all = 2 * s.lists + s.count;
+    const long long kept = (long long)batch * shape.kv_heads * keep;
+    EvictSizes s = {rounded(4 * kept), rounded(4LL * batch), 0, {0, 0}, 0};
+    const long long workers = (long long)batch * shape.kv_heads;
+    if (8 * workers < compute_units() && keep >= 1536 && keep >= 256 * workers)
+        s.codes = rounded(kept * shape.row_bytes), s.scales[0] = rounded(4 * kept * (shape.segments + 1)), s.scales[1] = rounded(4 * kept * shape.segments);
+    s.all = 2 * s.lists + s.count + 2 * s.codes + s.scales[0] + s.scales[1];
     return s;
 }
 
@@ -344,12 +389,21 @@ extern "C" void qtensor_hip_cache_evict(const qtensor_cache *cache, const qtenso
     a.table = at.table, a.lengths = at.lengths, a.table_stride = at.table_stride, a.table_pages = at.table_pages, a.batch = at.batch;
     uint8_t *p = (uint8_t *)workspace;
     a.from = (int *)p, a.to = (int *)(p + size.lists), a.count = (int *)(p + 2 * size.lists);
+    p += 2 * size.lists + size.count;
+    a.apart[0] = p, a.apart[1] = p + size.codes, a.apart[2] = p + 2 * size.codes, a.apart[3] = a.apart[2] + size.scales[0];
     for (int i = 0; i < 2; ++i) a.codes[i] = cache->codes[i], a.scales[i] = cache->scales[i];
     a.totals = totals, a.total_sequence = total_sequence, a.total_head = total_head;
     const long long most = 0x7fffffff;
     a.keep = (int)kept, a.recent = (int)(recent < most ? recent : most), a.sinks = (int)(sinks < most ? sinks : most);
     a.new_lengths = new_lengths;
     hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)a.shape.kv_heads, (unsigned)a.batch), dim3(kChooseThreads), 0, (hipStream_t)stream, a);
-    hipLaunchKernelGGL(evict_move_kernel, dim3(4, (unsigned)a.shape.kv_heads, (unsigned)a.batch), dim3(kMoveThreads), 0, (hipStream_t)stream, a);
+    if (size.codes) {
+        const long long pieces = kept * (a.shape.row_bytes / 16 > a.shape.segments + 1 ? a.shape.row_bytes / 16 : a.shape.segments + 1), each = kCopyThreads * kCopyItems;
+        const dim3 grid((unsigned)((pieces + each - 1) / each), 4 * (unsigned)a.shape.kv_heads, (unsigned)a.batch);
+        hipLaunchKernelGGL(evict_copy_kernel<false>, grid, dim3(kCopyThreads), 0, (hipStream_t)stream, a);
+        hipLaunchKernelGGL(evict_copy_kernel<true>, grid, dim3(kCopyThreads), 0, (hipStream_t)stream, a);
+    } else {
+        hipLaunchKernelGGL(evict_move_kernel, dim3(4, (unsigned)a.shape.kv_heads, (unsigned)a.batch), dim3(kMoveThreads), 0, (hipStream_t)stream, a);
+    }
     launch_ok(what);
 }

@@ -271,7 +271,8 @@ class QTensorCache:
             raise ValueError(f"{places.batch} sequences are too many for one call.")
         keep, recent, sinks = (min(n, 2 ** 62) for n in (keep, recent, sinks))
         cache = self._ref()
-        size = F.lib.qtensor_hip_cache_evict_workspace(cache, places, keep)
+        with torch.cuda.device(totals.device):
+            size = F.lib.qtensor_hip_cache_evict_workspace(cache, places, keep)
         scratch = torch.empty(size, dtype=torch.uint8, device=totals.device)
         out = torch.empty(places.batch, dtype=torch.int32, device=totals.device)
         F._call(F.lib.qtensor_hip_cache_evict, totals.device, cache, places, totals.data_ptr(), totals.stride(0), totals.stride(1), keep, recent, sinks,

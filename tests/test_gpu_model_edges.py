@@ -214,3 +214,34 @@ def test_rows_of_prompts_cut_into_parts(lengths, news, heads, kv_heads, dim, win
         assert bool((off <= limit).all()), f"sequence {b}: off by {float((off / limit).max()):.3g} of the bound"
         assert torch.equal(totals[b, :, n:], before[b, :, n:])
         at, first = at + new, first + n
+
+
+@pytest.mark.parametrize("lengths,kv_heads,dim,blocksize,keep", [([9000, 40, 2500], 2, 128, 64, 2000), ([20000], 1, 80, 128, 9000), ([5000], 4, 256, 64, 1536), ([1700, 0], 1, 33, 256, 4000)])
+def test_few_sequences_cut_down_through_room_of_their_own(lengths, kv_heads, dim, blocksize, keep):
+    from qtensor.cache import QTensorCache
+    width = -(-max(lengths) // 64) + 1
+    cache = QTensorCache(len(lengths) * width + 2, kv_heads, dim, page_size=64, blocksize=blocksize)
+    table = torch.randperm(cache.pages, generator=torch.Generator().manual_seed(60))[:len(lengths) * width].view(len(lengths), width).to(torch.int32).cuda()
+    starts = torch.tensor([sum(lengths[:b]) for b in range(len(lengths) + 1)], dtype=torch.int32, device="cuda")
+    counts = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    k, v = random((sum(lengths), kv_heads, dim), 61), random((sum(lengths), kv_heads, dim), 62)
+    cache.write(k, v, table, counts, starts)
+    table[0, 3] = -1
+    before = cache.read(table, counts, starts, tokens=sum(lengths))
+    totals = torch.rand(cache.totals(table).shape, generator=torch.Generator().manual_seed(63)).cuda()
+    was = totals.clone()
+    new = cache.evict(totals, table, counts, keep, recent=30, sinks=5)
+    after = cache.read(table, counts, starts, tokens=sum(lengths))
+    for b, n in enumerate(lengths):
+        there = [not (b == 0 and 192 <= t < 256) for t in range(n)]
+        at = int(starts[b])
+        for h in range(kv_heads):
+            source, target = E.evict(was[b, h, :n].tolist(), n, keep, 30, 5, there)
+            assert int(new[b]) == (target[-1] + 1 if target else 0)
+            i, j = torch.tensor(source, dtype=torch.long, device="cuda"), torch.tensor(target, dtype=torch.long, device="cuda")
+            for x, y in zip(before, after):
+                assert torch.equal(y[at + j, h], x[at + i, h])
+            assert torch.equal(totals[b, h, j], was[b, h, i])
+            stay = torch.ones(totals.shape[2], dtype=torch.bool, device="cuda")
+            stay[j] = False
+            assert torch.equal(totals[b, h][stay], was[b, h][stay])
