@@ -200,6 +200,14 @@ void launch_few(const LinearArgs &a, int groups, hipStream_t stream) {
     else hipLaunchKernelGGL((linear_few_kernel<BF16, T, R, WAVES, 1, T == 1>), grid, dim3(64 * WAVES), 0, stream, a);
 }
 
+// One tile of tokens to a workgroup: MOST waves where more than 2048 inputs give each of them blocks, else eight.  One token, 14336 inputs, 4096 outputs in bf16 9.3 us of 16
+// waves, 11.4 of 8; in fp32 4096 inputs, 4096 outputs 6.2 and 7.3, 14336 outputs 10.0 and 11.1, where bf16 has 7.3 and 7.4 (32 tokens 15.8 and 15.2).
+template <bool BF16, int R, int MOST>
+void launch_few_long(const LinearArgs &a, int groups, hipStream_t stream) {
+    if (MOST > 8 && a.blocks > 16) launch_few<BF16, 1, R, MOST>(a, groups, stream);
+    else launch_few<BF16, 1, R, 8>(a, groups, stream);
+}
+
 // Many tokens as soon as the kernel for them has a workgroup for seven of eight units: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 15.1 us here
 // and 25.8 there, 384 and 4096 (192) 22.0 and 26.1, 128 and 14336 (224) 29.4 and 26.9, in fp32 70.6 and 57.4.
 // Its tile is of 64 tokens: 32 tokens, 128000 outputs 74 us here and 80 there, 33 126 and 80, in fp32 48 217 and 203, 32 147 and 188, one 67 and 213.
@@ -213,9 +221,9 @@ template <bool BF16>
 void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
     const long long tiles = (a.outputs + 15) / 16, rows = (a.tokens + 15) / 16, units = compute_units();
     if (a.tokens > (BF16 ? 32 : 48) && 8 * linear_many_workgroups(a) >= 7 * units) return launch_linear_many(a, BF16, groups, stream);
-    if (tiles * rows <= units) return launch_few<BF16, 1, 1, 8>(a, groups, stream);
-    if ((tiles + 1) / 2 * rows <= units) return launch_few<BF16, 1, 2, 8>(a, groups, stream);
-    if ((tiles + 3) / 4 * rows <= units) return launch_few<BF16, 1, 4, 8>(a, groups, stream);
+    if (tiles * rows <= units) return launch_few_long<BF16, 1, 16>(a, groups, stream);
+    if ((tiles + 1) / 2 * rows <= units) return launch_few_long<BF16, 2, BF16 ? 8 : 16>(a, groups, stream);
+    if ((tiles + 3) / 4 * rows <= units) return launch_few_long<BF16, 4, BF16 ? 8 : 16>(a, groups, stream);
     if constexpr (BF16) {
         if (rows > 1 && (tiles + 3) / 4 * ((rows + 1) / 2) <= units) return launch_few<BF16, 2, 4, 8>(a, groups, stream);
         if (rows > 2 && (tiles + 3) / 4 * ((rows + 3) / 4) <= units) return launch_few<BF16, 4, 4, 8>(a, groups, stream);

@@ -200,13 +200,15 @@ __global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4
     }
 }
 
+bool linear_aligned(const LinearArgs &a) { return is_aligned(a.x, 16) && a.x_stride % 8 == 0; }
+
 template <bool BF16, int MT, int N, int SPLIT>
 void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
     const ManyGrid grid = {(a.tokens + 16 * MT - 1) / (16 * MT), (a.outputs + 64 * N - 1) / (64 * N), 8};
     const long long all = (long long)grid.rows * grid.columns, blocks = (all + kXcds - 1) / kXcds * kXcds;
     if (blocks >= kMostThreads / (SPLIT * kManyThreads)) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
     const int shift = scales_of_block == 2 ? 0 : 1 + a.scales_shift;
-    const bool aligned = is_aligned(a.x, 16) && a.x_stride % 8 == 0;
+    const bool aligned = linear_aligned(a);
     hipLaunchKernelGGL((linear_many_kernel<BF16, MT, N, SPLIT>), dim3((unsigned)blocks), dim3(SPLIT * kManyThreads), 0, stream, a, grid, shift, aligned);
 }
 
@@ -219,9 +221,10 @@ long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.to
 // 256 and 4096 99 and 80, 2048 and 11008 514 and 567.
 // With no more than one workgroup a unit, eight waves of it cover each other's loads: 512 tokens and 4096 outputs (256 workgroups) 26.9 us, of four waves 30.4, in fp32 58.7
 // and 74.5; 256 and 14336 (448) in fp32 112 and 97.6, as a unit's LDS holds one of them.
+// Rows that are not aligned go through registers, and take the smaller tile: 6000 tokens of 4100 inputs, 11008 outputs 691 us, the larger 783 (aligned 506).
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
     const long long large = bf16 ? (long long)((a.tokens + 127) / 128) * ((a.outputs + 255) / 256) : (long long)((a.tokens + 63) / 64) * ((a.outputs + 191) / 192);
-    if (large >= 4LL * compute_units()) {
+    if (large >= 4LL * compute_units() && (!bf16 || linear_aligned(a))) {
         if (bf16) launch_many<true, 8, 4, 1>(a, scales_of_block, stream);
         else launch_many<false, 4, 3, 1>(a, scales_of_block, stream);
     } else if (linear_many_workgroups(a) > compute_units()) {

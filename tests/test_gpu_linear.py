@@ -243,3 +243,15 @@ def test_few_tokens_and_as_many_outputs_as_a_vocabulary(Linear, tokens, inputs, 
     w, x = matrix(outputs, inputs, dtype, 34), matrix(tokens, inputs, dtype, 35)
     for blocksize in (64, 256):
         check(Linear(inputs, outputs, blocksize=blocksize).quantize(w.cuda()).product(x.cuda()), x, w, blocksize)
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 16, 40])
+@pytest.mark.parametrize("inputs", [2048, 2049, 2200, 9813])
+@pytest.mark.parametrize("outputs", [20, 2100, 5001, 9000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_long_inputs(Linear, tokens, inputs, outputs, dtype):
+    """More blocks of inputs than waves, fewer of the last ones, and as few as make eight waves enough."""
+    if inputs == 9813 and outputs > 2100:
+        outputs //= 4
+    w, x = matrix(outputs, inputs, dtype, 44), matrix(tokens, inputs, dtype, 45)
+    check(Linear(inputs, outputs).quantize(w.cuda()).product(x.cuda()), x, w, 64)
