@@ -4,7 +4,7 @@
 // of the sequence, then those with the largest totals, ties to the earlier one.  The nth token that stays moves to the place of the nth
 // token that is there, which is never behind it.
 //
-// Two launches: the choice (a workgroup a sequence and head), which lists where tokens come from and go to; the moves.
+// The choice (a workgroup a sequence and head), which lists where tokens come from and go to, then the moves.
 #include "qt_cache.h"
 
 namespace qt {
@@ -73,12 +73,12 @@ __device__ __forceinline__ uint32_t sum_before(uint32_t x, uint32_t *s_waves, ui
 }
 
 // Bound by the latency of its steps, and of fetching its instructions, which run once: loops stay loops (16384 keys in registers, all unrolled: 27 us for the
-// fewest tokens, 37 for 24 x 8 of 12000; so 13.5 and 23;
-// with loads and LDS reads asked for together, four copies of the counts and no look at ties that all stay 20.6).  The least key of those that stay is found eight bits at a time, from counts in LDS; lanes
-// that have the digit of the first one among them are counted together, as totals of one size are most of them.
+// fewest tokens, 37 for 24 x 8 of 12000; so 13.5 and 23; with loads and LDS reads asked for together, four copies of the counts, no look at ties that all
+// stay and the first digit counted with the tokens that are there, 20.2).  The least key of those that stay is found eight bits at a time, from counts in LDS;
+// lanes that have the digit of the first one among them are counted together, as totals of one size are most of them.
 __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const EvictArgs a) {
     __shared__ uint32_t s_key[kEach][kChooseThreads], s_waves[kChooseWaves];
-    __shared__ int s_count[kCopies][256], s_digit, s_above, s_same;
+    __shared__ int s_count[kCopies][256], s_digit, s_above, s_same, s_all[2];
     const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 63;
     const int length = max(a.lengths[b], 0), end = evict_end(a, b);
     const float *totals = a.totals + b * a.total_sequence + head * a.total_head;
@@ -115,16 +115,7 @@ __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const Evic
             }
         }
     };
-    int all_there = 0, all_protect = 0;
-#pragma unroll 1
-    for (int chunk = 0; chunk < chunks; ++chunk) {
-        load(chunk);
-        uint32_t all;
-        sum_before((uint32_t)__popc(there) | (uint32_t)__popc(anyhow) << 16, s_waves, all);
-        all_there += all & 0xffff, all_protect += all >> 16;
-    }
-    const int stay = min(all_there, a.keep);
-    int wanted = stay - all_protect;            // by their totals
+    int stay = 0, wanted = 0;                   // of the tokens that are there; by their totals
     // the least key of those that stay, and how many of the tokens with that key do
     uint32_t least = 0;
     bool all_ties = false;
@@ -133,10 +124,17 @@ __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const Evic
     for (int shift = 24; shift >= 0; shift -= 8) {
         __syncthreads();
         if (threadIdx.x < kCopies * 256) (&s_count[0][0])[threadIdx.x] = 0;
+        if (shift == 24 && threadIdx.x < 2) s_all[threadIdx.x] = 0;
         __syncthreads();
 #pragma unroll 1
         for (int chunk = 0; chunk < chunks; ++chunk) {
-            if (chunks > 1) load(chunk);
+            if (chunks > 1 || shift == 24) load(chunk);
+            if (shift == 24) {
+                uint32_t n = (uint32_t)__popc(there) | (uint32_t)__popc(anyhow) << 16;
+#pragma unroll
+                for (int off = 1; off < 64; off *= 2) n += (uint32_t)__shfl_xor((int)n, off, 64);
+                if (lane < 2) atomicAdd(&s_all[lane], (int)(lane ? n >> 16 : n & 0xffff));
+            }
 #pragma unroll 1
             for (int first = 0; first < each; first += 4) {
                 uint32_t key[4];
@@ -156,6 +154,7 @@ __global__ __launch_bounds__(kChooseThreads) void evict_choose_kernel(const Evic
             }
         }
         __syncthreads();
+        if (shift == 24) stay = min(s_all[0], a.keep), wanted = stay - s_all[1];
         if (threadIdx.x < 64) {
             // counts of the digits from this lane's four on
             int mine[4], above = 0;
