@@ -660,7 +660,9 @@ struct WeighGroups {
                 at = first + (Cost)nth * price;
                 return;
             }
-            look(a, block + 64);            // (at is in front of all groups' end)
+            // (at is in front of all groups' end, unless lengths have changed in between)
+            if (block + 64 >= a.at.batch) return;
+            look(a, block + 64);
         }
     }
     __device__ __forceinline__ bool next(const WeighArgs &a, WeighGroup &g) {
