@@ -34,9 +34,10 @@ __device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &colu
 // matrix instructions at a higher priority, in groups with the vector ones, or one tile ahead of them (512 to 529 us beside 513: the pipes are busy all the time, at a clock that falls to
 // 2.0 GHz).
 //
+// STAGED: tokens on their way in registers while a block is multiplied, for rows of bf16 that are not aligned to sixteen bytes.
 // SPLIT: two times four waves, which take the blocks of 128 inputs in turn and join their sums through LDS.
-template <bool BF16, int MT, int N, int SPLIT>
-__global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4 ? 3 : 2) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift, const bool aligned) {
+template <bool BF16, int MT, int N, int SPLIT, bool STAGED>
+__global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4 ? 3 : 2) void linear_many_kernel(const LinearArgs a, const ManyGrid grid, const int shift) {
     constexpr int P = Eight<BF16>::kPieces, GROUPS = 2, J = 4 / GROUPS, kBuffers = BF16 ? 2 : 1;
     constexpr int kPlane = MT * 4 * 64;             // sixteen bytes each
     __shared__ qt_u32x4 s_all[SPLIT][kBuffers * P * kPlane];
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4
         }
     };
     // a wave's part of a block of tokens: MT of the 4 MT pieces of 1 KB
-    Eight<BF16> raw[BF16 ? 1 : MT];
+    Eight<BF16> raw[STAGED || !BF16 ? MT : 1];
     // (four lanes side by side load 64 bytes of a token, in an order that keeps the lanes which read them off each other's banks)
     const int eighth = 8 * ((lane & 3) ^ quarter), mine = 4 * (lane & 15) + (quarter ^ ((lane >> 2) & 3));
     const uint8_t *from[MT / 4];
@@ -72,36 +73,55 @@ __global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4
         valid[i] = token < a.tokens ? a.inputs : 0;
         from[i] = (const uint8_t *)a.x + (long long)min(token, a.tokens - 1) * a.x_stride * (BF16 ? 2 : 4) + eighth * (BF16 ? 2 : 4);
     }
-    const auto load_tokens = [&](int block, int buffer) {
-        const int first = block * kLinearInputs;
-        if constexpr (BF16) {
-            if (aligned && first + kLinearInputs <= a.inputs) {
-                // (tokens behind the last are the last one again: their results are not stored)
+    // (tokens behind the last are the last one again, or zeros: their results are not stored)
+    const auto put = [&](const Eight<BF16> &x, int i, int buffer) {
+        bf16x8 pieces[P];
+        x.pieces(pieces);
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    __builtin_amdgcn_global_load_lds((const QT_GLOBAL void *)(from[i >> 2] + 2 * (first + 32 * (i & 3))),
-                                                     (QT_LDS void *)(s_x + buffer * kPlane + (wave * MT + i) * 64), 16, 0, 0);
-            } else {
+        for (int n = 0; n < P; ++n) s_x[(buffer * P + n) * kPlane + (wave * MT + i) * 64 + lane] = __builtin_bit_cast(qt_u32x4, pieces[n]);
+    };
+    const auto put_rest = [&](int first, int buffer) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    Eight<BF16> x;
-                    x.load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - eighth);
-                    s_x[buffer * kPlane + (wave * MT + i) * 64 + lane] = (qt_u32x4){x.raw[0], x.raw[1], x.raw[2], x.raw[3]};
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) raw[i].load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - eighth);
+        for (int i = 0; i < MT; ++i) {
+            Eight<BF16> x;
+            x.load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - eighth);
+            put(x, i, buffer);
         }
     };
-    const auto put_tokens = [&]() {
+    const auto load_tokens = [&](int block, int buffer) {
+        const int first = block * kLinearInputs;
+        if constexpr (!BF16) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) raw[i].load(from[i >> 2], first + 32 * (i & 3), valid[i >> 2] - eighth);
+        } else if constexpr (STAGED) {
+            // (nothing but whole blocks, so that they are waited for where they are used)
+            if (first + kLinearInputs <= a.inputs) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) raw[i].load(from[i >> 2], first + 32 * (i & 3));
+            }
+        } else if (first + kLinearInputs <= a.inputs) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                __builtin_amdgcn_global_load_lds((const QT_GLOBAL void *)(from[i >> 2] + 2 * (first + 32 * (i & 3))), (QT_LDS void *)(s_x + buffer * kPlane + (wave * MT + i) * 64),
+                                                 16, 0, 0);
+        } else {
+            put_rest(first, buffer);
+        }
+    };
+    const auto put_tokens = [&](int block, int buffer) {
+        if constexpr (BF16 && STAGED) {
+            const int first = block * kLinearInputs;
+            if (first + kLinearInputs <= a.inputs) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) put(raw[i], i, buffer);
+            } else {
+                put_rest(first, buffer);
+            }
+        }
         if constexpr (!BF16) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                bf16x8 pieces[P];
-                raw[i].pieces(pieces);
-#pragma unroll
-                for (int n = 0; n < P; ++n) s_x[n * kPlane + (wave * MT + i) * 64 + lane] = __builtin_bit_cast(qt_u32x4, pieces[n]);
+                put(raw[i], i, buffer);
                 __builtin_amdgcn_sched_barrier(0);          // (one at a time: registers)
             }
         }
@@ -114,7 +134,7 @@ __global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4
     if (turn < a.blocks) {
         load_tokens(turn, 0);
         load_weights(turn);
-        put_tokens();
+        put_tokens(turn, 0);
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -164,8 +184,8 @@ __global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4
         }
         if constexpr (!BF16) {
             __syncthreads();
-            if (more) put_tokens();
         }
+        if (more) put_tokens(block + SPLIT, BF16 ? buffer ^ 1 : 0);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
     }
@@ -202,14 +222,13 @@ __global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4
 
 bool linear_aligned(const LinearArgs &a) { return is_aligned(a.x, 16) && a.x_stride % 8 == 0; }
 
-template <bool BF16, int MT, int N, int SPLIT>
+template <bool BF16, int MT, int N, int SPLIT, bool STAGED>
 void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
     const ManyGrid grid = {(a.tokens + 16 * MT - 1) / (16 * MT), (a.outputs + 64 * N - 1) / (64 * N), 8};
     const long long all = (long long)grid.rows * grid.columns, blocks = (all + kXcds - 1) / kXcds * kXcds;
     if (blocks >= kMostThreads / (SPLIT * kManyThreads)) { set_error(kBadArgument, "linear_product: too many tokens and outputs (%d, %d)", a.tokens, a.outputs); return; }
     const int shift = scales_of_block == 2 ? 0 : 1 + a.scales_shift;
-    const bool aligned = linear_aligned(a);
-    hipLaunchKernelGGL((linear_many_kernel<BF16, MT, N, SPLIT>), dim3((unsigned)blocks), dim3(SPLIT * kManyThreads), 0, stream, a, grid, shift, aligned);
+    hipLaunchKernelGGL((linear_many_kernel<BF16, MT, N, SPLIT, STAGED>), dim3((unsigned)blocks), dim3(SPLIT * kManyThreads), 0, stream, a, grid, shift);
 }
 
 }  // namespace
@@ -221,18 +240,22 @@ long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.to
 // 256 and 4096 99 and 80, 2048 and 11008 514 and 567.
 // With no more than one workgroup a unit, eight waves of it cover each other's loads: 512 tokens and 4096 outputs (256 workgroups) 26.9 us, of four waves 30.4, in fp32 58.7
 // and 74.5; 256 and 14336 (448) in fp32 112 and 97.6, as a unit's LDS holds one of them.
-// Rows that are not aligned go through registers, and take the smaller tile: 6000 tokens of 4100 inputs, 11008 outputs 691 us, the larger 783 (aligned 506).
+// Rows that are not aligned are STAGED, and take the smaller tile: 6000 tokens of 4100 inputs, 11008 outputs 640 us (aligned 506; put into LDS as they come 695, by the larger tile 783),
+// 898 of 3140, 2202 outputs 37 us (3136 33; 56).
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
     const long long large = bf16 ? (long long)((a.tokens + 127) / 128) * ((a.outputs + 255) / 256) : (long long)((a.tokens + 63) / 64) * ((a.outputs + 191) / 192);
-    if (large >= 4LL * compute_units() && (!bf16 || linear_aligned(a))) {
-        if (bf16) launch_many<true, 8, 4, 1>(a, scales_of_block, stream);
-        else launch_many<false, 4, 3, 1>(a, scales_of_block, stream);
+    const bool aligned = linear_aligned(a);
+    if (large >= 4LL * compute_units() && (!bf16 || aligned)) {
+        if (bf16) launch_many<true, 8, 4, 1, false>(a, scales_of_block, stream);
+        else launch_many<false, 4, 3, 1, false>(a, scales_of_block, stream);
     } else if (linear_many_workgroups(a) > compute_units()) {
-        if (bf16) launch_many<true, 4, 2, 1>(a, scales_of_block, stream);
-        else launch_many<false, 4, 2, 1>(a, scales_of_block, stream);
+        if (!bf16) launch_many<false, 4, 2, 1, false>(a, scales_of_block, stream);
+        else if (aligned) launch_many<true, 4, 2, 1, false>(a, scales_of_block, stream);
+        else launch_many<true, 4, 2, 1, true>(a, scales_of_block, stream);
     } else {
-        if (bf16) launch_many<true, 4, 2, 2>(a, scales_of_block, stream);
-        else launch_many<false, 4, 2, 2>(a, scales_of_block, stream);
+        if (!bf16) launch_many<false, 4, 2, 2, false>(a, scales_of_block, stream);
+        else if (aligned) launch_many<true, 4, 2, 2, false>(a, scales_of_block, stream);
+        else launch_many<true, 4, 2, 2, true>(a, scales_of_block, stream);
     }
 }
 
