@@ -1,4 +1,6 @@
 // Products of weights held in 4 bits with many tokens (layout: qt_linear.h).
+#include <type_traits>
+
 #include "qt_linear.h"
 
 #define QT_LDS __attribute__((address_space(3)))
@@ -205,31 +207,35 @@ __global__ __launch_bounds__(SPLIT * kManyThreads, SPLIT == 1 && BF16 && MT == 4
 #pragma unroll
             for (int n = 0; n < N; ++n) sum[m][n] += s_sum[((wave * MT + m) * N + n) * 64 + lane];
     }
-    if constexpr (BF16) {
-        if ((first_tile + N) * kLinearOutputs <= a.outputs) {
-            // sixteen tokens at a time through LDS, so that a lane stores eight outputs side by side
-            constexpr int kRow = 16 * N + 8, kLanes = 2 * N;
-            uint16_t *const s_out = (uint16_t *)s_all[0] + wave * 16 * kRow;
-            float bias[N];
+    if ((first_tile + N) * kLinearOutputs <= a.outputs) {
+        // sixteen tokens at a time through LDS, so that a lane stores sixteen bytes of a token
+        typedef typename std::conditional<BF16, uint16_t, float>::type Number;
+        typedef typename std::conditional<BF16, Unaligned16, Unaligned16of4>::type Store;
+        constexpr int kEach = BF16 ? 8 : 4, kRow = 16 * N + kEach, kLanes = 16 * N / kEach;
+        Number *const s_out = (Number *)s_all[0] + wave * 16 * kRow;
+        float bias[N];
 #pragma unroll
-            for (int n = 0; n < N; ++n) bias[n] = linear_bias(a, (first_tile + n) * kLinearOutputs + (lane & 15));
+        for (int n = 0; n < N; ++n) bias[n] = linear_bias(a, (first_tile + n) * kLinearOutputs + (lane & 15));
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < MT; ++m) {
 #pragma unroll
-                for (int n = 0; n < N; ++n)
+            for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s_out[(4 * quarter + i) * kRow + 16 * n + (lane & 15)] = float_to_bf16_bits(sum[m][n][i] + bias[n]);
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-                for (int k = 0; k < 16 * kLanes / 64; ++k) {
-                    const int at = 64 * k + lane, token = first_token + 16 * m + at / kLanes, column = at % kLanes * 8;
-                    const qt_u32x4 y = *(const qt_u32x4 *)(s_out + at / kLanes * kRow + column);
-                    if (token < a.tokens) ((Unaligned16 *)((uint16_t *)a.out + token * a.out_stride + first_tile * kLinearOutputs + column))->v = y;
+                for (int i = 0; i < 4; ++i) {
+                    const float y = sum[m][n][i] + bias[n];
+                    if constexpr (BF16) s_out[(4 * quarter + i) * kRow + 16 * n + (lane & 15)] = float_to_bf16_bits(y);
+                    else s_out[(4 * quarter + i) * kRow + 16 * n + (lane & 15)] = y;
                 }
-                asm volatile("" ::: "memory");
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < 16 * kLanes / 64; ++k) {
+                const int at = 64 * k + lane, token = first_token + 16 * m + at / kLanes, column = at % kLanes * kEach;
+                const qt_u32x4 y = *(const qt_u32x4 *)(s_out + at / kLanes * kRow + column);
+                if (token < a.tokens) ((Store *)((Number *)a.out + token * a.out_stride + first_tile * kLinearOutputs + column))->v = y;
             }
-            return;
+            asm volatile("" ::: "memory");
         }
+        return;
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
