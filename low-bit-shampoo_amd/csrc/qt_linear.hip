@@ -75,12 +75,27 @@ __global__ __launch_bounds__(kCodeThreads) void linear_copy_kernel(const LinearC
                 const int first = 256 * pair + 128 * i + 32 * j + 8 * quarter;
                 const float scale = a.scales[(tile * a.segments + min(first / a.blocksize, a.segments - 1)) * kLinearOutputs + (lane & 15)];
                 const bf16x8 numbers = fp4_to_bf16(words[j]);
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = (float)numbers[e] * scale;
+                if (!there || first >= a.inputs) continue;
+                if (first + 8 <= a.inputs) {
+                    if constexpr (BF16) {
+                        ((Unaligned16 *)((uint16_t *)row + first))->v = (qt_u32x4){floats_to_bf16_pair(y[0], y[1]), floats_to_bf16_pair(y[2], y[3]), floats_to_bf16_pair(y[4], y[5]),
+                                                                                   floats_to_bf16_pair(y[6], y[7])};
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 8; h += 4)
+                            ((Unaligned16of4 *)((float *)row + first + h))->v =
+                                (qt_u32x4){__float_as_uint(y[h]), __float_as_uint(y[h + 1]), __float_as_uint(y[h + 2]), __float_as_uint(y[h + 3])};
+                    }
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const float y = (float)numbers[e] * scale;
-                    if (!there || first + e >= a.inputs) continue;
-                    if (BF16) ((uint16_t *)row)[first + e] = float_to_bf16_bits(y);
-                    else ((float *)row)[first + e] = y;
+                    if (first + e >= a.inputs) continue;
+                    if (BF16) ((uint16_t *)row)[first + e] = float_to_bf16_bits(y[e]);
+                    else ((float *)row)[first + e] = y[e];
                 }
             }
         }
@@ -209,7 +224,7 @@ void launch_few_long(const LinearArgs &a, int groups, hipStream_t stream) {
 }
 
 // Many tokens as soon as the kernel for them has a workgroup for seven of eight units: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 15.1 us here
-// and 25.8 there, 384 and 4096 (192) 22.0 and 26.1, 128 and 14336 (224) 29.4 and 26.9, in fp32 70.6 and 57.4.
+// and 22.2 there, 384 and 4096 (192) 21.0 and 22.4, 64 and 24000 (188) 24.7 and 22.4, in fp32 46.5 and 53.9, 54.7 and 53.8.
 // Its tile is of 64 tokens: 32 tokens, 128000 outputs 74 us here and 80 there, 33 126 and 80, in fp32 48 217 and 203, 32 147 and 188, one 67 and 213.
 // Else the smallest tile of a workgroup whose workgroups have a unit each: every one reads all of its tokens (from L2) and joins its waves, so
 // more of them than that cost more than they spread.  By tiles of outputs x tokens, before loads of tokens and joins were as they are: 16 tokens, 4096

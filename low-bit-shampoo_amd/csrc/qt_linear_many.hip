@@ -30,9 +30,9 @@ __device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &colu
 // numbers of the next block are on their way in registers.  They are exact in bf16, and scales multiply the sums of 64 inputs: four vector
 // operations beside every two matrix ones, and as many to expand the numbers, are what a wave does beside them.
 //
-// Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 506 us, 1070 TFLOP/s, where the
-// library's product of bf16 matrices takes 519 us; 1024 tokens through 4096 x 4096 43 us, 800 TFLOP/s; 2048 tokens through 11008 x 4096 in fp32 (three
-// matrix operations for each) 508 us, 364 TFLOP/s.  Four lanes side by side load a token's line: 547 us where sixteen tokens' lines were touched by each.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers), the
+// Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 460 us, 1175 TFLOP/s, where the
+// library's product of bf16 matrices takes 519 us; 1024 tokens through 4096 x 4096 39 us, 885 TFLOP/s; 2048 tokens through 11008 x 4096 in fp32 (three
+// matrix operations for each) 498 us, 371 TFLOP/s.  Results stored two bytes a lane: 510, 43 and 508 us.  Four lanes side by side load a token's line: 547 us where sixteen tokens' lines were touched by each.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers), the
 // matrix instructions at a higher priority, in groups with the vector ones, or one tile ahead of them (512 to 529 us beside 513: the pipes are busy all the time, at a clock that falls to
 // 2.0 GHz).
 //
@@ -271,9 +271,9 @@ long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.to
 // 64 x 128, as loads of tokens were then, 1024 tokens and 4096 outputs 101 and 43 us, 2048 and 11008 218 and 219, 6000 and 11008 545 and 634; in fp32 64 x 192 against 64 x 128,
 // 256 and 4096 99 and 80, 2048 and 11008 514 and 567.
 // With no more than one workgroup a unit, eight waves of it cover each other's loads: 512 tokens and 4096 outputs (256 workgroups) 26.9 us, of four waves 30.4, in fp32 58.7
-// and 74.5; 256 and 14336 (448) in fp32 112 and 97.6, as a unit's LDS holds one of them.
-// Rows that are not aligned are STAGED, and take the smaller tile: 6000 tokens of 4100 inputs, 11008 outputs 640 us (aligned 506; put into LDS as they come 695, by the larger tile 783),
-// 898 of 3140, 2202 outputs 37 us (3136 33; 56).
+// and 74.5; 256 and 14336 (448) in fp32 112 and 97.6, as a unit's LDS holds one of them (all with results stored two or four bytes a lane).
+// Rows that are not aligned are STAGED, and take the smaller tile: 6000 tokens of 4100 inputs, 11008 outputs 605 us (aligned 460; put into LDS as they come 60 more, by the larger tile 150),
+// 898 of 3140, 2202 outputs 33 us (3136 29).
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
     const long long large = bf16 ? (long long)((a.tokens + 127) / 128) * ((a.outputs + 255) / 256) : (long long)((a.tokens + 63) / 64) * ((a.outputs + 191) / 192);
     const bool aligned = linear_aligned(a);
