@@ -267,9 +267,9 @@ void launch_many(const LinearArgs &a, int scales_of_block, hipStream_t stream) {
 
 long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.tokens + 63) / 64) * ((a.outputs + 127) / 128); }
 
-// Large tiles use what they read more often, but leave units idle until there are four workgroups for each: 4096 inputs in bf16, 128 x 256 against
-// 64 x 128, as loads of tokens were then, 1024 tokens and 4096 outputs 101 and 43 us, 2048 and 11008 218 and 219, 6000 and 11008 545 and 634; in fp32 64 x 192 against 64 x 128,
-// 256 and 4096 99 and 80, 2048 and 11008 514 and 567.
+// Large tiles use what they read more often, but two of them fill a unit, and the last ones leave it half idle: from one and a half a unit on, in fp32 from three and a
+// half.  4096 inputs in bf16, 128 x 256 against 64 x 128, 1024 tokens and 11008 outputs (344 large) 104.8 and 100.5 us, 14336 (448) 112.4 and 120.9, 4096 and 4096 (512) 119 and
+// 137, 2048 and 11008 (688) 179 and 184.5; in fp32 64 x 192 against 64 x 128, 1024 and 4096 (352) 120 and 102, 8192 (688) 204 and 199.5, 11008 (928) 251 and 287.5.
 // With no more than one workgroup a unit, eight waves of it cover each other's loads: 512 tokens and 4096 outputs (256 workgroups) 26.9 us, of four waves 30.4, in fp32 58.7
 // and 74.5; 256 and 14336 (448) in fp32 112 and 97.6, as a unit's LDS holds one of them (all with results stored two or four bytes a lane).
 // Rows that are not aligned are STAGED, and take the smaller tile: 6000 tokens of 4100 inputs, 11008 outputs 605 us (aligned 460; put into LDS as they come 60 more, by the larger tile 150),
@@ -277,7 +277,7 @@ long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.to
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {
     const long long large = bf16 ? (long long)((a.tokens + 127) / 128) * ((a.outputs + 255) / 256) : (long long)((a.tokens + 63) / 64) * ((a.outputs + 191) / 192);
     const bool aligned = linear_aligned(a);
-    if (large >= 4LL * compute_units() && (!bf16 || aligned)) {
+    if (2 * large >= (bf16 ? 3LL : 7LL) * compute_units() && (!bf16 || aligned)) {
         if (bf16) launch_many<true, 8, 4, 1, false>(a, scales_of_block, stream);
         else launch_many<false, 4, 3, 1, false>(a, scales_of_block, stream);
     } else if (linear_many_workgroups(a) > compute_units()) {
