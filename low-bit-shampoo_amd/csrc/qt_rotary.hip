@@ -213,7 +213,7 @@ struct TurnWrite {
 
 // Bound by memory, with the places' look-up, cosines and sines in front of the first loads: the more heads a workgroup goes through, the less of
 // that, and tokens side by side in a head of the cache are written together.  9 prompts of up to 3500 tokens, 32 query heads, 8 of 128 in the cache, bf16:
-// 102 us for 397 MB, 3.9 TB/s, of which some 20 are cosines and sines of the keys' and of the queries' workgroups in 64 bits; turned, then written by two calls 114
+// 102 us for 397 MB, 3.9 TB/s, 9 us of them for cosines and sines in 64 bits (against the instructions for 32); turned, then written by two calls 114
 // (1 token of 32 sequences 5.8 and 9.2).  Tried: the first heads' loads in front of the places (registers: 125 us), keys' and queries' workgroups in turn (106),
 // more waves (105 to 194: registers), 16 tokens of the keys (105).
 template <bool BF16, bool LARGE>
