@@ -20,6 +20,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -191,16 +192,21 @@ PyObject *dequantize_checked(PyObject *const *args) {
 }
 
 // C++ exceptions (out of memory, a failed look-up) end here, with the interpreter's lock held: the caller's long way meets
-// the same one and raises it in torch's words.
+// the same one and raises it in torch's words.  Python's own go through: they come from hooks on what a gradient saves, which have been called by then, and may be
+// raised to be caught by whoever set them (a recomputed region ends in that way).
 template <PyObject *(*body)(PyObject *const *), Py_ssize_t COUNT>
 PyObject *guarded(PyObject *, PyObject *const *args, Py_ssize_t count) {
     if (count != COUNT || last_error == nullptr) Py_RETURN_NONE;
     try {
         return body(args);
+    } catch (python_error &e) {
+        e.restore();
+    } catch (pybind11::error_already_set &e) {
+        e.restore();
     } catch (...) {
-        PyErr_Clear();
-        Py_RETURN_NONE;
     }
+    if (PyErr_Occurred()) return nullptr;
+    Py_RETURN_NONE;
 }
 
 // bind(addresses): the sixteen entry points in the order of `entry`, the two of the error slot
@@ -649,8 +655,11 @@ PyObject *rotary_turn_checked(PyObject *const *args) {
         PyThreadState *state = PyEval_SaveThread();
         ~Unlocked() { PyEval_RestoreThread(state); }
     };
+    const bool saves = c10::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()));
+    // (what torch does not save: found out before hooks on the rest have been called)
+    if (saves && (angles.frequencies->is_inference() || positions.is_inference())) Py_RETURN_NONE;
     auto unlocked = std::make_unique<Unlocked>();
-    if (c10::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
+    if (saves) {
         const auto both = Turn::apply(q, k.defined() ? std::optional<at::Tensor>(k) : std::nullopt, positions, *angles.frequencies, angles.rotary.magnitude, (int64_t)angles.rotary.dims, angles.rotary.interleaved != 0, false);
         out = {both[0], both.size() > 1 ? both[1] : at::Tensor()};
     } else {
