@@ -54,6 +54,8 @@ bool in_memory(const at::Tensor &t, int device) {
            t.get_device() == device;
 }
 bool in_plain_memory(const at::Tensor &t, int device) { return in_memory(t, device) && t.is_contiguous(); }
+// Whether a derivative is asked for that a call without one would lose.
+bool differentiated(const at::Tensor &t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
 
 // A tensor that is itself (no subclass), in plain memory of the current GPU.
 const at::Tensor *plain(PyObject *obj, int device) {
@@ -301,7 +303,7 @@ const at::Tensor *vectors_of(PyObject *obj, const CacheCall &c, const at::Tensor
     const at::Tensor &t = THPVariable_Unpack(obj);
     if (!in_memory(t, c.device) || t.dim() != 3 || slot_of(t.scalar_type()) < 0 || t.size(2) != c.cache.head_dim || (t.size(2) > 1 && t.stride(2) != 1)) return nullptr;
     if ((like != nullptr && t.scalar_type() != like->scalar_type()) || (tokens >= 0 && t.size(0) != tokens) || (heads >= 0 && t.size(1) != heads)) return nullptr;
-    if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;
+    if (differentiated(t)) return nullptr;
     out = {t.data_ptr(), slot_of(t.scalar_type()), t.stride(0), t.stride(1)};
     return &t;
 }
@@ -538,14 +540,13 @@ PyObject *linear_product_checked(PyObject *const *args) {
         Py_RETURN_NONE;
     if (!THPVariable_CheckExact(args[5])) Py_RETURN_NONE;
     const at::Tensor &x = THPVariable_Unpack(args[5]);
-    if (!in_memory(x, device) || slot_of(x.scalar_type()) < 0 || x.dim() < 1 || x.size(-1) != inputs || (x.requires_grad() && c10::GradMode::is_enabled())) Py_RETURN_NONE;
+    if (!in_memory(x, device) || slot_of(x.scalar_type()) < 0 || x.dim() < 1 || x.size(-1) != inputs || differentiated(x)) Py_RETURN_NONE;
     if (x.dim() == 2 ? inputs > 1 && x.stride(1) != 1 : !x.is_contiguous()) Py_RETURN_NONE;
     const long long tokens = x.numel() / inputs;
     const at::Tensor *bias = nullptr;
     if (args[6] != Py_None) {
         bias = plain(args[6], device);
-        if (bias == nullptr || bias->numel() != outputs || (bias->scalar_type() != at::kFloat && bias->scalar_type() != x.scalar_type()) ||
-            (bias->requires_grad() && c10::GradMode::is_enabled()))
+        if (bias == nullptr || bias->numel() != outputs || (bias->scalar_type() != at::kFloat && bias->scalar_type() != x.scalar_type()) || differentiated(*bias))
             Py_RETURN_NONE;
     }
     at::Tensor out;
@@ -556,7 +557,7 @@ PyObject *linear_product_checked(PyObject *const *args) {
         if (!in_plain_memory(out, device)) Py_RETURN_NONE;
     } else {
         const at::Tensor *given = plain(args[7], device);
-        if (given == nullptr || given->scalar_type() != x.scalar_type() || given->dim() != x.dim() || given->size(-1) != outputs || !apart(*given, x) ||
+        if (given == nullptr || given->scalar_type() != x.scalar_type() || given->dim() != x.dim() || given->size(-1) != outputs || differentiated(*given) || !apart(*given, x) ||
             (bias != nullptr && !apart(*given, *bias)))
             Py_RETURN_NONE;
         for (int64_t d = 0; d + 1 < x.dim(); ++d)

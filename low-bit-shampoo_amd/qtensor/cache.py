@@ -323,8 +323,7 @@ class QTensorCache:
                              + (f" = {shape}." if min(shape) >= 0 else "."))
         if t.shape[2] > 1 and t.stride(2) != 1:
             raise ValueError(f"the last dimension of {name} must be contiguous.")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} requires a gradient, and a cache held in 4 bits has none: call it under torch.no_grad().")
+        F._check_derivatives("a cache", **{name: t})
 
     def _places(self, table: Tensor, lengths: Tensor, starts: Optional[Tensor], tokens: int) -> _Places:
         batch = lengths.numel()

@@ -172,6 +172,13 @@ def _check_buffer(t: Tensor, name: str, numel: int, dtype: torch.dtype, device: 
         raise ValueError(f"{name} must be contiguous.")
 
 
+def _check_derivatives(held: str, **tensors: Optional[Tensor]) -> None:
+    """Refuses tensors of a call without derivatives that ask for one."""
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires a gradient, which {held} held in 4 bits cannot give: call it under torch.no_grad().")
+
+
 def _overlap(a: Tensor, b: Tensor) -> bool:
     """Whether the memory between the first and the last element of two tensors meets."""
     def span(t):

@@ -101,8 +101,7 @@ class QTensorLinear:
         F._dtype_slot(x.dtype, "x")
         if x.dim() < 1 or x.shape[-1] != self.inputs:
             raise ValueError(f"x has shape {tuple(x.shape)}, expected [.., {self.inputs}].")
-        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-            raise RuntimeError("x or bias requires a gradient, and weights held in 4 bits have none: call it under torch.no_grad().")
+        F._check_derivatives("weights", x=x, bias=bias, out=out)
         rows = x if x.dim() == 2 else x.reshape(-1, self.inputs)
         self._check(rows, "x", (rows.shape[0], self.inputs), x.dtype)
         if bias is not None:
