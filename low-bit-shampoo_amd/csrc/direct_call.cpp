@@ -54,8 +54,10 @@ bool in_memory(const at::Tensor &t, int device) {
            t.get_device() == device;
 }
 bool in_plain_memory(const at::Tensor &t, int device) { return in_memory(t, device) && t.is_contiguous(); }
+// A forward-mode derivative (torch.autograd.forward_ad): an ordinary tensor carries it, whatever the mode of gradients is.
+bool has_tangent(const at::Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
 // Whether a derivative is asked for that a call without one would lose.
-bool differentiated(const at::Tensor &t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+bool differentiated(const at::Tensor &t) { return (t.requires_grad() && c10::GradMode::is_enabled()) || has_tangent(t); }
 
 // A tensor that is itself (no subclass), in plain memory of the current GPU.
 const at::Tensor *plain(PyObject *obj, int device) {
@@ -581,7 +583,7 @@ PyObject *linear_product_checked(PyObject *const *args) {
 bool turn_fits(const at::Tensor &t, const at::Tensor &first, int device, long long dims) {
     return in_memory(t, device) && t.scalar_type() == first.scalar_type() && slot_of(t.scalar_type()) >= 0 && (t.dim() == 3 || t.dim() == 4) && t.dim() == first.dim() &&
            t.size(-1) == first.size(-1) && t.size(-3) == first.size(-3) && t.size(0) == first.size(0) && t.size(-1) >= dims && t.size(-1) <= 1024 && t.size(-2) >= 1 &&
-           t.size(-2) <= 32767 && t.stride(-1) == 1;
+           t.size(-2) <= 32767 && t.stride(-1) == 1 && !has_tangent(t);
 }
 bool positions_fit(const at::Tensor &p, const at::Tensor &first, int device) {
     if (!in_memory(p, device) || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong) || p.dim() < 1 || p.dim() > first.dim() - 2) return false;

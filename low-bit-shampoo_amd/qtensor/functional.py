@@ -22,6 +22,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from qtensor.cextension import get_lib
 
@@ -173,10 +174,15 @@ def _check_buffer(t: Tensor, name: str, numel: int, dtype: torch.dtype, device: 
 
 
 def _check_derivatives(held: str, **tensors: Optional[Tensor]) -> None:
-    """Refuses tensors of a call without derivatives that ask for one."""
+    """Refuses tensors of a call without derivatives that ask for one: a gradient, or a forward-mode one (its tangent would be lost, and torch.no_grad() does
+    not stop it)."""
     for name, t in tensors.items():
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if t is None:
+            continue
+        if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError(f"{name} requires a gradient, which {held} held in 4 bits cannot give: call it under torch.no_grad().")
+        if forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} carries a forward-mode tangent, which {held} held in 4 bits cannot pass on: give its primal.")
 
 
 def _overlap(a: Tensor, b: Tensor) -> bool:

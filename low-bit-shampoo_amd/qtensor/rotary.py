@@ -91,7 +91,8 @@ class Rotary:
     def turn(self, q: Tensor, k: Optional[Tensor], positions: Tensor) -> Tuple[Tensor, Optional[Tensor]]:
         """(q, k) turned: [.., tokens, heads, head_dim] with at most one dimension in front (fp32 or bf16, the last dimension contiguous),
         heads of both may differ in number; k may be None.  positions: int32 or int64 [tokens] or [batch, tokens], any values.  The
-        gradients of q and k are theirs turned back."""
+        gradients of q and k are theirs turned back, in reverse mode and of every order; forward mode, torch.func's transformations and batched
+        gradients (is_grads_batched) raise."""
         if F._direct is not None:
             done = F._direct.rotary_turn(self.frequencies, self.magnitude, self.dims, self.interleaved, q, k, positions)
             if done is not None:
