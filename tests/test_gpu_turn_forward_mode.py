@@ -74,3 +74,19 @@ def test_the_cache_refuses_tangents(route):
         assert not cache.codes.any() and not totals.any()           # (nothing was launched)
         cache.write(k, k, table, lengths)
         assert cache.codes.any() and torch.allclose(cache.attend(q, table, lengths)[:, :2], k)
+
+
+def test_other_transformations_raise(route):
+    """Not lost: gradients by torch.func, batched calls and batched gradients."""
+    from qtensor.rotary import Rotary
+    rotary, q, at = Rotary(32), torch.ones(5, 4, 64, device="cuda"), torch.arange(5, device="cuda")
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda q: rotary.turn(q, None, at)[0].sum())(q)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda q: rotary.turn(q, None, at)[0], (q,), (q,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda q: rotary.turn(q, None, at)[0])(q.expand(3, 5, 4, 64))
+    leaf = q.clone().requires_grad_()
+    out = rotary.turn(leaf, None, at)[0]
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaf, torch.ones(3, 5, 4, 64, device="cuda"), is_grads_batched=True)
