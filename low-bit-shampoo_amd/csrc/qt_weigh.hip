@@ -269,7 +269,21 @@ __device__ __forceinline__ float2 join_parts(float2 x, float2 y) {
     return make_float2(m, x.y * __builtin_amdgcn_exp2f(x.x - by) + y.y * __builtin_amdgcn_exp2f(y.x - by));
 }
 
+// Whether a row's query has an infinite element: its scores are infinities of either sign or NaN, and the formula's weights NaN; minus infinities alone would pass for
+// tokens that are not seen.  Looked for where a row has nothing else (infinities made NaN in front of the products cost 2 % of a call).
+template <bool BF16>
+__device__ __forceinline__ bool row_is_infinite(const WeighArgs &a, const WeighSequence &v, int head, int row) {
+    const int i = (int)fastdiv((uint32_t)row, a.by_group);
+    const uint8_t *p = (const uint8_t *)a.q + ((v.start + i) * a.q_token + (head * a.group + row - i * a.group) * a.q_head) * (BF16 ? 2 : 4);
+    bool found = false;
+#pragma unroll 1
+    for (int d = 0; d < a.shape.head_dim; ++d)
+        found = found || (BF16 ? (((const uint16_t *)p)[d] & 0x7fffu) == 0x7f80u : (((const uint32_t *)p)[d] & 0x7fffffffu) == 0x7f800000u);
+    return found;
+}
+
 // (m, 1 / l) of the row `first_row` + lane % 16, from its parts; (0, 0) where nothing is seen, (infinity, 0) behind the last row.
+template <bool BF16>
 __device__ __forceinline__ float2 row_statistics(const WeighArgs &a, const WeighSequence &v, int head, int first_row) {
     const int lane = threadIdx.x & 63, quarter = lane >> 4, row = first_row + (lane & 15);
     float m = -INFINITY, l = 0.0f;
@@ -291,6 +305,7 @@ __device__ __forceinline__ float2 row_statistics(const WeighArgs &a, const Weigh
     m = quarters_max(m);
     m = m == -INFINITY ? 0.0f : m;
     l = quarters_sum(l * __builtin_amdgcn_exp2f(mine - m));
+    if (l == 0.0f && row < v.count * a.group && row_is_infinite<BF16>(a, v, head, row)) l = NAN;
     return row < v.count * a.group ? make_float2(m, l == 0.0f ? 0.0f : 1.0f / l) : make_float2(INFINITY, 0.0f);
 }
 
@@ -438,7 +453,7 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
     for (int r = 0; r < T; ++r) q[r].arrange();
     float m[T][4], l[T][4];             // WEIGHTS: 1 / l
     if constexpr (WEIGHTS) {
-        const float2 part = row_statistics(a, v, head, first_row);
+        const float2 part = row_statistics<BF16>(a, v, head, first_row);
 #pragma unroll
         for (int i = 0; i < 4; ++i) m[0][i] = __shfl(part.x, 4 * quarter + i, 64), l[0][i] = __shfl(part.y, 4 * quarter + i, 64);
     } else {
@@ -540,6 +555,8 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
             float2 part = s_part[0][threadIdx.x];
 #pragma unroll
             for (int w = 1; w < kWeighWaves; ++w) part = join_parts(part, s_part[w][threadIdx.x]);
+            // (a token of each sequence: when the parts are joined)
+            if (!(BF16 && T == 1) && part.x == -INFINITY && row_is_infinite<BF16>(a, v, head, first_row + (int)threadIdx.x)) part.y = NAN;
             put(part);
         }
     }
@@ -547,6 +564,7 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
 
 // Weights of the only token of a sequence from its scores: four tokens a thread.  Bound by latency, length to scores: 9.3 us for the step above, whose 25 MB
 // are 5 us at a copy's rate; 10.5 with the statistics in front of the loads.
+template <bool BF16>
 __global__ __launch_bounds__(kWeighThreads) void weigh_scores_kernel(const WeighArgs a) {
     __shared__ float2 s_row[16];
     const int head = blockIdx.y, b = blockIdx.z, first = (int)blockIdx.x * 4 * kWeighThreads;
@@ -570,7 +588,7 @@ __global__ __launch_bounds__(kWeighThreads) void weigh_scores_kernel(const Weigh
         before = ((const Unaligned16of4 *)total)->v;
     }
     if (threadIdx.x < 64) {
-        const float2 row = row_statistics(a, v, head, 0);
+        const float2 row = row_statistics<BF16>(a, v, head, 0);
         if (threadIdx.x < 16) s_row[threadIdx.x] = row;
     }
     __syncthreads();
@@ -894,7 +912,7 @@ void launch_weigh(WeighArgs a, bool few, hipStream_t stream) {
         launch_rows<BF16, STEPS, 1>(a, work, stream);
         if (a.scores) {
             const dim3 grid((unsigned)((covered + 4 * kWeighThreads - 1) / (4 * kWeighThreads)), a.shape.kv_heads, a.at.batch);
-            hipLaunchKernelGGL(weigh_scores_kernel, grid, dim3(kWeighThreads), 0, stream, a);
+            hipLaunchKernelGGL(weigh_scores_kernel<BF16>, grid, dim3(kWeighThreads), 0, stream, a);
         } else
             hipLaunchKernelGGL((weigh_rows_kernel<BF16, STEPS, 1, true>), work, dim3(kWeighThreads), 0, stream, a);
         return;
