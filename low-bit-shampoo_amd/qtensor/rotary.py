@@ -13,6 +13,7 @@ position * frequencies[p]: (a, b) becomes (a c - b s, b c + a s), c and s the fp
 the angle, which is worked out in 64 bits (in fp32 a position of 10^5 leaves it two digits).  Products and their sum are rounded to fp32, the
 result to its type; the elements behind `dims` stay as they are.
 """
+import copy
 import ctypes as ct
 import math
 from typing import Optional, Sequence, Tuple, Union
@@ -153,18 +154,24 @@ def _check_positions(positions: Tensor, device, shapes) -> None:
 class _Turn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rotary, back, q, k, positions):
-        ctx.rotary, ctx.back = rotary, back
+        # (its angles are kept as they are now, frequencies by torch, or where they were made in inference mode, which it does not save, as a copy)
+        speed = rotary.frequencies
+        ctx.rotary, ctx.back = copy.copy(rotary), back
+        ctx.rotary.frequencies = speed.clone() if speed.is_inference() else None
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions)
+        ctx.save_for_backward(positions, *([] if speed.is_inference() else [speed]))
         out = rotary._turned(back, [q] if k is None else [q, k], positions)
         return out[0], out[1] if k is not None else None
 
     @staticmethod
     def backward(ctx, dq, dk):
-        positions, = ctx.saved_tensors
+        rotary = copy.copy(ctx.rotary)
+        positions, *frequencies = ctx.saved_tensors
+        if frequencies:
+            rotary.frequencies, = frequencies
         wanted = [d if d is not None and need else None for d, need in zip((dq, dk), ctx.needs_input_grad[2:4])]
         given = [d if d.stride(-1) == 1 else d.contiguous() for d in wanted if d is not None]
         if not given:
             return None, None, None, None, None
-        turned = list(_Turn.apply(ctx.rotary, not ctx.back, given[0], given[1] if len(given) > 1 else None, positions))
+        turned = list(_Turn.apply(rotary, not ctx.back, given[0], given[1] if len(given) > 1 else None, positions))
         return None, None, *(turned.pop(0) if d is not None else None for d in wanted), None
