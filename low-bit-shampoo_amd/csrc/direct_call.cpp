@@ -28,6 +28,7 @@
 #include <array>
 #include <climits>
 #include <cmath>
+#include <initializer_list>
 #include <memory>
 #include <optional>
 #include <utility>
@@ -74,6 +75,9 @@ bool watched() {
                                              K::FuncTorchDynamicLayerBackMode});
     return c10::impl::tls_local_dispatch_key_set().included_.has_any(levels) || at::impl::torch_function_mode_enabled();
 }
+
+// Whether a tensor has the shape that it was made with: as many elements in another order are not what the kernels read.
+bool shaped(const at::Tensor &t, std::initializer_list<int64_t> sizes) { return t.sizes() == at::IntArrayRef(sizes.begin(), sizes.size()); }
 
 // A buffer of `numel` elements: false where what is given does not fit; made if nothing is given.
 bool buffer(PyObject *given, int device, long long numel, at::ScalarType type, const at::TensorOptions &like, at::Tensor &out) {
@@ -266,10 +270,9 @@ bool cache_of(PyObject *const *args, CacheCall &c) {
         return false;
     if (page_size < 16 || page_size > 4096 || heads < 1 || heads > 32767 || dim < 1 || dim > 256 || (blocksize != 64 && blocksize != 128 && blocksize != 256))
         return false;
-    if (codes->scalar_type() != at::kByte || scales->scalar_type() != at::kFloat || codes->dim() != 5 || scales->dim() != 5) return false;
+    if (codes->scalar_type() != at::kByte || scales->scalar_type() != at::kFloat || codes->dim() != 5) return false;
     const long long pages = codes->size(1), row = 16 * ((dim + 31) / 32), segments = (dim + blocksize - 1) / blocksize;
-    if (pages < 1 || pages > INT_MAX || codes->numel() != 2 * pages * heads * page_size * row || scales->numel() != 2 * pages * heads * page_size * segments)
-        return false;
+    if (pages < 1 || pages > INT_MAX || !shaped(*codes, {2, pages, heads, page_size, row}) || !shaped(*scales, {2, pages, heads, segments, page_size})) return false;
     auto *bytes = static_cast<unsigned char *>(codes->data_ptr());
     auto *floats = static_cast<float *>(scales->data_ptr());
     c.cache = {{bytes, bytes + codes->numel() / 2}, {floats, floats + scales->numel() / 2}, (int)pages, (int)page_size, (int)heads, (int)dim, (int)blocksize};
@@ -403,7 +406,7 @@ bool angles_of(PyObject *const *args, int device, long long most, Angles &a) {
     long long dims;
     a.frequencies = plain(args[0], device);
     if (a.frequencies == nullptr || !PyFloat_CheckExact(args[1]) || !whole(args[2], dims) || !PyBool_Check(args[3])) return false;
-    if (dims < 2 || dims % 2 != 0 || dims > most || a.frequencies->scalar_type() != at::kDouble || a.frequencies->numel() != dims / 2) return false;
+    if (dims < 2 || dims % 2 != 0 || dims > most || a.frequencies->scalar_type() != at::kDouble || !shaped(*a.frequencies, {dims / 2})) return false;
     a.rotary = {static_cast<const double *>(a.frequencies->data_ptr()), PyFloat_AS_DOUBLE(args[1]), (int)dims, args[3] == Py_True, 0};
     return true;
 }
@@ -537,8 +540,8 @@ PyObject *linear_product_checked(PyObject *const *args) {
     if (codes == nullptr || scales == nullptr || !whole(args[2], inputs) || !whole(args[3], outputs) || !whole(args[4], blocksize)) Py_RETURN_NONE;
     if (inputs < 1 || inputs > 1 << 24 || outputs < 1 || outputs > 1 << 24 || (blocksize != 64 && blocksize != 128 && blocksize != 256)) Py_RETURN_NONE;
     const long long tiles = (outputs + 15) / 16;
-    if (codes->scalar_type() != at::kByte || scales->scalar_type() != at::kFloat || codes->numel() != tiles * ((inputs + 127) / 128) * 1024 ||
-        scales->numel() != tiles * ((inputs + blocksize - 1) / blocksize) * 16)
+    if (codes->scalar_type() != at::kByte || scales->scalar_type() != at::kFloat || !shaped(*codes, {tiles, (inputs + 127) / 128, 1024}) ||
+        !shaped(*scales, {tiles, (inputs + blocksize - 1) / blocksize, 16}))
         Py_RETURN_NONE;
     if (!THPVariable_CheckExact(args[5])) Py_RETURN_NONE;
     const at::Tensor &x = THPVariable_Unpack(args[5]);
