@@ -306,10 +306,16 @@ extern "C" void qtensor_hip_linear_product(const qtensor_linear *weights, const 
     }
     if (call->tokens == 0) return;
     const int blocks = (weights->inputs + kLinearInputs - 1) / kLinearInputs;
-    const LinearArgs a = {weights->codes, weights->scales, call->x, call->bias, call->out, call->x_stride, call->out_stride, (int)call->tokens, weights->inputs, weights->outputs,
-                          blocks, (weights->inputs + weights->blocksize - 1) / weights->blocksize, weights->blocksize == 256, call->bias_is_bf16 != 0};
     const int groups = weights->blocksize == 64 ? 2 : 1;
-    if (call->is_bf16) launch_product<true>(a, groups, (hipStream_t)stream);
-    else launch_product<false>(a, groups, (hipStream_t)stream);
-    launch_ok(what);
+    // (a launch takes less than 2^24 workgroups, of 64 tokens and up to 256 outputs)
+    const long long most = 1LL << 24;
+    for (long long first = 0; first < call->tokens; first += most) {
+        const long long tokens = call->tokens - first < most ? call->tokens - first : most;
+        const LinearArgs a = {weights->codes, weights->scales, (const uint8_t *)call->x + first * call->x_stride * size, call->bias, (uint8_t *)call->out + first * call->out_stride * size,
+                              call->x_stride, call->out_stride, (int)tokens, weights->inputs, weights->outputs, blocks,
+                              (weights->inputs + weights->blocksize - 1) / weights->blocksize, weights->blocksize == 256, call->bias_is_bf16 != 0};
+        if (call->is_bf16) launch_product<true>(a, groups, (hipStream_t)stream);
+        else launch_product<false>(a, groups, (hipStream_t)stream);
+        if (!launch_ok(what)) return;
+    }
 }

@@ -91,8 +91,8 @@ class QTensorLinear:
 
     def product(self, x: Tensor, bias: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
         """W x + bias for every token: x [.., inputs] (fp32 or bf16) -> [.., outputs] of its type; bias [outputs] of fp32 or x's type.  Products are
-        exact and summed in fp32, the result is rounded once.  out: optional result, contiguous, that shares no memory with x or bias.  Any number of
-        tokens; sums in front of the scales, so up to 768 of x's largest magnitude, have to stay below 2^128."""
+        exact and summed in fp32, the result is rounded once.  out: optional result, contiguous, that shares no memory with x or bias.  Up to
+        2^31 - 256 tokens; sums in front of the scales, so up to 768 of x's largest magnitude, have to stay below 2^128."""
         if F._direct is not None:
             done = F._direct.linear_product(self.codes, self.scales, self.inputs, self.outputs, self.blocksize, x, bias, out)
             if done is not None:
