@@ -225,7 +225,8 @@ void launch_few_long(const LinearArgs &a, int groups, hipStream_t stream) {
 
 // Many tokens as soon as the kernel for them has a workgroup for seven of eight units: 4096 inputs in bf16, 256 tokens and 4096 outputs (128 workgroups) 15.1 us here
 // and 22.2 there, 384 and 4096 (192) 21.0 and 22.4, 64 and 24000 (188) 24.7 and 22.4, in fp32 46.5 and 53.9, 54.7 and 53.8.
-// Its tile is of 64 tokens: 32 tokens, 128000 outputs 74 us here and 80 there, 33 126 and 80, in fp32 48 217 and 203, 32 147 and 188, one 67 and 213.
+// Its tile is of 64 tokens: 32 tokens, 128000 outputs 74 us here and 80 there, 33 126 and 80, one in fp32 67 and 213; in fp32 from 48 on: 40 tokens 215 and 228, 48 218
+// and 198, 50000 outputs 91 and 107, 92 and 94, 28672 outputs 53 and 65, 54 and 53 (1000 inputs, 128000 outputs 33 77 and 56, 48 80 and 52).
 // Else the smallest tile of a workgroup whose workgroups have a unit each: every one reads all of its tokens (from L2) and joins its waves, so
 // more of them than that cost more than they spread.  By tiles of outputs x tokens, before loads of tokens and joins were as they are: 16 tokens, 4096
 // outputs 1 x 1 6.7 us, 2 x 1 7.9, 4 x 1 10.1; 14336 outputs 18.3, 12.6, 10.5; 64 tokens, 4096 outputs 4 x 1 10.5, 4 x 2 15.4; as they are, 64 tokens, 11008
@@ -235,7 +236,7 @@ void launch_few_long(const LinearArgs &a, int groups, hipStream_t stream) {
 template <bool BF16>
 void launch_product(const LinearArgs &a, int groups, hipStream_t stream) {
     const long long tiles = (a.outputs + 15) / 16, rows = (a.tokens + 15) / 16, units = compute_units();
-    if (a.tokens > (BF16 ? 32 : 48) && 8 * linear_many_workgroups(a) >= 7 * units) return launch_linear_many(a, BF16, groups, stream);
+    if (a.tokens >= (BF16 ? 33 : 48) && 8 * linear_many_workgroups(a) >= 7 * units) return launch_linear_many(a, BF16, groups, stream);
     if (tiles * rows <= units) return launch_few_long<BF16, 1, 16>(a, groups, stream);
     if ((tiles + 1) / 2 * rows <= units) return launch_few_long<BF16, 2, BF16 ? 8 : 16>(a, groups, stream);
     if ((tiles + 3) / 4 * rows <= units) return launch_few_long<BF16, 4, BF16 ? 8 : 16>(a, groups, stream);

@@ -12,7 +12,7 @@ pytestmark = pytest.mark.gpu
 # (outputs that take all routes of a product: few tokens with one, two, four and eight tiles of outputs to a workgroup, eight and sixteen waves, many with inputs shared by
 # halves of a workgroup, by one, and in large tiles)
 @pytest.mark.parametrize("tokens,inputs,outputs", [(1, 130, 33), (5, 300, 64), (8, 2100, 40), (9, 128, 16), (16, 300, 4096), (16, 2200, 8100), (16, 130, 16300), (13, 300, 20000),
-                                                   (40, 257, 4000), (48, 2177, 500), (256, 300, 7168), (300, 129, 5800), (512, 385, 4400), (1024, 260, 10900)])
+                                                   (40, 257, 4000), (47, 300, 28700), (48, 300, 28700), (48, 2177, 500), (256, 300, 7168), (300, 129, 5800), (512, 385, 4400), (1024, 260, 10900)])
 @pytest.mark.parametrize("blocksize", [64, 128, 256])
 @pytest.mark.parametrize("aligned", [True, False])
 def test_products(tokens, inputs, outputs, blocksize, aligned):
