@@ -14,7 +14,6 @@ namespace qt {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float fp4_f32x4 __attribute__((ext_vector_type(4)));
-typedef float fp4_f32x2 __attribute__((ext_vector_type(2)));
 
 // Numbers of N (4 or 8) elements of a segment whose largest magnitude has the bits `top` (NaN above infinity, so that a segment
 // with a NaN gets a NaN for its scale and reads as NaN): scale and quotients by correctly rounded division (qt_divide.h;
@@ -57,7 +56,8 @@ struct __attribute__((packed, aligned(2))) Unaligned16 { qt_u32x4 v; };
 struct __attribute__((packed, aligned(4))) Unaligned16of4 { qt_u32x4 v; };
 
 // An operand of eight elements as it lies in memory, and as the bf16 pieces that the matrix instructions multiply: one, or three whose
-// sum is the fp32 number (each piece cuts off eight bits, so every difference is exact; a number that is not finite is its first piece).
+// sum is the fp32 number (each piece cuts off eight bits, so every difference is exact; a number that is not finite is its first piece; bf16 ends at 2^-133,
+// and what an fp32 number has behind that is lost).
 template <bool BF16>
 struct Eight {
     static constexpr int kPieces = BF16 ? 1 : 3;

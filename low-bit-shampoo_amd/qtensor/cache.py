@@ -228,7 +228,8 @@ class QTensorCache:
               window: Optional[int] = None, sinks: int = 0) -> Tensor:
         """Adds to totals (fp32 [batch, kv_heads, n], n at least what the table has room for) the weights softmax(scale q k) that `attend`, called with the
         same arguments, multiplies values with: for every token of a sequence and head of the cache the sum over the call's queries and over the query
-        heads that read the head.  Sums are in fp32, in one order.  Returns totals."""
+        heads that read the head.  Sums are in fp32, in one order; six times a query's elements, added up, have to stay below 2^128, and what an fp32 query
+        has of bits below 2^-133 is cut off.  Returns totals."""
         if _native is not None:
             done = _native.cache_weigh(self.codes, self.scales, self.page_size, self.kv_heads, self.head_dim, self.blocksize, totals, q, table, lengths,
                                        starts, scale, window, sinks)

@@ -2,8 +2,9 @@
 
 No counterpart exists in the reference, whose low-bit tensors are the state of an optimizer; this is the attention cache's format
 (qtensor.cache) for the weights that a trained model generates with: segments of inputs, an fp32 scale each, 4 bits per weight.
-A step of generation is bound by reading its weights, and reads 0.56 bytes of each here; products are exact and summed in fp32, so the
-only error beside the result's rounding is that of the weights' 4 bits.  Everything runs on the GPU through libqtensor_hip.so, on
+A step of generation is bound by reading its weights, and reads 0.56 bytes of each here; products are exact and summed in fp32, so
+beside the weights' 4 bits and the result's rounding there are only the roundings of these sums, 2^-24 of the products' magnitudes added up for each step
+in them.  Everything runs on the GPU through libqtensor_hip.so, on
 torch's current stream.
 
     weights = QTensorLinear(inputs, outputs)
@@ -92,7 +93,8 @@ class QTensorLinear:
     def product(self, x: Tensor, bias: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
         """W x + bias for every token: x [.., inputs] (fp32 or bf16) -> [.., outputs] of its type; bias [outputs] of fp32 or x's type.  Products are
         exact and summed in fp32, the result is rounded once.  out: optional result, contiguous, that shares no memory with x or bias.  Up to
-        2^31 - 256 tokens; sums in front of the scales, so up to 768 of x's largest magnitude, have to stay below 2^128."""
+        2^31 - 256 tokens; sums in front of the scales, so up to 768 of x's largest magnitude, have to stay below 2^128, and
+        what an fp32 x has of bits below 2^-133 is cut off."""
         if F._direct is not None:
             done = F._direct.linear_product(self.codes, self.scales, self.inputs, self.outputs, self.blocksize, x, bias, out)
             if done is not None:

@@ -33,6 +33,20 @@ def test_products(tokens, inputs, outputs, blocksize, aligned):
         assert bool((off <= limit).all()), f"elements from {first} on: off by {float((off / limit.clamp(min=1e-300)).max()):.3g} of the bound"
 
 
+@pytest.mark.parametrize("power", [-100, -118, -126, -140])
+@pytest.mark.parametrize("tokens,outputs", [(16, 64), (512, 4400)])
+def test_products_of_tokens_so_small_that_pieces_end(power, tokens, outputs):
+    """bf16 ends at 2^-133: an element loses what it has behind that, times a number and its scale."""
+    from qtensor.linear import QTensorLinear
+    w = torch.randn(outputs, 128, generator=torch.Generator().manual_seed(1)) * 2.0 ** 100
+    held = C.held(w, 64)
+    x, where = A.one_each(tokens, 128, 3, seed=4)
+    x *= 2.0 ** power
+    want, limit = A.product(x, where, held)
+    off = (QTensorLinear(128, outputs).quantize(w.cuda()).product(x.cuda()).double().cpu() - want).abs()
+    assert bool((off <= limit + 2.0 ** -133 * held[:, where].T.abs()).all())
+
+
 def placed(lengths, kv_heads, dim, blocksize, wide=0):
     from qtensor.cache import QTensorCache
     width = -(-max(lengths) // 16)
