@@ -30,11 +30,11 @@ __device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &colu
 // numbers of the next block are on their way in registers.  They are exact in bf16, and scales multiply the sums of 64 inputs: four vector
 // operations beside every two matrix ones, and as many to expand the numbers, are what a wave does beside them.
 //
-// Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 460 us, 1175 TFLOP/s, where the
+// Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 449 to 462 us, 1170 to 1200 TFLOP/s, where the
 // library's product of bf16 matrices takes 519 us; 1024 tokens through 4096 x 4096 39 us, 885 TFLOP/s; 2048 tokens through 11008 x 4096 in fp32 (three
 // matrix operations for each) 498 us, 371 TFLOP/s.  Results stored two bytes a lane: 510, 43 and 508 us.  Four lanes side by side load a token's line: 547 us where sixteen tokens' lines were touched by each.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers), the
-// matrix instructions at a higher priority, in groups with the vector ones, or one tile ahead of them (512 to 529 us beside 513: the pipes are busy all the time, at a clock that falls to
-// 2.0 GHz).
+// matrix instructions at a higher priority, in groups with the vector ones, or one tile ahead of them (512 to 529 us beside 513).  Of all cycles, at a clock that falls to 2.0 GHz, matrix instructions take 53 % and vector ones 55 %, in the
+// 1.8 waves that a SIMD has on average.
 //
 // STAGED: tokens on their way in registers while a block is multiplied, for rows of bf16 that are not aligned to sixteen bytes.
 // SPLIT: two times four waves, which take the blocks of 128 inputs in turn and join their sums through LDS.
@@ -270,8 +270,8 @@ long long linear_many_workgroups(const LinearArgs &a) { return (long long)((a.to
 // Large tiles use what they read more often, but two of them fill a unit, and the last ones leave it half idle: from one and a half a unit on, in fp32 from three and a
 // half.  4096 inputs in bf16, 128 x 256 against 64 x 128, 1024 tokens and 11008 outputs (344 large) 104.8 and 100.5 us, 14336 (448) 112.4 and 120.9, 4096 and 4096 (512) 119 and
 // 137, 2048 and 11008 (688) 179 and 184.5; in fp32 64 x 192 against 64 x 128, 1024 and 4096 (352) 120 and 102, 8192 (688) 204 and 199.5, 11008 (928) 251 and 287.5.
-// With no more than one workgroup a unit, eight waves of it cover each other's loads: 512 tokens and 4096 outputs (256 workgroups) 26.9 us, of four waves 30.4, in fp32 58.7
-// and 74.5; 256 and 14336 (448) in fp32 112 and 97.6, as a unit's LDS holds one of them (all with results stored two or four bytes a lane).
+// With no more than one workgroup a unit, eight waves of it cover each other's loads: 512 tokens and 4096 outputs (256 workgroups) 23.1 us, of four waves 26.6, in fp32 56
+// and 72; 256 and 14336 (448) in fp32 108 and 95, as a unit's LDS holds one of them, in bf16 37 and 38.
 // Rows that are not aligned are STAGED, and take the smaller tile: 6000 tokens of 4100 inputs, 11008 outputs 605 us (aligned 460; put into LDS as they come 60 more, by the larger tile 150),
 // 898 of 3140, 2202 outputs 33 us (3136 29).
 void launch_linear_many(const LinearArgs &a, bool bf16, int scales_of_block, hipStream_t stream) {

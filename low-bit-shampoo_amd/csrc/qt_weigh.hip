@@ -400,9 +400,10 @@ __device__ __forceinline__ bool find_work(const WeighArgs &a, int index, WeighWo
 //
 // A step of 32 sequences of 100 to 8000 tokens, 8 heads of 128, groups of 4, bf16: 26 us for 85 MB of keys and scores written, 3.3 TB/s; 4 us are the
 // launch and the work found, 2.5 to 5 the first keys (length, page, keys: three loads that wait for each other), and a part has so few tokens that this is a third of its
-// time.  The last 1 to 27 tokens of four prompts of up to 32768, two tiles of rows at a time: 29 us, bound by the vector instructions (exponentials, scales, numbers
-// expanded; 45 % of all cycles) and the loads before them.  Tried: scores of a step transposed, so that no lane works on rows that are not there (31 us against 28: more
-// registers), all tiles' products in front (31 against 29).
+// time.  The last 1 to 27 tokens of four prompts of up to 32768, two tiles of rows at a time: 29 us.  No pipe is full (vector instructions, exponentials, scales and numbers
+// expanded, in 51 % of all cycles, matrix ones in 11 %): too few waves, 1.5 a SIMD on average, hide each other's loads and results, as each holds two tiles of rows and four
+// of keys in registers.  Tried: scores of a step transposed, so that no lane works on rows that are not there (31 us against 28: more registers), all tiles' products in
+// front (31 against 29).
 template <bool BF16, int STEPS, int T, bool WEIGHTS>
 __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 : 3) void weigh_rows_kernel(const WeighArgs a) {
     static_assert(T == 1 || !WEIGHTS, "weights of sixteen rows");
@@ -702,8 +703,8 @@ struct WeighGroups {
 // a workgroup have the same tokens and take rows in turn.  Then the next tokens, whose keys and first rows are on their way by then: one round of waves has
 // all tokens, a round for each four tokens' tiles took 179 us where this takes 118 (the last 100 tokens of six prompts of up to 9000, 8 heads of 128, groups of 4, bf16).
 //
-// Bound by the vector instructions, an exponential, a multiplication, two fused ones and a difference for each score and lane (4 us of 33 for the four prompts above are
-// matrix instructions), and with two waves a SIMD by what they wait for: rows' 16 bytes a lane touch sixteen lines an instruction where four lanes side by side load a
+// Bound by having few waves, two a SIMD at most and 1.3 on average, as four tiles' expanded keys alone are 64 registers: 32 us for the four prompts above, with vector
+// instructions (an exponential, a multiplication, two fused ones and a difference for each score and lane) in 36 % of all cycles, matrix ones in 8 %.  What waves wait for shows: rows' 16 bytes a lane touch sixteen lines an instruction where four lanes side by side load a
 // row, else 64 (36 us, 129 for the six prompts), and products of all tiles go first (35, 122).  Tried: 32 tokens a wave and four waves a SIMD, 57 us.
 template <bool BF16, int STEPS, bool SHARED>
 __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void weigh_tokens_kernel(const WeighArgs a) {
@@ -720,7 +721,7 @@ __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void wei
     WeighGroup g;
     if (!groups.next(a, g)) return;
     WeighKeys<STEPS, N> keys;
-    WeighRows<BF16, STEPS, BF16> q;            // (fp32: 17 rows over 32000 tokens 77 us, side by side 79)
+    WeighRows<BF16, STEPS, BF16> q;            // (fp32: a prompt of 2000 tokens, 8 heads, groups of 4 202 us, side by side 213)
     qt_u32x4 next[2];
     const auto fetch_rows = [&](const WeighSequence &v, int at) {
         q.fetch(a, v, head, at);
@@ -943,7 +944,8 @@ void launch_weigh_type(const WeighArgs &a, bool few, hipStream_t stream) {
 constexpr long long kMostScores = 1LL << 29;
 struct WeighSizes { long long partial, scores, stride, all; int parts, row_parts; bool few; };
 // Parts of the rows that see a token, where the tokens alone do not make two workgroups for each unit, of at least 256 rows on average.  A prompt of 1487 tokens, 3
-// heads, groups of 8, a window of 349, bf16: 76 us, whole 237; three of 371, 2 heads, groups of 4 36 and 42.
+// heads of 128, groups of 8, a window of 349, bf16: 47.7 us, whole 72; of 3950, one head, groups of 5 79 and 223; of 2000, 8 heads, groups of 4 103 and 128; three of 371, 2
+// heads, groups of 4 28 and 35.
 int weigh_row_parts(const CacheShape &shape, const CachePlaces &at, int group, long long room) {
     const int tokens = shape.head_dim > 128 ? 32 : 64;
     const long long groups = (room + tokens - 1) / tokens * at.batch * shape.kv_heads, rows = (long long)at.tokens * group / at.batch;
