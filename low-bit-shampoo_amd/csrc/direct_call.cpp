@@ -56,7 +56,7 @@ bool in_memory(const at::Tensor &t, int device) {
 }
 bool in_plain_memory(const at::Tensor &t, int device) { return in_memory(t, device) && t.is_contiguous(); }
 // A forward-mode derivative (torch.autograd.forward_ad): an ordinary tensor carries it, whatever the mode of gradients is.
-bool has_tangent(const at::Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const at::Tensor &t) { return t.unsafeGetTensorImpl()->autograd_meta() != nullptr && t._fw_grad(/*level=*/0).defined(); }
 // Whether a derivative is asked for that a call without one would lose.
 bool differentiated(const at::Tensor &t) { return (t.requires_grad() && c10::GradMode::is_enabled()) || has_tangent(t); }
 
