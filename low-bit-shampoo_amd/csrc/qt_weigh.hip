@@ -276,9 +276,13 @@ __device__ __forceinline__ bool row_is_infinite(const WeighArgs &a, const WeighS
     const int i = (int)fastdiv((uint32_t)row, a.by_group);
     const uint8_t *p = (const uint8_t *)a.q + ((v.start + i) * a.q_token + (head * a.group + row - i * a.group) * a.q_head) * (BF16 ? 2 : 4);
     bool found = false;
-#pragma unroll 1
-    for (int d = 0; d < a.shape.head_dim; ++d)
-        found = found || (BF16 ? (((const uint16_t *)p)[d] & 0x7fffu) == 0x7f80u : (((const uint32_t *)p)[d] & 0x7fffffffu) == 0x7f800000u);
+#pragma unroll 4
+    for (int d = 0; d < a.shape.head_dim; d += 8) {
+        Eight<BF16> x;
+        x.load(p, d, a.shape.head_dim);
+#pragma unroll
+        for (const uint32_t r : x.raw) found |= BF16 ? (r & 0x7fffu) == 0x7f80u || (r & 0x7fff0000u) == 0x7f800000u : (r & 0x7fffffffu) == 0x7f800000u;
+    }
     return found;
 }
 
@@ -556,8 +560,9 @@ __global__ __launch_bounds__(kWeighThreads, STEPS == 8 || T > 1 ? 2 : BF16 ? 4 :
             float2 part = s_part[0][threadIdx.x];
 #pragma unroll
             for (int w = 1; w < kWeighWaves; ++w) part = join_parts(part, s_part[w][threadIdx.x]);
-            // (a token of each sequence: when the parts are joined)
-            if (!(BF16 && T == 1) && part.x == -INFINITY && row_is_infinite<BF16>(a, v, head, first_row + (int)threadIdx.x)) part.y = NAN;
+            // (a token of each sequence: when the parts are joined; not for rows in front of the part: 20 over 8193 tokens 19.8 us, else 21.4)
+            const int row = first_row + (int)threadIdx.x;
+            if (!(BF16 && T == 1) && part.x == -INFINITY && v.position(a, row) >= tile_at(from) << 4 && row_is_infinite<BF16>(a, v, head, row)) part.y = NAN;
             put(part);
         }
     }
