@@ -633,10 +633,16 @@ struct Turn : torch::autograd::Function<Turn> {
             whose.push_back(i);
         }
         if (given.empty()) return out;
+        // (what was saved comes back from hooks, which may give anything, and gradients are of whoever calls: a kernel reads them)
         const auto saved = ctx->get_saved_variables();
+        const int device = (int)given[0].get_device();
+        const int64_t dims = ctx->saved_data["dims"].toInt();
+        for (const at::Tensor &d : given) TORCH_CHECK(turn_fits(d, given[0], device, dims), "gradients of turned queries and keys that are not in the GPU's memory");
+        TORCH_CHECK(positions_fit(saved[0], given[0], device) && in_plain_memory(saved[1], device) && saved[1].scalar_type() == at::kDouble && shaped(saved[1], {dims / 2}),
+                    "positions or frequencies that have come back from saved-tensor hooks as something else");
         const c10::OptionalDeviceGuard guard(given[0].device());
         const auto back = Turn::apply(given[0], given.size() > 1 ? std::optional<at::Tensor>(given[1]) : std::nullopt, saved[0], saved[1], ctx->saved_data["magnitude"].toDouble(),
-                                      ctx->saved_data["dims"].toInt(), ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["back"].toBool());
+                                      dims, ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["back"].toBool());
         for (size_t n = 0; n < whose.size(); ++n) out[whose[n]] = back[n];
         return out;
     }
