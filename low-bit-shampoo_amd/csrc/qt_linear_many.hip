@@ -33,8 +33,8 @@ __device__ __forceinline__ bool many_tile(const ManyGrid &g, int &row, int &colu
 // Bound by the matrix instructions and the vector operations between them: 6000 tokens through 11008 x 4096 in bf16 449 to 462 us, 1170 to 1200 TFLOP/s, where the
 // library's product of bf16 matrices takes 519 us; 1024 tokens through 4096 x 4096 39 us, 885 TFLOP/s; 2048 tokens through 11008 x 4096 in fp32 (three
 // matrix operations for each) 498 us, 371 TFLOP/s.  Results stored two bytes a lane: 510, 43 and 508 us.  Four lanes side by side load a token's line: 547 us where sixteen tokens' lines were touched by each.  Tried: the next operands read from LDS in front of the matrix instructions (620 us: registers), the
-// matrix instructions at a higher priority, in groups with the vector ones, or one tile ahead of them (512 to 529 us beside 513).  Of all cycles, at a clock that falls to 2.0 GHz, matrix instructions take 53 % and vector ones 55 %, in the
-// 1.8 waves that a SIMD has on average.
+// matrix instructions at a higher priority, in groups with the vector ones, or one tile ahead of them (512 to 529 us beside 513).  Of all cycles, at a clock that falls to 2.0 GHz, matrix instructions take 52 % and vector ones 55 %, in the
+// 1.7 waves that a SIMD has on average.
 //
 // STAGED: tokens on their way in registers while a block is multiplied, for rows of bf16 that are not aligned to sixteen bytes.
 // SPLIT: two times four waves, which take the blocks of 128 inputs in turn and join their sums through LDS.

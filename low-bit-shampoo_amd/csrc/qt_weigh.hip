@@ -405,7 +405,7 @@ __device__ __forceinline__ bool find_work(const WeighArgs &a, int index, WeighWo
 // A step of 32 sequences of 100 to 8000 tokens, 8 heads of 128, groups of 4, bf16: 26 us for 85 MB of keys and scores written, 3.3 TB/s; 4 us are the
 // launch and the work found, 2.5 to 5 the first keys (length, page, keys: three loads that wait for each other), and a part has so few tokens that this is a third of its
 // time.  The last 1 to 27 tokens of four prompts of up to 32768, two tiles of rows at a time: 29 us.  No pipe is full (vector instructions, exponentials, scales and numbers
-// expanded, in 51 % of all cycles, matrix ones in 11 %): too few waves, 1.5 a SIMD on average, hide each other's loads and results, as each holds two tiles of rows and four
+// expanded, in 50 % of all cycles, matrix ones in 11 %): too few waves, 1.6 a SIMD on average, hide each other's loads and results, as each holds two tiles of rows and four
 // of keys in registers.  Tried: scores of a step transposed, so that no lane works on rows that are not there (31 us against 28: more registers), all tiles' products in
 // front (31 against 29).
 template <bool BF16, int STEPS, int T, bool WEIGHTS>
@@ -709,7 +709,7 @@ struct WeighGroups {
 // all tokens, a round for each four tokens' tiles took 179 us where this takes 118 (the last 100 tokens of six prompts of up to 9000, 8 heads of 128, groups of 4, bf16).
 //
 // Bound by having few waves, two a SIMD at most and 1.3 on average, as four tiles' expanded keys alone are 64 registers: 32 us for the four prompts above, with vector
-// instructions (an exponential, a multiplication, two fused ones and a difference for each score and lane) in 36 % of all cycles, matrix ones in 8 %.  What waves wait for shows: rows' 16 bytes a lane touch sixteen lines an instruction where four lanes side by side load a
+// instructions (an exponential, a multiplication, two fused ones and a difference for each score and lane) in 37 % of all cycles, matrix ones in 8 %.  What waves wait for shows: rows' 16 bytes a lane touch sixteen lines an instruction where four lanes side by side load a
 // row, else 64 (36 us, 129 for the six prompts), and products of all tiles go first (35, 122).  Tried: 32 tokens a wave and four waves a SIMD, 57 us.
 template <bool BF16, int STEPS, bool SHARED>
 __global__ __launch_bounds__(kWeighThreads, BF16 && STEPS == 2 ? 3 : 2) void weigh_tokens_kernel(const WeighArgs a) {
